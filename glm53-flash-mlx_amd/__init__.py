@@ -37,6 +37,7 @@ from .grouped_fp8 import (
     restore_and_reduce,
 )
 from .loader import install_packed_decode_moe, install_packed_grouped_moe, install_packed_moe
+from .norms import residual_norm, rms_norm
 from .ownership import (
     ResidentTensor,
     TensorLayout,
@@ -64,5 +65,5 @@ __all__ = [
     "SortedGroupedFP8MoE", "PrefillPlan", "install_packed_moe", "install_packed_grouped_moe",
     "install_packed_decode_moe", "BankHandle", "RoutedDiagnostic", "ResidentTensor", "TensorLayout", "TensorLease", "TensorOwnership",
     "TensorOwnershipError", "borrowed_ephemeral_tensor", "borrowed_stable_tensor", "materialize_owned",
-    "owned_tensor", "require_resident", "resident_concatenate",
+    "owned_tensor", "require_resident", "resident_concatenate", "rms_norm", "residual_norm",
 ]

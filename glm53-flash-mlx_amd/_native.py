@@ -85,6 +85,41 @@ class PlanCounters(ctypes.Structure):
     ]
 
 
+# glm53_norm: gate kinds and f32_mask bits
+GATE_NONE, GATE_COLUMNS, GATE_ROWS, GATE_FULL = 0, 1, 2, 3
+NORM_F32_RESIDUAL, NORM_F32_OUT, NORM_F32_POST, NORM_F32_GATE, NORM_F32_NEXT, NORM_F32_Y = 1, 2, 4, 8, 16, 32
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [
+        ("rows", I64),
+        ("width", I64),
+        ("rows_per_gate", I64),
+        ("residual", P),
+        ("out", P),
+        ("post_weight", P),
+        ("gate", P),
+        ("next_weight", P),
+        ("new_residual", P),
+        ("y", P),
+        ("stats", P),
+        ("d_new_residual", P),
+        ("d_y", P),
+        ("d_residual", P),
+        ("d_out", P),
+        ("d_post_weight", P),
+        ("d_gate", P),
+        ("d_next_weight", P),
+        ("workspace", P),
+        ("workspace_bytes", SZ),
+        ("gate_kind", I32),
+        ("post_norm", I32),
+        ("f32_mask", I32),
+        ("scale", F32),
+        ("eps", F32),
+    ]
+
+
 _SIGNATURES = {
     "glm53_last_error": (ctypes.c_char_p, []),
     "glm53_abi_version": (ctypes.c_int, []),
@@ -138,6 +173,9 @@ _SIGNATURES = {
     "glm53_prefill_plan_scratch": (ctypes.c_int, [P, I32, P, P]),
     "glm53_prefill_plan_counters": (ctypes.c_int, [P, P]),
     "glm53_prefill_plan_identities": (ctypes.c_int, [P, P, I32, P]),
+    "glm53_residual_norm": (ctypes.c_int, [P, P]),
+    "glm53_residual_norm_workspace_bytes": (SZ, [I64, I64, I64]),
+    "glm53_residual_norm_backward": (ctypes.c_int, [P, P]),
     "glm53_synth_fp8": (ctypes.c_int, [P, P, I64, I64, ctypes.c_uint64, F32, P]),
     "glm53_synth_f32": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, F32, F32, I32, P]),
     "glm53_synth_bf16": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, P]),
@@ -192,6 +230,25 @@ def stream_handle(device: torch.device | None = None) -> int:
     if _raw_stream is None:
         return torch.cuda.current_stream(index).cuda_stream
     return _raw_stream(torch.cuda.current_device() if index is None else index)
+
+
+def run(device: torch.device, fn, *args) -> None:
+    """`fn(*args, stream)` on torch's current stream of `device`, which is made
+    the current device for the call where it is not."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, stream_handle(device)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, stream_handle(device)))
+
+
+def require_same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """One ROCm device for every tensor given (None: absent)."""
+    require_device(first)
+    for t in others:
+        if t is not None and t.device != first.device:
+            require_device(t)
+            raise ValueError(f"tensors on {first.device} and {t.device}: one device is needed")
 
 
 def require_device(*tensors: torch.Tensor) -> None:

@@ -19,7 +19,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OUT = PKG / "libglm53_moe.so"
 BUILD = PKG / "_build"
-SOURCES = ["decode.hip", "step.hip", "grouped.hip", "dense.hip", "router.hip", "layout.hip", "synth.hip", "api.cpp"]
+SOURCES = ["decode.hip", "step.hip", "grouped.hip", "dense.hip", "router.hip", "layout.hip", "synth.hip", "norms.hip",
+           "api.cpp", "api_block.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

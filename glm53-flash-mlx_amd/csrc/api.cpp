@@ -14,6 +14,7 @@
 #include <string>
 #include <vector>
 
+#include "api_util.h"
 #include "dense.h"
 #include "grouped.h"
 #include "kernels.h"
@@ -25,36 +26,6 @@ using namespace glm53;
 namespace {
 
 thread_local std::string g_error;
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_error = buf;
-  return code;
-}
-
-int hip_fail(hipError_t e, const char* what) {
-  return fail(GLM53_DEVICE_ERROR, "%s: %s", what, hipGetErrorString(e));
-}
-
-#define HIP_TRY(expr, what)                      \
-  do {                                           \
-    hipError_t _e = (expr);                      \
-    if (_e != hipSuccess) return hip_fail(_e, what); \
-  } while (0)
-
-#define CHECK_ARG(cond, ...)                                        \
-  do {                                                              \
-    if (!(cond)) return fail(GLM53_INVALID_ARGUMENT, __VA_ARGS__);  \
-  } while (0)
-
-inline hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
-inline size_t round_up(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
 // Bytes of the hi/lo/scale split of a [rows, cols] activation matrix.
 size_t split_bytes(int64_t rows, int64_t cols) {
@@ -287,6 +258,16 @@ int route_tokens(const glm53_router* r, const void* x, int64_t T, float* space, 
 }
 
 }  // namespace
+
+int glm53::fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_error = buf;
+  return code;
+}
 
 extern "C" {
 

@@ -1,0 +1,414 @@
+// Norms before and after a block, fused with the block's gate and residual
+// scale, and their gradients.
+//
+//   s = o r_o p,  r_o = (mean o^2 + eps)^-1/2     (without a post norm: s = o)
+//   x' = x + a g s
+//   y = x' r' w,  r' = (mean x'^2 + eps)^-1/2
+//
+// One workgroup holds a row in registers from its load to its store, so each
+// tensor crosses HBM once: the kernels are bound by those bytes.  All values
+// between load and store are fp32; y is made of the x' that has not been
+// rounded yet.
+#include "common.h"
+#include "norms.h"
+
+namespace glm53 {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <int VEC>
+struct Raw;
+template <>
+struct Raw<8> {
+  u32x4 lo, hi;
+};
+template <>
+struct Raw<1> {
+  uint32_t v;
+};
+
+// VEC elements from element index i, as stored; converted by to_float once
+// every load of the row is on its way.
+template <int VEC>
+__device__ __forceinline__ Raw<VEC> load_raw(const Tensor& t, int64_t i) {
+  Raw<VEC> r;
+  if constexpr (VEC == 8) {
+    if (t.f32) {
+      const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(t.p) + i);
+      r.lo = p[0];
+      r.hi = p[1];
+    } else {
+      r.lo = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(t.p) + i);
+    }
+  } else {
+    if (t.f32)
+      r.v = static_cast<const uint32_t*>(t.p)[i];
+    else
+      r.v = static_cast<const uint16_t*>(t.p)[i];
+  }
+  return r;
+}
+
+template <int VEC>
+__device__ __forceinline__ void to_float(const Raw<VEC>& r, bool f32, float* v) {
+  if constexpr (VEC == 8) {
+    if (f32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = __uint_as_float(r.lo[e]);
+        v[4 + e] = __uint_as_float(r.hi[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = __uint_as_float(r.lo[e] << 16);
+        v[2 * e + 1] = __uint_as_float(r.lo[e] & 0xFFFF0000u);
+      }
+    }
+  } else {
+    v[0] = __uint_as_float(f32 ? r.v : r.v << 16);
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void store(const Tensor& t, int64_t i, const float* v) {
+  if constexpr (VEC == 8) {
+    if (t.f32) {
+      u32x4* p = reinterpret_cast<u32x4*>(static_cast<float*>(t.p) + i);
+      u32x4 lo, hi;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = __float_as_uint(v[e]);
+        hi[e] = __float_as_uint(v[4 + e]);
+      }
+      p[0] = lo;
+      p[1] = hi;
+    } else {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = f32_to_bf16(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16(v[2 * e + 1])) << 16;
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(t.p) + i) = w;
+    }
+  } else {
+    if (t.f32)
+      static_cast<float*>(t.p)[i] = v[0];
+    else
+      static_cast<uint16_t*>(t.p)[i] = f32_to_bf16(v[0]);
+  }
+}
+
+__device__ __forceinline__ float scalar(const Tensor& t, int64_t i) {
+  return t.f32 ? static_cast<const float*>(t.p)[i] : bf16_to_f32(static_cast<const uint16_t*>(t.p)[i]);
+}
+
+// Sum over the T threads of a row, in every one of them.  `turn` alternates
+// between two sets of LDS words, so one barrier a sum is enough.
+template <int T>
+__device__ __forceinline__ float row_sum(float v, float (*words)[T / kWave], int& turn) {
+  v = wave_sum(v);
+  if constexpr (T == kWave) return v;
+  float* w = words[turn];
+  turn ^= 1;
+  if ((threadIdx.x & (kWave - 1)) == 0) w[threadIdx.x / kWave] = v;
+  __syncthreads();
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < T / kWave; ++i) s += w[i];
+  return s;
+}
+
+// A row's threads and how its elements lie on them: T threads, C chunks of
+// VEC consecutive elements each, chunk c of thread t at (c T + t) VEC.
+template <int T, int VEC, int C>
+struct Row {
+  static constexpr int kN = VEC * C;
+  __device__ static __forceinline__ int64_t at(int c) { return (static_cast<int64_t>(c) * T + threadIdx.x) * VEC; }
+
+  // Row elements [base, base + width) of t; elements past the width read 0.
+  __device__ static __forceinline__ void raw(const Tensor& t, int64_t base, int64_t width, Raw<VEC> (&r)[C]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      r[c] = Raw<VEC>{};
+      if (t.p != nullptr && at(c) < width) r[c] = load_raw<VEC>(t, base + at(c));
+    }
+  }
+  __device__ static __forceinline__ void floats(const Raw<VEC> (&r)[C], const Tensor& t, float (&v)[kN]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) to_float<VEC>(r[c], t.f32, v + c * VEC);
+  }
+  __device__ static __forceinline__ void put(const Tensor& t, int64_t base, int64_t width, const float (&v)[kN]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (at(c) < width) store<VEC>(t, base + at(c), v + c * VEC);
+  }
+  // Column values of a weight that may be absent (1).
+  __device__ static __forceinline__ void weight(const Tensor& t, int64_t base, int64_t width, float (&v)[kN]) {
+    if (t.p == nullptr) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) v[e] = 1.0f;
+      return;
+    }
+    Raw<VEC> r[C];
+    raw(t, base, width, r);
+    floats(r, t, v);
+  }
+};
+
+__device__ __forceinline__ int64_t gate_base(const NormArgs& a, int64_t row) {
+  return a.gate_kind == kGateFull ? row * a.width : row / a.rows_per_gate * a.width;
+}
+
+template <int T, int VEC, int C>
+__device__ __forceinline__ void gate_values(const NormArgs& a, int64_t row, float (&g)[VEC * C]) {
+  using R = Row<T, VEC, C>;
+  if (a.gate_kind == kGateRows) {
+    const float v = scalar(a.gate, row);
+#pragma unroll
+    for (int e = 0; e < VEC * C; ++e) g[e] = v;
+  } else if (a.gate_kind == kGateNone) {
+#pragma unroll
+    for (int e = 0; e < VEC * C; ++e) g[e] = 1.0f;
+  } else {
+    R::weight(a.gate, gate_base(a, row), a.width, g);
+  }
+}
+
+template <int T, int VEC, int C, bool POST>
+__global__ __launch_bounds__(T) void norm_forward_kernel(NormArgs a) {
+  using R = Row<T, VEC, C>;
+  constexpr int N = R::kN;
+  __shared__ float words[2][T / kWave];
+  int turn = 0;
+  const float inv_width = 1.0f / static_cast<float>(a.width);
+  const int64_t row = blockIdx.x, base = row * a.width;
+  Raw<VEC> rx[C], ro[C];
+  R::raw(a.residual, base, a.width, rx);
+  if (POST) R::raw(a.out, base, a.width, ro);
+  float x[N];
+  R::floats(rx, a.residual, x);
+  if (POST) {
+    float o[N], g[N];
+    R::floats(ro, a.out, o);
+    gate_values<T, VEC, C>(a, row, g);
+    float r_o = 1.0f;
+    if (a.post_norm) {
+      float p[N];
+      R::weight(a.post, 0, a.width, p);
+      float ss = 0.0f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) ss += o[e] * o[e];
+      r_o = 1.0f / sqrtf(row_sum<T>(ss, words, turn) * inv_width + a.eps);
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = o[e] * r_o * p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] += a.scale * g[e] * o[e];
+    R::put(a.new_residual, base, a.width, x);
+    if (a.stats != nullptr && threadIdx.x == 0) a.stats[2 * row] = r_o;
+  }
+  if (a.y.p == nullptr) return;
+  float w[N];
+  R::weight(a.next, 0, a.width, w);
+  float ss = 0.0f;
+  // elements past the width: x is 0 there
+#pragma unroll
+  for (int e = 0; e < N; ++e) ss += x[e] * x[e];
+  const float r = 1.0f / sqrtf(row_sum<T>(ss, words, turn) * inv_width + a.eps);
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = x[e] * r * w[e];
+  R::put(a.y, base, a.width, x);
+  if (a.stats != nullptr && threadIdx.x == 0) a.stats[2 * row + 1] = r;
+}
+
+// Rows [first, last) of backward workgroup `slice`, which lie in one gate group.
+struct Slice {
+  int64_t first, last;
+};
+__device__ __forceinline__ Slice slice_rows(int64_t rows, int64_t groups, int64_t slices, int64_t slice) {
+  const int64_t per = rows / groups, each = slices / groups, chunk = (per + each - 1) / each;
+  const int64_t g = slice / each, s = slice % each;
+  const int64_t first = g * per + min(s * chunk, per);
+  return {first, g * per + min((s + 1) * chunk, per)};
+}
+
+// Each workgroup takes a run of rows and keeps the column sums of d_post,
+// d_gate (kGateColumns) and d_next in registers, written once as one row of
+// fp32 partial sums: 3 width floats against 16 rows or more of five tensors.
+// The order of the sums is the rows', whatever runs when.
+template <int T, int VEC, int C, bool POST>
+__global__ __launch_bounds__(T) void norm_backward_kernel(NormArgs a, int64_t groups, int64_t slices) {
+  using R = Row<T, VEC, C>;
+  constexpr int N = R::kN;
+  __shared__ float words[2][T / kWave];
+  int turn = 0;
+  const float inv_width = 1.0f / static_cast<float>(a.width);
+  float s_next[N], s_post[N], s_gate[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) s_next[e] = s_post[e] = s_gate[e] = 0.0f;
+  const Slice rows = slice_rows(a.rows, groups, slices, blockIdx.x);
+  for (int64_t row = rows.first; row < rows.last; ++row) {
+    const int64_t base = row * a.width;
+    Raw<VEC> rx[C], ro[C], rn[C], ry[C];
+    R::raw(a.residual, base, a.width, rx);
+    if (POST) R::raw(a.out, base, a.width, ro);
+    R::raw(a.d_new, base, a.width, rn);
+    R::raw(a.d_y, base, a.width, ry);
+    const float r_o = POST && a.post_norm ? a.stats[2 * row] : 1.0f;
+    float x[N], o[N], g[N], p[N], d[N];
+    R::floats(rx, a.residual, x);
+    R::floats(rn, a.d_new, d);
+    if (POST) {
+      R::floats(ro, a.out, o);
+      gate_values<T, VEC, C>(a, row, g);
+      R::weight(a.post, 0, a.width, p);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        o[e] *= r_o;
+        x[e] += a.scale * g[e] * (o[e] * p[e]);
+      }
+    }
+    if (a.d_y.p != nullptr) {
+      const float r = a.stats[2 * row + 1];
+      float dy[N], w[N], dot = 0.0f;
+      R::floats(ry, a.d_y, dy);
+      R::weight(a.next, 0, a.width, w);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        x[e] *= r;
+        s_next[e] += dy[e] * x[e];
+        dy[e] *= w[e];
+        dot += dy[e] * x[e];
+      }
+      const float m = row_sum<T>(dot, words, turn) * inv_width;
+#pragma unroll
+      for (int e = 0; e < N; ++e) d[e] += r * (dy[e] - x[e] * m);
+    }
+    if (a.d_residual.p != nullptr) R::put(a.d_residual, base, a.width, d);
+    if (!POST) continue;
+    if (a.d_gate.p != nullptr) {
+      float dg[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) dg[e] = a.scale * (o[e] * p[e]) * d[e];
+      if (a.gate_kind == kGateColumns) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) s_gate[e] += dg[e];
+      } else if (a.gate_kind == kGateFull) {
+        R::put(a.d_gate, base, a.width, dg);
+      } else {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += dg[e];
+        sum = row_sum<T>(sum, words, turn);
+        if (threadIdx.x == 0) store<1>(a.d_gate, row, &sum);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] *= a.scale * g[e];
+    if (a.post_norm) {
+      float dot = 0.0f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        s_post[e] += d[e] * o[e];
+        d[e] *= p[e];
+        dot += d[e] * o[e];
+      }
+      const float m = row_sum<T>(dot, words, turn) * inv_width;
+#pragma unroll
+      for (int e = 0; e < N; ++e) d[e] = r_o * (d[e] - o[e] * m);
+    }
+    if (a.d_out.p != nullptr) R::put(a.d_out, base, a.width, d);
+  }
+  const Tensor part = {a.partial, true};
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kNormSums * a.width;
+  if (a.d_next.p != nullptr) R::put(part, at, a.width, s_next);
+  if (a.d_post.p != nullptr) R::put(part, at + a.width, a.width, s_post);
+  if (a.d_gate.p != nullptr && a.gate_kind == kGateColumns) R::put(part, at + 2 * a.width, a.width, s_gate);
+}
+
+// Adds the partial rows: out[v][column] = sum over rows first_v .. of sum v,
+// blockIdx.y = 0 d_next, 1 d_post, 2 + g d_gate of gate group g.  16 row
+// slices of 64 columns a workgroup, joined in LDS in their order.
+constexpr int kJoin = 16;
+__global__ __launch_bounds__(kWave* kJoin) void norm_join_kernel(NormArgs a, int64_t groups, int64_t slices) {
+  __shared__ float part[kJoin][kWave];
+  const int v = blockIdx.y < 2 ? blockIdx.y : 2;
+  const Tensor out = v == 0 ? a.d_next : v == 1 ? a.d_post : a.d_gate;
+  if (out.p == nullptr || (v == 2 && a.gate_kind != kGateColumns)) return;
+  const int64_t each = slices / groups, g = v == 2 ? blockIdx.y - 2 : 0;
+  const int64_t first = v == 2 ? g * each : 0, count = v == 2 ? each : slices;
+  const int lane = threadIdx.x & (kWave - 1), slot = threadIdx.x / kWave;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kWave + lane;
+  float sum = 0.0f;
+  if (col < a.width)
+    for (int64_t s = slot; s < count; s += kJoin) sum += a.partial[((first + s) * kNormSums + v) * a.width + col];
+  part[slot][lane] = sum;
+  __syncthreads();
+  if (slot != 0 || col >= a.width) return;
+  sum = part[0][lane];
+#pragma unroll
+  for (int i = 1; i < kJoin; ++i) sum += part[i][lane];
+  store<1>(out, g * a.width + col, &sum);
+}
+
+template <int T, int VEC, int C>
+hipError_t launch_shape(const NormArgs& a, bool backward, int64_t groups, int64_t slices, hipStream_t st) {
+  const bool post = a.out.p != nullptr;
+  if (!backward) {
+    const dim3 grid(static_cast<uint32_t>(a.rows));
+    if (post)
+      norm_forward_kernel<T, VEC, C, true><<<grid, T, 0, st>>>(a);
+    else
+      norm_forward_kernel<T, VEC, C, false><<<grid, T, 0, st>>>(a);
+  } else {
+    const dim3 grid(static_cast<uint32_t>(slices));
+    if (post)
+      norm_backward_kernel<T, VEC, C, true><<<grid, T, 0, st>>>(a, groups, slices);
+    else
+      norm_backward_kernel<T, VEC, C, false><<<grid, T, 0, st>>>(a, groups, slices);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_any(const NormArgs& a, bool vec, bool backward, int64_t groups, int64_t slices, hipStream_t st) {
+  const int64_t w = a.width;
+  if (vec) {
+    if (w <= 512) return launch_shape<64, 8, 1>(a, backward, groups, slices, st);
+    if (w <= 2048) return launch_shape<256, 8, 1>(a, backward, groups, slices, st);
+    if (w <= 4096) return launch_shape<256, 8, 2>(a, backward, groups, slices, st);
+    if (w <= 8192) return launch_shape<512, 8, 2>(a, backward, groups, slices, st);
+    return launch_shape<1024, 8, 2>(a, backward, groups, slices, st);
+  }
+  if (w <= 512) return launch_shape<64, 1, 8>(a, backward, groups, slices, st);
+  if (w <= 2048) return launch_shape<256, 1, 8>(a, backward, groups, slices, st);
+  return launch_shape<1024, 1, 8>(a, backward, groups, slices, st);
+}
+
+int64_t gate_groups(const NormArgs& a) {
+  return a.gate_kind == kGateColumns && a.rows > 0 ? a.rows / a.rows_per_gate : 1;
+}
+
+}  // namespace
+
+int64_t norm_slices(int64_t rows, int64_t groups) {
+  const int64_t per = rows / groups;
+  const int64_t each = 512 / groups;
+  return groups * (each < 1 ? 1 : each > per ? per : each);
+}
+
+hipError_t launch_norm_forward(const NormArgs& a, bool vec, hipStream_t st) {
+  return launch_any(a, vec, false, 1, 1, st);
+}
+
+hipError_t launch_norm_backward(const NormArgs& a, bool vec, hipStream_t st) {
+  const int64_t groups = gate_groups(a), slices = norm_slices(a.rows, groups);
+  if (slices > 0)  // without rows the sums are zero
+    if (hipError_t e = launch_any(a, vec, true, groups, slices, st); e != hipSuccess) return e;
+  const bool gates = a.d_gate.p != nullptr && a.gate_kind == kGateColumns;
+  if (a.d_next.p == nullptr && a.d_post.p == nullptr && !gates) return hipSuccess;
+  const dim3 grid(static_cast<uint32_t>((a.width + kWave - 1) / kWave), static_cast<uint32_t>(2 + (gates ? groups : 0)));
+  norm_join_kernel<<<grid, kWave * kJoin, 0, st>>>(a, groups, slices);
+  return hipGetLastError();
+}
+
+}  // namespace glm53

@@ -15,7 +15,10 @@ and FakeTensor / meta propagation gets the output shapes without a device.
 * ``glm53::moe_prefill(x, owner, expert_ids?, scores?)`` -- the grouped
   prefill of a ``SortedGroupedFP8MoE``;
 * ``glm53::moe_direct(x, owner)`` -- a batch below a ``SortedGroupedFP8MoE``'s
-  min_routes as one prefill in the Direct order.
+  min_routes as one prefill in the Direct order;
+* ``glm53::residual_norm(residual, out?, post_weight?, gate?, next_weight?,
+  ...)`` and ``glm53::residual_norm_backward`` -- ``rms_norm`` (without out)
+  and ``residual_norm``, differentiable.
 
 The MoE ops take the module by an integer key (``register_owner``): the
 module keeps its weights, its per-(device, stream) native plans and its
@@ -86,6 +89,12 @@ def direct(*tensors) -> bool:
     return True
 
 
+def eager(*tensors) -> bool:
+    """As ``direct``, but with reverse-mode differentiation allowed: a call
+    that nothing else acts on may run as a torch.autograd.Function."""
+    return not _dispatch_acts() and all(t is None or type(t) in _PLAIN_TENSORS for t in tensors)
+
+
 def _owner(key: int):
     ref = _OWNERS.get(int(key))
     module = ref() if ref is not None else None
@@ -151,3 +160,59 @@ def moe_direct(x: torch.Tensor, owner: int) -> torch.Tensor:
 @moe_direct.register_fake
 def _(x, owner):
     return torch.empty_like(x)
+
+
+@torch.library.custom_op("glm53::residual_norm", mutates_args=())
+def residual_norm(residual: torch.Tensor, out: Optional[torch.Tensor], post_weight: Optional[torch.Tensor],
+                  gate: Optional[torch.Tensor], next_weight: Optional[torch.Tensor], kind: int, rows_per_gate: int,
+                  scale: float, eps: float, normed: bool,
+                  y_f32: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from .norms import native_residual_norm
+
+    return native_residual_norm(residual, out, post_weight, gate, next_weight, kind, rows_per_gate, scale, eps, normed,
+                                y_f32)
+
+
+@residual_norm.register_fake
+def _(residual, out, post_weight, gate, next_weight, kind, rows_per_gate, scale, eps, normed, y_f32):
+    y_type = torch.float32 if y_f32 else torch.bfloat16
+    rows = residual.numel() // residual.shape[-1]
+    return (residual.new_empty(residual.shape if out is not None else 0),
+            residual.new_empty(residual.shape if normed else 0, dtype=y_type),
+            residual.new_empty((rows, 2), dtype=torch.float32))
+
+
+@torch.library.custom_op("glm53::residual_norm_backward", mutates_args=())
+def residual_norm_backward(residual: torch.Tensor, out: Optional[torch.Tensor], post_weight: Optional[torch.Tensor],
+                           gate: Optional[torch.Tensor], next_weight: Optional[torch.Tensor], stats: torch.Tensor,
+                           d_new: Optional[torch.Tensor], d_y: Optional[torch.Tensor], kind: int, rows_per_gate: int,
+                           scale: float, eps: float, y_f32: bool, wanted: list[bool]) -> list[torch.Tensor]:
+    from .norms import native_residual_norm_backward
+
+    return native_residual_norm_backward(residual, out, post_weight, gate, next_weight, stats, d_new, d_y, kind,
+                                         rows_per_gate, scale, eps, y_f32, wanted)
+
+
+@residual_norm_backward.register_fake
+def _(residual, out, post_weight, gate, next_weight, stats, d_new, d_y, kind, rows_per_gate, scale, eps, y_f32, wanted):
+    inputs = (residual, out, post_weight, gate, next_weight)
+    return [t.new_empty(t.shape) if t is not None and w else residual.new_empty(0) for t, w in zip(inputs, wanted)]
+
+
+def _residual_norm_context(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:5], output[2])
+    ctx.form = inputs[5:]
+    ctx.set_materialize_grads(False)
+
+
+def _residual_norm_backward(ctx, d_new, d_y, _):
+    saved = ctx.saved_tensors
+    kind, rows_per_gate, scale, eps, normed, y_f32 = ctx.form
+    wanted = [bool(w) for w in ctx.needs_input_grad[:5]]
+    grads = torch.ops.glm53.residual_norm_backward(*saved, d_new if saved[1] is not None else None,
+                                                   d_y if normed else None, kind, rows_per_gate, scale, eps, y_f32,
+                                                   wanted)
+    return (*(g if w else None for g, w in zip(grads, wanted)), None, None, None, None, None, None)
+
+
+residual_norm.register_autograd(_residual_norm_backward, setup_context=_residual_norm_context)

@@ -521,6 +521,65 @@ int glm53_prefill_plan_identities(const glm53_prefill_plan* plan, uint64_t* out,
 int glm53_prefill_plan_scratch(glm53_prefill_plan* plan, int32_t which, void** ptr, size_t* bytes);
 
 /* ------------------------------------------------------------------------
+ * Norms around a block (no reference counterpart: the reference's layers take
+ * them from mlx-vlm).  Every feed-forward of this library takes a normalised
+ * input and returns what is still to be added to the residual stream.
+ * ---------------------------------------------------------------------- */
+#define GLM53_GATE_NONE 0
+#define GLM53_GATE_COLUMNS 1 /* gate [rows / rows_per_gate, width]: row r takes gate row r / rows_per_gate */
+#define GLM53_GATE_ROWS 2    /* gate [rows] */
+#define GLM53_GATE_FULL 3    /* gate [rows, width] */
+/* f32_mask: tensors that are FP32 instead of BF16 */
+#define GLM53_NORM_F32_RESIDUAL 1 /* residual, new_residual and their gradients */
+#define GLM53_NORM_F32_OUT 2
+#define GLM53_NORM_F32_POST 4
+#define GLM53_NORM_F32_GATE 8
+#define GLM53_NORM_F32_NEXT 16
+#define GLM53_NORM_F32_Y 32
+/*   s = out / rms(out) * post_weight     (post_norm 0: s = out)
+ *   new_residual = residual + scale * gate * s
+ *   y = new_residual / rms(new_residual) * next_weight
+ * with rms(v) = sqrt(mean(v^2) + eps), over contiguous rows of `width`
+ * elements (at most 16384; above 8192 a multiple of 8 with every tensor
+ * 16-byte aligned).  FP32 throughout, each output rounded once; y is made of
+ * the new residual before it is rounded.  NULL: out (then y is the norm of
+ * `residual` alone), post_weight and next_weight (ones), gate (one), y (not
+ * computed), stats.  new_residual may be `residual` or `out` itself, y may be
+ * `out` or (without out) `residual`.  stats f32 [rows, 2] keeps 1 / rms(out)
+ * and 1 / rms(new_residual) for the backward call. */
+typedef struct glm53_norm {
+  int64_t rows, width, rows_per_gate;
+  const void* residual;
+  const void* out;
+  const void* post_weight; /* [width] */
+  const void* gate;
+  const void* next_weight; /* [width] */
+  void* new_residual;
+  void* y;
+  float* stats;
+  /* backward only; d_new_residual, d_y NULL: zero; results NULL: not wanted */
+  const void* d_new_residual;
+  const void* d_y;
+  void* d_residual;
+  void* d_out;
+  void* d_post_weight;
+  void* d_gate; /* as gate */
+  void* d_next_weight;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t gate_kind, post_norm, f32_mask;
+  float scale, eps;
+} glm53_norm;
+int glm53_residual_norm(const glm53_norm* norm, void* stream);
+/* The gradients, from the forward call's inputs and stats.  Sums over rows
+ * (d_post_weight, d_gate of GLM53_GATE_COLUMNS, d_next_weight) are FP32 in a
+ * fixed order.  Workspace (16-byte aligned) for gate_rows = rows /
+ * rows_per_gate gate rows, 1 for the other kinds.  No output may overlap an
+ * input, except that d_residual may be d_new_residual. */
+size_t glm53_residual_norm_workspace_bytes(int64_t rows, int64_t width, int64_t gate_rows);
+int glm53_residual_norm_backward(const glm53_norm* norm, void* stream);
+
+/* ------------------------------------------------------------------------
  * Seeded synthetic inputs (no reference counterpart: the reference loads a
  * checkpoint).  Element i of stream `seed` is N(0, std) (or U(lo, hi)). */
 int glm53_synth_fp8(uint8_t* codes, float* scale_inv, int64_t rows, int64_t cols, uint64_t seed,

@@ -1,0 +1,78 @@
+"""CPU checks of the dense feed-forward block's C entry points: arguments are
+refused before any device work (status 1 with a message), sizes of
+workspaces, and no CPU fallback in the Python functions."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from conftest import pkg, submodule
+
+FAKE = 1 << 20  # never dereferenced: every call here is refused or has nothing to do
+
+
+@pytest.fixture(scope="module")
+def N():
+    return submodule("_native")
+
+
+@pytest.fixture(scope="module")
+def libso(N):
+    return N.load_library()
+
+
+def _norm(N, **changes):
+    n = N.Norm(rows=4, width=64, rows_per_gate=4, residual=FAKE, out=FAKE, post_weight=FAKE, gate=FAKE, next_weight=FAKE,
+               new_residual=FAKE, y=FAKE, stats=FAKE, gate_kind=N.GATE_COLUMNS, post_norm=1, scale=1.0, eps=1e-6)
+    for name, value in changes.items():
+        setattr(n, name, value)
+    return ctypes.byref(n)
+
+
+@pytest.mark.parametrize("changes, message", [
+    (dict(rows=-1), "invalid shape"), (dict(width=0), "invalid shape"), (dict(rows=1 << 31), "invalid shape"),
+    (dict(width=16392), "exceeds"), (dict(width=8193), "multiple of 8"), (dict(width=12288, y=FAKE + 2), "multiple of 8"),
+    (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(f32_mask=64), "f32_mask"),
+    (dict(gate_kind=4), "gate kind"), (dict(gate=None), "gate"), (dict(gate_kind=0), "gate"),
+    (dict(rows_per_gate=0), "rows_per_gate"), (dict(rows_per_gate=3), "rows_per_gate"),
+    (dict(out=None), "without a block output"), (dict(post_norm=0), "post_weight"),
+    (dict(residual=None), "null"), (dict(new_residual=None), "null"),
+    (dict(out=None, gate=None, gate_kind=0, post_weight=None, post_norm=0, y=None), "nothing to compute"),
+])
+def test_norm_refusals(N, libso, changes, message):
+    assert libso.glm53_residual_norm(_norm(N, **changes), None) == N.INVALID_ARGUMENT
+    assert message in libso.glm53_last_error().decode()
+
+
+@pytest.mark.parametrize("changes, message", [
+    (dict(), "workspace"), (dict(workspace=FAKE, workspace_bytes=16), "workspace"),
+    (dict(workspace=FAKE + 4, workspace_bytes=1 << 30), "workspace"), (dict(stats=None), "null"),
+    (dict(gate=None, gate_kind=0, d_gate=FAKE), "d_gate"),
+    (dict(post_norm=0, post_weight=None, d_post_weight=FAKE), "d_post_weight"),
+    (dict(out=None, gate=None, gate_kind=0, post_weight=None, post_norm=0, d_out=FAKE), "d_out"),
+])
+def test_norm_backward_refusals(N, libso, changes, message):
+    assert libso.glm53_residual_norm_backward(_norm(N, **changes), None) == N.INVALID_ARGUMENT
+    assert message in libso.glm53_last_error().decode()
+
+
+def test_norm_without_rows_and_workspace_sizes(N, libso):
+    assert libso.glm53_residual_norm(None, None) == N.INVALID_ARGUMENT
+    assert libso.glm53_residual_norm(_norm(N, rows=0, residual=None), None) == N.OK
+    size = libso.glm53_residual_norm_workspace_bytes
+    assert size(0, 64, 1) == size(4, 0, 1) == size(4, 64, 5) == size(4, 64, 0) == 0
+    assert size(4, 64, 1) == 4 * 3 * 64 * 4
+    assert size(8192, 4096, 1) <= 512 * 3 * 4096 * 4
+    assert size(8192, 64, 8192) == 8192 * 3 * 64 * 4
+
+
+def test_python_functions_refuse_cpu_tensors():
+    import torch
+
+    M = pkg()
+    x, w = torch.zeros(2, 64, dtype=torch.bfloat16), torch.ones(64)
+    for call in (lambda: M.rms_norm(x, w), lambda: M.residual_norm(x, x, next_weight=w)):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
