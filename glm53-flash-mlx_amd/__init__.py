@@ -26,6 +26,7 @@ from .fp8 import (
     block_fp8_linear,
     swiglu,
 )
+from .gated import GatedMLP, gated_mlp
 from .grouped_fp8 import (
     GROUPED_TILE_ROWS,
     PrefillPlan,
@@ -65,5 +66,5 @@ __all__ = [
     "SortedGroupedFP8MoE", "PrefillPlan", "install_packed_moe", "install_packed_grouped_moe",
     "install_packed_decode_moe", "BankHandle", "RoutedDiagnostic", "ResidentTensor", "TensorLayout", "TensorLease", "TensorOwnership",
     "TensorOwnershipError", "borrowed_ephemeral_tensor", "borrowed_stable_tensor", "materialize_owned",
-    "owned_tensor", "require_resident", "resident_concatenate", "rms_norm", "residual_norm",
+    "owned_tensor", "require_resident", "resident_concatenate", "rms_norm", "residual_norm", "gated_mlp", "GatedMLP",
 ]

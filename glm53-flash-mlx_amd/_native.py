@@ -120,6 +120,29 @@ class Norm(ctypes.Structure):
     ]
 
 
+class GatedMLP(ctypes.Structure):
+    _fields_ = [
+        ("rows", I64),
+        ("hidden", I64),
+        ("intermediate", I64),
+        ("x", P),
+        ("gate_weight", P),
+        ("up_weight", P),
+        ("down_weight", P),
+        ("y", P),
+        ("gate", P),
+        ("up", P),
+        ("d_y", P),
+        ("d_x", P),
+        ("d_gate_weight", P),
+        ("d_up_weight", P),
+        ("d_down_weight", P),
+        ("workspace", P),
+        ("workspace_bytes", SZ),
+        ("limit", F32),
+    ]
+
+
 _SIGNATURES = {
     "glm53_last_error": (ctypes.c_char_p, []),
     "glm53_abi_version": (ctypes.c_int, []),
@@ -176,6 +199,10 @@ _SIGNATURES = {
     "glm53_residual_norm": (ctypes.c_int, [P, P]),
     "glm53_residual_norm_workspace_bytes": (SZ, [I64, I64, I64]),
     "glm53_residual_norm_backward": (ctypes.c_int, [P, P]),
+    "glm53_gated_mlp_workspace_bytes": (SZ, [I64, I64, I64]),
+    "glm53_gated_mlp": (ctypes.c_int, [P, P]),
+    "glm53_gated_mlp_backward_workspace_bytes": (SZ, [I64, I64, I64]),
+    "glm53_gated_mlp_backward": (ctypes.c_int, [P, P]),
     "glm53_synth_fp8": (ctypes.c_int, [P, P, I64, I64, ctypes.c_uint64, F32, P]),
     "glm53_synth_f32": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, F32, F32, I32, P]),
     "glm53_synth_bf16": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, P]),

@@ -1,6 +1,7 @@
 // C ABI of the dense feed-forward block (declared in include/glm53_moe.h):
-// the norms around it.
+// the norms around it and the gated MLP.
 #include "api_util.h"
+#include "gated.h"
 #include "norms.h"
 
 using namespace glm53;
@@ -103,6 +104,86 @@ int glm53_residual_norm_backward(const glm53_norm* norm, void* stream) {
   bool vec;
   if (int rc = norm_args(norm, true, a, vec)) return rc;
   HIP_TRY(launch_norm_backward(a, vec, S(stream)), "norm gradient launch");
+  return GLM53_OK;
+}
+
+}  // extern "C"
+
+// ----------------------------------------------------------- gated MLP ----
+
+namespace {
+
+constexpr int64_t kGatedMaxWidth = int64_t{1} << 22;  // 256 rows of a tile within 32-bit byte offsets
+
+int gated_args(const glm53_gated_mlp_desc* d, GatedArgs& a) {
+  CHECK_ARG(d != nullptr, "gated MLP descriptor is null");
+  CHECK_ARG(d->rows >= 0 && d->rows < (int64_t{1} << 31) && d->hidden > 0 && d->intermediate > 0,
+            "invalid shape rows=%lld hidden=%lld intermediate=%lld", (long long)d->rows, (long long)d->hidden,
+            (long long)d->intermediate);
+  CHECK_ARG(d->hidden % 8 == 0 && d->intermediate % 8 == 0, "hidden %lld and intermediate %lld must be multiples of 8",
+            (long long)d->hidden, (long long)d->intermediate);
+  CHECK_ARG(d->hidden <= kGatedMaxWidth && d->intermediate <= kGatedMaxWidth, "widths above %lld",
+            (long long)kGatedMaxWidth);
+  CHECK_ARG(d->limit > 0.0f, "limit must be positive (infinity: no clamp)");
+  a = GatedArgs{};
+  a.x = static_cast<const uint16_t*>(d->x);
+  a.wg = static_cast<const uint16_t*>(d->gate_weight);
+  a.wu = static_cast<const uint16_t*>(d->up_weight);
+  a.wd = static_cast<const uint16_t*>(d->down_weight);
+  a.rows = d->rows;
+  a.hidden = d->hidden;
+  a.inter = d->intermediate;
+  a.limit = d->limit;
+  a.y = static_cast<uint16_t*>(d->y);
+  a.gate = d->gate;
+  a.up = d->up;
+  a.dy = static_cast<const uint16_t*>(d->d_y);
+  a.dx = static_cast<uint16_t*>(d->d_x);
+  a.d_wg = static_cast<uint16_t*>(d->d_gate_weight);
+  a.d_wu = static_cast<uint16_t*>(d->d_up_weight);
+  a.d_wd = static_cast<uint16_t*>(d->d_down_weight);
+  a.space = d->workspace;
+  const void* every[] = {a.x, a.wg, a.wu, a.wd, a.y, a.gate, a.up, a.dy, a.dx, a.d_wg, a.d_wu, a.d_wd};
+  for (const void* p : every) CHECK_ARG(aligned(p, 16), "gated MLP tensors must be 16-byte aligned");
+  CHECK_ARG((a.gate == nullptr) == (a.up == nullptr), "gate and up are kept together");
+  return GLM53_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t glm53_gated_mlp_workspace_bytes(int64_t rows, int64_t hidden, int64_t intermediate) {
+  if (rows <= 0 || hidden <= 0 || intermediate <= 0) return 0;
+  return gated_space(rows, hidden, intermediate, false);
+}
+
+size_t glm53_gated_mlp_backward_workspace_bytes(int64_t rows, int64_t hidden, int64_t intermediate) {
+  if (rows <= 0 || hidden <= 0 || intermediate <= 0) return 0;
+  return gated_space(rows, hidden, intermediate, true);
+}
+
+int glm53_gated_mlp(const glm53_gated_mlp_desc* desc, void* stream) {
+  GatedArgs a;
+  if (int rc = gated_args(desc, a)) return rc;
+  if (a.rows == 0) return GLM53_OK;
+  CHECK_ARG(a.x && a.wg && a.wu && a.wd && a.y, "null pointer argument");
+  const size_t need = glm53_gated_mlp_workspace_bytes(a.rows, a.hidden, a.inter);
+  CHECK_ARG(a.space && desc->workspace_bytes >= need && aligned(a.space, 256),
+            "the gated MLP needs a 256-byte aligned workspace of %zu bytes", need);
+  HIP_TRY(launch_gated(a, S(stream)), "gated MLP launch");
+  return GLM53_OK;
+}
+
+int glm53_gated_mlp_backward(const glm53_gated_mlp_desc* desc, void* stream) {
+  GatedArgs a;
+  if (int rc = gated_args(desc, a)) return rc;
+  CHECK_ARG(a.rows > 0, "gradients of an MLP over no rows are zero: nothing to compute");
+  CHECK_ARG(a.x && a.wg && a.wu && a.wd && a.gate && a.up && a.dy, "null pointer argument");
+  const size_t need = glm53_gated_mlp_backward_workspace_bytes(a.rows, a.hidden, a.inter);
+  CHECK_ARG(a.space && desc->workspace_bytes >= need && aligned(a.space, 256),
+            "the gated MLP's gradients need a 256-byte aligned workspace of %zu bytes", need);
+  HIP_TRY(launch_gated_backward(a, S(stream)), "gated MLP gradient launch");
   return GLM53_OK;
 }
 

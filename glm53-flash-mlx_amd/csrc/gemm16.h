@@ -1,0 +1,405 @@
+// Tiled matrix products of 16-bit operands on the bf16 MFMA, the core of the
+// gated MLP and of the 4-bit linear over many rows:
+//
+//   out[m, n] = sum_k a(m, k) b(n, k),  FP32 accumulation
+//
+// A workgroup computes a BM x BN tile, its wavefronts a grid of them.  Each K
+// step of 64 stages both operands in LDS while the step before is
+// multiplied (two stages, one barrier a step).  An operand is stored either
+// with k contiguous (rows of 64 k: "row" form) or with m or n contiguous
+// ("column" form, the contraction over rows: gradients), which is read from
+// LDS by the transposing ds_read_b64_tr_b16, so no operand is ever
+// transposed in memory.
+#pragma once
+
+#include "common.h"
+
+namespace glm53 {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kStepK = 64;          // contraction columns of one LDS stage
+constexpr int kOperandTile = 2048;  // 16 rows x 64 k, or its share of a column stage
+
+// One product's operands, or one segment of a contraction over several.
+struct Gemm16Pair {
+  const uint16_t* a;  // row form [m, lda], column form [k, lda]
+  const uint16_t* b;
+  uint16_t* out;      // [m, ldo]
+  int64_t lda, ldb, ldo, m, n;
+};
+
+struct Gemm16Args {
+  Gemm16Pair pair[3];
+  int64_t k;       // of each pair
+  int problems;    // pairs that are products of their own
+  int segments;    // pairs whose contractions are added into pair[0].out
+  int splits;      // parts of the contraction, each to `partial`
+  float* partial;  // [splits][planes][m][n]
+  int64_t tiles;   // output tiles of all problems
+  int group_m;     // tile rows that one XCD's neighbouring workgroups share
+  // SwiGLU: pair[0].b gate and pair[1].b up rows, out = h; gate/up (f32
+  // [m, n]) null or what the gradient needs.  Its gradient (out unused): reads
+  // gate and up, writes d_gate, d_up and h.
+  float limit;
+  float* gate;
+  float* up;
+  uint16_t* d_gate;
+  uint16_t* d_up;
+  uint16_t* h;
+  // 4-bit b: codes [n, k / 2], scales and offsets [n, k / group], bias [n]
+  const uint8_t* codes;
+  const void* scales;
+  const void* offsets;  // null: -8 scale
+  const void* bias;     // or null
+  bool scales_f32;
+  int group_log2;
+};
+
+enum Gemm16Epilogue { kStore, kSwiglu, kSwigluGrad };
+
+__device__ __forceinline__ float sigmoid_f32(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
+
+// g' = min(g, L), u' = clip(u, -L, L); a NaN stays one.
+__device__ __forceinline__ float clamp_gate(float g, float limit) { return g > limit ? limit : g; }
+__device__ __forceinline__ float clamp_up(float u, float limit) { return u > limit ? limit : u < -limit ? -limit : u; }
+
+__device__ __forceinline__ u32x2 pack_bf16x4(f32x4 v) {
+  return (u32x2){f32_to_bf16(v[0]) | static_cast<uint32_t>(f32_to_bf16(v[1])) << 16,
+                 f32_to_bf16(v[2]) | static_cast<uint32_t>(f32_to_bf16(v[3])) << 16};
+}
+
+__device__ __forceinline__ float table_value(const void* t, bool f32, int64_t i) {
+  return f32 ? static_cast<const float*>(t)[i] : bf16_to_f32(static_cast<const uint16_t*>(t)[i]);
+}
+
+// Outputs n .. n + 3 of row m (m and n in range; n % 4 == 0).
+__device__ __forceinline__ void store_plain(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n, f32x4 v) {
+  *reinterpret_cast<u32x2*>(p.out + m * p.ldo + n) = pack_bf16x4(v);
+}
+
+// h = silu(min(g, L)) clip(u, -L, L).  G and U themselves are kept in FP32
+// where a gradient follows: rounded to bf16 they would put an error the size
+// of the results' own rounding into every gradient.
+__device__ __forceinline__ void store_swiglu(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n, f32x4 gate,
+                                             f32x4 up) {
+  const int64_t at = m * p.n + n;
+  if (g.gate != nullptr) {
+    *reinterpret_cast<f32x4*>(g.gate + at) = gate;
+    *reinterpret_cast<f32x4*>(g.up + at) = up;
+  }
+  f32x4 h;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float c = clamp_gate(gate[i], g.limit);
+    h[i] = c * sigmoid_f32(c) * clamp_up(up[i], g.limit);
+  }
+  *reinterpret_cast<u32x2*>(p.out + m * p.ldo + n) = pack_bf16x4(h);
+}
+
+// With dh: dU = dh silu(g') [|u| <= L], dG = dh u' silu'(g') [g <= L], and h
+// again for the down projection's gradient.
+__device__ __forceinline__ void store_swiglu_grad(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n,
+                                                  f32x4 dh) {
+  const int64_t at = m * p.n + n;
+  const f32x4 gate = *reinterpret_cast<const f32x4*>(g.gate + at);
+  const f32x4 up = *reinterpret_cast<const f32x4*>(g.up + at);
+  f32x4 dg, du, h;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float c = clamp_gate(gate[i], g.limit), u = clamp_up(up[i], g.limit);
+    const float s = sigmoid_f32(c), silu = c * s;
+    h[i] = silu * u;
+    du[i] = fabsf(up[i]) > g.limit ? 0.0f : dh[i] * silu;
+    dg[i] = gate[i] > g.limit ? 0.0f : dh[i] * u * (s * (1.0f + c * (1.0f - s)));
+  }
+  *reinterpret_cast<u32x2*>(g.d_gate + at) = pack_bf16x4(dg);
+  *reinterpret_cast<u32x2*>(g.d_up + at) = pack_bf16x4(du);
+  if (g.h != nullptr) *reinterpret_cast<u32x2*>(g.h + at) = pack_bf16x4(h);
+}
+
+// ------------------------------------------------------------- staging ---
+//
+// Row form: operand tiles of 16 rows x 128 bytes, row r's 16-byte piece p in
+// slot p ^ (r % 8) ^ (r / 8 % 2) of its row, the permutation the FP8 kernels
+// measured at the LDS's full 16-byte read rate.  A lane reads pieces 2 (l /
+// 16) and 2 (l / 16) + 1 of row l % 16, so MFMA j of a step contracts k =
+// 16 (l / 16) + 8 j + 0..7.
+//
+// Column form: 64 rows of R columns.  ds_read_b64_tr_b16 gives lane i of each
+// 16 the 4 rows x 1 column that the 16 lanes' 8 bytes hold, lane a reading
+// row a / 4, columns 4 (a % 4) .. + 3.  Its 64 lanes read 32-byte pieces of 16
+// rows at one column; piece c of row k lies at c ^ f(k), f(k) = k % 4 + 4 (k /
+// 16 % 2), which puts the 8 rows that 32 lanes read on distinct banks.
+
+__device__ __forceinline__ int column_swizzle(int k) { return (k & 3) | ((k >> 2) & 4); }
+
+// Direct global -> LDS load of 16 bytes a lane to lds_base + 16 lane.  Inline
+// assembly, so that the compiler puts no wait of its own before LDS reads;
+// stage_wait counts them.
+__device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_base)
+               : "memory", "m0");
+}
+
+// All of this wavefront's loads and LDS accesses are done, and every
+// wavefront of the workgroup is here.
+__device__ __forceinline__ void stage_wait() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// The share of one wavefront in staging an operand tile of R rows (row form)
+// or columns (column form): loads `wave`, wave + W, ... of R / 8, 1 KB each.
+template <int R, int W, bool COLUMN>
+struct Stager {
+  static constexpr int kLoads = R / 8 / W;
+  static_assert(R % (8 * W) == 0, "whole loads a wavefront");
+  static constexpr int kLanes = R / 8;  // column form: lanes a row
+  uint32_t off[kLoads];                 // byte offset of this lane's piece from the tile's base
+
+  // which row (row form) or k (column form) of the tile load i's lane holds,
+  // and its first k or column
+  __device__ static __forceinline__ int outer(int i, int wave, int lane) {
+    const int li = wave + W * i;
+    return COLUMN ? li * (64 / kLanes) + lane / kLanes : 8 * li + (lane >> 3);
+  }
+  __device__ static __forceinline__ int inner(int i, int wave, int lane) {
+    const int li = wave + W * i;
+    if (!COLUMN) return 8 * ((lane & 7) ^ (lane >> 3) ^ (li & 1));
+    const int p = lane % kLanes, c = (p >> 1) ^ (column_swizzle(outer(i, wave, lane)) & (R / 16 - 1));
+    return 16 * c + 8 * (p & 1);
+  }
+  // `left`: rows (row form) or columns (column form) of the matrix from the
+  // tile's first on; what lies past them repeats the last ones and never
+  // reaches an output.
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int64_t left) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      int o = outer(i, wave, lane), c = inner(i, wave, lane);
+      if (!COLUMN && o >= left) o = static_cast<int>(left) - 1;
+      if (COLUMN && c >= left) c = static_cast<int>(left) - 8;
+      off[i] = static_cast<uint32_t>((o * ld + c) * 2);
+    }
+  }
+  __device__ __forceinline__ void issue(const uint16_t* base, int wave, uint32_t lds) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_lds16(base, off[i], lds + (wave + W * i) * 1024);
+  }
+  // The last, partial step: k_left k's (of which the row form has a multiple
+  // of 8), zeros after them.
+  __device__ __forceinline__ void issue_tail(const uint16_t* base, int wave, int lane, int k_left, uint8_t* lds) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      u32x4 v = {0, 0, 0, 0};
+      const int k = COLUMN ? outer(i, wave, lane) : inner(i, wave, lane);
+      if (k < k_left) v = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(base) + off[i]);
+      *reinterpret_cast<u32x4*>(lds + (wave + W * i) * 1024 + 16 * lane) = v;
+    }
+  }
+};
+
+// MFMA operand j (0, 1) of 16-row or 16-column tile t of a stage.
+template <int R, bool COLUMN>
+struct Reader {
+  uint32_t lo, hi;  // row form: a tile's two pieces; column form: row base and swizzle
+  __device__ __forceinline__ Reader(int lane) {
+    const int r = lane & 15, kq = lane >> 4;
+    if (!COLUMN) {
+      const int g = (r & 7) ^ (r >> 3);
+      lo = 128 * r + 16 * ((2 * kq) ^ g);
+      hi = 128 * r + 16 * ((2 * kq + 1) ^ g);
+    } else {
+      lo = (16 * kq + (r >> 2)) * (2 * R) + 8 * (r & 3);
+      hi = ((r >> 2) | ((kq & 1) << 2)) & (R / 16 - 1);
+    }
+  }
+  __device__ __forceinline__ bf16x8 operator()(const uint8_t* stage, int t, int j) const {
+    if constexpr (!COLUMN) {
+      return *reinterpret_cast<const bf16x8*>(stage + t * kOperandTile + (j ? hi : lo));
+    } else {
+      typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+      const uint8_t* p = stage + lo + 32 * (static_cast<uint32_t>(t) ^ hi) + 8 * j * (2 * R);
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
+      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * (2 * R)));
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+};
+
+// Tile number t of `tiles` for workgroup b: consecutive workgroups go to the
+// XCDs in turn, so workgroup b takes number b / 8 of XCD b % 8's run of
+// consecutive tiles, which share rows and columns in that XCD's L2.
+__device__ __forceinline__ int64_t xcd_tile(int64_t b, int64_t tiles) {
+  const int64_t q = tiles / 8, r = tiles % 8, x = b % 8;
+  return x * q + (x < r ? x : r) + b / 8;
+}
+
+// Tile (row, column) number t of rows x cols, in bands of `group` tile rows.
+__device__ __forceinline__ void band_tile(int64_t t, int64_t rows, int64_t cols, int group, int64_t& tm, int64_t& tn) {
+  const int64_t band = t / (group * cols), first = band * group;
+  const int64_t high = rows - first < group ? rows - first : group;
+  const int64_t in = t - band * group * cols;
+  tm = first + in % high;
+  tn = in / high;
+}
+
+// WM x WN wavefronts, each MT x NT MFMA tiles of 16 x 16.
+template <int WM, int WN, int MT, int NT, bool A_COLUMN, bool B_COLUMN, Gemm16Epilogue EPI>
+struct Gemm16 {
+  static constexpr int W = WM * WN, kThreads = 64 * W;
+  static constexpr int BM = 16 * WM * MT, BN = 16 * WN * NT;
+  static constexpr bool kPairB = EPI == kSwiglu;           // half the tile gate columns, half up
+  static constexpr int kColumns = kPairB ? BN / 2 : BN;    // output columns of a tile
+  static constexpr int kStageA = BM * 128, kStage = kStageA + BN * 128;
+  static constexpr int kLds = 2 * kStage;
+
+  __device__ static __forceinline__ void run(const Gemm16Args& g, uint8_t* lds) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    // tile, split and problem
+    const int64_t unit = xcd_tile(blockIdx.x, g.tiles * g.splits);
+    const int split = static_cast<int>(unit / g.tiles);
+    int64_t t = unit % g.tiles;
+    int q = 0;
+    int64_t rows = (g.pair[0].m + BM - 1) / BM, cols = (g.pair[0].n + kColumns - 1) / kColumns;
+    while (q + 1 < g.problems && t >= rows * cols) {
+      t -= rows * cols;
+      ++q;
+      rows = (g.pair[q].m + BM - 1) / BM;
+      cols = (g.pair[q].n + kColumns - 1) / kColumns;
+    }
+    const Gemm16Pair& p = g.pair[q];
+    int64_t tm, tn;
+    band_tile(t, rows, cols, g.group_m, tm, tn);
+    const int64_t m0 = tm * BM, n0 = tn * kColumns;
+
+    // K steps of this split
+    const int64_t steps = (g.k + kStepK - 1) / kStepK, all = steps * g.segments;
+    const int64_t each = (all + g.splits - 1) / g.splits;
+    const int64_t first = split * each, last = first + each < all ? first + each : all;
+    const int tail = static_cast<int>(g.k % kStepK);
+
+    Stager<BM, W, A_COLUMN> sa;
+    sa.init(wave, lane, p.lda, p.m - m0);
+    constexpr int kHalves = kPairB ? 2 : 1;
+    Stager<BN / kHalves, W, B_COLUMN> sb;
+    sb.init(wave, lane, p.ldb, p.n - n0);
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    const auto issue = [&](int64_t step, int slot) {
+      const int s = g.segments > 1 ? static_cast<int>(step / steps) : 0;
+      const int64_t kk = (step - s * steps) * kStepK;
+      const Gemm16Pair& o = g.segments > 1 ? g.pair[s] : p;
+      const uint16_t* a = o.a + (A_COLUMN ? kk * p.lda + m0 : m0 * p.lda + kk);
+      const int64_t b_at = B_COLUMN ? kk * p.ldb + n0 : n0 * p.ldb + kk;
+      const bool partial = tail != 0 && kk + kStepK > g.k;
+      if (partial)
+        sa.issue_tail(a, wave, lane, tail, lds + slot * kStage);
+      else
+        sa.issue(a, wave, lds_at + slot * kStage);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const uint16_t* b = (kPairB ? g.pair[h].b : o.b) + b_at;
+        const uint32_t at = slot * kStage + kStageA + h * (BN / kHalves) * 128;
+        if (partial)
+          sb.issue_tail(b, wave, lane, tail, lds + at);
+        else
+          sb.issue(b, wave, lds_at + at);
+      }
+    };
+
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int c = 0; c < NT; ++c) acc[i][c] = (f32x4){0, 0, 0, 0};
+    const Reader<BM, A_COLUMN> ra(lane);
+    const Reader<BN / kHalves, B_COLUMN> rb(lane);
+    // LDS tile of the wavefront's column tile c: in a pair, the first half of
+    // its tiles are gate columns, the others the up columns of the same outputs
+    const auto b_tile = [&](int c) {
+      return kPairB ? (c < NT / 2 ? wn * (NT / 2) + c : BN / 32 + wn * (NT / 2) + c - NT / 2) : wn * NT + c;
+    };
+
+    if (first < last) issue(first, 0);
+    int slot = 0;
+    for (int64_t step = first; step < last; ++step, slot ^= 1) {
+      stage_wait();
+      if (step + 1 < last) issue(step + 1, slot ^ 1);
+      const uint8_t* stage = lds + slot * kStage;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        bf16x8 a[MT], b[NT];
+#pragma unroll
+        for (int c = 0; c < NT; ++c) b[c] = rb(stage + kStageA, b_tile(c), j);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) a[i] = ra(stage, wm * MT + i, j);
+        // columns as the MFMA's rows: a lane's four results are four
+        // consecutive outputs of one row
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+            acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[c], a[i], acc[i][c], 0, 0, 0);
+      }
+    }
+
+    const int64_t plane = p.m * p.n;
+    float* part = g.partial + split * (kPairB ? 2 : 1) * plane;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int64_t m = m0 + 16 * (wm * MT + i) + (lane & 15);
+      if (m >= p.m) continue;
+#pragma unroll
+      for (int c = 0; c < (kPairB ? NT / 2 : NT); ++c) {
+        const int64_t n = n0 + 16 * (wn * (kPairB ? NT / 2 : NT) + c) + 4 * (lane >> 4);
+        if (n >= p.n) continue;
+        if (g.splits > 1) {
+          *reinterpret_cast<f32x4*>(part + m * p.n + n) = acc[i][c];
+          if constexpr (kPairB) *reinterpret_cast<f32x4*>(part + plane + m * p.n + n) = acc[i][c + NT / 2];
+        } else if constexpr (EPI == kStore) {
+          store_plain(g, p, m, n, acc[i][c]);
+        } else if constexpr (EPI == kSwiglu) {
+          store_swiglu(g, p, m, n, acc[i][c], acc[i][c + NT / 2]);
+        } else {
+          store_swiglu_grad(g, p, m, n, acc[i][c]);
+        }
+      }
+    }
+  }
+};
+
+template <class G>
+__global__ __launch_bounds__(G::kThreads) void gemm16_kernel(Gemm16Args g) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  G::run(g, lds);
+}
+
+// Adds the splits' partial results, in their order, and finishes them.
+template <Gemm16Epilogue EPI>
+__global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
+  const Gemm16Pair& p = g.pair[0];
+  const int64_t plane = p.m * p.n, at = 4 * (blockIdx.x * int64_t{256} + threadIdx.x);
+  if (at >= plane) return;
+  constexpr int kPlanes = EPI == kSwiglu ? 2 : 1;
+  f32x4 v[kPlanes];
+#pragma unroll
+  for (int h = 0; h < kPlanes; ++h) {
+    v[h] = *reinterpret_cast<const f32x4*>(g.partial + h * plane + at);
+    for (int s = 1; s < g.splits; ++s)
+      v[h] += *reinterpret_cast<const f32x4*>(g.partial + (s * kPlanes + h) * plane + at);
+  }
+  const int64_t m = at / p.n, n = at % p.n;
+  if constexpr (EPI == kStore)
+    store_plain(g, p, m, n, v[0]);
+  else if constexpr (EPI == kSwiglu)
+    store_swiglu(g, p, m, n, v[0], v[1]);
+  else
+    store_swiglu_grad(g, p, m, n, v[0]);
+}
+
+}  // namespace glm53

@@ -18,7 +18,10 @@ and FakeTensor / meta propagation gets the output shapes without a device.
   min_routes as one prefill in the Direct order;
 * ``glm53::residual_norm(residual, out?, post_weight?, gate?, next_weight?,
   ...)`` and ``glm53::residual_norm_backward`` -- ``rms_norm`` (without out)
-  and ``residual_norm``, differentiable.
+  and ``residual_norm``, differentiable;
+* ``glm53::gated_mlp(x, gate_weight, up_weight, down_weight, limit, keep)``
+  and ``glm53::gated_mlp_backward`` -- ``gated_mlp``, differentiable where
+  `keep` has it return G and U.
 
 The MoE ops take the module by an integer key (``register_owner``): the
 module keeps its weights, its per-(device, stream) native plans and its
@@ -216,3 +219,52 @@ def _residual_norm_backward(ctx, d_new, d_y, _):
 
 
 residual_norm.register_autograd(_residual_norm_backward, setup_context=_residual_norm_context)
+
+
+@torch.library.custom_op("glm53::gated_mlp", mutates_args=())
+def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, down_weight: torch.Tensor,
+              limit: float, keep: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from .gated import native_gated_mlp
+
+    return native_gated_mlp(x, gate_weight, up_weight, down_weight, limit, keep)
+
+
+@gated_mlp.register_fake
+def _(x, gate_weight, up_weight, down_weight, limit, keep):
+    rows = x.numel() // x.shape[-1]
+    kept = (rows, gate_weight.shape[0]) if keep else (0,)
+    return (x.new_empty(x.shape), x.new_empty(kept, dtype=torch.float32), x.new_empty(kept, dtype=torch.float32))
+
+
+@torch.library.custom_op("glm53::gated_mlp_backward", mutates_args=())
+def gated_mlp_backward(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, down_weight: torch.Tensor,
+                       gate: torch.Tensor, up: torch.Tensor, d_y: torch.Tensor, limit: float,
+                       wanted: list[bool]) -> list[torch.Tensor]:
+    from .gated import native_gated_mlp_backward
+
+    return native_gated_mlp_backward(x, gate_weight, up_weight, down_weight, gate, up, d_y, limit, wanted)
+
+
+@gated_mlp_backward.register_fake
+def _(x, gate_weight, up_weight, down_weight, gate, up, d_y, limit, wanted):
+    inputs = (x, gate_weight, up_weight, down_weight)
+    return [t.new_empty(t.shape) if w else x.new_empty(0) for t, w in zip(inputs, wanted)]
+
+
+def _gated_mlp_context(ctx, inputs, output):
+    if not inputs[5]:
+        raise RuntimeError("glm53::gated_mlp without keep has no gradient")
+    ctx.save_for_backward(*inputs[:4], output[1], output[2])
+    ctx.limit = inputs[4]
+    ctx.set_materialize_grads(False)
+
+
+def _gated_mlp_backward(ctx, d_y, _gate, _up):
+    if d_y is None:
+        return (None,) * 6
+    wanted = [bool(w) for w in ctx.needs_input_grad[:4]]
+    grads = torch.ops.glm53.gated_mlp_backward(*ctx.saved_tensors, d_y, ctx.limit, wanted)
+    return (*(g if w else None for g, w in zip(grads, wanted)), None, None)
+
+
+gated_mlp.register_autograd(_gated_mlp_backward, setup_context=_gated_mlp_context)

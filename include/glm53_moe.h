@@ -580,6 +580,44 @@ size_t glm53_residual_norm_workspace_bytes(int64_t rows, int64_t width, int64_t 
 int glm53_residual_norm_backward(const glm53_norm* norm, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Gated MLP in BF16 weights, with its gradients (the reference's dense MLP,
+ * patch.py:114-129, is frozen and FP8).
+ * ---------------------------------------------------------------------- */
+/*   G = x Wg^T, U = x Wu^T, h = silu(min(G, L)) clip(U, -L, L), y = h Wd^T
+ * over contiguous BF16 tensors, 16-byte aligned; hidden and intermediate
+ * multiples of 8; limit L > 0, INFINITY for none.  Sums, G, U and the
+ * activation are FP32, h and y are rounded once.  gate, up: f32 [rows,
+ * intermediate], NULL or where G and U are kept for the gradients. */
+typedef struct glm53_gated_mlp_desc {
+  int64_t rows, hidden, intermediate;
+  const void* x;           /* [rows, hidden] */
+  const void* gate_weight; /* [intermediate, hidden] */
+  const void* up_weight;   /* [intermediate, hidden] */
+  const void* down_weight; /* [hidden, intermediate] */
+  void* y;                 /* [rows, hidden]; forward only */
+  float* gate;
+  float* up;
+  /* backward only; results NULL: not wanted */
+  const void* d_y;
+  void* d_x;
+  void* d_gate_weight;
+  void* d_up_weight;
+  void* d_down_weight;
+  void* workspace; /* 256-byte aligned, of the *_workspace_bytes below; needs no initialisation */
+  size_t workspace_bytes;
+  float limit;
+} glm53_gated_mlp_desc;
+size_t glm53_gated_mlp_workspace_bytes(int64_t rows, int64_t hidden, int64_t intermediate);
+int glm53_gated_mlp(const glm53_gated_mlp_desc* desc, void* stream);
+/* dh = d_y Wd; dU = dh silu(min(G, L)) where |U| <= L, else 0; dG = dh
+ * clip(U) silu'(min(G, L)) where G <= L, else 0; d_x = dG Wg + dU Wu, d_gate_weight
+ * = dG^T x, d_up_weight = dU^T x, d_down_weight = d_y^T h.  dG, dU and h are
+ * rounded to BF16 as operands of these products, sums are FP32 in a fixed
+ * order.  rows > 0.  Results may not overlap inputs. */
+size_t glm53_gated_mlp_backward_workspace_bytes(int64_t rows, int64_t hidden, int64_t intermediate);
+int glm53_gated_mlp_backward(const glm53_gated_mlp_desc* desc, void* stream);
+
+/* ------------------------------------------------------------------------
  * Seeded synthetic inputs (no reference counterpart: the reference loads a
  * checkpoint).  Element i of stream `seed` is N(0, std) (or U(lo, hi)). */
 int glm53_synth_fp8(uint8_t* codes, float* scale_inv, int64_t rows, int64_t cols, uint64_t seed,
