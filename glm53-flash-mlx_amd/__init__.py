@@ -37,6 +37,7 @@ from .grouped_fp8 import (
     grouped_fp8_linear,
     restore_and_reduce,
 )
+from .int4 import Int4Linear, Int4MLP, int4_linear, quantize_int4
 from .loader import install_packed_decode_moe, install_packed_grouped_moe, install_packed_moe
 from .norms import residual_norm, rms_norm
 from .ownership import (
@@ -67,4 +68,5 @@ __all__ = [
     "install_packed_decode_moe", "BankHandle", "RoutedDiagnostic", "ResidentTensor", "TensorLayout", "TensorLease", "TensorOwnership",
     "TensorOwnershipError", "borrowed_ephemeral_tensor", "borrowed_stable_tensor", "materialize_owned",
     "owned_tensor", "require_resident", "resident_concatenate", "rms_norm", "residual_norm", "gated_mlp", "GatedMLP",
+    "int4_linear", "quantize_int4", "Int4Linear", "Int4MLP",
 ]

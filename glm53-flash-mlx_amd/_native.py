@@ -143,6 +143,19 @@ class GatedMLP(ctypes.Structure):
     ]
 
 
+class Int4Weight(ctypes.Structure):
+    _fields_ = [
+        ("codes", P),
+        ("scales", P),
+        ("offsets", P),
+        ("bias", P),
+        ("out_features", I64),
+        ("in_features", I64),
+        ("group", I32),
+        ("tables_f32", I32),
+    ]
+
+
 _SIGNATURES = {
     "glm53_last_error": (ctypes.c_char_p, []),
     "glm53_abi_version": (ctypes.c_int, []),
@@ -203,6 +216,8 @@ _SIGNATURES = {
     "glm53_gated_mlp": (ctypes.c_int, [P, P]),
     "glm53_gated_mlp_backward_workspace_bytes": (SZ, [I64, I64, I64]),
     "glm53_gated_mlp_backward": (ctypes.c_int, [P, P]),
+    "glm53_int4_linear_workspace_bytes": (SZ, [I64, I64, I64]),
+    "glm53_int4_linear": (ctypes.c_int, [P, P, I64, P, P, SZ, P]),
     "glm53_synth_fp8": (ctypes.c_int, [P, P, I64, I64, ctypes.c_uint64, F32, P]),
     "glm53_synth_f32": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, F32, F32, I32, P]),
     "glm53_synth_bf16": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, P]),

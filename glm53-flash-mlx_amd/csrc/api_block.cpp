@@ -1,7 +1,8 @@
 // C ABI of the dense feed-forward block (declared in include/glm53_moe.h):
-// the norms around it and the gated MLP.
+// the norms around it, the gated MLP and the 4-bit linear.
 #include "api_util.h"
 #include "gated.h"
+#include "int4.h"
 #include "norms.h"
 
 using namespace glm53;
@@ -184,6 +185,49 @@ int glm53_gated_mlp_backward(const glm53_gated_mlp_desc* desc, void* stream) {
   CHECK_ARG(a.space && desc->workspace_bytes >= need && aligned(a.space, 256),
             "the gated MLP's gradients need a 256-byte aligned workspace of %zu bytes", need);
   HIP_TRY(launch_gated_backward(a, S(stream)), "gated MLP gradient launch");
+  return GLM53_OK;
+}
+
+}  // extern "C"
+
+// --------------------------------------------------------- 4-bit linear ---
+
+extern "C" {
+
+size_t glm53_int4_linear_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features) {
+  if (rows <= 0 || out_features <= 0 || in_features <= 0) return 0;
+  return int4_space(rows, out_features, in_features);
+}
+
+int glm53_int4_linear(const glm53_int4_weight* w, const void* x, int64_t rows, void* y, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  CHECK_ARG(w != nullptr, "4-bit weight is null");
+  const int64_t N = w->out_features, K = w->in_features;
+  CHECK_ARG(rows >= 0 && rows < (int64_t{1} << 31) && N > 0 && K > 0, "invalid shape rows=%lld out=%lld in=%lld",
+            (long long)rows, (long long)N, (long long)K);
+  CHECK_ARG(w->group == 32 || w->group == 64 || w->group == 128, "group must be 32, 64 or 128, got %d", w->group);
+  CHECK_ARG(K % w->group == 0, "in_features %lld is not a multiple of the group %d", (long long)K, w->group);
+  CHECK_ARG(K <= kGatedMaxWidth && N < (int64_t{1} << 31), "weight too large");
+  if (rows == 0) return GLM53_OK;
+  CHECK_ARG(w->codes && w->scales && x && y, "null pointer argument");
+  CHECK_ARG(aligned(w->codes, 16) && aligned(x, 16) && aligned(y, 16), "codes, x and y must be 16-byte aligned");
+  const size_t need = glm53_int4_linear_workspace_bytes(rows, N, K);
+  CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 256)),
+            "the 4-bit linear needs a 256-byte aligned workspace of %zu bytes", need);
+  Int4Args a{};
+  a.x = static_cast<const uint16_t*>(x);
+  a.codes = w->codes;
+  a.scales = w->scales;
+  a.offsets = w->offsets;
+  a.bias = w->bias;
+  a.tables_f32 = w->tables_f32 != 0;
+  a.group_log2 = w->group == 32 ? 5 : w->group == 64 ? 6 : 7;
+  a.rows = rows;
+  a.N = N;
+  a.K = K;
+  a.y = static_cast<uint16_t*>(y);
+  a.space = workspace;
+  HIP_TRY(launch_int4(a, S(stream)), "4-bit linear launch");
   return GLM53_OK;
 }
 

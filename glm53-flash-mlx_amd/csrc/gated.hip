@@ -25,10 +25,10 @@ hipError_t launch_tiles(Gemm16Args g, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <bool A_COLUMN, bool B_COLUMN, Gemm16Epilogue EPI>
+template <bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI>
 hipError_t launch_product(Gemm16Args g, hipStream_t st) {
   g.splits = 1;
-  return launch_tiles<Gemm16<2, 2, 4, 4, A_COLUMN, B_COLUMN, EPI>>(g, st);
+  return launch_tiles<Gemm16<2, 2, 4, 4, A_COLUMN, B, EPI>>(g, st);
 }
 
 Gemm16Pair pair(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb, uint16_t* out, int64_t m, int64_t n) {
@@ -58,10 +58,10 @@ hipError_t launch_gated(const GatedArgs& a, hipStream_t st) {
   g.limit = a.limit;
   g.gate = a.gate;
   g.up = a.up;
-  if (hipError_t e = launch_product<false, false, kSwiglu>(g, st); e != hipSuccess) return e;
+  if (hipError_t e = launch_product<false, kRow, kSwiglu>(g, st); e != hipSuccess) return e;
   Gemm16Args d = product(a.inter);
   d.pair[0] = pair(h, a.inter, a.wd, a.inter, a.y, a.rows, a.hidden);
-  return launch_product<false, false, kStore>(d, st);
+  return launch_product<false, kRow, kStore>(d, st);
 }
 
 hipError_t launch_gated_backward(const GatedArgs& a, hipStream_t st) {
@@ -78,13 +78,13 @@ hipError_t launch_gated_backward(const GatedArgs& a, hipStream_t st) {
   g.d_gate = dg;
   g.d_up = du;
   g.h = a.d_wd != nullptr ? h : nullptr;
-  if (hipError_t e = launch_product<false, true, kSwigluGrad>(g, st); e != hipSuccess) return e;
+  if (hipError_t e = launch_product<false, kColumn, kSwigluGrad>(g, st); e != hipSuccess) return e;
   if (a.dx != nullptr) {
     Gemm16Args x = product(a.inter);
     x.segments = 2;
     x.pair[0] = pair(dg, a.inter, a.wg, a.hidden, a.dx, a.rows, a.hidden);
     x.pair[1] = pair(du, a.inter, a.wu, a.hidden, a.dx, a.rows, a.hidden);
-    if (hipError_t e = launch_product<false, true, kStore>(x, st); e != hipSuccess) return e;
+    if (hipError_t e = launch_product<false, kColumn, kStore>(x, st); e != hipSuccess) return e;
   }
   Gemm16Args w = product(a.rows);
   w.problems = 0;
@@ -92,7 +92,7 @@ hipError_t launch_gated_backward(const GatedArgs& a, hipStream_t st) {
   if (a.d_wu) w.pair[w.problems++] = pair(du, a.inter, a.x, a.hidden, a.d_wu, a.inter, a.hidden);
   if (a.d_wd) w.pair[w.problems++] = pair(a.dy, a.hidden, h, a.inter, a.d_wd, a.hidden, a.inter);
   if (w.problems == 0) return hipSuccess;
-  return launch_product<true, true, kStore>(w, st);
+  return launch_product<true, kColumn, kStore>(w, st);
 }
 
 }  // namespace glm53

@@ -39,7 +39,7 @@ struct Gemm16Args {
   int problems;    // pairs that are products of their own
   int segments;    // pairs whose contractions are added into pair[0].out
   int splits;      // parts of the contraction, each to `partial`
-  float* partial;  // [splits][planes][m][n]
+  float* partial;  // [splits][planes][m][partial_ld(n)]
   int64_t tiles;   // output tiles of all problems
   int group_m;     // tile rows that one XCD's neighbouring workgroups share
   // SwiGLU: pair[0].b gate and pair[1].b up rows, out = h; gate/up (f32
@@ -60,7 +60,11 @@ struct Gemm16Args {
   int group_log2;
 };
 
-enum Gemm16Epilogue { kStore, kSwiglu, kSwigluGrad };
+enum Gemm16Epilogue { kStore, kSwiglu, kSwigluGrad, kBias };
+enum OperandForm { kRow, kColumn, kCodes };
+
+// Row length of the partial results: whole groups of four.
+__host__ __device__ __forceinline__ int64_t partial_ld(int64_t n) { return (n + 3) & ~int64_t{3}; }
 
 __device__ __forceinline__ float sigmoid_f32(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
@@ -80,6 +84,25 @@ __device__ __forceinline__ float table_value(const void* t, bool f32, int64_t i)
 // Outputs n .. n + 3 of row m (m and n in range; n % 4 == 0).
 __device__ __forceinline__ void store_plain(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n, f32x4 v) {
   *reinterpret_cast<u32x2*>(p.out + m * p.ldo + n) = pack_bf16x4(v);
+}
+
+// The same plus a bias, for any number of columns: outputs past the last one
+// are left out, and rows whose length is no multiple of 4 have no aligned
+// group of four.
+__device__ __forceinline__ void store_bias(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n, f32x4 v) {
+  uint16_t* out = p.out + m * p.ldo + n;
+  if (g.bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.n) v[i] += table_value(g.bias, g.scales_f32, n + i);
+  }
+  if ((p.ldo & 3) == 0) {
+    *reinterpret_cast<u32x2*>(out) = pack_bf16x4(v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < p.n) out[i] = f32_to_bf16(v[i]);
 }
 
 // h = silu(min(g, L)) clip(u, -L, L).  G and U themselves are kept in FP32
@@ -202,6 +225,59 @@ struct Stager {
   }
 };
 
+// 4-bit rows into a row-form stage of R rows by T threads: a thread takes 32
+// codes (16 bytes, within one group) of a row, fetched a step ahead, and
+// writes them as bf16 w = scale q + offset.  That rounding, half a step of
+// bf16 as the activations carry, makes the weights an MFMA operand; over the
+// rows this form is used for, sums of scaled group products in FP32 instead
+// would cost the vector units as many cycles as the product.
+template <int R, int T>
+struct CodeStager {
+  static_assert(R * 2 == T, "32 codes a thread");
+  u32x4 codes;
+  float scale, offset;
+  const uint8_t* row;
+  int64_t table;
+  int at;  // byte of the row's piece 0 in the stage, without the slot
+  int mix, half;
+
+  __device__ __forceinline__ void init(const Gemm16Args& g, int64_t n0, int64_t n, int64_t k) {
+    const int r = threadIdx.x >> 1;
+    half = threadIdx.x & 1;
+    const int64_t nr = n0 + r < n ? n0 + r : n - 1;
+    row = g.codes + nr * (k >> 1);
+    table = nr * (k >> g.group_log2);
+    at = (r >> 4) * kOperandTile + (r & 15) * 128;
+    mix = (r & 7) ^ ((r >> 3) & 1);
+  }
+  __device__ __forceinline__ void fetch(const Gemm16Args& g, int64_t kk) {
+    const int64_t k = kk + 32 * half;
+    if (k >= g.k) {  // the half step past the last k
+      codes = (u32x4){0, 0, 0, 0};
+      scale = offset = 0.0f;
+      return;
+    }
+    codes = *reinterpret_cast<const u32x4*>(row + (k >> 1));
+    const int64_t t = table + (k >> g.group_log2);
+    scale = table_value(g.scales, g.scales_f32, t);
+    offset = g.offsets != nullptr ? table_value(g.offsets, g.scales_f32, t) : -8.0f * scale;
+  }
+  __device__ __forceinline__ void write(uint8_t* stage) const {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const uint32_t even = codes[d] & 0x0F0F0F0Fu, odd = (codes[d] >> 4) & 0x0F0F0F0Fu;
+      u32x4 w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float a = fmaf(static_cast<float>((even >> (8 * i)) & 0xFFu), scale, offset);
+        const float b = fmaf(static_cast<float>((odd >> (8 * i)) & 0xFFu), scale, offset);
+        w[i] = f32_to_bf16(a) | static_cast<uint32_t>(f32_to_bf16(b)) << 16;
+      }
+      *reinterpret_cast<u32x4*>(stage + at + 16 * ((4 * half + d) ^ mix)) = w;
+    }
+  }
+};
+
 // MFMA operand j (0, 1) of 16-row or 16-column tile t of a stage.
 template <int R, bool COLUMN>
 struct Reader {
@@ -225,7 +301,6 @@ struct Reader {
       const uint8_t* p = stage + lo + 32 * (static_cast<uint32_t>(t) ^ hi) + 8 * j * (2 * R);
       const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
       const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * (2 * R)));
-      typedef short s16x8 __attribute__((ext_vector_type(8)));
       return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
@@ -249,10 +324,11 @@ __device__ __forceinline__ void band_tile(int64_t t, int64_t rows, int64_t cols,
 }
 
 // WM x WN wavefronts, each MT x NT MFMA tiles of 16 x 16.
-template <int WM, int WN, int MT, int NT, bool A_COLUMN, bool B_COLUMN, Gemm16Epilogue EPI>
+template <int WM, int WN, int MT, int NT, bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI>
 struct Gemm16 {
   static constexpr int W = WM * WN, kThreads = 64 * W;
   static constexpr int BM = 16 * WM * MT, BN = 16 * WN * NT;
+  static constexpr bool B_COLUMN = B == kColumn;
   static constexpr bool kPairB = EPI == kSwiglu;           // half the tile gate columns, half up
   static constexpr int kColumns = kPairB ? BN / 2 : BN;    // output columns of a tile
   static constexpr int kStageA = BM * 128, kStage = kStageA + BN * 128;
@@ -290,6 +366,8 @@ struct Gemm16 {
     Stager<BN / kHalves, W, B_COLUMN> sb;
     sb.init(wave, lane, p.ldb, p.n - n0);
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    CodeStager<B == kCodes ? BN : kThreads / 2, kThreads> sq;
+    if constexpr (B == kCodes) sq.init(g, n0, p.n, g.k);
     const auto issue = [&](int64_t step, int slot) {
       const int s = g.segments > 1 ? static_cast<int>(step / steps) : 0;
       const int64_t kk = (step - s * steps) * kStepK;
@@ -301,6 +379,7 @@ struct Gemm16 {
         sa.issue_tail(a, wave, lane, tail, lds + slot * kStage);
       else
         sa.issue(a, wave, lds_at + slot * kStage);
+      if constexpr (B == kCodes) return;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
         const uint16_t* b = (kPairB ? g.pair[h].b : o.b) + b_at;
@@ -325,11 +404,24 @@ struct Gemm16 {
       return kPairB ? (c < NT / 2 ? wn * (NT / 2) + c : BN / 32 + wn * (NT / 2) + c - NT / 2) : wn * NT + c;
     };
 
+    if constexpr (B == kCodes) {
+      if (first < last) {
+        sq.fetch(g, first * kStepK);
+        sq.write(lds + kStageA);
+        if (first + 1 < last) sq.fetch(g, (first + 1) * kStepK);
+      }
+    }
     if (first < last) issue(first, 0);
     int slot = 0;
     for (int64_t step = first; step < last; ++step, slot ^= 1) {
       stage_wait();
+      if constexpr (B == kCodes) {  // codes before the direct loads: the compiler's wait for them drains both
+        if (step + 1 < last) sq.write(lds + (slot ^ 1) * kStage + kStageA);
+      }
       if (step + 1 < last) issue(step + 1, slot ^ 1);
+      if constexpr (B == kCodes) {
+        if (step + 2 < last) sq.fetch(g, (step + 2) * kStepK);
+      }
       const uint8_t* stage = lds + slot * kStage;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -348,7 +440,7 @@ struct Gemm16 {
       }
     }
 
-    const int64_t plane = p.m * p.n;
+    const int64_t ldp = partial_ld(p.n), plane = p.m * ldp;
     float* part = g.partial + split * (kPairB ? 2 : 1) * plane;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -359,10 +451,12 @@ struct Gemm16 {
         const int64_t n = n0 + 16 * (wn * (kPairB ? NT / 2 : NT) + c) + 4 * (lane >> 4);
         if (n >= p.n) continue;
         if (g.splits > 1) {
-          *reinterpret_cast<f32x4*>(part + m * p.n + n) = acc[i][c];
-          if constexpr (kPairB) *reinterpret_cast<f32x4*>(part + plane + m * p.n + n) = acc[i][c + NT / 2];
+          *reinterpret_cast<f32x4*>(part + m * ldp + n) = acc[i][c];
+          if constexpr (kPairB) *reinterpret_cast<f32x4*>(part + plane + m * ldp + n) = acc[i][c + NT / 2];
         } else if constexpr (EPI == kStore) {
           store_plain(g, p, m, n, acc[i][c]);
+        } else if constexpr (EPI == kBias) {
+          store_bias(g, p, m, n, acc[i][c]);
         } else if constexpr (EPI == kSwiglu) {
           store_swiglu(g, p, m, n, acc[i][c], acc[i][c + NT / 2]);
         } else {
@@ -383,7 +477,7 @@ __global__ __launch_bounds__(G::kThreads) void gemm16_kernel(Gemm16Args g) {
 template <Gemm16Epilogue EPI>
 __global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
   const Gemm16Pair& p = g.pair[0];
-  const int64_t plane = p.m * p.n, at = 4 * (blockIdx.x * int64_t{256} + threadIdx.x);
+  const int64_t ldp = partial_ld(p.n), plane = p.m * ldp, at = 4 * (blockIdx.x * int64_t{256} + threadIdx.x);
   if (at >= plane) return;
   constexpr int kPlanes = EPI == kSwiglu ? 2 : 1;
   f32x4 v[kPlanes];
@@ -393,9 +487,11 @@ __global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
     for (int s = 1; s < g.splits; ++s)
       v[h] += *reinterpret_cast<const f32x4*>(g.partial + (s * kPlanes + h) * plane + at);
   }
-  const int64_t m = at / p.n, n = at % p.n;
+  const int64_t m = at / ldp, n = at % ldp;
   if constexpr (EPI == kStore)
     store_plain(g, p, m, n, v[0]);
+  else if constexpr (EPI == kBias)
+    store_bias(g, p, m, n, v[0]);
   else if constexpr (EPI == kSwiglu)
     store_swiglu(g, p, m, n, v[0], v[1]);
   else

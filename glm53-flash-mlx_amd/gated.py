@@ -127,3 +127,10 @@ class GatedMLP(torch.nn.Module):
 
     def forward(self, x):
         return gated_mlp(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, self.limit)
+
+    def to_int4(self, group_size: int = 64, symmetric: bool = False):
+        """The served form: an Int4MLP of these weights."""
+        from .int4 import Int4MLP
+
+        return Int4MLP.from_weights(self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, self.limit,
+                                    group_size=group_size, symmetric=symmetric)

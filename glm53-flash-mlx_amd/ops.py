@@ -21,7 +21,9 @@ and FakeTensor / meta propagation gets the output shapes without a device.
   and ``residual_norm``, differentiable;
 * ``glm53::gated_mlp(x, gate_weight, up_weight, down_weight, limit, keep)``
   and ``glm53::gated_mlp_backward`` -- ``gated_mlp``, differentiable where
-  `keep` has it return G and U.
+  `keep` has it return G and U;
+* ``glm53::int4_linear(x, weight, scales, offsets?, bias?)`` -- ``int4_linear``,
+  and ``glm53::joined_swiglu(joined, limit)``, the activation of ``Int4MLP``.
 
 The MoE ops take the module by an integer key (``register_owner``): the
 module keeps its weights, its per-(device, stream) native plans and its
@@ -268,3 +270,28 @@ def _gated_mlp_backward(ctx, d_y, _gate, _up):
 
 
 gated_mlp.register_autograd(_gated_mlp_backward, setup_context=_gated_mlp_context)
+
+
+@torch.library.custom_op("glm53::int4_linear", mutates_args=())
+def int4_linear(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, offsets: Optional[torch.Tensor],
+                bias: Optional[torch.Tensor]) -> torch.Tensor:
+    from .int4 import native_int4_linear
+
+    return native_int4_linear(x, weight, scales, offsets, bias)
+
+
+@int4_linear.register_fake
+def _(x, weight, scales, offsets, bias):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))
+
+
+@torch.library.custom_op("glm53::joined_swiglu", mutates_args=())
+def joined_swiglu(joined: torch.Tensor, limit: float) -> torch.Tensor:
+    from .int4 import native_joined_swiglu
+
+    return native_joined_swiglu(joined, limit)
+
+
+@joined_swiglu.register_fake
+def _(joined, limit):
+    return joined.new_empty((*joined.shape[:-1], joined.shape[-1] // 2))

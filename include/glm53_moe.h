@@ -618,6 +618,33 @@ size_t glm53_gated_mlp_backward_workspace_bytes(int64_t rows, int64_t hidden, in
 int glm53_gated_mlp_backward(const glm53_gated_mlp_desc* desc, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Linear with 4-bit weights and group scales (no reference counterpart: its
+ * weights are FP8).
+ * ---------------------------------------------------------------------- */
+/* W[n, k] = scales[n, k / group] q[n, k] + offsets[n, k / group], q in 0..15;
+ * codes u8 [out, in / 2], column 2 j in the low half of byte j and 2 j + 1 in
+ * the high half; scales and offsets [out, in / group], bias [out], all BF16 or
+ * (tables_f32) all FP32; offsets NULL: -8 scale; bias NULL: none.  group 32,
+ * 64 or 128, dividing in_features.  codes 16-byte aligned. */
+typedef struct glm53_int4_weight {
+  const uint8_t* codes;
+  const void* scales;
+  const void* offsets;
+  const void* bias;
+  int64_t out_features, in_features;
+  int32_t group;
+  int32_t tables_f32;
+} glm53_int4_weight;
+/* y[m] = T(x[m] . W^T + bias), x BF16 [rows, in], y BF16 [rows, out], both
+ * contiguous and 16-byte aligned; FP32 sums.  Up to 16 rows multiply by the
+ * codes themselves and scale the group sums in FP32; more rows multiply by W
+ * rounded to BF16.  Workspace (256-byte aligned; NULL where 0 bytes) needs no
+ * initialisation. */
+size_t glm53_int4_linear_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features);
+int glm53_int4_linear(const glm53_int4_weight* weight, const void* x, int64_t rows, void* y, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Seeded synthetic inputs (no reference counterpart: the reference loads a
  * checkpoint).  Element i of stream `seed` is N(0, std) (or U(lo, hi)). */
 int glm53_synth_fp8(uint8_t* codes, float* scale_inv, int64_t rows, int64_t cols, uint64_t seed,

@@ -101,12 +101,71 @@ def test_gated_empty_calls_and_workspace_sizes(N, libso):
         assert size(4, 64, 32) >= 4 * 32 * 2
 
 
+def _int4(N, **changes):
+    w = N.Int4Weight(codes=FAKE, scales=FAKE, offsets=FAKE, bias=FAKE, out_features=48, in_features=128, group=64)
+    for name, value in changes.items():
+        setattr(w, name, value)
+    return ctypes.byref(w)
+
+
+@pytest.mark.parametrize("changes, message", [
+    (dict(out_features=0), "invalid shape"), (dict(in_features=0), "invalid shape"), (dict(group=16), "group"),
+    (dict(group=0), "group"), (dict(in_features=96), "multiple of the group"), (dict(codes=None), "null"),
+    (dict(scales=None), "null"), (dict(codes=FAKE + 8), "aligned"), (dict(in_features=1 << 23), "too large"),
+])
+def test_int4_refusals(N, libso, changes, message):
+    assert libso.glm53_int4_linear(_int4(N, **changes), FAKE, 4, FAKE, FAKE, 1 << 30, None) == N.INVALID_ARGUMENT
+    assert message in libso.glm53_last_error().decode()
+
+
+def test_int4_refuses_call_arguments(N, libso):
+    for x, rows, y in ((FAKE, -1, FAKE), (FAKE, 1 << 31, FAKE), (None, 4, FAKE), (FAKE, 4, None), (FAKE + 2, 4, FAKE),
+                       (FAKE, 4, FAKE + 8)):
+        assert libso.glm53_int4_linear(_int4(N), x, rows, y, FAKE, 1 << 30, None) == N.INVALID_ARGUMENT
+    assert libso.glm53_int4_linear(None, FAKE, 4, FAKE, None, 0, None) == N.INVALID_ARGUMENT
+    assert libso.glm53_int4_linear(_int4(N), None, 0, None, None, 0, None) == N.OK
+    size = libso.glm53_int4_linear_workspace_bytes
+    assert size(0, 48, 128) == size(4, 0, 128) == size(4, 48, 0) == 0
+
+
+def test_quantize_int4_gives_the_nearest_codes():
+    """Codes, scales and offsets made on the CPU: nearest codes for the rounded
+    tables, constant and zero groups, and refusals."""
+    import torch
+
+    M = pkg()
+    g = torch.Generator()
+    g.manual_seed(0)
+    w = torch.randn(6, 128, generator=g)
+    w[0, :64], w[1, 64:] = 0.0, 0.75
+    for symmetric in (False, True):
+        for dtype in (torch.bfloat16, torch.float32):
+            codes, scales, offsets = M.quantize_int4(w, 64, symmetric, dtype)
+            assert codes.shape == (6, 64) and scales.shape == (6, 2) and scales.dtype == dtype
+            q = torch.stack([codes & 15, codes >> 4], 2).view(6, 2, 64).double()
+            s = scales.double()[:, :, None]
+            o = -8 * s if symmetric else offsets.double()[:, :, None]
+            v = w.double().view(6, 2, 64)
+            every = s[..., None] * torch.arange(16) + o[..., None]  # [6, 2, 1, 16]
+            best = (every - v[..., None]).abs().amin(3)
+            assert ((q * s + o - v).abs() <= best + 1e-6).all()
+            assert ((q * s + o)[0, 0] == 0).all()
+    for bad in (lambda: M.quantize_int4(w, 48), lambda: M.quantize_int4(w[:, :96], 64), lambda: M.quantize_int4(w[0], 64),
+                lambda: M.quantize_int4(w.int(), 64), lambda: M.quantize_int4(w, 64, dtype=torch.float16),
+                lambda: M.quantize_int4(w / 0, 64), lambda: M.Int4Linear(96, 8, group_size=64),
+                lambda: M.Int4MLP(M.Int4Linear(64, 64), M.Int4Linear(64, 64)),
+                lambda: M.Int4MLP.from_weights(w, w[:3], w.t())):
+        with pytest.raises(ValueError):
+            bad()
+
+
 def test_python_functions_refuse_cpu_tensors():
     import torch
 
     M = pkg()
     x, w = torch.zeros(2, 64, dtype=torch.bfloat16), torch.ones(64)
     for call in (lambda: M.rms_norm(x, w), lambda: M.residual_norm(x, x, next_weight=w),
-                 lambda: M.gated_mlp(x, x, x, x.t())):
+                 lambda: M.gated_mlp(x, x, x, x.t()),
+                 lambda: M.int4_linear(x, torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1))):
         with pytest.raises((RuntimeError, ValueError)):
             call()
