@@ -15,6 +15,7 @@ from .abi import (
     PACKED_DECODE_KERNEL_ABI,
     PACKED_EXPERT_BANK_ABI,
 )
+from .block import FeedForwardBlock, run_blocks
 from .checkpoint import CheckpointError, load_moe_layer
 from .fp8 import (
     BLOCK_SIZE,
@@ -68,5 +69,5 @@ __all__ = [
     "install_packed_decode_moe", "BankHandle", "RoutedDiagnostic", "ResidentTensor", "TensorLayout", "TensorLease", "TensorOwnership",
     "TensorOwnershipError", "borrowed_ephemeral_tensor", "borrowed_stable_tensor", "materialize_owned",
     "owned_tensor", "require_resident", "resident_concatenate", "rms_norm", "residual_norm", "gated_mlp", "GatedMLP",
-    "int4_linear", "quantize_int4", "Int4Linear", "Int4MLP",
+    "int4_linear", "quantize_int4", "Int4Linear", "Int4MLP", "FeedForwardBlock", "run_blocks",
 ]
