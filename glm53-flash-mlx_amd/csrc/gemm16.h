@@ -61,7 +61,7 @@ struct Gemm16Args {
 };
 
 enum Gemm16Epilogue { kStore, kSwiglu, kSwigluGrad, kBias };
-enum OperandForm { kRow, kColumn, kCodes };
+enum OperandForm { kRow, kColumn, kCodes, kCodesF32 };  // 4-bit codes with bf16 or FP32 tables
 
 // Row length of the partial results: whole groups of four.
 __host__ __device__ __forceinline__ int64_t partial_ld(int64_t n) { return (n + 3) & ~int64_t{3}; }
@@ -231,7 +231,7 @@ struct Stager {
 // bf16 as the activations carry, makes the weights an MFMA operand; over the
 // rows this form is used for, sums of scaled group products in FP32 instead
 // would cost the vector units as many cycles as the product.
-template <int R, int T>
+template <int R, int T, bool F32>
 struct CodeStager {
   static_assert(R * 2 == T, "32 codes a thread");
   u32x4 codes;
@@ -259,18 +259,21 @@ struct CodeStager {
     }
     codes = *reinterpret_cast<const u32x4*>(row + (k >> 1));
     const int64_t t = table + (k >> g.group_log2);
-    scale = table_value(g.scales, g.scales_f32, t);
-    offset = g.offsets != nullptr ? table_value(g.offsets, g.scales_f32, t) : -8.0f * scale;
+    scale = table_value(g.scales, F32, t);
+    // without offsets: the scale, read again, so that both loads are on their
+    // way before either is waited for
+    offset = table_value(g.offsets != nullptr ? g.offsets : g.scales, F32, t);
   }
-  __device__ __forceinline__ void write(uint8_t* stage) const {
+  __device__ __forceinline__ void write(uint8_t* stage, bool offsets) const {
+    const float base = offsets ? offset : -8.0f * offset;
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
       const uint32_t even = codes[d] & 0x0F0F0F0Fu, odd = (codes[d] >> 4) & 0x0F0F0F0Fu;
       u32x4 w;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float a = fmaf(static_cast<float>((even >> (8 * i)) & 0xFFu), scale, offset);
-        const float b = fmaf(static_cast<float>((odd >> (8 * i)) & 0xFFu), scale, offset);
+        const float a = fmaf(static_cast<float>((even >> (8 * i)) & 0xFFu), scale, base);
+        const float b = fmaf(static_cast<float>((odd >> (8 * i)) & 0xFFu), scale, base);
         w[i] = f32_to_bf16(a) | static_cast<uint32_t>(f32_to_bf16(b)) << 16;
       }
       *reinterpret_cast<u32x4*>(stage + at + 16 * ((4 * half + d) ^ mix)) = w;
@@ -328,7 +331,7 @@ template <int WM, int WN, int MT, int NT, bool A_COLUMN, OperandForm B, Gemm16Ep
 struct Gemm16 {
   static constexpr int W = WM * WN, kThreads = 64 * W;
   static constexpr int BM = 16 * WM * MT, BN = 16 * WN * NT;
-  static constexpr bool B_COLUMN = B == kColumn;
+  static constexpr bool B_COLUMN = B == kColumn, kFromCodes = B == kCodes || B == kCodesF32;
   static constexpr bool kPairB = EPI == kSwiglu;           // half the tile gate columns, half up
   static constexpr int kColumns = kPairB ? BN / 2 : BN;    // output columns of a tile
   static constexpr int kStageA = BM * 128, kStage = kStageA + BN * 128;
@@ -366,8 +369,8 @@ struct Gemm16 {
     Stager<BN / kHalves, W, B_COLUMN> sb;
     sb.init(wave, lane, p.ldb, p.n - n0);
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    CodeStager<B == kCodes ? BN : kThreads / 2, kThreads> sq;
-    if constexpr (B == kCodes) sq.init(g, n0, p.n, g.k);
+    CodeStager<kFromCodes ? BN : kThreads / 2, kThreads, B == kCodesF32> sq;
+    if constexpr (kFromCodes) sq.init(g, n0, p.n, g.k);
     const auto issue = [&](int64_t step, int slot) {
       const int s = g.segments > 1 ? static_cast<int>(step / steps) : 0;
       const int64_t kk = (step - s * steps) * kStepK;
@@ -379,7 +382,7 @@ struct Gemm16 {
         sa.issue_tail(a, wave, lane, tail, lds + slot * kStage);
       else
         sa.issue(a, wave, lds_at + slot * kStage);
-      if constexpr (B == kCodes) return;
+      if constexpr (kFromCodes) return;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
         const uint16_t* b = (kPairB ? g.pair[h].b : o.b) + b_at;
@@ -404,10 +407,10 @@ struct Gemm16 {
       return kPairB ? (c < NT / 2 ? wn * (NT / 2) + c : BN / 32 + wn * (NT / 2) + c - NT / 2) : wn * NT + c;
     };
 
-    if constexpr (B == kCodes) {
+    if constexpr (kFromCodes) {
       if (first < last) {
         sq.fetch(g, first * kStepK);
-        sq.write(lds + kStageA);
+        sq.write(lds + kStageA, g.offsets != nullptr);
         if (first + 1 < last) sq.fetch(g, (first + 1) * kStepK);
       }
     }
@@ -415,11 +418,11 @@ struct Gemm16 {
     int slot = 0;
     for (int64_t step = first; step < last; ++step, slot ^= 1) {
       stage_wait();
-      if constexpr (B == kCodes) {  // codes before the direct loads: the compiler's wait for them drains both
-        if (step + 1 < last) sq.write(lds + (slot ^ 1) * kStage + kStageA);
+      if constexpr (kFromCodes) {  // codes before the direct loads: the compiler's wait for them drains both
+        if (step + 1 < last) sq.write(lds + (slot ^ 1) * kStage + kStageA, g.offsets != nullptr);
       }
       if (step + 1 < last) issue(step + 1, slot ^ 1);
-      if constexpr (B == kCodes) {
+      if constexpr (kFromCodes) {
         if (step + 2 < last) sq.fetch(g, (step + 2) * kStepK);
       }
       const uint8_t* stage = lds + slot * kStage;

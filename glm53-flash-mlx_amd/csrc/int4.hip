@@ -30,8 +30,6 @@ hipError_t launch_tiles(Gemm16Args g, hipStream_t st) {
 // Operands: rows of x as the MFMA's rows, so that a lane's four results have
 // one output column, one scale and one offset.
 constexpr int kFewRows = 16;
-constexpr int kFewWaves = 8;
-constexpr int kFewBlocks = 4;  // blocks of 128 columns that a wavefront has in flight
 
 // Quarter q's dword s of four becomes quarter s's dword q.
 __device__ __forceinline__ void exchange_quarters(u32x4& v) {
@@ -68,102 +66,198 @@ __device__ __forceinline__ bf16x8 codes_order(u32x4 x) {
 }
 
 // One output in the formula's own order: for results that the kernel below
-// cannot tell from inf - inf of its two sums.
-__device__ __attribute__((noinline)) float one_output(const Int4Args& a, int64_t m, int64_t n) {
+// cannot tell from inf - inf of its two sums.  Its pointers come one by one:
+// with the argument block's address taken, every load of the kernel would go
+// by flat addresses and wait for the one before.
+__device__ __forceinline__ float one_output(const uint16_t* x, const uint8_t* codes, const void* scales,
+                                                      const void* offsets, bool f32, int group_log2, int k_all) {
   float y = 0.0f;
-  for (int64_t k = 0; k < a.K; ++k) {
-    const int64_t t = n * (a.K >> a.group_log2) + (k >> a.group_log2);
-    const float scale = table_value(a.scales, a.tables_f32, t);
-    const float offset = a.offsets != nullptr ? table_value(a.offsets, a.tables_f32, t) : -8.0f * scale;
-    const int q = (a.codes[(n * a.K + k) >> 1] >> (4 * (k & 1))) & 15;
-    y += bf16_to_f32(a.x[m * a.K + k]) * fmaf(static_cast<float>(q), scale, offset);
+  for (int k = 0; k < k_all; ++k) {
+    const float scale = table_value(scales, f32, k >> group_log2);
+    const float offset = offsets != nullptr ? table_value(offsets, f32, k >> group_log2) : -8.0f * scale;
+    const int q = (codes[k >> 1] >> (4 * (k & 1))) & 15;
+    y += bf16_to_f32(x[k]) * fmaf(static_cast<float>(q), scale, offset);
   }
   return y;
 }
 
-template <int GROUP_LOG2>
-__global__ __launch_bounds__(64 * kFewWaves) void int4_few_kernel(Int4Args a) {
-  constexpr int kGroups = 128 >> GROUP_LOG2;           // groups of a block
-  constexpr int kSteps = 1 << (GROUP_LOG2 - 5);        // MFMAs of a group
-  __shared__ float part[kFewWaves][kFewRows][16];
+template <class T>
+__device__ __forceinline__ T load_at(const void* base, uint32_t off) {
+  return *reinterpret_cast<const T*>(static_cast<const uint8_t*>(base) + off);
+}
+template <bool F32>
+__device__ __forceinline__ float table_load(const void* base, uint32_t off) {
+  if (F32) return load_at<float>(base, off);
+  return bf16_to_f32(load_at<uint16_t>(base, off));
+}
+
+constexpr int64_t kFewXBytes = 32768;  // x of a phase in LDS
+constexpr int kPhase = 8192;  // columns whose tables (and x) a workgroup has in LDS at a time
+
+// Table entries (scale, offset - 128 scale) of an output column and phase in
+// LDS: its groups, then zeros for a block's groups.
+__host__ __device__ constexpr int few_table_groups(int columns, int group_log2) {
+  return ((columns + 127) / 128 << (7 - group_log2)) + (128 >> group_log2);
+}
+
+// Entries from one column to the next: odd, so that the 16 columns' entries of a
+// group, which 16 lanes read at once, lie on different banks.
+__host__ __device__ constexpr int few_table_ld(int columns, int group_log2) {
+  return few_table_groups(columns, group_log2) | 1;
+}
+
+// XLDS: x lies in LDS, [columns / 8][rows] pieces of 8 in the codes' order (few
+// rows, whose x fits); otherwise each wavefront reads its part from L2.
+template <int W, int U, int GROUP_LOG2, bool F32, bool OFFSETS, bool XLDS>
+__global__ __launch_bounds__(64 * W) void int4_few_kernel(Int4Args a) {
+  constexpr int kGroups = 128 >> GROUP_LOG2;     // groups of a block
+  constexpr int kSteps = 1 << (GROUP_LOG2 - 5);  // MFMAs of a group
+  constexpr int kTable = F32 ? 4 : 2;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  extern __shared__ __align__(16) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, q = lane >> 4;
+  const int r = lane & 15, q = lane >> 4, K = static_cast<int>(a.K), rows = static_cast<int>(a.rows);
   const int64_t n0 = 16 * static_cast<int64_t>(blockIdx.x);
-  const int64_t n = n0 + r < a.N ? n0 + r : a.N - 1;
-  const int64_t m = r < a.rows ? r : a.rows - 1;
-  const uint8_t* row = a.codes + n * (a.K >> 1) + 16 * q;
-  const uint16_t* x = a.x + m * a.K + 8 * q;
-  const int64_t table = n * (a.K >> GROUP_LOG2);
-  const int64_t blocks = (a.K + 127) / 128;
-  const int64_t each = (blocks + kFewWaves - 1) / kFewWaves;
-  const int64_t first = wave * each, last = first + each < blocks ? first + each : blocks;
+  const int cols = a.N - n0 < 16 ? static_cast<int>(a.N - n0) : 16;
+  const int nr = r < cols ? r : cols - 1, mr = r < rows ? r : rows - 1;
+  const int groups = K >> GROUP_LOG2;
+  // bases of the workgroup and a lane's byte offsets from them
+  const uint8_t* codes = a.codes + n0 * (a.K >> 1);
+  const uint8_t* scales = static_cast<const uint8_t*>(a.scales) + n0 * groups * kTable;
+  const uint8_t* offsets = OFFSETS ? static_cast<const uint8_t*>(a.offsets) + n0 * groups * kTable : nullptr;
+  const uint32_t code_off = static_cast<uint32_t>(nr) * (K >> 1);
+  const uint32_t x_off = static_cast<uint32_t>(mr) * (2 * K) + 16 * q;
+  const int phase_columns = K < kPhase ? K : kPhase;
+  f32x2* tables = reinterpret_cast<f32x2*>(lds);
+  const int table_ld = few_table_ld(phase_columns, GROUP_LOG2);
+  uint8_t* x_lds = lds + 128 * table_ld;
+
   f32x4 total = {0, 0, 0, 0};
   const u32x4 one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
   const bf16x8 ones = __builtin_bit_cast(bf16x8, one);
-  for (int64_t b0 = first; b0 < last; b0 += kFewBlocks) {
-    u32x4 code[kFewBlocks], xs[kFewBlocks][4];
-    float scale[kFewBlocks][kGroups], offset[kFewBlocks][kGroups];
+  for (int k0 = 0; k0 < K; k0 += kPhase) {
+    const int columns = K - k0 < kPhase ? K - k0 : kPhase;
+    const int blocks = (columns + 127) / 128, each = (blocks + W - 1) / W;
+    const int first = wave * each, last = first + each < blocks ? first + each : blocks;
+    // Codes and x of U blocks, without a branch: what lies past the
+    // wavefront's blocks or past K reads an address that is there and meets
+    // scale 0.  Branches around the steps would have the compiler move each
+    // step's loads behind them.
+    u32x4 code[2][U], xs[2][XLDS ? 1 : U][4];
+    const auto load = [&](int b, int to) {
 #pragma unroll
-    for (int u = 0; u < kFewBlocks; ++u) {
-      const int64_t k = 128 * (b0 + u);
-      if (b0 + u >= last) break;
-      code[u] = (u32x4){0, 0, 0, 0};
-      if (k + 32 * q < a.K) code[u] = *reinterpret_cast<const u32x4*>(row + (k >> 1));
+      for (int u = 0; u < U; ++u) {
+        const int bb = b + u < last ? b + u : last - 1, k = k0 + 128 * bb;
+        const uint32_t piece = k + 128 <= K || k + 32 * q < K ? 16 * q : 0;
+        code[to][u] = load_at<u32x4>(codes, code_off + (k >> 1) + piece);
+        if constexpr (!XLDS) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (k + 32 * s < a.K) xs[u][s] = *reinterpret_cast<const u32x4*>(x + k + 32 * s);
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        if (k + (g << GROUP_LOG2) >= a.K) break;
-        const int64_t t = table + (k >> GROUP_LOG2) + g;
-        scale[u][g] = table_value(a.scales, a.tables_f32, t);
-        offset[u][g] = a.offsets != nullptr ? table_value(a.offsets, a.tables_f32, t) : -8.0f * scale[u][g];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kFewBlocks; ++u) {
-      const int64_t k = 128 * (b0 + u);
-      if (b0 + u >= last) break;
-      exchange_quarters(code[u]);
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) {
-        if (k + (g << GROUP_LOG2) >= a.K) break;
-        f32x4 d = {0, 0, 0, 0}, sum = {0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const bf16x8 v = codes_order(xs[u][g * kSteps + s]);
-          d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, codes_operand(code[u][g * kSteps + s]), d, 0, 0, 0);
-          sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ones, sum, 0, 0, 0);
+          for (int s = 0; s < 4; ++s) xs[to][u][s] = load_at<u32x4>(a.x, x_off + 2 * (k + 32 * s < K ? k + 32 * s : k));
         }
-        const float c = offset[u][g] - 128.0f * scale[u][g];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) total[i] += scale[u][g] * d[i] + c * sum[i];
       }
+    };
+    if (first < last) load(first, 0);
+    if (k0 > 0) __syncthreads();  // the phase before is read
+    const int entries = few_table_groups(columns, GROUP_LOG2), phase_groups = columns >> GROUP_LOG2;
+    for (int c = wave; c < 16; c += W)  // a column's groups are consecutive in memory and in LDS
+      for (int g = lane; g < entries; g += 64) {
+        f32x2 v = {0.0f, 0.0f};
+        if (g < phase_groups && c < cols) {
+          const uint32_t at = (static_cast<uint32_t>(c) * groups + (k0 >> GROUP_LOG2) + g) * kTable;
+          const float scale = table_load<F32>(scales, at);
+          v = (f32x2){scale, OFFSETS ? table_load<F32>(offsets, at) - 128.0f * scale : -136.0f * scale};
+        }
+        tables[c * table_ld + g] = v;
+      }
+    if constexpr (XLDS) {
+      for (int m = 0; m < rows; ++m)
+        for (int c = threadIdx.x; c < columns / 8; c += 64 * W)
+          *reinterpret_cast<bf16x8*>(x_lds + 16 * (c * rows + m)) = codes_order(load_at<u32x4>(a.x, 2 * (m * K + k0) + 16 * c));
+    }
+    __syncthreads();
+    const int zeros = entries - kGroups;
+    const auto compute = [&](int b, int from) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool in = b + u < last;
+        u32x4 cd = code[from][u];
+        exchange_quarters(cd);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const f32x2 t = tables[r * table_ld + (in ? (b + u) * kGroups : zeros) + g];
+          f32x4 d = {0, 0, 0, 0}, sum = {0, 0, 0, 0};
+#pragma unroll
+          for (int s = g * kSteps; s < (g + 1) * kSteps; ++s) {
+            bf16x8 v;
+            if constexpr (XLDS) {
+              const int at = in && 128 * (b + u) + 32 * s < columns ? 16 * (b + u) + 4 * s : 0;
+              v = *reinterpret_cast<const bf16x8*>(x_lds + 16 * ((at + q) * rows + mr));
+            } else {
+              v = codes_order(xs[from][u][s]);
+            }
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, codes_operand(cd[s]), d, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ones, sum, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) total[i] += t[0] * d[i] + t[1] * sum[i];
+        }
+      }
+    };
+    for (int b = first; b < last; b += 2 * U) {
+      if (b + U < last) load(b + U, 1);
+      compute(b, 0);
+      if (b + 2 * U < last) load(b + 2 * U, 0);
+      if (b + U < last) compute(b + U, 1);
     }
   }
+  __syncthreads();  // the last phase is read; its place holds the partial sums
+  float(*part)[kFewRows][16] = reinterpret_cast<float(*)[kFewRows][16]>(lds);
 #pragma unroll
   for (int i = 0; i < 4; ++i) part[wave][4 * q + i][r] = total[i];
   __syncthreads();
   if (threadIdx.x >= 16 * kFewRows) return;
-  const int col = threadIdx.x & 15, mm = threadIdx.x >> 4;
-  if (mm >= a.rows || n0 + col >= a.N) return;
-  float y = part[0][mm][col];
+  const int col = threadIdx.x & 15, m = threadIdx.x >> 4;
+  if (m >= rows || col >= cols) return;
+  float y = part[0][m][col];
 #pragma unroll
-  for (int w = 1; w < kFewWaves; ++w) y += part[w][mm][col];
-  if (!(fabsf(y) < INFINITY)) y = one_output(a, mm, n0 + col);
+  for (int w = 1; w < W; ++w) y += part[w][m][col];
+  if (!(fabsf(y) < INFINITY))
+    y = one_output(a.x + m * a.K, codes + static_cast<int64_t>(col) * (K >> 1), scales + int64_t{col} * groups * kTable,
+                   OFFSETS ? offsets + int64_t{col} * groups * kTable : nullptr, F32, GROUP_LOG2, K);
   if (a.bias != nullptr) y += table_value(a.bias, a.tables_f32, n0 + col);
-  a.y[mm * a.N + n0 + col] = f32_to_bf16(y);
+  a.y[m * a.N + n0 + col] = f32_to_bf16(y);
 }
 
+template <int W, int U, int GROUP_LOG2, bool XLDS>
 hipError_t launch_few(const Int4Args& a, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>(cdiv(a.N, 16)));
-  if (a.group_log2 == 5)
-    int4_few_kernel<5><<<grid, 64 * kFewWaves, 0, st>>>(a);
-  else if (a.group_log2 == 6)
-    int4_few_kernel<6><<<grid, 64 * kFewWaves, 0, st>>>(a);
-  else
-    int4_few_kernel<7><<<grid, 64 * kFewWaves, 0, st>>>(a);
+  const dim3 grid(static_cast<uint32_t>(cdiv(a.N, 16))), block(64 * W);
+  const int columns = static_cast<int>(a.K < kPhase ? a.K : kPhase);
+  const size_t staged = 128 * few_table_ld(columns, GROUP_LOG2) + (XLDS ? 2 * static_cast<size_t>(a.rows * columns) : 0);
+  const size_t lds = staged > 1024 * W ? staged : 1024 * W;
+  if (a.tables_f32) {
+    if (a.offsets != nullptr)
+      int4_few_kernel<W, U, GROUP_LOG2, true, true, XLDS><<<grid, block, lds, st>>>(a);
+    else
+      int4_few_kernel<W, U, GROUP_LOG2, true, false, XLDS><<<grid, block, lds, st>>>(a);
+  } else {
+    if (a.offsets != nullptr)
+      int4_few_kernel<W, U, GROUP_LOG2, false, true, XLDS><<<grid, block, lds, st>>>(a);
+    else
+      int4_few_kernel<W, U, GROUP_LOG2, false, false, XLDS><<<grid, block, lds, st>>>(a);
+  }
   return hipGetLastError();
+}
+
+template <int W, int U, bool XLDS>
+hipError_t launch_few_group(const Int4Args& a, hipStream_t st) {
+  if (a.group_log2 == 5) return launch_few<W, U, 5, XLDS>(a, st);
+  if (a.group_log2 == 6) return launch_few<W, U, 6, XLDS>(a, st);
+  return launch_few<W, U, 7, XLDS>(a, st);
+}
+
+hipError_t launch_few_rows(const Int4Args& a, hipStream_t st) {
+  if (2 * a.rows * (a.K < kPhase ? a.K : kPhase) <= kFewXBytes) return launch_few_group<16, 1, true>(a, st);
+  return launch_few_group<16, 1, false>(a, st);
 }
 
 }  // namespace
@@ -171,7 +265,7 @@ hipError_t launch_few(const Int4Args& a, hipStream_t st) {
 size_t int4_space(int64_t rows, int64_t N, int64_t K) { return 0; }
 
 hipError_t launch_int4(const Int4Args& a, hipStream_t st) {
-  if (a.rows <= kFewRows) return launch_few(a, st);
+  if (a.rows <= kFewRows) return launch_few_rows(a, st);
   Gemm16Args g{};
   g.k = a.K;
   g.problems = g.segments = g.splits = 1;
@@ -182,6 +276,7 @@ hipError_t launch_int4(const Int4Args& a, hipStream_t st) {
   g.bias = a.bias;
   g.scales_f32 = a.tables_f32;
   g.group_log2 = a.group_log2;
+  if (a.tables_f32) return launch_tiles<Gemm16<2, 2, 4, 4, false, kCodesF32, kBias>>(g, st);
   return launch_tiles<Gemm16<2, 2, 4, 4, false, kCodes, kBias>>(g, st);
 }
 
