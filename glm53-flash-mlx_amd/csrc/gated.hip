@@ -7,6 +7,9 @@
 //   dWg = dG^T x, dWu = dU^T x, dWd = dy^T h (one launch).
 // Operands of a product are bf16 and its sums FP32: h, dG and dU are rounded
 // to bf16 once, as MFMA operands, everything before them is FP32.
+#include <algorithm>
+#include <initializer_list>
+
 #include "gated.h"
 #include "gemm16.h"
 
@@ -15,21 +18,6 @@ namespace {
 
 size_t round_up(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-template <class G>
-hipError_t launch_tiles(Gemm16Args g, hipStream_t st) {
-  g.tiles = 0;
-  for (int q = 0; q < g.problems; ++q) g.tiles += cdiv(g.pair[q].m, G::BM) * cdiv(g.pair[q].n, G::kColumns);
-  g.group_m = 8;
-  gemm16_kernel<G><<<static_cast<uint32_t>(g.tiles * g.splits), G::kThreads, G::kLds, st>>>(g);
-  return hipGetLastError();
-}
-
-template <bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI>
-hipError_t launch_product(Gemm16Args g, hipStream_t st) {
-  g.splits = 1;
-  return launch_tiles<Gemm16<2, 2, 4, 4, A_COLUMN, B, EPI>>(g, st);
-}
 
 // ------------------------------------------------------------- few rows ---
 //
@@ -150,59 +138,118 @@ Gemm16Args product(int64_t k) {
   return g;
 }
 
-}  // namespace
-
-size_t gated_space(int64_t rows, int64_t hidden, int64_t inter, bool backward) {
-  const size_t values = static_cast<size_t>(rows) * static_cast<size_t>(inter);
-  if (backward) return 3 * round_up(2 * values);
-  return round_up((rows <= kFewRows ? 4 : 2) * values);
+// The workspace: h, and backward dG and dU (bf16 [rows, inter] each), then the
+// partial results of one product at a time.
+struct Space {
+  uint16_t *h, *dg, *du;
+  float* partial;
+};
+Space carve(const GatedArgs& a, bool backward) {
+  uint8_t* p = static_cast<uint8_t*>(a.space);
+  const size_t plane = round_up(2 * static_cast<size_t>(a.rows) * static_cast<size_t>(a.inter));
+  Space s{};
+  s.h = reinterpret_cast<uint16_t*>(p);
+  if (backward) {
+    s.dg = reinterpret_cast<uint16_t*>(p + plane);
+    s.du = reinterpret_cast<uint16_t*>(p + 2 * plane);
+  }
+  s.partial = reinterpret_cast<float*>(p + (backward ? 3 : 1) * plane);
+  return s;
 }
 
-hipError_t launch_gated(const GatedArgs& a, hipStream_t st) {
-  if (a.rows <= kFewRows) return launch_few(a, st);
-  uint16_t* h = static_cast<uint16_t*>(a.space);
+Gemm16Args gate_up(const GatedArgs& a, const Space& s) {
   Gemm16Args g = product(a.hidden);
-  g.pair[0] = pair(a.x, a.hidden, a.wg, a.hidden, h, a.rows, a.inter);
+  g.pair[0] = pair(a.x, a.hidden, a.wg, a.hidden, s.h, a.rows, a.inter);
   g.pair[1] = g.pair[0];
   g.pair[1].b = a.wu;
   g.limit = a.limit;
   g.gate = a.gate;
   g.up = a.up;
-  if (hipError_t e = launch_product<false, kRow, kSwiglu>(g, st); e != hipSuccess) return e;
-  Gemm16Args d = product(a.inter);
-  d.pair[0] = pair(h, a.inter, a.wd, a.inter, a.y, a.rows, a.hidden);
-  return launch_product<false, kRow, kStore>(d, st);
+  g.partial = s.partial;
+  return g;
 }
-
-hipError_t launch_gated_backward(const GatedArgs& a, hipStream_t st) {
-  uint8_t* space = static_cast<uint8_t*>(a.space);
-  const size_t plane = round_up(2 * static_cast<size_t>(a.rows) * static_cast<size_t>(a.inter));
-  uint16_t* dg = reinterpret_cast<uint16_t*>(space);
-  uint16_t* du = reinterpret_cast<uint16_t*>(space + plane);
-  uint16_t* h = reinterpret_cast<uint16_t*>(space + 2 * plane);
+Gemm16Args down(const GatedArgs& a, const Space& s) {
+  Gemm16Args g = product(a.inter);
+  g.pair[0] = pair(s.h, a.inter, a.wd, a.inter, a.y, a.rows, a.hidden);
+  g.partial = s.partial;
+  return g;
+}
+Gemm16Args hidden_grad(const GatedArgs& a, const Space& s) {
   Gemm16Args g = product(a.hidden);
   g.pair[0] = pair(a.dy, a.hidden, a.wd, a.inter, nullptr, a.rows, a.inter);
   g.limit = a.limit;
   g.gate = a.gate;
   g.up = a.up;
-  g.d_gate = dg;
-  g.d_up = du;
-  g.h = a.d_wd != nullptr ? h : nullptr;
-  if (hipError_t e = launch_product<false, kColumn, kSwigluGrad>(g, st); e != hipSuccess) return e;
-  if (a.dx != nullptr) {
-    Gemm16Args x = product(a.inter);
-    x.segments = 2;
-    x.pair[0] = pair(dg, a.inter, a.wg, a.hidden, a.dx, a.rows, a.hidden);
-    x.pair[1] = pair(du, a.inter, a.wu, a.hidden, a.dx, a.rows, a.hidden);
-    if (hipError_t e = launch_product<false, kColumn, kStore>(x, st); e != hipSuccess) return e;
+  g.d_gate = s.dg;
+  g.d_up = s.du;
+  g.h = a.d_wd != nullptr ? s.h : nullptr;
+  g.partial = s.partial;
+  return g;
+}
+Gemm16Args input_grad(const GatedArgs& a, const Space& s) {
+  Gemm16Args g = product(a.inter);
+  g.segments = 2;
+  g.pair[0] = pair(s.dg, a.inter, a.wg, a.hidden, a.dx, a.rows, a.hidden);
+  g.pair[1] = pair(s.du, a.inter, a.wu, a.hidden, a.dx, a.rows, a.hidden);
+  g.partial = s.partial;
+  return g;
+}
+// Those weights' gradients that are wanted (`every`: all, for their room).
+Gemm16Args weight_grads(const GatedArgs& a, const Space& s, bool every) {
+  Gemm16Args g = product(a.rows);
+  g.problems = 0;
+  if (every || a.d_wg) g.pair[g.problems++] = pair(s.dg, a.inter, a.x, a.hidden, a.d_wg, a.inter, a.hidden);
+  if (every || a.d_wu) g.pair[g.problems++] = pair(s.du, a.inter, a.x, a.hidden, a.d_wu, a.inter, a.hidden);
+  if (every || a.d_wd) g.pair[g.problems++] = pair(a.dy, a.hidden, s.h, a.inter, a.d_wd, a.hidden, a.inter);
+  g.partial = s.partial;
+  return g;
+}
+
+int64_t most(std::initializer_list<int64_t> v) { return std::max(v); }
+
+}  // namespace
+
+size_t gated_space(int64_t rows, int64_t hidden, int64_t inter, bool backward) {
+  const size_t values = static_cast<size_t>(rows) * static_cast<size_t>(inter);
+  GatedArgs a{};
+  a.rows = rows;
+  a.hidden = hidden;
+  a.inter = inter;
+  const Space s{};
+  if (backward) {
+    int64_t partial = most({gemm16_plan(hidden_grad(a, s), false).partial,
+                            gemm16_plan(input_grad(a, s), false).partial});
+    for (int n = 1; n <= 3; ++n) {  // any of the weights' gradients may not be wanted
+      Gemm16Args w = weight_grads(a, s, true);
+      w.problems = n;
+      partial = most({partial, gemm16_plan(w, false).partial});
+    }
+    return 3 * round_up(2 * values) + sizeof(float) * static_cast<size_t>(partial);
   }
-  Gemm16Args w = product(a.rows);
-  w.problems = 0;
-  if (a.d_wg) w.pair[w.problems++] = pair(dg, a.inter, a.x, a.hidden, a.d_wg, a.inter, a.hidden);
-  if (a.d_wu) w.pair[w.problems++] = pair(du, a.inter, a.x, a.hidden, a.d_wu, a.inter, a.hidden);
-  if (a.d_wd) w.pair[w.problems++] = pair(a.dy, a.hidden, h, a.inter, a.d_wd, a.hidden, a.inter);
+  if (rows <= kFewRows) return round_up(4 * values);
+  const int64_t partial = most({gemm16_plan(gate_up(a, s), true).partial, gemm16_plan(down(a, s), false).partial});
+  return round_up(2 * values) + sizeof(float) * static_cast<size_t>(partial);
+}
+
+hipError_t launch_gated(const GatedArgs& a, hipStream_t st) {
+  if (a.rows <= kFewRows) return launch_few(a, st);
+  const Space s = carve(a, false);
+  const Gemm16Args g = gate_up(a, s), d = down(a, s);
+  if (hipError_t e = gemm16<false, kRow, kSwiglu>(g, gemm16_plan(g, true), st); e != hipSuccess) return e;
+  return gemm16<false, kRow, kStore>(d, gemm16_plan(d, false), st);
+}
+
+hipError_t launch_gated_backward(const GatedArgs& a, hipStream_t st) {
+  const Space s = carve(a, true);
+  const Gemm16Args g = hidden_grad(a, s);
+  if (hipError_t e = gemm16<false, kColumn, kSwigluGrad>(g, gemm16_plan(g, false), st); e != hipSuccess) return e;
+  if (a.dx != nullptr) {
+    const Gemm16Args x = input_grad(a, s);
+    if (hipError_t e = gemm16<false, kColumn, kStore>(x, gemm16_plan(x, false), st); e != hipSuccess) return e;
+  }
+  const Gemm16Args w = weight_grads(a, s, false);
   if (w.problems == 0) return hipSuccess;
-  return launch_product<true, kColumn, kStore>(w, st);
+  return gemm16<true, kColumn, kStore>(w, gemm16_plan(w, false), st);
 }
 
 }  // namespace glm53

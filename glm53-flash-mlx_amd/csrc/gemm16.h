@@ -39,8 +39,9 @@ struct Gemm16Args {
   int problems;    // pairs that are products of their own
   int segments;    // pairs whose contractions are added into pair[0].out
   int splits;      // parts of the contraction, each to `partial`
-  float* partial;  // [splits][planes][m][partial_ld(n)]
-  int64_t tiles;   // output tiles of all problems
+  float* partial;  // of each problem [splits][planes][m][partial_ld(n)], at partial_at floats
+  int64_t partial_at[3];
+  int64_t tiles;   // output tiles of all problems; tiles * splits below 2^31
   int group_m;     // tile rows that one XCD's neighbouring workgroups share
   // SwiGLU: pair[0].b gate and pair[1].b up rows, out = h; gate/up (f32
   // [m, n]) null or what the gradient needs.  Its gradient (out unused): reads
@@ -161,10 +162,21 @@ __device__ __forceinline__ void store_swiglu_grad(const Gemm16Args& g, const Gem
 
 __device__ __forceinline__ int column_swizzle(int k) { return (k & 3) | ((k >> 2) & 4); }
 
+// A wave-uniform pointer in scalar registers, where the compiler does not see
+// that it is one.
+__device__ __forceinline__ const void* uniform_pointer(const void* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));  // an int: not to be sign-extended
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+  return reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 // Direct global -> LDS load of 16 bytes a lane to lds_base + 16 lane.  Inline
 // assembly, so that the compiler puts no wait of its own before LDS reads;
 // stage_wait counts them.
 __device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint32_t lds_base) {
+  base = uniform_pointer(base);
+  lds_base = __builtin_amdgcn_readfirstlane(lds_base);
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_base)
                : "memory", "m0");
 }
@@ -312,56 +324,83 @@ struct Reader {
 // Tile number t of `tiles` for workgroup b: consecutive workgroups go to the
 // XCDs in turn, so workgroup b takes number b / 8 of XCD b % 8's run of
 // consecutive tiles, which share rows and columns in that XCD's L2.
-__device__ __forceinline__ int64_t xcd_tile(int64_t b, int64_t tiles) {
-  const int64_t q = tiles / 8, r = tiles % 8, x = b % 8;
+__device__ __forceinline__ int xcd_tile(int b, int tiles) {
+  const int q = tiles / 8, r = tiles % 8, x = b % 8;
   return x * q + (x < r ? x : r) + b / 8;
 }
 
 // Tile (row, column) number t of rows x cols, in bands of `group` tile rows.
-__device__ __forceinline__ void band_tile(int64_t t, int64_t rows, int64_t cols, int group, int64_t& tm, int64_t& tn) {
-  const int64_t band = t / (group * cols), first = band * group;
-  const int64_t high = rows - first < group ? rows - first : group;
-  const int64_t in = t - band * group * cols;
+__device__ __forceinline__ void band_tile(int t, int rows, int cols, int group, int& tm, int& tn) {
+  const int band = t / (group * cols), first = band * group;
+  const int high = rows - first < group ? rows - first : group;
+  const int in = t - band * group * cols;
   tm = first + in % high;
   tn = in / high;
 }
 
-// WM x WN wavefronts, each MT x NT MFMA tiles of 16 x 16.
-template <int WM, int WN, int MT, int NT, bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI>
+// Tiles of `size` over m or n, which are below 2^31.
+__device__ __forceinline__ int tiles_of(int64_t n, int size) {
+  return static_cast<int>((static_cast<uint32_t>(n) + static_cast<uint32_t>(size) - 1) / static_cast<uint32_t>(size));
+}
+
+// WM x WN wavefronts, each MT x NT MFMA tiles of 16 x 16; SUB blocks of 64 k a
+// step and stage: small tiles multiply a block faster than its loads return, so
+// they take two blocks between barriers.
+template <int WM, int WN, int MT, int NT, int SUB, bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI>
 struct Gemm16 {
   static constexpr int W = WM * WN, kThreads = 64 * W;
   static constexpr int BM = 16 * WM * MT, BN = 16 * WN * NT;
   static constexpr bool B_COLUMN = B == kColumn, kFromCodes = B == kCodes || B == kCodesF32;
   static constexpr bool kPairB = EPI == kSwiglu;           // half the tile gate columns, half up
   static constexpr int kColumns = kPairB ? BN / 2 : BN;    // output columns of a tile
-  static constexpr int kStageA = BM * 128, kStage = kStageA + BN * 128;
+  static constexpr int kStageA = BM * 128, kBlock = kStageA + BN * 128, kStage = SUB * kBlock;
   static constexpr int kLds = 2 * kStage;
+
+  static constexpr int kReadA = A_COLUMN ? 2 : 1, kReadB = B_COLUMN ? 2 : 1;  // LDS reads of an operand
+  static constexpr int kAhead = 2;
+
+  __device__ static __forceinline__ void schedule_step() {
+    constexpr int kMfma = 0x008, kLdsRead = 0x100;
+    constexpr int kGroups = MT / kAhead;
+    __builtin_amdgcn_sched_group_barrier(kLdsRead, NT * kReadB + kAhead * kReadA, 0);
+#pragma unroll
+    for (int j = 0; j < 2 * SUB; ++j) {
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        if (i + 1 < kGroups)
+          __builtin_amdgcn_sched_group_barrier(kLdsRead, kAhead * kReadA, 0);
+        else if (j + 1 < 2 * SUB)
+          __builtin_amdgcn_sched_group_barrier(kLdsRead, NT * kReadB + kAhead * kReadA, 0);
+        __builtin_amdgcn_sched_group_barrier(kMfma, kAhead * NT, 0);
+      }
+    }
+  }
 
   __device__ static __forceinline__ void run(const Gemm16Args& g, uint8_t* lds) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     // tile, split and problem
-    const int64_t unit = xcd_tile(blockIdx.x, g.tiles * g.splits);
-    const int split = static_cast<int>(unit / g.tiles);
-    int64_t t = unit % g.tiles;
-    int q = 0;
-    int64_t rows = (g.pair[0].m + BM - 1) / BM, cols = (g.pair[0].n + kColumns - 1) / kColumns;
+    const int tiles = static_cast<int>(g.tiles), unit = xcd_tile(blockIdx.x, tiles * g.splits);
+    const int split = g.splits > 1 ? unit / tiles : 0;
+    int t = unit - split * tiles, q = 0;
+    int rows = tiles_of(g.pair[0].m, BM), cols = tiles_of(g.pair[0].n, kColumns);
     while (q + 1 < g.problems && t >= rows * cols) {
       t -= rows * cols;
       ++q;
-      rows = (g.pair[q].m + BM - 1) / BM;
-      cols = (g.pair[q].n + kColumns - 1) / kColumns;
+      rows = tiles_of(g.pair[q].m, BM);
+      cols = tiles_of(g.pair[q].n, kColumns);
     }
     const Gemm16Pair& p = g.pair[q];
-    int64_t tm, tn;
+    int tm, tn;
     band_tile(t, rows, cols, g.group_m, tm, tn);
-    const int64_t m0 = tm * BM, n0 = tn * kColumns;
+    const int64_t m0 = static_cast<int64_t>(tm) * BM, n0 = static_cast<int64_t>(tn) * kColumns;
 
-    // K steps of this split
-    const int64_t steps = (g.k + kStepK - 1) / kStepK, all = steps * g.segments;
-    const int64_t each = (all + g.splits - 1) / g.splits;
-    const int64_t first = split * each, last = first + each < all ? first + each : all;
-    const int tail = static_cast<int>(g.k % kStepK);
+    // K steps of this split, counted over all segments
+    constexpr int kStep = SUB * kStepK;
+    const int steps = static_cast<int>((g.k + kStep - 1) / kStep), all = steps * g.segments;
+    const int each = (all + g.splits - 1) / g.splits;
+    const int first = split * each, last = first + each < all ? first + each : all;
+    const int tail = static_cast<int>(g.k % kStep);
 
     Stager<BM, W, A_COLUMN> sa;
     sa.init(wave, lane, p.lda, p.m - m0);
@@ -369,29 +408,58 @@ struct Gemm16 {
     Stager<BN / kHalves, W, B_COLUMN> sb;
     sb.init(wave, lane, p.ldb, p.n - n0);
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    CodeStager<kFromCodes ? BN : kThreads / 2, kThreads, B == kCodesF32> sq;
-    if constexpr (kFromCodes) sq.init(g, n0, p.n, g.k);
-    const auto issue = [&](int64_t step, int slot) {
-      const int s = g.segments > 1 ? static_cast<int>(step / steps) : 0;
-      const int64_t kk = (step - s * steps) * kStepK;
-      const Gemm16Pair& o = g.segments > 1 ? g.pair[s] : p;
-      const uint16_t* a = o.a + (A_COLUMN ? kk * p.lda + m0 : m0 * p.lda + kk);
-      const int64_t b_at = B_COLUMN ? kk * p.ldb + n0 : n0 * p.ldb + kk;
-      const bool partial = tail != 0 && kk + kStepK > g.k;
-      if (partial)
-        sa.issue_tail(a, wave, lane, tail, lds + slot * kStage);
-      else
-        sa.issue(a, wave, lds_at + slot * kStage);
-      if constexpr (kFromCodes) return;
+    CodeStager<kFromCodes ? BN : kThreads / 2, kThreads, B == kCodesF32> sq[SUB];
+    if constexpr (kFromCodes) {
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const uint16_t* b = (kPairB ? g.pair[h].b : o.b) + b_at;
-        const uint32_t at = slot * kStage + kStageA + h * (BN / kHalves) * 128;
+      for (int u = 0; u < SUB; ++u) sq[u].init(g, n0, p.n, g.k);
+    }
+    const auto fetch_codes = [&](int step) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) sq[u].fetch(g, static_cast<int64_t>(step) * kStep + u * kStepK);
+    };
+    const auto write_codes = [&](int slot) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) sq[u].write(lds + slot * kStage + u * kBlock + kStageA, g.offsets != nullptr);
+    };
+    // Where the next step's operands start; a step on costs two additions.
+    const uint16_t *pa, *pb[kHalves];
+    int left;  // steps of the segment still to issue
+    const auto seek = [&](int segment, int step) {
+      const Gemm16Pair& o = g.pair[g.segments > 1 ? segment : q];
+      const int64_t kk = static_cast<int64_t>(step) * kStep;
+      pa = o.a + (A_COLUMN ? kk * p.lda + m0 : m0 * p.lda + kk);
+      const int64_t b_at = B_COLUMN ? kk * p.ldb + n0 : n0 * p.ldb + kk;
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) pb[h] = (kPairB ? g.pair[h].b : o.b) + b_at;
+      left = steps - step;
+    };
+    int segment = first / steps;
+    seek(segment, first - segment * steps);
+    const int64_t next_a = A_COLUMN ? kStepK * p.lda : kStepK, next_b = B_COLUMN ? kStepK * p.ldb : kStepK;
+    const auto issue = [&](int slot) {
+      const bool partial = tail != 0 && left == 1;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const uint32_t at = slot * kStage + u * kBlock;
+        const int k_left = tail - u * kStepK;  // in a partial step: may be none
         if (partial)
-          sb.issue_tail(b, wave, lane, tail, lds + at);
+          sa.issue_tail(pa, wave, lane, k_left, lds + at);
         else
-          sb.issue(b, wave, lds_at + at);
+          sa.issue(pa, wave, lds_at + at);
+        pa += next_a;
+        if constexpr (!kFromCodes) {
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            const uint32_t b_lds = at + kStageA + h * (BN / kHalves) * 128;
+            if (partial)
+              sb.issue_tail(pb[h], wave, lane, k_left, lds + b_lds);
+            else
+              sb.issue(pb[h], wave, lds_at + b_lds);
+            pb[h] += next_b;
+          }
+        }
       }
+      if (--left == 0 && ++segment < g.segments) seek(segment, 0);
     };
 
     f32x4 acc[MT][NT];
@@ -409,30 +477,31 @@ struct Gemm16 {
 
     if constexpr (kFromCodes) {
       if (first < last) {
-        sq.fetch(g, first * kStepK);
-        sq.write(lds + kStageA, g.offsets != nullptr);
-        if (first + 1 < last) sq.fetch(g, (first + 1) * kStepK);
+        fetch_codes(first);
+        write_codes(0);
+        if (first + 1 < last) fetch_codes(first + 1);
       }
     }
-    if (first < last) issue(first, 0);
+    if (first < last) issue(0);
     int slot = 0;
-    for (int64_t step = first; step < last; ++step, slot ^= 1) {
+    for (int step = first; step < last; ++step, slot ^= 1) {
       stage_wait();
       if constexpr (kFromCodes) {  // codes before the direct loads: the compiler's wait for them drains both
-        if (step + 1 < last) sq.write(lds + (slot ^ 1) * kStage + kStageA, g.offsets != nullptr);
+        if (step + 1 < last) write_codes(slot ^ 1);
       }
-      if (step + 1 < last) issue(step + 1, slot ^ 1);
+      if (step + 1 < last) issue(slot ^ 1);
       if constexpr (kFromCodes) {
-        if (step + 2 < last) sq.fetch(g, (step + 2) * kStepK);
+        if (step + 2 < last) fetch_codes(step + 2);
       }
       const uint8_t* stage = lds + slot * kStage;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2 * SUB; ++j) {
         bf16x8 a[MT], b[NT];
+        const uint8_t* block = stage + (j >> 1) * kBlock;
 #pragma unroll
-        for (int c = 0; c < NT; ++c) b[c] = rb(stage + kStageA, b_tile(c), j);
+        for (int c = 0; c < NT; ++c) b[c] = rb(block + kStageA, b_tile(c), j & 1);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) a[i] = ra(stage, wm * MT + i, j);
+        for (int i = 0; i < MT; ++i) a[i] = ra(block, wm * MT + i, j & 1);
         // columns as the MFMA's rows: a lane's four results are four
         // consecutive outputs of one row
 #pragma unroll
@@ -441,10 +510,14 @@ struct Gemm16 {
           for (int c = 0; c < NT; ++c)
             acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[c], a[i], acc[i][c], 0, 0, 0);
       }
+      // The order of a step's LDS reads and products: rows' operands are read
+      // one group of kAhead row tiles ahead of the products that take them
+      // (left alone, the compiler reads each pair just before its products).
+      schedule_step();
     }
 
     const int64_t ldp = partial_ld(p.n), plane = p.m * ldp;
-    float* part = g.partial + split * (kPairB ? 2 : 1) * plane;
+    float* part = g.partial + g.partial_at[q] + split * (kPairB ? 2 : 1) * plane;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int64_t m = m0 + 16 * (wm * MT + i) + (lane & 15);
@@ -476,21 +549,24 @@ __global__ __launch_bounds__(G::kThreads) void gemm16_kernel(Gemm16Args g) {
   G::run(g, lds);
 }
 
-// Adds the splits' partial results, in their order, and finishes them.
+// Adds the splits' partial results, in their order, and finishes them; problem
+// blockIdx.y.
 template <Gemm16Epilogue EPI>
 __global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
-  const Gemm16Pair& p = g.pair[0];
+  const Gemm16Pair& p = g.pair[blockIdx.y];
+  const float* partial = g.partial + g.partial_at[blockIdx.y];
   const int64_t ldp = partial_ld(p.n), plane = p.m * ldp, at = 4 * (blockIdx.x * int64_t{256} + threadIdx.x);
   if (at >= plane) return;
   constexpr int kPlanes = EPI == kSwiglu ? 2 : 1;
   f32x4 v[kPlanes];
 #pragma unroll
   for (int h = 0; h < kPlanes; ++h) {
-    v[h] = *reinterpret_cast<const f32x4*>(g.partial + h * plane + at);
+    v[h] = *reinterpret_cast<const f32x4*>(partial + h * plane + at);
     for (int s = 1; s < g.splits; ++s)
-      v[h] += *reinterpret_cast<const f32x4*>(g.partial + (s * kPlanes + h) * plane + at);
+      v[h] += *reinterpret_cast<const f32x4*>(partial + (s * kPlanes + h) * plane + at);
   }
   const int64_t m = at / ldp, n = at % ldp;
+  if (n >= p.n) return;
   if constexpr (EPI == kStore)
     store_plain(g, p, m, n, v[0]);
   else if constexpr (EPI == kBias)
@@ -499,6 +575,50 @@ __global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
     store_swiglu(g, p, m, n, v[0], v[1]);
   else
     store_swiglu_grad(g, p, m, n, v[0]);
+}
+
+// ---------------------------------------------------------------- host ---
+
+enum Gemm16Tile { kTile64, kTile128, kTile256 };
+struct Gemm16Plan {
+  Gemm16Tile tile;
+  int splits;
+  int64_t partial;  // floats of the splits' partial results
+};
+// The tile and the number of splits for g's products; pair_b: gate and up
+// columns in one product.
+Gemm16Plan gemm16_plan(const Gemm16Args& g, bool pair_b);
+
+template <class G, Gemm16Epilogue EPI>
+hipError_t gemm16_launch(Gemm16Args g, hipStream_t st) {
+  g.tiles = 0;
+  int64_t most = 0, at = 0;
+  for (int q = 0; q < g.problems; ++q) {
+    const Gemm16Pair& p = g.pair[q];
+    g.tiles += ((p.m + G::BM - 1) / G::BM) * ((p.n + G::kColumns - 1) / G::kColumns);
+    const int64_t plane = p.m * partial_ld(p.n);
+    g.partial_at[q] = at;
+    at += plane * g.splits * (EPI == kSwiglu ? 2 : 1);
+    most = most > plane ? most : plane;
+  }
+  g.group_m = 8;
+  if (g.tiles * g.splits >= (int64_t{1} << 31) || most / 1024 >= (int64_t{1} << 31)) return hipErrorInvalidValue;
+  gemm16_kernel<G><<<static_cast<uint32_t>(g.tiles * g.splits), G::kThreads, G::kLds, st>>>(g);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess || g.splits == 1) return e;
+  const dim3 grid(static_cast<uint32_t>((most + 1023) / 1024), static_cast<uint32_t>(g.problems));
+  gemm16_join_kernel<EPI><<<grid, 256, 0, st>>>(g);
+  return hipGetLastError();
+}
+
+// g's products in the plan's shape; g.partial has the plan's room.
+template <bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI>
+hipError_t gemm16(Gemm16Args g, const Gemm16Plan& plan, hipStream_t st) {
+  g.splits = plan.splits;
+  switch (plan.tile) {
+    case kTile64: return gemm16_launch<Gemm16<1, 4, 4, 2, 2, A_COLUMN, B, EPI>, EPI>(g, st);  // 64 x 128
+    case kTile128: return gemm16_launch<Gemm16<2, 2, 4, 4, 1, A_COLUMN, B, EPI>, EPI>(g, st);
+    default: return gemm16_launch<Gemm16<2, 4, 8, 4, 1, A_COLUMN, B, EPI>, EPI>(g, st);
+  }
 }
 
 }  // namespace glm53

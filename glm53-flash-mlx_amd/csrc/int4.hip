@@ -8,14 +8,6 @@ namespace {
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <class G>
-hipError_t launch_tiles(Gemm16Args g, hipStream_t st) {
-  g.tiles = cdiv(g.pair[0].m, G::BM) * cdiv(g.pair[0].n, G::kColumns);
-  g.group_m = 8;
-  gemm16_kernel<G><<<static_cast<uint32_t>(g.tiles * g.splits), G::kThreads, G::kLds, st>>>(g);
-  return hipGetLastError();
-}
-
 // ------------------------------------------------------------- few rows ---
 //
 // Up to 16 rows: the call costs the codes' bytes.  A workgroup makes 16
@@ -262,13 +254,47 @@ hipError_t launch_few_rows(const Int4Args& a, hipStream_t st) {
 
 }  // namespace
 
-size_t int4_space(int64_t rows, int64_t N, int64_t K) { return 0; }
+namespace {
+// The weights as bf16, W = scale q + offset rounded once, [N, K]: a thread
+// takes 32 codes (16 bytes, within one group).
+template <bool F32>
+__global__ __launch_bounds__(256) void int4_expand_kernel(Int4Args a, uint16_t* w) {
+  const int64_t at = blockIdx.x * int64_t{256} + threadIdx.x, pieces = a.K >> 5;
+  const int64_t n = at / pieces, k = (at - n * pieces) << 5;
+  if (n >= a.N) return;
+  const u32x4 codes = *reinterpret_cast<const u32x4*>(a.codes + (at << 4));
+  const int64_t t = n * (a.K >> a.group_log2) + (k >> a.group_log2);
+  const float scale = table_value(a.scales, F32, t);
+  // without offsets: the scale, read again, so that both loads are on their
+  // way before either is waited for
+  const float second = table_value(a.offsets != nullptr ? a.offsets : a.scales, F32, t);
+  const float offset = a.offsets != nullptr ? second : -8.0f * second;
+  u32x4* out = reinterpret_cast<u32x4*>(w + (at << 5));
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const uint32_t even = codes[d] & 0x0F0F0F0Fu, odd = (codes[d] >> 4) & 0x0F0F0F0Fu;
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = fmaf(static_cast<float>((even >> (8 * i)) & 0xFFu), scale, offset);
+      const float y = fmaf(static_cast<float>((odd >> (8 * i)) & 0xFFu), scale, offset);
+      v[i] = f32_to_bf16(x) | static_cast<uint32_t>(f32_to_bf16(y)) << 16;
+    }
+    out[d] = v;
+  }
+}
 
-hipError_t launch_int4(const Int4Args& a, hipStream_t st) {
-  if (a.rows <= kFewRows) return launch_few_rows(a, st);
+// From 17 to this many rows the codes become weights in the tiled product's own
+// stage, tile row by tile row; beyond, in memory once, for the product of bf16
+// weights, whose larger tiles the conversion would hold up (4096 x 4096: 64
+// rows 23 us staged, 32 expanded; 128 rows 35 and 38; 300 rows 66 and 45;
+// 2,048 rows 110 and 81).
+constexpr int64_t kStagedRows = 128;
+
+Gemm16Args product(const Int4Args& a) {
   Gemm16Args g{};
   g.k = a.K;
-  g.problems = g.segments = g.splits = 1;
+  g.problems = g.segments = 1;
   g.pair[0] = {a.x, nullptr, a.y, a.K, a.K, a.N, a.rows, a.N};
   g.codes = a.codes;
   g.scales = a.scales;
@@ -276,8 +302,52 @@ hipError_t launch_int4(const Int4Args& a, hipStream_t st) {
   g.bias = a.bias;
   g.scales_f32 = a.tables_f32;
   g.group_log2 = a.group_log2;
-  if (a.tables_f32) return launch_tiles<Gemm16<2, 2, 4, 4, false, kCodesF32, kBias>>(g, st);
-  return launch_tiles<Gemm16<2, 2, 4, 4, false, kCodes, kBias>>(g, st);
+  return g;
+}
+
+// 64 x 128 tiles; as many parts of the contraction as fill the chip once.
+Gemm16Plan staged_plan(const Int4Args& a) {
+  const int64_t tiles = cdiv(a.rows, 64) * cdiv(a.N, 128), steps = cdiv(a.K, 128);
+  int splits = 1;
+  while (splits < 16 && tiles * splits < 192 && steps >= 4 * splits) splits *= 2;
+  return {kTile64, splits, splits > 1 ? splits * a.rows * partial_ld(a.N) : 0};
+}
+
+size_t weight_bytes(int64_t N, int64_t K) { return (2 * static_cast<size_t>(N) * static_cast<size_t>(K) + 255) & ~size_t{255}; }
+
+}  // namespace
+
+size_t int4_space(int64_t rows, int64_t N, int64_t K) {
+  if (rows <= kFewRows) return 0;
+  Int4Args a{};
+  a.rows = rows;
+  a.N = N;
+  a.K = K;
+  if (rows <= kStagedRows) return sizeof(float) * static_cast<size_t>(staged_plan(a).partial);
+  return weight_bytes(N, K) + sizeof(float) * static_cast<size_t>(gemm16_plan(product(a), false).partial);
+}
+
+hipError_t launch_int4(const Int4Args& a, hipStream_t st) {
+  if (a.rows <= kFewRows) return launch_few_rows(a, st);
+  Gemm16Args g = product(a);
+  if (a.rows <= kStagedRows) {
+    const Gemm16Plan plan = staged_plan(a);
+    g.splits = plan.splits;
+    g.partial = static_cast<float*>(a.space);
+    if (a.tables_f32) return gemm16_launch<Gemm16<1, 4, 4, 2, 2, false, kCodesF32, kBias>, kBias>(g, st);
+    return gemm16_launch<Gemm16<1, 4, 4, 2, 2, false, kCodes, kBias>, kBias>(g, st);
+  }
+  uint16_t* w = static_cast<uint16_t*>(a.space);
+  g.pair[0].b = w;
+  g.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.space) + weight_bytes(a.N, a.K));
+  if (cdiv(a.N * (a.K >> 5), 256) >= (int64_t{1} << 31)) return hipErrorInvalidValue;
+  const uint32_t blocks = static_cast<uint32_t>(cdiv(a.N * (a.K >> 5), 256));
+  if (a.tables_f32)
+    int4_expand_kernel<true><<<blocks, 256, 0, st>>>(a, w);
+  else
+    int4_expand_kernel<false><<<blocks, 256, 0, st>>>(a, w);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  return gemm16<false, kRow, kBias>(g, gemm16_plan(g, false), st);
 }
 
 }  // namespace glm53
