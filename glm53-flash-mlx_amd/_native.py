@@ -132,6 +132,7 @@ class GatedMLP(ctypes.Structure):
         ("y", P),
         ("gate", P),
         ("up", P),
+        ("h", P),
         ("d_y", P),
         ("d_x", P),
         ("d_gate_weight", P),
@@ -274,23 +275,41 @@ def stream_handle(device: torch.device | None = None) -> int:
     return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
-def run(device: torch.device, fn, *args) -> None:
-    """`fn(*args, stream)` on torch's current stream of `device`, which is made
-    the current device for the call where it is not."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, stream_handle(device)))
-    else:
-        with torch.cuda.device(device):
-            check(fn(*args, stream_handle(device)))
+# a private name, ~0.5 us a call below torch.cuda.current_device
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def require_same_device(first: torch.Tensor, *others: torch.Tensor | None) -> None:
-    """One ROCm device for every tensor given (None: absent)."""
-    require_device(first)
+def run(index: int, fn, *args) -> None:
+    """`fn(*args, stream)` on torch's current stream of device `index`, which
+    is made the current device for the call where it is not."""
+    if index == _current_device():
+        status = fn(*args, torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index))
+        if status:
+            check(status)
+        return
+    with torch.cuda.device(index):
+        check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+
+
+def same_device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The index of the ROCm device that every tensor given lies on (None:
+    absent); an error where there is none."""
+    index = first.get_device()
+    if index < 0:
+        require_device(first)
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             require_device(t)
             raise ValueError(f"tensors on {first.device} and {t.device}: one device is needed")
+    return index
+
+
+def operand(t: torch.Tensor) -> torch.Tensor:
+    """`t`, or a contiguous copy at a 16-byte aligned address where it is not
+    both."""
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
 
 
 def require_device(*tensors: torch.Tensor) -> None:

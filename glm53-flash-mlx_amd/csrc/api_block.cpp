@@ -138,15 +138,17 @@ int gated_args(const glm53_gated_mlp_desc* d, GatedArgs& a) {
   a.y = static_cast<uint16_t*>(d->y);
   a.gate = d->gate;
   a.up = d->up;
+  a.h = static_cast<uint16_t*>(d->h);
   a.dy = static_cast<const uint16_t*>(d->d_y);
   a.dx = static_cast<uint16_t*>(d->d_x);
   a.d_wg = static_cast<uint16_t*>(d->d_gate_weight);
   a.d_wu = static_cast<uint16_t*>(d->d_up_weight);
   a.d_wd = static_cast<uint16_t*>(d->d_down_weight);
   a.space = d->workspace;
-  const void* every[] = {a.x, a.wg, a.wu, a.wd, a.y, a.gate, a.up, a.dy, a.dx, a.d_wg, a.d_wu, a.d_wd};
+  const void* every[] = {a.x, a.wg, a.wu, a.wd, a.y, a.gate, a.up, a.h, a.dy, a.dx, a.d_wg, a.d_wu, a.d_wd};
   for (const void* p : every) CHECK_ARG(aligned(p, 16), "gated MLP tensors must be 16-byte aligned");
-  CHECK_ARG((a.gate == nullptr) == (a.up == nullptr), "gate and up are kept together");
+  CHECK_ARG((a.gate == nullptr) == (a.up == nullptr) && (a.gate == nullptr) == (a.h == nullptr),
+            "gate, up and h are kept together");
   return GLM53_OK;
 }
 

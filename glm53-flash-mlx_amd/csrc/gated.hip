@@ -2,9 +2,9 @@
 // Wd^T, and its gradients, as products of gemm16.h: gate and up projections
 // with the activation and the product as one kernel's epilogue, the down
 // projection, and backward
-//   dh = dy Wd, in whose epilogue dG, dU and h are made,
+//   dh = dy Wd, in whose epilogue dG and dU are made,
 //   dx = dG Wg + dU Wu (one contraction over both),
-//   dWg = dG^T x, dWu = dU^T x, dWd = dy^T h (one launch).
+//   dWg = dG^T x, dWu = dU^T x, dWd = dy^T h.
 // Operands of a product are bf16 and its sums FP32: h, dG and dU are rounded
 // to bf16 once, as MFMA operands, everything before them is FP32.
 #include <algorithm>
@@ -105,8 +105,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_up_kernel(GatedArgs a
     a.gate[at] = gate;
     a.up[at] = up;
   }
-  const float c = clamp_gate(gate, a.limit);
-  h[at] = c * sigmoid_f32(c) * clamp_up(up, a.limit);
+  const float c = clamp_gate(gate, a.limit), v = c * sigmoid_f32(c) * clamp_up(up, a.limit);
+  h[at] = v;
+  if (a.h != nullptr) a.h[at] = f32_to_bf16(v);
 }
 
 __global__ __launch_bounds__(64 * kFewWaves) void few_down_kernel(GatedArgs a, const float* h) {
@@ -138,8 +139,8 @@ Gemm16Args product(int64_t k) {
   return g;
 }
 
-// The workspace: h, and backward dG and dU (bf16 [rows, inter] each), then the
-// partial results of one product at a time.
+// The workspace: forward h where it is not kept, backward dG and dU (bf16
+// [rows, inter] each); then the partial results of one product at a time.
 struct Space {
   uint16_t *h, *dg, *du;
   float* partial;
@@ -148,12 +149,14 @@ Space carve(const GatedArgs& a, bool backward) {
   uint8_t* p = static_cast<uint8_t*>(a.space);
   const size_t plane = round_up(2 * static_cast<size_t>(a.rows) * static_cast<size_t>(a.inter));
   Space s{};
-  s.h = reinterpret_cast<uint16_t*>(p);
+  s.h = a.h;
   if (backward) {
-    s.dg = reinterpret_cast<uint16_t*>(p + plane);
-    s.du = reinterpret_cast<uint16_t*>(p + 2 * plane);
+    s.dg = reinterpret_cast<uint16_t*>(p);
+    s.du = reinterpret_cast<uint16_t*>(p + plane);
+  } else if (s.h == nullptr) {
+    s.h = reinterpret_cast<uint16_t*>(p);
   }
-  s.partial = reinterpret_cast<float*>(p + (backward ? 3 : 1) * plane);
+  s.partial = reinterpret_cast<float*>(p + (backward ? 2 : 1) * plane);
   return s;
 }
 
@@ -182,7 +185,6 @@ Gemm16Args hidden_grad(const GatedArgs& a, const Space& s) {
   g.up = a.up;
   g.d_gate = s.dg;
   g.d_up = s.du;
-  g.h = a.d_wd != nullptr ? s.h : nullptr;
   g.partial = s.partial;
   return g;
 }
@@ -194,13 +196,14 @@ Gemm16Args input_grad(const GatedArgs& a, const Space& s) {
   g.partial = s.partial;
   return g;
 }
-// Those weights' gradients that are wanted (`every`: all, for their room).
-Gemm16Args weight_grads(const GatedArgs& a, const Space& s, bool every) {
+// Those of the weights' gradients, dWg, dWu and dWd, that `which` (bits 1, 2
+// and 4) names.
+Gemm16Args weight_grads(const GatedArgs& a, const Space& s, int which) {
   Gemm16Args g = product(a.rows);
   g.problems = 0;
-  if (every || a.d_wg) g.pair[g.problems++] = pair(s.dg, a.inter, a.x, a.hidden, a.d_wg, a.inter, a.hidden);
-  if (every || a.d_wu) g.pair[g.problems++] = pair(s.du, a.inter, a.x, a.hidden, a.d_wu, a.inter, a.hidden);
-  if (every || a.d_wd) g.pair[g.problems++] = pair(a.dy, a.hidden, s.h, a.inter, a.d_wd, a.hidden, a.inter);
+  if (which & 1) g.pair[g.problems++] = pair(s.dg, a.inter, a.x, a.hidden, a.d_wg, a.inter, a.hidden);
+  if (which & 2) g.pair[g.problems++] = pair(s.du, a.inter, a.x, a.hidden, a.d_wu, a.inter, a.hidden);
+  if (which & 4) g.pair[g.problems++] = pair(a.dy, a.hidden, s.h, a.inter, a.d_wd, a.hidden, a.inter);
   g.partial = s.partial;
   return g;
 }
@@ -217,14 +220,10 @@ size_t gated_space(int64_t rows, int64_t hidden, int64_t inter, bool backward) {
   a.inter = inter;
   const Space s{};
   if (backward) {
-    int64_t partial = most({gemm16_plan(hidden_grad(a, s), false).partial,
-                            gemm16_plan(input_grad(a, s), false).partial});
-    for (int n = 1; n <= 3; ++n) {  // any of the weights' gradients may not be wanted
-      Gemm16Args w = weight_grads(a, s, true);
-      w.problems = n;
-      partial = most({partial, gemm16_plan(w, false).partial});
-    }
-    return 3 * round_up(2 * values) + sizeof(float) * static_cast<size_t>(partial);
+    int64_t partial = most({gemm16_plan(hidden_grad(a, s), false).partial, gemm16_plan(input_grad(a, s), false).partial});
+    for (int which : {1, 3, 7})  // one, two or all three of the products, which are of one size
+      partial = most({partial, gemm16_plan(weight_grads(a, s, which), false).partial});
+    return 2 * round_up(2 * values) + sizeof(float) * static_cast<size_t>(partial);
   }
   if (rows <= kFewRows) return round_up(4 * values);
   const int64_t partial = most({gemm16_plan(gate_up(a, s), true).partial, gemm16_plan(down(a, s), false).partial});
@@ -241,15 +240,29 @@ hipError_t launch_gated(const GatedArgs& a, hipStream_t st) {
 
 hipError_t launch_gated_backward(const GatedArgs& a, hipStream_t st) {
   const Space s = carve(a, true);
-  const Gemm16Args g = hidden_grad(a, s);
-  if (hipError_t e = gemm16<false, kColumn, kSwigluGrad>(g, gemm16_plan(g, false), st); e != hipSuccess) return e;
+  const auto weights = [&](int which) {
+    const Gemm16Args g = weight_grads(a, s, which);
+    return g.problems == 0 ? hipSuccess : gemm16<true, kColumn, kStore>(g, gemm16_plan(g, false), st);
+  };
+  const int pair = (a.d_wg ? 1 : 0) | (a.d_wu ? 2 : 0), down = a.d_wd ? 4 : 0;
+  if (a.dx != nullptr || pair != 0) {
+    const Gemm16Args g = hidden_grad(a, s);
+    if (hipError_t e = gemm16<false, kColumn, kSwigluGrad>(g, gemm16_plan(g, false), st); e != hipSuccess) return e;
+  }
   if (a.dx != nullptr) {
     const Gemm16Args x = input_grad(a, s);
     if (hipError_t e = gemm16<false, kColumn, kStore>(x, gemm16_plan(x, false), st); e != hipSuccess) return e;
   }
-  const Gemm16Args w = weight_grads(a, s, false);
-  if (w.problems == 0) return hipSuccess;
-  return gemm16<true, kColumn, kStore>(w, gemm16_plan(w, false), st);
+  // The weights' gradients in one launch, or the down projection's apart, where
+  // the numbers of tiles fill the chip's rounds better: 8,192 rows, 4096 x 2048
+  // (256 and 128 large tiles): 420 us in one launch, 384 in two.
+  if (pair != 0 && down != 0 &&
+      gemm16_plan(weight_grads(a, s, pair | down), false).us >
+          gemm16_plan(weight_grads(a, s, pair), false).us + gemm16_plan(weight_grads(a, s, down), false).us) {
+    if (hipError_t e = weights(pair); e != hipSuccess) return e;
+    return weights(down);
+  }
+  return weights(pair | down);
 }
 
 }  // namespace glm53

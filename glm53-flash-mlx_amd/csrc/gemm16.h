@@ -45,13 +45,12 @@ struct Gemm16Args {
   int group_m;     // tile rows that one XCD's neighbouring workgroups share
   // SwiGLU: pair[0].b gate and pair[1].b up rows, out = h; gate/up (f32
   // [m, n]) null or what the gradient needs.  Its gradient (out unused): reads
-  // gate and up, writes d_gate, d_up and h.
+  // gate and up, writes d_gate and d_up.
   float limit;
   float* gate;
   float* up;
   uint16_t* d_gate;
   uint16_t* d_up;
-  uint16_t* h;
   // 4-bit b: codes [n, k / 2], scales and offsets [n, k / group], bias [n]
   const uint8_t* codes;
   const void* scales;
@@ -125,25 +124,20 @@ __device__ __forceinline__ void store_swiglu(const Gemm16Args& g, const Gemm16Pa
   *reinterpret_cast<u32x2*>(p.out + m * p.ldo + n) = pack_bf16x4(h);
 }
 
-// With dh: dU = dh silu(g') [|u| <= L], dG = dh u' silu'(g') [g <= L], and h
-// again for the down projection's gradient.
+// With dh: dU = dh silu(g') [|u| <= L], dG = dh u' silu'(g') [g <= L].
 __device__ __forceinline__ void store_swiglu_grad(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n,
-                                                  f32x4 dh) {
+                                                  f32x4 dh, f32x4 gate, f32x4 up) {
   const int64_t at = m * p.n + n;
-  const f32x4 gate = *reinterpret_cast<const f32x4*>(g.gate + at);
-  const f32x4 up = *reinterpret_cast<const f32x4*>(g.up + at);
-  f32x4 dg, du, h;
+  f32x4 dg, du;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float c = clamp_gate(gate[i], g.limit), u = clamp_up(up[i], g.limit);
-    const float s = sigmoid_f32(c), silu = c * s;
-    h[i] = silu * u;
-    du[i] = fabsf(up[i]) > g.limit ? 0.0f : dh[i] * silu;
+    const float s = sigmoid_f32(c);
+    du[i] = fabsf(up[i]) > g.limit ? 0.0f : dh[i] * (c * s);
     dg[i] = gate[i] > g.limit ? 0.0f : dh[i] * u * (s * (1.0f + c * (1.0f - s)));
   }
   *reinterpret_cast<u32x2*>(g.d_gate + at) = pack_bf16x4(dg);
   *reinterpret_cast<u32x2*>(g.d_up + at) = pack_bf16x4(du);
-  if (g.h != nullptr) *reinterpret_cast<u32x2*>(g.h + at) = pack_bf16x4(h);
 }
 
 // ------------------------------------------------------------- staging ---
@@ -518,13 +512,43 @@ struct Gemm16 {
 
     const int64_t ldp = partial_ld(p.n), plane = p.m * ldp;
     float* part = g.partial + g.partial_at[q] + split * (kPairB ? 2 : 1) * plane;
+    constexpr int kOut = kPairB ? NT / 2 : NT;  // column tiles of outputs
+    const auto row = [&](int i) { return m0 + 16 * (wm * MT + i) + (lane & 15); };
+    const auto col = [&](int c) { return n0 + 16 * (wn * kOut + c) + 4 * (lane >> 4); };
+    if constexpr (EPI == kSwigluGrad) {
+      if (g.splits == 1) {
+        // G and U of a row of tiles come while the row before is finished;
+        // without a branch around the loads (past an edge they repeat it),
+        // which would have each wait for the one before.
+        f32x4 gate[2][NT], up[2][NT];
+        const auto load = [&](int i) {
+          const int64_t m = row(i) < p.m ? row(i) : p.m - 1;
+#pragma unroll
+          for (int c = 0; c < NT; ++c) {
+            const int64_t at = m * p.n + (col(c) < p.n ? col(c) : p.n - 4);
+            gate[i & 1][c] = *reinterpret_cast<const f32x4*>(g.gate + at);
+            up[i & 1][c] = *reinterpret_cast<const f32x4*>(g.up + at);
+          }
+        };
+        load(0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          if (i + 1 < MT) load(i + 1);
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+            if (row(i) < p.m && col(c) < p.n)
+              store_swiglu_grad(g, p, row(i), col(c), acc[i][c], gate[i & 1][c], up[i & 1][c]);
+        }
+        return;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const int64_t m = m0 + 16 * (wm * MT + i) + (lane & 15);
+      const int64_t m = row(i);
       if (m >= p.m) continue;
 #pragma unroll
-      for (int c = 0; c < (kPairB ? NT / 2 : NT); ++c) {
-        const int64_t n = n0 + 16 * (wn * (kPairB ? NT / 2 : NT) + c) + 4 * (lane >> 4);
+      for (int c = 0; c < kOut; ++c) {
+        const int64_t n = col(c);
         if (n >= p.n) continue;
         if (g.splits > 1) {
           *reinterpret_cast<f32x4*>(part + m * ldp + n) = acc[i][c];
@@ -535,8 +559,6 @@ struct Gemm16 {
           store_bias(g, p, m, n, acc[i][c]);
         } else if constexpr (EPI == kSwiglu) {
           store_swiglu(g, p, m, n, acc[i][c], acc[i][c + NT / 2]);
-        } else {
-          store_swiglu_grad(g, p, m, n, acc[i][c]);
         }
       }
     }
@@ -574,7 +596,8 @@ __global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
   else if constexpr (EPI == kSwiglu)
     store_swiglu(g, p, m, n, v[0], v[1]);
   else
-    store_swiglu_grad(g, p, m, n, v[0]);
+    store_swiglu_grad(g, p, m, n, v[0], *reinterpret_cast<const f32x4*>(g.gate + m * p.n + n),
+                      *reinterpret_cast<const f32x4*>(g.up + m * p.n + n));
 }
 
 // ---------------------------------------------------------------- host ---
@@ -584,6 +607,7 @@ struct Gemm16Plan {
   Gemm16Tile tile;
   int splits;
   int64_t partial;  // floats of the splits' partial results
+  float us;         // expected time
 };
 // The tile and the number of splits for g's products; pair_b: gate and up
 // columns in one product.
@@ -592,6 +616,7 @@ Gemm16Plan gemm16_plan(const Gemm16Args& g, bool pair_b);
 template <class G, Gemm16Epilogue EPI>
 hipError_t gemm16_launch(Gemm16Args g, hipStream_t st) {
   g.tiles = 0;
+  g.group_m = 8;
   int64_t most = 0, at = 0;
   for (int q = 0; q < g.problems; ++q) {
     const Gemm16Pair& p = g.pair[q];
@@ -601,7 +626,6 @@ hipError_t gemm16_launch(Gemm16Args g, hipStream_t st) {
     at += plane * g.splits * (EPI == kSwiglu ? 2 : 1);
     most = most > plane ? most : plane;
   }
-  g.group_m = 8;
   if (g.tiles * g.splits >= (int64_t{1} << 31) || most / 1024 >= (int64_t{1} << 31)) return hipErrorInvalidValue;
   gemm16_kernel<G><<<static_cast<uint32_t>(g.tiles * g.splits), G::kThreads, G::kLds, st>>>(g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || g.splits == 1) return e;

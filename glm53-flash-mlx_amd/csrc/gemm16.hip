@@ -2,6 +2,27 @@
 #include "gemm16.h"
 
 namespace glm53 {
+namespace {
+
+struct Shape {
+  Gemm16Tile tile;
+  int rows, cols, step;
+  int64_t slots;
+  float step_us, step_full_us, fixed_us;
+};
+constexpr Shape kShapes[] = {{kTile64, 64, 128, 128, 256, 1.3f, 1.3f, 4.0f},
+                             {kTile128, 128, 128, 64, 512, 0.95f, 1.05f, 6.0f},
+                             {kTile256, 256, 256, 64, 256, 1.6f, 1.6f, 12.0f}};
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+int64_t tiles_of(const Gemm16Args& g, const Shape& s, int planes) {
+  int64_t tiles = 0;
+  for (int q = 0; q < g.problems; ++q) tiles += cdiv(g.pair[q].m, s.rows) * cdiv(g.pair[q].n, s.cols / planes);
+  return tiles;
+}
+
+}  // namespace
 
 // By the time that each shape is expected to take, from what the shapes
 // measured over 16 to 8,192 rows, 1,000 to 8,192 columns and contractions of
@@ -17,35 +38,18 @@ namespace glm53 {
 // 300 x 4096 x 4096 in 128 x 128 tiles: 66 us whole, 44 in 2 parts, 35 in 4;
 // 2,048 rows: 71 whole, 91 in 2; 4,096 rows: 135, and 113 in 256 x 256 tiles.
 Gemm16Plan gemm16_plan(const Gemm16Args& g, bool pair_b) {
-  struct Shape {
-    Gemm16Tile tile;
-    int rows, cols, step;
-    int64_t slots;
-    float step_us, step_full_us, fixed_us;
-  };
-  static constexpr Shape kShapes[] = {{kTile64, 64, 128, 128, 256, 1.3f, 1.3f, 4.0f},
-                                      {kTile128, 128, 128, 64, 512, 0.95f, 1.05f, 6.0f},
-                                      {kTile256, 256, 256, 64, 256, 1.6f, 1.6f, 12.0f}};
   const int planes = pair_b ? 2 : 1;
   int64_t outputs = 0;
   for (int q = 0; q < g.problems; ++q) outputs += g.pair[q].m * partial_ld(g.pair[q].n) * planes;
-  Gemm16Plan best{kTile128, 1, 0};
-  float best_us = 0.0f;
+  Gemm16Plan best{};
   for (const Shape& s : kShapes) {
-    int64_t tiles = 0;
-    for (int q = 0; q < g.problems; ++q)
-      tiles += ((g.pair[q].m + s.rows - 1) / s.rows) * ((g.pair[q].n + s.cols / planes - 1) / (s.cols / planes));
-    const int64_t steps = (g.k + s.step - 1) / s.step * g.segments;
+    const int64_t tiles = tiles_of(g, s, planes), steps = cdiv(g.k, s.step) * g.segments;
     for (int splits = 1; splits <= 16 && (splits == 1 || steps >= 2 * splits); splits *= 2) {
-      const int64_t units = tiles * splits, rounds = (units + s.slots - 1) / s.slots;
-      const float step_us = units > 256 ? s.step_full_us : s.step_us;
-      float us = static_cast<float>(rounds) * (static_cast<float>((steps + splits - 1) / splits) * step_us);
+      const int64_t units = tiles * splits, rounds = cdiv(units, s.slots);
+      float us = static_cast<float>(rounds * cdiv(steps, splits)) * (units > 256 ? s.step_full_us : s.step_us);
       us += s.tile == kTile256 ? static_cast<float>(rounds) * s.fixed_us : s.fixed_us;
       if (splits > 1) us += 3.0f + 8.0f * static_cast<float>(outputs) * static_cast<float>(splits) / 6.5e6f;
-      if (best_us == 0.0f || us < best_us) {
-        best_us = us;
-        best = {s.tile, splits, splits > 1 ? outputs * splits : 0};
-      }
+      if (best.splits == 0 || us < best.us) best = {s.tile, splits, splits > 1 ? outputs * splits : 0, us};
     }
   }
   return best;

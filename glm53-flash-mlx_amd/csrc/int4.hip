@@ -310,7 +310,7 @@ Gemm16Plan staged_plan(const Int4Args& a) {
   const int64_t tiles = cdiv(a.rows, 64) * cdiv(a.N, 128), steps = cdiv(a.K, 128);
   int splits = 1;
   while (splits < 16 && tiles * splits < 192 && steps >= 4 * splits) splits *= 2;
-  return {kTile64, splits, splits > 1 ? splits * a.rows * partial_ld(a.N) : 0};
+  return {kTile64, splits, splits > 1 ? splits * a.rows * partial_ld(a.N) : 0, 0.0f};
 }
 
 size_t weight_bytes(int64_t N, int64_t K) { return (2 * static_cast<size_t>(N) * static_cast<size_t>(K) + 255) & ~size_t{255}; }

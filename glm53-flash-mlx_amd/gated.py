@@ -6,8 +6,8 @@ weights (patch.py:114-129 of the reference).
 Gate and up projections, activation and product are one kernel; sums, G, U
 and the activation are FP32, h and y are rounded to bf16 once each (the FP8
 path keeps the reference's rounding after every step instead).  A call that
-may be differentiated keeps G and U in FP32, 8 bytes an intermediate value,
-for the backward pass.
+may be differentiated keeps G and U in FP32 and h, 10 bytes an intermediate
+value, for the backward pass.
 """
 
 from __future__ import annotations
@@ -29,16 +29,17 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
     [intermediate, hidden], down_weight bfloat16 [hidden, intermediate], both
     widths multiples of 8; limit None: no clamp.  Differentiable (first order)
     in all four tensors."""
-    N.require_same_device(x, gate_weight, up_weight, down_weight)
+    N.same_device(x, gate_weight, up_weight, down_weight)
     weights = (gate_weight, up_weight, down_weight)
-    for t in (x, *weights):
-        if t.dtype != torch.bfloat16:
-            raise ValueError(f"the gated MLP takes bfloat16 tensors, got {t.dtype}")
-    if any(w.dim() != 2 for w in weights) or x.dim() < 1:
+    x_shape, shape = x.shape, gate_weight.shape
+    bf16 = torch.bfloat16
+    if x.dtype is not bf16 or gate_weight.dtype is not bf16 or up_weight.dtype is not bf16 or down_weight.dtype is not bf16:
+        raise ValueError(f"the gated MLP takes bfloat16 tensors, got {[t.dtype for t in (x, *weights)]}")
+    if len(shape) != 2 or not x_shape:
         raise ValueError("the gated MLP takes x [..., hidden] and 2-D weights")
-    inter, hidden = gate_weight.shape
-    if up_weight.shape != (inter, hidden) or down_weight.shape != (hidden, inter) or x.shape[-1] != hidden:
-        raise ValueError(f"shapes do not match: x {tuple(x.shape)}, gate {tuple(gate_weight.shape)}, "
+    inter, hidden = shape
+    if up_weight.shape != shape or down_weight.shape != (hidden, inter) or x_shape[-1] != hidden:
+        raise ValueError(f"shapes do not match: x {tuple(x_shape)}, gate {tuple(shape)}, "
                          f"up {tuple(up_weight.shape)}, down {tuple(down_weight.shape)}")
     if hidden % 8 or inter % 8 or hidden == 0 or inter == 0:
         raise ValueError(f"hidden {hidden} and intermediate {inter} must be multiples of 8")
@@ -53,66 +54,60 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
     return torch.ops.glm53.gated_mlp(x, *weights, limit, keep)[0]
 
 
-def _ready(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned."""
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
 def native_gated_mlp(x, gate_weight, up_weight, down_weight, limit: float, keep: bool):
-    """The native call behind glm53::gated_mlp: y, and G and U where kept
-    (empty tensors otherwise)."""
-    x, gate_weight, up_weight, down_weight = _ready(x), _ready(gate_weight), _ready(up_weight), _ready(down_weight)
+    """The native call behind glm53::gated_mlp: y, and G, U and h where kept."""
+    x, gate_weight, up_weight, down_weight = map(N.operand, (x, gate_weight, up_weight, down_weight))
     inter, hidden = gate_weight.shape
     rows = x.numel() // hidden
     y = torch.empty_like(x)
-    gate = torch.empty((rows, inter) if keep else 0, dtype=torch.float32, device=x.device)
-    up = torch.empty_like(gate)
+    gate = up = h = p_gate = p_up = p_h = None
+    if keep:
+        gate = x.new_empty((rows, inter), dtype=torch.float32)
+        up = torch.empty_like(gate)
+        h = x.new_empty((rows, inter))
+        p_gate, p_up, p_h = gate.data_ptr(), up.data_ptr(), h.data_ptr()
     if rows:
         lib = N.lib()
         ws_bytes = lib.glm53_gated_mlp_workspace_bytes(rows, hidden, inter)
         ws = N.workspace(ws_bytes, x.device)
         d = N.GatedMLP(rows, hidden, inter, x.data_ptr(), gate_weight.data_ptr(), up_weight.data_ptr(),
-                       down_weight.data_ptr(), y.data_ptr(), gate.data_ptr() if keep else None,
-                       up.data_ptr() if keep else None, None, None, None, None, None, ws.data_ptr(), ws_bytes,
-                       limit)
-        N.run(x.device, lib.glm53_gated_mlp, ctypes.byref(d))
-    return y, gate, up
+                       down_weight.data_ptr(), y.data_ptr(), p_gate, p_up, p_h, None, None, None, None, None, ws.data_ptr(),
+                       ws_bytes, limit)
+        N.run(x.get_device(), lib.glm53_gated_mlp, ctypes.byref(d))
+    return y, gate, up, h
 
 
-def native_gated_mlp_backward(x, gate_weight, up_weight, down_weight, gate, up, d_y, limit: float, wanted: list[bool]):
+def native_gated_mlp_backward(x, gate_weight, up_weight, down_weight, gate, up, h, d_y, limit: float, wanted: list[bool]):
     """The native call behind glm53::gated_mlp_backward: the gradients of x
-    and the weights that are `wanted`, empty tensors in place of the others."""
-    inputs = [_ready(t) for t in (x, gate_weight, up_weight, down_weight)]
-    d_y = _ready(d_y)
+    and the weights that are `wanted`, None in place of the others."""
+    inputs = [N.operand(t) for t in (x, gate_weight, up_weight, down_weight)]
+    d_y = N.operand(d_y)
     inter, hidden = gate_weight.shape
     rows = x.numel() // hidden
     grads = [torch.empty_like(t) if w else None for t, w in zip(inputs, wanted)]
     if rows == 0:
-        return [x.new_empty(0) if g is None else g.zero_() for g in grads]
+        return [None if g is None else g.zero_() for g in grads]
     lib = N.lib()
     ws_bytes = lib.glm53_gated_mlp_backward_workspace_bytes(rows, hidden, inter)
     ws = N.workspace(ws_bytes, x.device)
     d = N.GatedMLP(rows, hidden, inter, *(t.data_ptr() for t in inputs), None, gate.data_ptr(), up.data_ptr(),
-                   d_y.data_ptr(), *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), ws_bytes, limit)
-    N.run(x.device, lib.glm53_gated_mlp_backward, ctypes.byref(d))
-    return [x.new_empty(0) if g is None else g for g in grads]
+                   h.data_ptr(), d_y.data_ptr(), *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), ws_bytes, limit)
+    N.run(x.get_device(), lib.glm53_gated_mlp_backward, ctypes.byref(d))
+    return grads
 
 
 class _GatedMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_weight, up_weight, down_weight, limit):
-        y, gate, up = native_gated_mlp(x, gate_weight, up_weight, down_weight, limit, True)
-        ctx.save_for_backward(x, gate_weight, up_weight, down_weight, gate, up)
+        y, *kept = native_gated_mlp(x, gate_weight, up_weight, down_weight, limit, True)
+        ctx.save_for_backward(x, gate_weight, up_weight, down_weight, *kept)
         ctx.limit = limit
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_y):
-        wanted = [bool(w) for w in ctx.needs_input_grad[:4]]
-        grads = native_gated_mlp_backward(*ctx.saved_tensors, d_y, ctx.limit, wanted)
-        return (*(g if w else None for g, w in zip(grads, wanted)), None)
+        return (*native_gated_mlp_backward(*ctx.saved_tensors, d_y, ctx.limit, ctx.needs_input_grad), None)
 
 
 class GatedMLP(torch.nn.Module):

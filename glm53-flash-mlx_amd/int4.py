@@ -19,6 +19,7 @@ from . import _native as N
 from . import ops as _ops
 
 GROUP_SIZES = (32, 64, 128)
+FEW_ROWS = 16  # up to here the codes are multiplied as they are, and no workspace is taken
 
 
 def int4_linear(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor | None = None,
@@ -27,54 +28,51 @@ def int4_linear(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, off
 
     x bfloat16 [..., in]; weight uint8 [out, in / 2]; scales and offsets [out,
     in / g], bias [out], all bfloat16 or all float32; offsets None: -8 scales."""
-    N.require_same_device(x, weight, scales, offsets, bias)
-    if x.dtype != torch.bfloat16:
+    N.same_device(x, weight, scales, offsets, bias)
+    x_shape, w_shape, s_shape, table = x.shape, weight.shape, scales.shape, scales.dtype
+    if x.dtype is not torch.bfloat16:
         raise ValueError(f"activations must be bfloat16, got {x.dtype}")
-    if weight.dtype != torch.uint8 or weight.dim() != 2:
-        raise ValueError(f"expected 2-D uint8 codes, got {tuple(weight.shape)} {weight.dtype}")
-    out_features, in_features = weight.shape[0], 2 * weight.shape[1]
-    if x.dim() < 1 or x.shape[-1] != in_features:
-        raise ValueError(f"input {tuple(x.shape)} does not end in the weight's width {in_features}")
-    if scales.dtype not in (torch.bfloat16, torch.float32) or scales.dim() != 2 or scales.shape[0] != out_features:
-        raise ValueError(f"scales must be bfloat16 or float32 [{out_features}, groups], got {tuple(scales.shape)} "
-                         f"{scales.dtype}")
-    groups = scales.shape[1]
+    if weight.dtype is not torch.uint8 or len(w_shape) != 2:
+        raise ValueError(f"expected 2-D uint8 codes, got {tuple(w_shape)} {weight.dtype}")
+    out_features, in_features = w_shape[0], 2 * w_shape[1]
+    if not x_shape or x_shape[-1] != in_features:
+        raise ValueError(f"input {tuple(x_shape)} does not end in the weight's width {in_features}")
+    if (table is not torch.bfloat16 and table is not torch.float32) or len(s_shape) != 2 or s_shape[0] != out_features:
+        raise ValueError(f"scales must be bfloat16 or float32 [{out_features}, groups], got {tuple(s_shape)} {table}")
+    groups = s_shape[1]
     if out_features == 0 or groups == 0 or in_features not in (32 * groups, 64 * groups, 128 * groups):
         raise ValueError(f"{groups} groups over {in_features} columns: groups hold {GROUP_SIZES} columns")
-    if offsets is not None and (offsets.shape != scales.shape or offsets.dtype != scales.dtype):
+    if offsets is not None and (offsets.shape != s_shape or offsets.dtype is not table):
         raise ValueError(f"offsets must match scales, got {tuple(offsets.shape)} {offsets.dtype}")
-    if bias is not None and (bias.shape != (out_features,) or bias.dtype != scales.dtype):
-        raise ValueError(f"bias must be {scales.dtype} [{out_features}], got {tuple(bias.shape)} {bias.dtype}")
+    if bias is not None and (bias.shape != (out_features,) or bias.dtype is not table):
+        raise ValueError(f"bias must be {table} [{out_features}], got {tuple(bias.shape)} {bias.dtype}")
     if _ops.direct(x, weight, scales, offsets, bias):
         return native_int4_linear(x, weight, scales, offsets, bias)
     return torch.ops.glm53.int4_linear(x, weight, scales, offsets, bias)
 
 
-def _ready(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned."""
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
 def native_int4_linear(x, weight, scales, offsets, bias):
     """The native call behind glm53::int4_linear (arguments validated)."""
-    out_features, in_features = weight.shape[0], 2 * weight.shape[1]
-    x, weight, scales = _ready(x), _ready(weight), scales.contiguous()
+    out_features, half = weight.shape
+    in_features = 2 * half
+    x, weight, scales = N.operand(x), N.operand(weight), scales.contiguous()
     if offsets is not None:
         offsets = offsets.contiguous()
     if bias is not None:
         bias = bias.contiguous()
     rows = x.numel() // in_features
-    y = torch.empty((*x.shape[:-1], out_features), dtype=torch.bfloat16, device=x.device)
+    y = x.new_empty((rows, out_features) if x.dim() == 2 else (*x.shape[:-1], out_features))
     if rows == 0:
         return y
     lib = N.lib()
-    ws_bytes = lib.glm53_int4_linear_workspace_bytes(rows, out_features, in_features)
-    ws = N.workspace(ws_bytes, x.device)
+    ws, ws_bytes = None, 0
+    if rows > FEW_ROWS:  # fewer take no workspace
+        ws_bytes = lib.glm53_int4_linear_workspace_bytes(rows, out_features, in_features)
+        ws = N.workspace(ws_bytes, x.device)
     w = N.Int4Weight(weight.data_ptr(), scales.data_ptr(), None if offsets is None else offsets.data_ptr(),
                      None if bias is None else bias.data_ptr(), out_features, in_features,
-                     in_features // scales.shape[1], int(scales.dtype is torch.float32))
-    N.run(x.device, lib.glm53_int4_linear, ctypes.byref(w), x.data_ptr(), rows, y.data_ptr(),
+                     in_features // scales.shape[1], scales.dtype is torch.float32)
+    N.run(x.get_device(), lib.glm53_int4_linear, ctypes.byref(w), x.data_ptr(), rows, y.data_ptr(),
           None if ws is None else ws.data_ptr(), ws_bytes)
     return y
 
@@ -143,7 +141,7 @@ def native_joined_swiglu(joined: torch.Tensor, limit: float) -> torch.Tensor:
     joined = joined.contiguous()
     width = joined.shape[-1] // 2
     h = torch.empty((*joined.shape[:-1], width), dtype=torch.bfloat16, device=joined.device)
-    N.run(joined.device, N.lib().glm53_activate_gate_up, joined.data_ptr(), h.numel() // width, width, limit, h.data_ptr())
+    N.run(joined.get_device(), N.lib().glm53_activate_gate_up, joined.data_ptr(), h.numel() // width, width, limit, h.data_ptr())
     return h
 
 

@@ -34,7 +34,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
     """``x / rms(x) * weight`` over the last axis, in ``dtype`` (x's own).
 
     x, weight and the result are bfloat16 or float32, each its own."""
-    N.require_same_device(x, weight)
+    N.same_device(x, weight)
     dtype = x.dtype if dtype is None else dtype
     width = _check_rows("x", x)
     _check_weight("weight", weight, width)
@@ -54,16 +54,18 @@ def residual_norm(residual: torch.Tensor, out: torch.Tensor, *, post_weight: tor
     residual's type, `normed` out's.  gate broadcasts against them: a value a
     channel ([width]), a token ([..., 1]), a sequence ([batch, 1, width]) or
     an element.  All tensors are bfloat16 or float32, each its own."""
-    N.require_same_device(residual, out, post_weight, gate, next_weight)
+    N.same_device(residual, out, post_weight, gate, next_weight)
     width = _check_rows("residual", residual)
-    if out.shape != residual.shape:
-        raise ValueError(f"out {tuple(out.shape)} must have residual's shape {tuple(residual.shape)}")
-    _check_rows("out", out)
+    shape = residual.shape
+    if out.shape != shape:
+        raise ValueError(f"out {tuple(out.shape)} must have residual's shape {tuple(shape)}")
+    if out.dtype not in _TYPES:
+        raise ValueError(f"out must be bfloat16 or float32, got {out.dtype}")
     _check_weight("post_weight", post_weight, width)
     _check_weight("next_weight", next_weight, width)
     kind, rows_per_gate = N.GATE_NONE, 1
     if gate is not None:
-        gate, kind, rows_per_gate = _gate_form(gate, residual.shape)
+        gate, kind, rows_per_gate = _gate_form(gate, shape)
     form = (kind, rows_per_gate, float(scale), float(eps), next_weight is not None, out.dtype is torch.float32)
     x, y = _call(residual, out, post_weight, gate, next_weight, form)
     return x, y if next_weight is not None else None
@@ -72,13 +74,14 @@ def residual_norm(residual: torch.Tensor, out: torch.Tensor, *, post_weight: tor
 def _check_rows(name: str, t: torch.Tensor) -> int:
     if t.dtype not in _TYPES:
         raise ValueError(f"{name} must be bfloat16 or float32, got {t.dtype}")
-    if t.dim() < 1 or t.shape[-1] < 1:
-        raise ValueError(f"{name} must have a last axis of one element or more, got {tuple(t.shape)}")
-    return t.shape[-1]
+    shape = t.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"{name} must have a last axis of one element or more, got {tuple(shape)}")
+    return shape[-1]
 
 
 def _check_weight(name: str, t: torch.Tensor | None, width: int) -> None:
-    if t is not None and (t.dtype not in _TYPES or t.dim() != 1 or t.shape[0] != width):
+    if t is not None and (t.dtype not in _TYPES or t.shape != (width,)):
         raise ValueError(f"{name} must be a bfloat16 or float32 [{width}] tensor, got {tuple(t.shape)} {t.dtype}")
 
 
@@ -91,6 +94,8 @@ def _gate_form(gate: torch.Tensor, shape) -> tuple[torch.Tensor, int, int]:
     if gate.dtype not in _TYPES:
         raise ValueError(f"gate must be bfloat16 or float32, got {gate.dtype}")
     width, rows = shape[-1], math.prod(shape[:-1])
+    if gate.shape == (width,) and rows > 0:  # a value a channel
+        return gate, N.GATE_COLUMNS, rows
     own = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
     if len(own) != len(shape) or any(g != s and g != 1 for g, s in zip(own, shape)):
         raise ValueError(f"gate {tuple(gate.shape)} does not broadcast to {tuple(shape)}")
@@ -113,84 +118,96 @@ def _gate_form(gate: torch.Tensor, shape) -> tuple[torch.Tensor, int, int]:
 def _call(residual, out, post_weight, gate, next_weight, form):
     tensors = (residual, out, post_weight, gate, next_weight)
     if _ops.direct(*tensors):
-        return native_residual_norm(*tensors, *form, False)[:2]
+        x, y, _ = native_residual_norm(*tensors, *form, False)
+        return x, y
     if _ops.eager(*tensors):
         return _ResidualNorm.apply(*tensors, form)
     return torch.ops.glm53.residual_norm(*tensors, *form)[:2]
 
 
-def _ready(t: torch.Tensor | None) -> torch.Tensor | None:
-    """Contiguous and, as far as its values' order needs it, 16-byte aligned."""
+def _taken(t: torch.Tensor | None):
+    """(t as the kernels take it, its address); (None, None) where absent."""
     if t is None:
-        return None
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 and t.dim() and t.shape[-1] % 8 == 0 else t
+        return None, None
+    if not t.is_contiguous():
+        t = t.contiguous()
+    p = t.data_ptr()
+    if p & 15:  # a copy at an aligned address gives the bits that an aligned tensor does
+        t = t.clone()
+        p = t.data_ptr()
+    return t, p
+
+
+def _f32(t: torch.Tensor | None, bit: int) -> int:
+    return bit if t is not None and t.dtype is torch.float32 else 0
 
 
 def _mask(residual, out, post_weight, gate, next_weight, y_f32) -> int:
-    m = N.NORM_F32_Y if y_f32 else 0
-    for bit, t in ((N.NORM_F32_RESIDUAL, residual), (N.NORM_F32_OUT, out), (N.NORM_F32_POST, post_weight),
-                   (N.NORM_F32_GATE, gate), (N.NORM_F32_NEXT, next_weight)):
-        if t is not None and t.dtype is torch.float32:
-            m |= bit
-    return m
-
-
-def _p(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
+    return (_f32(residual, N.NORM_F32_RESIDUAL) | _f32(out, N.NORM_F32_OUT) | _f32(post_weight, N.NORM_F32_POST)
+            | _f32(gate, N.NORM_F32_GATE) | _f32(next_weight, N.NORM_F32_NEXT) | (N.NORM_F32_Y if y_f32 else 0))
 
 
 def native_residual_norm(residual, out, post_weight, gate, next_weight, kind: int, rows_per_gate: int, scale: float,
                          eps: float, normed: bool, y_f32: bool, keep: bool = True):
-    """The native call behind glm53::residual_norm: (new residual, or an empty
-    tensor without out; normed, or an empty tensor; stats where kept)."""
-    residual, out, gate = _ready(residual), _ready(out), _ready(gate)
-    post_weight, next_weight = _ready(post_weight), _ready(next_weight)
-    width = residual.shape[-1]
+    """The native call behind glm53::residual_norm: (new residual, normed, stats),
+    None for what is not made."""
+    residual, p_residual = _taken(residual)
+    out, p_out = _taken(out)
+    post_weight, p_post = _taken(post_weight)
+    gate, p_gate = _taken(gate)
+    next_weight, p_next = _taken(next_weight)
+    shape = residual.shape
+    width = shape[-1]
     rows = residual.numel() // width
-    device = residual.device
-    x = torch.empty_like(residual) if out is not None else residual.new_empty(0)
-    y = torch.empty(residual.shape if normed else 0, dtype=torch.float32 if y_f32 else torch.bfloat16, device=device)
-    stats = torch.empty((rows, 2) if keep else 0, dtype=torch.float32, device=device) if keep else None
-    n = N.Norm(rows, width, rows_per_gate, residual.data_ptr(), _p(out), _p(post_weight), _p(gate), _p(next_weight),
-               x.data_ptr() if out is not None else None, y.data_ptr() if normed else None, _p(stats), None, None, None,
-               None, None, None, None, None, 0, kind, int(post_weight is not None),
-               _mask(residual, out, post_weight, gate, next_weight, y_f32), scale, eps)
+    x = p_x = y = p_y = stats = p_stats = None
+    if out is not None:
+        x = torch.empty_like(residual)
+        p_x = x.data_ptr()
+    if normed:
+        if y_f32 == (residual.dtype is torch.float32):
+            y = torch.empty_like(residual)
+        else:
+            y = residual.new_empty(shape, dtype=torch.float32 if y_f32 else torch.bfloat16)
+        p_y = y.data_ptr()
+    if keep:
+        stats = residual.new_empty((rows, 2), dtype=torch.float32)
+        p_stats = stats.data_ptr()
     if rows:
-        N.run(device, N.lib().glm53_residual_norm, ctypes.byref(n))
+        n = N.Norm(rows, width, rows_per_gate, p_residual, p_out, p_post, p_gate, p_next, p_x, p_y, p_stats, None, None,
+                   None, None, None, None, None, None, 0, kind, post_weight is not None,
+                   _mask(residual, out, post_weight, gate, next_weight, y_f32), scale, eps)
+        N.run(residual.get_device(), N.lib().glm53_residual_norm, ctypes.byref(n))
     return x, y, stats
 
 
 def native_residual_norm_backward(residual, out, post_weight, gate, next_weight, stats, d_new, d_y, kind: int,
                                   rows_per_gate: int, scale: float, eps: float, y_f32: bool, wanted: list[bool]):
     """The native call behind glm53::residual_norm_backward: the gradients of
-    residual, out, post_weight, gate and next_weight that are `wanted`, empty
-    tensors in place of the others."""
-    inputs = [_ready(t) for t in (residual, out, post_weight, gate, next_weight)]
-    residual, out, post_weight, gate, next_weight = inputs
-    d_new, d_y = _ready(d_new), _ready(d_y)
+    residual, out, post_weight, gate and next_weight that are `wanted`, None in
+    place of the others."""
+    (residual, out, post_weight, gate, next_weight), addresses = zip(*map(_taken, (residual, out, post_weight, gate,
+                                                                                   next_weight)))
+    d_new, p_new = _taken(d_new)
+    d_y, p_y = _taken(d_y)
     width = residual.shape[-1]
     rows = residual.numel() // width
-    device = residual.device
-    grads = [torch.empty_like(t) if t is not None and w else None for t, w in zip(inputs, wanted)]
+    grads = [torch.empty_like(t) if t is not None and w else None
+             for t, w in zip((residual, out, post_weight, gate, next_weight), wanted)]
     if rows == 0 or (d_new is None and d_y is None):
-        return [residual.new_empty(0) if g is None else g.zero_() for g in grads]
+        return [None if g is None else g.zero_() for g in grads]
     lib = N.lib()
+    p_grads = [None if g is None else g.data_ptr() for g in grads]
     if d_y is None and grads[4] is not None:
         grads[4].zero_()
+        p_grads[4] = None
     gate_rows = rows // rows_per_gate if kind == N.GATE_COLUMNS else 1
     ws_bytes = lib.glm53_residual_norm_workspace_bytes(rows, width, gate_rows)
-    ws = N.workspace(ws_bytes, device)
-    n = N.Norm(rows, width, rows_per_gate, residual.data_ptr(), _p(out), _p(post_weight), _p(gate), _p(next_weight),
-               None, None, stats.data_ptr(), _p(d_new), _p(d_y), _p(grads[0]), _p(grads[1]), _p(grads[2]), _p(grads[3]),
-               _p(grads[4]) if d_y is not None else None, ws.data_ptr(), ws_bytes, kind, int(post_weight is not None),
-               _mask(residual, out, post_weight, gate, next_weight, y_f32), scale, eps)
-    N.run(device, lib.glm53_residual_norm_backward, ctypes.byref(n))
-    return [residual.new_empty(0) if g is None else g for g in grads]
-
-
-def _given(grads, wanted):
-    return [g if w else None for g, w in zip(grads, wanted)]
+    ws = residual.new_empty(ws_bytes, dtype=torch.uint8)
+    n = N.Norm(rows, width, rows_per_gate, *addresses, None, None, stats.data_ptr(), p_new, p_y, *p_grads, ws.data_ptr(),
+               ws_bytes, kind, post_weight is not None, _mask(residual, out, post_weight, gate, next_weight, y_f32),
+               scale, eps)
+    N.run(residual.get_device(), lib.glm53_residual_norm_backward, ctypes.byref(n))
+    return grads
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -200,15 +217,11 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.save_for_backward(residual, out, post_weight, gate, next_weight, stats)
         ctx.form = form
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*([x] if out is None else []), *([] if form[4] else [y]))
         return x, y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_new, d_y):
-        saved = ctx.saved_tensors
-        kind, rows_per_gate, scale, eps, normed, y_f32 = ctx.form
-        wanted = [bool(w) for w in ctx.needs_input_grad[:5]]
-        grads = native_residual_norm_backward(*saved, d_new if saved[1] is not None else None, d_y if normed else None,
-                                              kind, rows_per_gate, scale, eps, y_f32, wanted)
-        return (*_given(grads, wanted), None)
+        kind, rows_per_gate, scale, eps, _, y_f32 = ctx.form
+        return (*native_residual_norm_backward(*ctx.saved_tensors, d_new, d_y, kind, rows_per_gate, scale, eps, y_f32,
+                                               ctx.needs_input_grad), None)

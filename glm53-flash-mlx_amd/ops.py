@@ -21,7 +21,7 @@ and FakeTensor / meta propagation gets the output shapes without a device.
   and ``residual_norm``, differentiable;
 * ``glm53::gated_mlp(x, gate_weight, up_weight, down_weight, limit, keep)``
   and ``glm53::gated_mlp_backward`` -- ``gated_mlp``, differentiable where
-  `keep` has it return G and U;
+  `keep` has it return G, U and h;
 * ``glm53::int4_linear(x, weight, scales, offsets?, bias?)`` -- ``int4_linear``,
   and ``glm53::joined_swiglu(joined, limit)``, the activation of ``Int4MLP``.
 
@@ -174,8 +174,10 @@ def residual_norm(residual: torch.Tensor, out: Optional[torch.Tensor], post_weig
                   y_f32: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     from .norms import native_residual_norm
 
-    return native_residual_norm(residual, out, post_weight, gate, next_weight, kind, rows_per_gate, scale, eps, normed,
-                                y_f32)
+    x, y, stats = native_residual_norm(residual, out, post_weight, gate, next_weight, kind, rows_per_gate, scale, eps,
+                                       normed, y_f32)
+    y_type = torch.float32 if y_f32 else torch.bfloat16
+    return (residual.new_empty(0) if x is None else x, residual.new_empty(0, dtype=y_type) if y is None else y, stats)
 
 
 @residual_norm.register_fake
@@ -194,8 +196,9 @@ def residual_norm_backward(residual: torch.Tensor, out: Optional[torch.Tensor], 
                            scale: float, eps: float, y_f32: bool, wanted: list[bool]) -> list[torch.Tensor]:
     from .norms import native_residual_norm_backward
 
-    return native_residual_norm_backward(residual, out, post_weight, gate, next_weight, stats, d_new, d_y, kind,
-                                         rows_per_gate, scale, eps, y_f32, wanted)
+    grads = native_residual_norm_backward(residual, out, post_weight, gate, next_weight, stats, d_new, d_y, kind,
+                                          rows_per_gate, scale, eps, y_f32, wanted)
+    return [residual.new_empty(0) if g is None else g for g in grads]
 
 
 @residual_norm_backward.register_fake
@@ -225,30 +228,35 @@ residual_norm.register_autograd(_residual_norm_backward, setup_context=_residual
 
 @torch.library.custom_op("glm53::gated_mlp", mutates_args=())
 def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, down_weight: torch.Tensor,
-              limit: float, keep: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+              limit: float, keep: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     from .gated import native_gated_mlp
 
-    return native_gated_mlp(x, gate_weight, up_weight, down_weight, limit, keep)
+    y, gate, up, h = native_gated_mlp(x, gate_weight, up_weight, down_weight, limit, keep)
+    if keep:
+        return y, gate, up, h
+    return y, x.new_empty(0, dtype=torch.float32), x.new_empty(0, dtype=torch.float32), x.new_empty(0)
 
 
 @gated_mlp.register_fake
 def _(x, gate_weight, up_weight, down_weight, limit, keep):
     rows = x.numel() // x.shape[-1]
     kept = (rows, gate_weight.shape[0]) if keep else (0,)
-    return (x.new_empty(x.shape), x.new_empty(kept, dtype=torch.float32), x.new_empty(kept, dtype=torch.float32))
+    return (x.new_empty(x.shape), x.new_empty(kept, dtype=torch.float32), x.new_empty(kept, dtype=torch.float32),
+            x.new_empty(kept))
 
 
 @torch.library.custom_op("glm53::gated_mlp_backward", mutates_args=())
 def gated_mlp_backward(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, down_weight: torch.Tensor,
-                       gate: torch.Tensor, up: torch.Tensor, d_y: torch.Tensor, limit: float,
+                       gate: torch.Tensor, up: torch.Tensor, h: torch.Tensor, d_y: torch.Tensor, limit: float,
                        wanted: list[bool]) -> list[torch.Tensor]:
     from .gated import native_gated_mlp_backward
 
-    return native_gated_mlp_backward(x, gate_weight, up_weight, down_weight, gate, up, d_y, limit, wanted)
+    grads = native_gated_mlp_backward(x, gate_weight, up_weight, down_weight, gate, up, h, d_y, limit, wanted)
+    return [x.new_empty(0) if g is None else g for g in grads]
 
 
 @gated_mlp_backward.register_fake
-def _(x, gate_weight, up_weight, down_weight, gate, up, d_y, limit, wanted):
+def _(x, gate_weight, up_weight, down_weight, gate, up, h, d_y, limit, wanted):
     inputs = (x, gate_weight, up_weight, down_weight)
     return [t.new_empty(t.shape) if w else x.new_empty(0) for t, w in zip(inputs, wanted)]
 
@@ -256,12 +264,12 @@ def _(x, gate_weight, up_weight, down_weight, gate, up, d_y, limit, wanted):
 def _gated_mlp_context(ctx, inputs, output):
     if not inputs[5]:
         raise RuntimeError("glm53::gated_mlp without keep has no gradient")
-    ctx.save_for_backward(*inputs[:4], output[1], output[2])
+    ctx.save_for_backward(*inputs[:4], *output[1:])
     ctx.limit = inputs[4]
     ctx.set_materialize_grads(False)
 
 
-def _gated_mlp_backward(ctx, d_y, _gate, _up):
+def _gated_mlp_backward(ctx, d_y, _gate, _up, _h):
     if d_y is None:
         return (None,) * 6
     wanted = [bool(w) for w in ctx.needs_input_grad[:4]]

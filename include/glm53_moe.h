@@ -586,8 +586,9 @@ int glm53_residual_norm_backward(const glm53_norm* norm, void* stream);
 /*   G = x Wg^T, U = x Wu^T, h = silu(min(G, L)) clip(U, -L, L), y = h Wd^T
  * over contiguous BF16 tensors, 16-byte aligned; hidden and intermediate
  * multiples of 8; limit L > 0, INFINITY for none.  Sums, G, U and the
- * activation are FP32, h and y are rounded once.  gate, up: f32 [rows,
- * intermediate], NULL or where G and U are kept for the gradients. */
+ * activation are FP32, h and y are rounded once (up to 16 rows h not at all).
+ * gate, up (f32) and h (BF16) [rows, intermediate]: all NULL, or where G, U
+ * and h are kept for the gradients. */
 typedef struct glm53_gated_mlp_desc {
   int64_t rows, hidden, intermediate;
   const void* x;           /* [rows, hidden] */
@@ -597,6 +598,7 @@ typedef struct glm53_gated_mlp_desc {
   void* y;                 /* [rows, hidden]; forward only */
   float* gate;
   float* up;
+  void* h;
   /* backward only; results NULL: not wanted */
   const void* d_y;
   void* d_x;

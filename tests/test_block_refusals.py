@@ -70,7 +70,7 @@ def test_norm_without_rows_and_workspace_sizes(N, libso):
 
 def _gated(N, **changes):
     d = N.GatedMLP(rows=4, hidden=64, intermediate=32, x=FAKE, gate_weight=FAKE, up_weight=FAKE, down_weight=FAKE, y=FAKE,
-                   gate=FAKE, up=FAKE, d_y=FAKE, workspace=FAKE, workspace_bytes=1 << 30, limit=1.0)
+                   gate=FAKE, up=FAKE, h=FAKE, d_y=FAKE, workspace=FAKE, workspace_bytes=1 << 30, limit=1.0)
     for name, value in changes.items():
         setattr(d, name, value)
     return ctypes.byref(d)
@@ -81,7 +81,7 @@ def _gated(N, **changes):
     (dict(intermediate=0), "invalid shape"), (dict(hidden=60), "multiples of 8"), (dict(intermediate=4), "multiples of 8"),
     (dict(hidden=1 << 23), "widths"), (dict(limit=0.0), "limit"), (dict(limit=-1.0), "limit"),
     (dict(limit=float("nan")), "limit"), (dict(x=FAKE + 2), "aligned"), (dict(down_weight=FAKE + 8), "aligned"),
-    (dict(up=None), "together"), (dict(x=None), "null"), (dict(gate_weight=None), "null"),
+    (dict(up=None), "together"), (dict(h=None), "together"), (dict(x=None), "null"), (dict(gate_weight=None), "null"),
     (dict(workspace=None), "workspace"), (dict(workspace=FAKE + 16), "workspace"), (dict(workspace_bytes=8), "workspace"),
 ])
 def test_gated_refusals(N, libso, changes, message):
@@ -95,7 +95,7 @@ def test_gated_empty_calls_and_workspace_sizes(N, libso):
     assert libso.glm53_gated_mlp(_gated(N, rows=0, x=None), None) == N.OK
     assert libso.glm53_gated_mlp(_gated(N, y=None), None) == N.INVALID_ARGUMENT
     assert libso.glm53_gated_mlp_backward(_gated(N, rows=0), None) == N.INVALID_ARGUMENT
-    assert libso.glm53_gated_mlp_backward(_gated(N, gate=None, up=None), None) == N.INVALID_ARGUMENT
+    assert libso.glm53_gated_mlp_backward(_gated(N, gate=None, up=None, h=None), None) == N.INVALID_ARGUMENT
     for size in (libso.glm53_gated_mlp_workspace_bytes, libso.glm53_gated_mlp_backward_workspace_bytes):
         assert size(0, 64, 32) == size(4, 0, 32) == size(4, 64, 0) == 0
         assert size(4, 64, 32) >= 4 * 32 * 2

@@ -246,9 +246,9 @@ def test_other_stream_and_captured_graph(dev, rows):
 
     def both():
         args = (i["x"], i["gate"], i["up"], i["down"])
-        y, g, u = gated.native_gated_mlp(*args, 2.0, True)
+        y, *kept = gated.native_gated_mlp(*args, 2.0, True)
         z = gated.native_gated_mlp(*args, 2.0, False)[0]
-        return [y, z] + gated.native_gated_mlp_backward(*args, g, u, i["dy"], 2.0, [True] * 4)
+        return [y, z] + gated.native_gated_mlp_backward(*args, *kept, i["dy"], 2.0, [True] * 4)
 
     with torch.cuda.stream(s):
         both()
