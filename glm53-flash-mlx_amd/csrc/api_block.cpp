@@ -18,7 +18,7 @@ int64_t gate_groups(const glm53_norm* n) {
 }
 
 // Checks a descriptor and makes the kernels' argument block of it.
-int norm_args(const glm53_norm* n, bool backward, NormArgs& a, bool& vec) {
+int norm_args(const glm53_norm* n, bool backward, NormArgs& a) {
   CHECK_ARG(n != nullptr, "norm descriptor is null");
   CHECK_ARG(n->rows >= 0 && n->rows < (int64_t{1} << 31) && n->width > 0, "invalid shape rows=%lld width=%lld",
             (long long)n->rows, (long long)n->width);
@@ -72,13 +72,6 @@ int norm_args(const glm53_norm* n, bool backward, NormArgs& a, bool& vec) {
               "norm gradients need a 16-byte aligned workspace of %zu bytes", need);
     a.partial = static_cast<float*>(n->workspace);
   }
-  const void* every[] = {a.residual.p, a.out.p, a.post.p, a.gate_kind == kGateRows ? nullptr : a.gate.p, a.next.p,
-                         a.new_residual.p, a.y.p, a.d_new.p, a.d_y.p, a.d_residual.p, a.d_out.p};
-  vec = n->width % 8 == 0;
-  for (const void* p : every) vec = vec && aligned(p, 16);
-  if (a.gate_kind != kGateRows) vec = vec && aligned(a.d_gate.p, 16);
-  CHECK_ARG(vec || n->width <= kNormMaxScalarWidth,
-            "a width above %lld must be a multiple of 8 with 16-byte aligned tensors", (long long)kNormMaxScalarWidth);
   return GLM53_OK;
 }
 
@@ -88,23 +81,21 @@ extern "C" {
 
 size_t glm53_residual_norm_workspace_bytes(int64_t rows, int64_t width, int64_t gate_rows) {
   if (rows <= 0 || width <= 0 || gate_rows <= 0 || gate_rows > rows) return 0;
-  return sizeof(float) * static_cast<size_t>(norm_slices(rows, gate_rows)) * kNormSums * static_cast<size_t>(width);
+  return sizeof(float) * static_cast<size_t>(norm_slices(rows, gate_rows, width)) * kNormSums * static_cast<size_t>(width);
 }
 
 int glm53_residual_norm(const glm53_norm* norm, void* stream) {
   NormArgs a;
-  bool vec;
-  if (int rc = norm_args(norm, false, a, vec)) return rc;
+  if (int rc = norm_args(norm, false, a)) return rc;
   if (a.rows == 0) return GLM53_OK;
-  HIP_TRY(launch_norm_forward(a, vec, S(stream)), "norm launch");
+  HIP_TRY(launch_norm_forward(a, S(stream)), "norm launch");
   return GLM53_OK;
 }
 
 int glm53_residual_norm_backward(const glm53_norm* norm, void* stream) {
   NormArgs a;
-  bool vec;
-  if (int rc = norm_args(norm, true, a, vec)) return rc;
-  HIP_TRY(launch_norm_backward(a, vec, S(stream)), "norm gradient launch");
+  if (int rc = norm_args(norm, true, a)) return rc;
+  HIP_TRY(launch_norm_backward(a, S(stream)), "norm gradient launch");
   return GLM53_OK;
 }
 

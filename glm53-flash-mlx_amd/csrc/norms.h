@@ -37,15 +37,14 @@ struct NormArgs {
   float* partial;       // [slices(), sums(), width]
 };
 
-constexpr int64_t kNormMaxWidth = 16384;        // rows whose values a workgroup holds in registers
-constexpr int64_t kNormMaxScalarWidth = 8192;   // of any width or alignment; above: 8 elements a load
+constexpr int64_t kNormMaxWidth = 16384;  // rows whose values a workgroup holds in registers
 
 // Workgroups of a backward pass over `rows` rows in `groups` equal groups,
-// each writing one row of column sums, and column sums a row.
-int64_t norm_slices(int64_t rows, int64_t groups);
+// each writing one row of kNormSums column sums.
+int64_t norm_slices(int64_t rows, int64_t groups, int64_t width);
 constexpr int kNormSums = 3;
 
-hipError_t launch_norm_forward(const NormArgs& a, bool vec, hipStream_t st);
-hipError_t launch_norm_backward(const NormArgs& a, bool vec, hipStream_t st);
+hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st);
+hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st);
 
 }  // namespace glm53

@@ -17,84 +17,96 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-template <int VEC>
-struct Raw;
-template <>
-struct Raw<8> {
+constexpr int kVec = 8;  // elements a thread loads at once
+
+// 16 bytes at any element's address: rows of odd widths, and views, start
+// anywhere, and the memory takes such loads whole.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+
+struct Raw {
   u32x4 lo, hi;
 };
-template <>
-struct Raw<1> {
-  uint32_t v;
-};
 
-// VEC elements from element index i, as stored; converted by to_float once
-// every load of the row is on its way.
-template <int VEC>
-__device__ __forceinline__ Raw<VEC> load_raw(const Tensor& t, int64_t i) {
-  Raw<VEC> r;
-  if constexpr (VEC == 8) {
-    if (t.f32) {
-      const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(t.p) + i);
-      r.lo = p[0];
-      r.hi = p[1];
-    } else {
-      r.lo = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(t.p) + i);
+// How a row's last elements are taken where the width is no multiple of kVec.
+// kWhole: it is one.  kOverlap: the last load is the row's last kVec elements,
+// whose first ones another thread has too: both compute and store the same
+// values for them, and one of the two leaves them out of the row's sums.
+// kSingly (rows shorter than kVec): one by one.
+enum Ends { kWhole, kOverlap, kSingly };
+
+// kVec elements from element index i, as stored (kSingly: `left` of them, the
+// others 0); converted by to_float once every load of the row is on its way.
+template <Ends E>
+__device__ __forceinline__ Raw load_raw(const Tensor& t, int64_t i, int64_t left) {
+  Raw r{};
+  if constexpr (E == kSingly) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      if (e >= left) break;
+      if (t.f32) {
+        const uint32_t v = static_cast<const uint32_t*>(t.p)[i + e];
+        if (e < 4)
+          r.lo[e] = v;
+        else
+          r.hi[e - 4] = v;
+      } else {
+        r.lo[e / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(t.p)[i + e]) << (16 * (e & 1));
+      }
     }
+  } else if (t.f32) {
+    const u32x4_any* p = reinterpret_cast<const u32x4_any*>(static_cast<const float*>(t.p) + i);
+    r.lo = p[0];
+    r.hi = p[1];
   } else {
-    if (t.f32)
-      r.v = static_cast<const uint32_t*>(t.p)[i];
-    else
-      r.v = static_cast<const uint16_t*>(t.p)[i];
+    r.lo = *reinterpret_cast<const u32x4_any*>(static_cast<const uint16_t*>(t.p) + i);
   }
   return r;
 }
 
-template <int VEC>
-__device__ __forceinline__ void to_float(const Raw<VEC>& r, bool f32, float* v) {
-  if constexpr (VEC == 8) {
-    if (f32) {
+__device__ __forceinline__ void to_float(const Raw& r, bool f32, float* v) {
+  if (f32) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = __uint_as_float(r.lo[e]);
-        v[4 + e] = __uint_as_float(r.hi[e]);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[2 * e] = __uint_as_float(r.lo[e] << 16);
-        v[2 * e + 1] = __uint_as_float(r.lo[e] & 0xFFFF0000u);
-      }
+    for (int e = 0; e < 4; ++e) {
+      v[e] = __uint_as_float(r.lo[e]);
+      v[4 + e] = __uint_as_float(r.hi[e]);
     }
   } else {
-    v[0] = __uint_as_float(f32 ? r.v : r.v << 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = __uint_as_float(r.lo[e] << 16);
+      v[2 * e + 1] = __uint_as_float(r.lo[e] & 0xFFFF0000u);
+    }
   }
 }
 
-template <int VEC>
-__device__ __forceinline__ void store(const Tensor& t, int64_t i, const float* v) {
-  if constexpr (VEC == 8) {
-    if (t.f32) {
-      u32x4* p = reinterpret_cast<u32x4*>(static_cast<float*>(t.p) + i);
-      u32x4 lo, hi;
+__device__ __forceinline__ void store_one(const Tensor& t, int64_t i, float v) {
+  if (t.f32)
+    static_cast<float*>(t.p)[i] = v;
+  else
+    static_cast<uint16_t*>(t.p)[i] = f32_to_bf16(v);
+}
+
+template <Ends E>
+__device__ __forceinline__ void store(const Tensor& t, int64_t i, int64_t left, const float* v) {
+  if constexpr (E == kSingly) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        lo[e] = __float_as_uint(v[e]);
-        hi[e] = __float_as_uint(v[4 + e]);
-      }
-      p[0] = lo;
-      p[1] = hi;
-    } else {
-      u32x4 w;
+    for (int e = 0; e < kVec; ++e)
+      if (e < left) store_one(t, i + e, v[e]);
+  } else if (t.f32) {
+    u32x4_any* p = reinterpret_cast<u32x4_any*>(static_cast<float*>(t.p) + i);
+    u32x4 lo, hi;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = f32_to_bf16(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16(v[2 * e + 1])) << 16;
-      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(t.p) + i) = w;
+    for (int e = 0; e < 4; ++e) {
+      lo[e] = __float_as_uint(v[e]);
+      hi[e] = __float_as_uint(v[4 + e]);
     }
+    p[0] = lo;
+    p[1] = hi;
   } else {
-    if (t.f32)
-      static_cast<float*>(t.p)[i] = v[0];
-    else
-      static_cast<uint16_t*>(t.p)[i] = f32_to_bf16(v[0]);
+    u32x4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = f32_to_bf16(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16(v[2 * e + 1])) << 16;
+    *reinterpret_cast<u32x4_any*>(static_cast<uint16_t*>(t.p) + i) = w;
   }
 }
 
@@ -119,28 +131,54 @@ __device__ __forceinline__ float row_sum(float v, float (*words)[T / kWave], int
 }
 
 // A row's threads and how its elements lie on them: T threads, C chunks of
-// VEC consecutive elements each, chunk c of thread t at (c T + t) VEC.
-template <int T, int VEC, int C>
+// kVec consecutive elements each, chunk c of thread t at (c T + t) kVec.
+template <int T, int C, Ends E>
 struct Row {
-  static constexpr int kN = VEC * C;
-  __device__ static __forceinline__ int64_t at(int c) { return (static_cast<int64_t>(c) * T + threadIdx.x) * VEC; }
+  static constexpr int kN = kVec * C;
+  __device__ static __forceinline__ int64_t chunk(int c) { return (static_cast<int64_t>(c) * T + threadIdx.x) * kVec; }
+  // where chunk c starts, in a row that has it
+  __device__ static __forceinline__ int64_t at(int c, int64_t width) {
+    const int64_t i = chunk(c);
+    return E == kOverlap && i + kVec > width ? width - kVec : i;
+  }
+  // whether element e counts in a row's sum: it is no second copy
+  __device__ static __forceinline__ bool counts(int e, int64_t width) {
+    if (E != kOverlap) return true;
+    const int64_t i = chunk(e / kVec);
+    return i + kVec <= width || e % kVec >= i + kVec - width;
+  }
 
   // Row elements [base, base + width) of t; elements past the width read 0.
-  __device__ static __forceinline__ void raw(const Tensor& t, int64_t base, int64_t width, Raw<VEC> (&r)[C]) {
+  __device__ static __forceinline__ void raw(const Tensor& t, int64_t base, int64_t width, Raw (&r)[C]) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      r[c] = Raw<VEC>{};
-      if (t.p != nullptr && at(c) < width) r[c] = load_raw<VEC>(t, base + at(c));
+      r[c] = Raw{};
+      if (t.p != nullptr && chunk(c) < width) r[c] = load_raw<E>(t, base + at(c, width), width - chunk(c));
     }
   }
-  __device__ static __forceinline__ void floats(const Raw<VEC> (&r)[C], const Tensor& t, float (&v)[kN]) {
+  __device__ static __forceinline__ void floats(const Raw (&r)[C], const Tensor& t, float (&v)[kN]) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) to_float<VEC>(r[c], t.f32, v + c * VEC);
+    for (int c = 0; c < C; ++c) to_float(r[c], t.f32, v + c * kVec);
   }
   __device__ static __forceinline__ void put(const Tensor& t, int64_t base, int64_t width, const float (&v)[kN]) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      if (at(c) < width) store<VEC>(t, base + at(c), v + c * VEC);
+      if (chunk(c) < width) store<E>(t, base + at(c, width), width - chunk(c), v + c * kVec);
+  }
+  // Every thread has its part of the row before any thread stores over it: the
+  // overlapping ends belong to two.
+  __device__ static __forceinline__ void all_loaded() {
+    if (E == kOverlap && T > kWave) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    }
+  }
+  // sum_e v_e w_e over the row's elements of this thread
+  __device__ static __forceinline__ float dot(const float (&v)[kN], const float (&w)[kN], int64_t width) {
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kN; ++e) s += counts(e, width) ? v[e] * w[e] : 0.0f;
+    return s;
   }
   // Column values of a weight that may be absent (1).
   __device__ static __forceinline__ void weight(const Tensor& t, int64_t base, int64_t width, float (&v)[kN]) {
@@ -149,7 +187,7 @@ struct Row {
       for (int e = 0; e < kN; ++e) v[e] = 1.0f;
       return;
     }
-    Raw<VEC> r[C];
+    Raw r[C];
     raw(t, base, width, r);
     floats(r, t, v);
   }
@@ -159,46 +197,43 @@ __device__ __forceinline__ int64_t gate_base(const NormArgs& a, int64_t row) {
   return a.gate_kind == kGateFull ? row * a.width : row / a.rows_per_gate * a.width;
 }
 
-template <int T, int VEC, int C>
-__device__ __forceinline__ void gate_values(const NormArgs& a, int64_t row, float (&g)[VEC * C]) {
-  using R = Row<T, VEC, C>;
+template <class R>
+__device__ __forceinline__ void gate_values(const NormArgs& a, int64_t row, float (&g)[R::kN]) {
   if (a.gate_kind == kGateRows) {
     const float v = scalar(a.gate, row);
 #pragma unroll
-    for (int e = 0; e < VEC * C; ++e) g[e] = v;
+    for (int e = 0; e < R::kN; ++e) g[e] = v;
   } else if (a.gate_kind == kGateNone) {
 #pragma unroll
-    for (int e = 0; e < VEC * C; ++e) g[e] = 1.0f;
+    for (int e = 0; e < R::kN; ++e) g[e] = 1.0f;
   } else {
     R::weight(a.gate, gate_base(a, row), a.width, g);
   }
 }
 
-template <int T, int VEC, int C, bool POST>
+template <int T, int C, Ends E, bool POST>
 __global__ __launch_bounds__(T) void norm_forward_kernel(NormArgs a) {
-  using R = Row<T, VEC, C>;
+  using R = Row<T, C, E>;
   constexpr int N = R::kN;
   __shared__ float words[2][T / kWave];
   int turn = 0;
   const float inv_width = 1.0f / static_cast<float>(a.width);
   const int64_t row = blockIdx.x, base = row * a.width;
-  Raw<VEC> rx[C], ro[C];
+  Raw rx[C], ro[C];
   R::raw(a.residual, base, a.width, rx);
   if (POST) R::raw(a.out, base, a.width, ro);
   float x[N];
   R::floats(rx, a.residual, x);
+  R::all_loaded();
   if (POST) {
     float o[N], g[N];
     R::floats(ro, a.out, o);
-    gate_values<T, VEC, C>(a, row, g);
+    gate_values<R>(a, row, g);
     float r_o = 1.0f;
     if (a.post_norm) {
       float p[N];
       R::weight(a.post, 0, a.width, p);
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < N; ++e) ss += o[e] * o[e];
-      r_o = 1.0f / sqrtf(row_sum<T>(ss, words, turn) * inv_width + a.eps);
+      r_o = 1.0f / sqrtf(row_sum<T>(R::dot(o, o, a.width), words, turn) * inv_width + a.eps);
 #pragma unroll
       for (int e = 0; e < N; ++e) o[e] = o[e] * r_o * p[e];
     }
@@ -210,11 +245,7 @@ __global__ __launch_bounds__(T) void norm_forward_kernel(NormArgs a) {
   if (a.y.p == nullptr) return;
   float w[N];
   R::weight(a.next, 0, a.width, w);
-  float ss = 0.0f;
-  // elements past the width: x is 0 there
-#pragma unroll
-  for (int e = 0; e < N; ++e) ss += x[e] * x[e];
-  const float r = 1.0f / sqrtf(row_sum<T>(ss, words, turn) * inv_width + a.eps);
+  const float r = 1.0f / sqrtf(row_sum<T>(R::dot(x, x, a.width), words, turn) * inv_width + a.eps);  // x past the width: 0
 #pragma unroll
   for (int e = 0; e < N; ++e) x[e] = x[e] * r * w[e];
   R::put(a.y, base, a.width, x);
@@ -236,9 +267,9 @@ __device__ __forceinline__ Slice slice_rows(int64_t rows, int64_t groups, int64_
 // d_gate (kGateColumns) and d_next in registers, written once as one row of
 // fp32 partial sums: 3 width floats against 16 rows or more of five tensors.
 // The order of the sums is the rows', whatever runs when.
-template <int T, int VEC, int C, bool POST>
+template <int T, int C, Ends E, bool POST>
 __global__ __launch_bounds__(T) void norm_backward_kernel(NormArgs a, int64_t groups, int64_t slices) {
-  using R = Row<T, VEC, C>;
+  using R = Row<T, C, E>;
   constexpr int N = R::kN;
   __shared__ float words[2][T / kWave];
   int turn = 0;
@@ -247,20 +278,37 @@ __global__ __launch_bounds__(T) void norm_backward_kernel(NormArgs a, int64_t gr
 #pragma unroll
   for (int e = 0; e < N; ++e) s_next[e] = s_post[e] = s_gate[e] = 0.0f;
   const Slice rows = slice_rows(a.rows, groups, slices, blockIdx.x);
+  // The next row's tensors are on their way while a row is worked on (with two
+  // loads a thread and tensor they would take the registers of half the
+  // wavefronts).
+  constexpr bool kAhead = C == 1;
+  struct {
+    Raw x[C], o[C], n[C], y[C];
+    float r_o, r;
+  } f;
+  const auto fetch = [&](int64_t row) {
+    const int64_t base = row * a.width;
+    R::raw(a.residual, base, a.width, f.x);
+    if (POST) R::raw(a.out, base, a.width, f.o);
+    R::raw(a.d_new, base, a.width, f.n);
+    R::raw(a.d_y, base, a.width, f.y);
+    f.r_o = a.stats[2 * row];
+    f.r = a.stats[2 * row + 1];
+  };
+  if (kAhead && rows.first < rows.last) fetch(rows.first);
   for (int64_t row = rows.first; row < rows.last; ++row) {
     const int64_t base = row * a.width;
-    Raw<VEC> rx[C], ro[C], rn[C], ry[C];
-    R::raw(a.residual, base, a.width, rx);
-    if (POST) R::raw(a.out, base, a.width, ro);
-    R::raw(a.d_new, base, a.width, rn);
-    R::raw(a.d_y, base, a.width, ry);
-    const float r_o = POST && a.post_norm ? a.stats[2 * row] : 1.0f;
-    float x[N], o[N], g[N], p[N], d[N];
-    R::floats(rx, a.residual, x);
-    R::floats(rn, a.d_new, d);
+    if (!kAhead) fetch(row);
+    const float r_o = POST && a.post_norm ? f.r_o : 1.0f, r = f.r;
+    float x[N], o[N], g[N], p[N], d[N], dy[N];
+    R::floats(f.x, a.residual, x);
+    R::floats(f.n, a.d_new, d);
+    R::floats(f.y, a.d_y, dy);
+    if (POST) R::floats(f.o, a.out, o);
+    R::all_loaded();
+    if (kAhead && row + 1 < rows.last) fetch(row + 1);
     if (POST) {
-      R::floats(ro, a.out, o);
-      gate_values<T, VEC, C>(a, row, g);
+      gate_values<R>(a, row, g);
       R::weight(a.post, 0, a.width, p);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
@@ -269,18 +317,15 @@ __global__ __launch_bounds__(T) void norm_backward_kernel(NormArgs a, int64_t gr
       }
     }
     if (a.d_y.p != nullptr) {
-      const float r = a.stats[2 * row + 1];
-      float dy[N], w[N], dot = 0.0f;
-      R::floats(ry, a.d_y, dy);
+      float w[N];
       R::weight(a.next, 0, a.width, w);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         x[e] *= r;
         s_next[e] += dy[e] * x[e];
         dy[e] *= w[e];
-        dot += dy[e] * x[e];
       }
-      const float m = row_sum<T>(dot, words, turn) * inv_width;
+      const float m = row_sum<T>(R::dot(dy, x, a.width), words, turn) * inv_width;
 #pragma unroll
       for (int e = 0; e < N; ++e) d[e] += r * (dy[e] - x[e] * m);
     }
@@ -298,22 +343,20 @@ __global__ __launch_bounds__(T) void norm_backward_kernel(NormArgs a, int64_t gr
       } else {
         float sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < N; ++e) sum += dg[e];
+        for (int e = 0; e < N; ++e) sum += R::counts(e, a.width) ? dg[e] : 0.0f;
         sum = row_sum<T>(sum, words, turn);
-        if (threadIdx.x == 0) store<1>(a.d_gate, row, &sum);
+        if (threadIdx.x == 0) store_one(a.d_gate, row, sum);
       }
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) d[e] *= a.scale * g[e];
     if (a.post_norm) {
-      float dot = 0.0f;
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         s_post[e] += d[e] * o[e];
         d[e] *= p[e];
-        dot += d[e] * o[e];
       }
-      const float m = row_sum<T>(dot, words, turn) * inv_width;
+      const float m = row_sum<T>(R::dot(d, o, a.width), words, turn) * inv_width;
 #pragma unroll
       for (int e = 0; e < N; ++e) d[e] = r_o * (d[e] - o[e] * m);
     }
@@ -341,6 +384,7 @@ __global__ __launch_bounds__(kWave* kJoin) void norm_join_kernel(NormArgs a, int
   const int64_t col = static_cast<int64_t>(blockIdx.x) * kWave + lane;
   float sum = 0.0f;
   if (col < a.width)
+#pragma unroll 8
     for (int64_t s = slot; s < count; s += kJoin) sum += a.partial[((first + s) * kNormSums + v) * a.width + col];
   part[slot][lane] = sum;
   __syncthreads();
@@ -348,41 +392,50 @@ __global__ __launch_bounds__(kWave* kJoin) void norm_join_kernel(NormArgs a, int
   sum = part[0][lane];
 #pragma unroll
   for (int i = 1; i < kJoin; ++i) sum += part[i][lane];
-  store<1>(out, g * a.width + col, &sum);
+  store_one(out, g * a.width + col, sum);
 }
 
-template <int T, int VEC, int C>
+template <int T, int C, Ends E>
 hipError_t launch_shape(const NormArgs& a, bool backward, int64_t groups, int64_t slices, hipStream_t st) {
   const bool post = a.out.p != nullptr;
   if (!backward) {
     const dim3 grid(static_cast<uint32_t>(a.rows));
     if (post)
-      norm_forward_kernel<T, VEC, C, true><<<grid, T, 0, st>>>(a);
+      norm_forward_kernel<T, C, E, true><<<grid, T, 0, st>>>(a);
     else
-      norm_forward_kernel<T, VEC, C, false><<<grid, T, 0, st>>>(a);
+      norm_forward_kernel<T, C, E, false><<<grid, T, 0, st>>>(a);
   } else {
     const dim3 grid(static_cast<uint32_t>(slices));
     if (post)
-      norm_backward_kernel<T, VEC, C, true><<<grid, T, 0, st>>>(a, groups, slices);
+      norm_backward_kernel<T, C, E, true><<<grid, T, 0, st>>>(a, groups, slices);
     else
-      norm_backward_kernel<T, VEC, C, false><<<grid, T, 0, st>>>(a, groups, slices);
+      norm_backward_kernel<T, C, E, false><<<grid, T, 0, st>>>(a, groups, slices);
   }
   return hipGetLastError();
 }
 
-hipError_t launch_any(const NormArgs& a, bool vec, bool backward, int64_t groups, int64_t slices, hipStream_t st) {
-  const int64_t w = a.width;
-  if (vec) {
-    if (w <= 512) return launch_shape<64, 8, 1>(a, backward, groups, slices, st);
-    if (w <= 2048) return launch_shape<256, 8, 1>(a, backward, groups, slices, st);
-    if (w <= 4096) return launch_shape<256, 8, 2>(a, backward, groups, slices, st);
-    if (w <= 8192) return launch_shape<512, 8, 2>(a, backward, groups, slices, st);
-    return launch_shape<1024, 8, 2>(a, backward, groups, slices, st);
+// Threads a row, so that each holds one or two loads of every tensor.
+int row_threads(int64_t width) { return width <= 512 ? 64 : width <= 1024 ? 128 : width <= 4096 ? 256 : width <= 8192 ? 512 : 1024; }
+
+template <Ends E>
+hipError_t launch_any(const NormArgs& a, bool backward, int64_t groups, int64_t slices, hipStream_t st) {
+  switch (row_threads(a.width)) {
+    case 64: return launch_shape<64, 1, E>(a, backward, groups, slices, st);
+    case 128: return launch_shape<128, 1, E>(a, backward, groups, slices, st);
+    case 256:
+      if (a.width <= 2048) return launch_shape<256, 1, E>(a, backward, groups, slices, st);
+      return launch_shape<256, 2, E>(a, backward, groups, slices, st);
+    case 512: return launch_shape<512, 2, E>(a, backward, groups, slices, st);
+    default: return launch_shape<1024, 2, E>(a, backward, groups, slices, st);
   }
-  if (w <= 512) return launch_shape<64, 1, 8>(a, backward, groups, slices, st);
-  if (w <= 2048) return launch_shape<256, 1, 8>(a, backward, groups, slices, st);
-  return launch_shape<1024, 1, 8>(a, backward, groups, slices, st);
 }
+
+hipError_t launch(const NormArgs& a, bool backward, int64_t groups, int64_t slices, hipStream_t st) {
+  if (a.width < kVec) return launch_shape<64, 1, kSingly>(a, backward, groups, slices, st);
+  return a.width % kVec ? launch_any<kOverlap>(a, backward, groups, slices, st) : launch_any<kWhole>(a, backward, groups, slices, st);
+}
+
+constexpr int64_t kNormSlices = 512;  // workgroups of 256 threads or more, two a CU
 
 int64_t gate_groups(const NormArgs& a) {
   return a.gate_kind == kGateColumns && a.rows > 0 ? a.rows / a.rows_per_gate : 1;
@@ -390,20 +443,18 @@ int64_t gate_groups(const NormArgs& a) {
 
 }  // namespace
 
-int64_t norm_slices(int64_t rows, int64_t groups) {
-  const int64_t per = rows / groups;
-  const int64_t each = 512 / groups;
+int64_t norm_slices(int64_t rows, int64_t groups, int64_t width) {
+  const int64_t per = rows / groups, threads = row_threads(width);
+  const int64_t each = (threads < 256 ? kNormSlices * 256 / threads : kNormSlices) / groups;
   return groups * (each < 1 ? 1 : each > per ? per : each);
 }
 
-hipError_t launch_norm_forward(const NormArgs& a, bool vec, hipStream_t st) {
-  return launch_any(a, vec, false, 1, 1, st);
-}
+hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) { return launch(a, false, 1, 1, st); }
 
-hipError_t launch_norm_backward(const NormArgs& a, bool vec, hipStream_t st) {
-  const int64_t groups = gate_groups(a), slices = norm_slices(a.rows, groups);
+hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
+  const int64_t groups = gate_groups(a), slices = norm_slices(a.rows, groups, a.width);
   if (slices > 0)  // without rows the sums are zero
-    if (hipError_t e = launch_any(a, vec, true, groups, slices, st); e != hipSuccess) return e;
+    if (hipError_t e = launch(a, true, groups, slices, st); e != hipSuccess) return e;
   const bool gates = a.d_gate.p != nullptr && a.gate_kind == kGateColumns;
   if (a.d_next.p == nullptr && a.d_post.p == nullptr && !gates) return hipSuccess;
   const dim3 grid(static_cast<uint32_t>((a.width + kWave - 1) / kWave), static_cast<uint32_t>(2 + (gates ? groups : 0)));

@@ -131,11 +131,7 @@ def _taken(t: torch.Tensor | None):
         return None, None
     if not t.is_contiguous():
         t = t.contiguous()
-    p = t.data_ptr()
-    if p & 15:  # a copy at an aligned address gives the bits that an aligned tensor does
-        t = t.clone()
-        p = t.data_ptr()
-    return t, p
+    return t, t.data_ptr()
 
 
 def _f32(t: torch.Tensor | None, bit: int) -> int:

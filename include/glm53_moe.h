@@ -540,8 +540,7 @@ int glm53_prefill_plan_scratch(glm53_prefill_plan* plan, int32_t which, void** p
  *   new_residual = residual + scale * gate * s
  *   y = new_residual / rms(new_residual) * next_weight
  * with rms(v) = sqrt(mean(v^2) + eps), over contiguous rows of `width`
- * elements (at most 16384; above 8192 a multiple of 8 with every tensor
- * 16-byte aligned).  FP32 throughout, each output rounded once; y is made of
+ * elements (at most 16384), aligned to their elements.  FP32 throughout, each output rounded once; y is made of
  * the new residual before it is rounded.  NULL: out (then y is the norm of
  * `residual` alone), post_weight and next_weight (ones), gate (one), y (not
  * computed), stats.  new_residual may be `residual` or `out` itself, y may be

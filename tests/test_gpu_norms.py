@@ -139,7 +139,7 @@ def _check(i, scale, eps, post_norm=True, rows=None):
     assert torch.equal(x0, x) and torch.equal(y0, y)
 
 
-@pytest.mark.parametrize("width", [1, 7, 64, 511, 512, 520, 1001, 2048, 2049, 4096, 5000, 8191, 8192, 12288, 16384])
+@pytest.mark.parametrize("width", [1, 7, 64, 511, 512, 520, 1001, 2048, 2049, 4096, 5000, 8191, 8192, 9001, 12288, 16383, 16384])
 def test_widths(dev, width):
     _check(_inputs(5, width, "bbb", "channel"), 0.5, 1e-6)
 
@@ -360,7 +360,7 @@ def test_refusals(dev):
         lambda: M.rms_norm(x.half(), w), lambda: M.rms_norm(x, w.half()), lambda: M.rms_norm(x, w[:8]),
         lambda: M.rms_norm(x, w.view(1, 16)), lambda: M.rms_norm(x, w, dtype=torch.float16),
         lambda: M.rms_norm(x[:, :0], None), lambda: M.rms_norm(x, w.cpu()), lambda: M.rms_norm(x, w, -1.0),
-        lambda: M.rms_norm(torch.zeros(2, 16392, device=dev)), lambda: M.rms_norm(torch.zeros(2, 8193, device=dev)),
+        lambda: M.rms_norm(torch.zeros(2, 16385, device=dev)),
         lambda: M.residual_norm(x, x[:2]), lambda: M.residual_norm(x, x.half()),
         lambda: M.residual_norm(x, x, gate=w[:8]), lambda: M.residual_norm(x, x, gate=torch.ones(3, 1, device=dev)),
         lambda: M.residual_norm(x, x, gate=torch.ones(1, 4, 16, device=dev)),
@@ -370,3 +370,50 @@ def test_refusals(dev):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {k} was not refused")
+
+
+@pytest.mark.parametrize("width", [5, 64, 100, 1001, 2050, 5003, 9001])
+@pytest.mark.parametrize("post_norm", [True, False])
+def test_in_place(dev, width, post_norm):
+    """The C entry points where an output is an input's own memory: the new
+    residual over residual or out, y over out or residual, d_residual over
+    d_new_residual; each gives the bits of separate memory."""
+    import ctypes
+
+    import torch
+
+    N, norms = submodule("_native"), submodule("norms")
+    i = _inputs(7, width, "bbb", "none", seed=width)
+    post = i["post"] if post_norm else None
+    form = (N.GATE_NONE, 1, 0.5, 1e-6)
+    x, y, stats = norms.native_residual_norm(i["residual"], i["out"], post, None, i["next"], *form, True, False)
+    alone = norms.native_residual_norm(i["residual"], None, None, None, i["next"], N.GATE_NONE, 1, 1.0, 1e-6, True, False)[1]
+
+    def call(residual, out, new, normed):
+        n = N.Norm(rows=7, width=width, rows_per_gate=1, residual=residual.data_ptr(), next_weight=i["next"].data_ptr(),
+                   out=None if out is None else out.data_ptr(), new_residual=None if new is None else new.data_ptr(),
+                   post_weight=None if post is None or out is None else post.data_ptr(), y=normed.data_ptr(),
+                   post_norm=int(post is not None and out is not None), scale=0.5, eps=1e-6)
+        N.run(residual.get_device(), N.lib().glm53_residual_norm, ctypes.byref(n))
+
+    for new_at, y_at in (("residual", "out"), ("out", "fresh"), ("residual", "fresh"), ("fresh", "out")):
+        t = dict(residual=i["residual"].clone(), out=i["out"].clone(), fresh=torch.empty_like(i["out"]))
+        call(t["residual"], t["out"], t[new_at], t[y_at])
+        assert torch.equal(t[new_at], x) and torch.equal(t[y_at], y), (new_at, y_at)
+    t = i["residual"].clone()
+    call(t, None, None, t)
+    assert torch.equal(t, alone)
+
+    for d_y in (i["d_y"], None):
+        want = norms.native_residual_norm_backward(i["residual"], i["out"], post, None, i["next"], stats, i["d_new"], d_y,
+                                                   *form, False, [True, True, False, False, False])
+        d = i["d_new"].clone()
+        d_out = torch.empty_like(i["out"])
+        ws = torch.empty(N.lib().glm53_residual_norm_workspace_bytes(7, width, 1), dtype=torch.uint8, device=dev)
+        n = N.Norm(rows=7, width=width, rows_per_gate=1, residual=i["residual"].data_ptr(), out=i["out"].data_ptr(),
+                   post_weight=None if post is None else post.data_ptr(), next_weight=i["next"].data_ptr(),
+                   stats=stats.data_ptr(), d_new_residual=d.data_ptr(), d_y=None if d_y is None else d_y.data_ptr(),
+                   d_residual=d.data_ptr(), d_out=d_out.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=ws.numel(),
+                   post_norm=int(post is not None), scale=0.5, eps=1e-6)
+        N.run(d.get_device(), N.lib().glm53_residual_norm_backward, ctypes.byref(n))
+        assert torch.equal(d, want[0]) and torch.equal(d_out, want[1])
