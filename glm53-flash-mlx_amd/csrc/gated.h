@@ -17,7 +17,7 @@ struct GatedArgs {
   uint16_t* y;            // [rows, hidden]
   float* gate;            // [rows, inter] kept for the gradient, or null
   float* up;
-  uint16_t* h;            // [rows, inter] kept with them
+  uint16_t* h;            // [rows, inter] kept with them; up to 16 rows [2, rows, inter], high and low parts
   // backward: gradients that are not wanted are null
   const uint16_t* dy;
   uint16_t* dx;

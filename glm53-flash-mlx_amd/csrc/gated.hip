@@ -6,7 +6,10 @@
 //   dx = dG Wg + dU Wu (one contraction over both),
 //   dWg = dG^T x, dWu = dU^T x, dWd = dy^T h.
 // Operands of a product are bf16 and its sums FP32: h, dG and dU are rounded
-// to bf16 once, as MFMA operands, everything before them is FP32.
+// to bf16 once, as MFMA operands, everything before them is FP32.  Over many
+// rows those roundings average out to about the results' own; up to kFewRows
+// rows, where a gradient holds few of them, they are carried as a high and a
+// low bf16 part, both multiplied.
 #include <algorithm>
 #include <initializer_list>
 
@@ -33,11 +36,6 @@ constexpr int kFewSteps = 4;  // K steps of 32 that a wavefront has in flight
 // y[m, n] = sum_k x[m, k] w(n)[k] of the 16 rows that row(n) gives, per wavefront
 // into part.  X: float rows are split into two bf16 operands, whose products
 // are added: no rounding of x.
-__device__ __forceinline__ float low_part(float f, uint16_t high) {
-  const float h = bf16_to_f32(high);  // an infinity or NaN is in the high part alone
-  return fabsf(h) < INFINITY ? f - h : 0.0f;
-}
-
 template <class X>
 __device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w_row, int K, float (*part)[16][16]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -107,7 +105,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_up_kernel(GatedArgs a
   }
   const float c = clamp_gate(gate, a.limit), v = c * sigmoid_f32(c) * clamp_up(up, a.limit);
   h[at] = v;
-  if (a.h != nullptr) a.h[at] = f32_to_bf16(v);
+  if (a.h != nullptr) {
+    const uint16_t high = f32_to_bf16(v);
+    a.h[at] = high;
+    a.h[a.rows * a.inter + at] = f32_to_bf16(low_part(v, high));
+  }
 }
 
 __global__ __launch_bounds__(64 * kFewWaves) void few_down_kernel(GatedArgs a, const float* h) {
@@ -139,15 +141,23 @@ Gemm16Args product(int64_t k) {
   return g;
 }
 
-// The workspace: forward h where it is not kept, backward dG and dU (bf16
-// [rows, inter] each); then the partial results of one product at a time.
+// Parts that h, dG and dU are carried in, one after the other.
+int parts(int64_t rows) { return rows <= kFewRows ? 2 : 1; }
+
+// Bytes of h, dG or dU.
+size_t plane_bytes(int64_t rows, int64_t inter) {
+  return round_up(2 * static_cast<size_t>(parts(rows)) * static_cast<size_t>(rows) * static_cast<size_t>(inter));
+}
+
+// The workspace: forward h where it is not kept, backward dG and dU; then the
+// partial results of one product at a time.
 struct Space {
   uint16_t *h, *dg, *du;
   float* partial;
 };
 Space carve(const GatedArgs& a, bool backward) {
   uint8_t* p = static_cast<uint8_t*>(a.space);
-  const size_t plane = round_up(2 * static_cast<size_t>(a.rows) * static_cast<size_t>(a.inter));
+  const size_t plane = plane_bytes(a.rows, a.inter);
   Space s{};
   s.h = a.h;
   if (backward) {
@@ -185,26 +195,40 @@ Gemm16Args hidden_grad(const GatedArgs& a, const Space& s) {
   g.up = a.up;
   g.d_gate = s.dg;
   g.d_up = s.du;
+  g.low = parts(a.rows) == 2 ? a.rows * a.inter : 0;
   g.partial = s.partial;
   return g;
 }
 Gemm16Args input_grad(const GatedArgs& a, const Space& s) {
   Gemm16Args g = product(a.inter);
-  g.segments = 2;
-  g.pair[0] = pair(s.dg, a.inter, a.wg, a.hidden, a.dx, a.rows, a.hidden);
-  g.pair[1] = pair(s.du, a.inter, a.wu, a.hidden, a.dx, a.rows, a.hidden);
+  g.segments = 0;
+  for (int part = 0; part < parts(a.rows); ++part) {
+    const int64_t at = part * a.rows * a.inter;
+    g.pair[g.segments++] = pair(s.dg + at, a.inter, a.wg, a.hidden, a.dx, a.rows, a.hidden);
+    g.pair[g.segments++] = pair(s.du + at, a.inter, a.wu, a.hidden, a.dx, a.rows, a.hidden);
+  }
   g.partial = s.partial;
   return g;
 }
+Gemm16Pair weight_grad(const GatedArgs& a, const Space& s, int which, int part) {
+  const int64_t at = part * a.rows * a.inter;
+  if (which == 1) return pair(s.dg + at, a.inter, a.x, a.hidden, a.d_wg, a.inter, a.hidden);
+  if (which == 2) return pair(s.du + at, a.inter, a.x, a.hidden, a.d_wu, a.inter, a.hidden);
+  return pair(a.dy, a.hidden, s.h + at, a.inter, a.d_wd, a.hidden, a.inter);
+}
 // Those of the weights' gradients, dWg, dWu and dWd, that `which` (bits 1, 2
-// and 4) names.
+// and 4) names; a single one where they are carried in two parts.
 Gemm16Args weight_grads(const GatedArgs& a, const Space& s, int which) {
   Gemm16Args g = product(a.rows);
-  g.problems = 0;
-  if (which & 1) g.pair[g.problems++] = pair(s.dg, a.inter, a.x, a.hidden, a.d_wg, a.inter, a.hidden);
-  if (which & 2) g.pair[g.problems++] = pair(s.du, a.inter, a.x, a.hidden, a.d_wu, a.inter, a.hidden);
-  if (which & 4) g.pair[g.problems++] = pair(a.dy, a.hidden, s.h, a.inter, a.d_wd, a.hidden, a.inter);
   g.partial = s.partial;
+  if (parts(a.rows) == 2) {
+    g.segments = 2;
+    for (int part = 0; part < 2; ++part) g.pair[part] = weight_grad(a, s, which, part);
+    return g;
+  }
+  g.problems = 0;
+  for (int one : {1, 2, 4})
+    if (which & one) g.pair[g.problems++] = weight_grad(a, s, one, 0);
   return g;
 }
 
@@ -213,7 +237,7 @@ int64_t most(std::initializer_list<int64_t> v) { return std::max(v); }
 }  // namespace
 
 size_t gated_space(int64_t rows, int64_t hidden, int64_t inter, bool backward) {
-  const size_t values = static_cast<size_t>(rows) * static_cast<size_t>(inter);
+  const size_t plane = plane_bytes(rows, inter);
   GatedArgs a{};
   a.rows = rows;
   a.hidden = hidden;
@@ -221,13 +245,15 @@ size_t gated_space(int64_t rows, int64_t hidden, int64_t inter, bool backward) {
   const Space s{};
   if (backward) {
     int64_t partial = most({gemm16_plan(hidden_grad(a, s), false).partial, gemm16_plan(input_grad(a, s), false).partial});
-    for (int which : {1, 3, 7})  // one, two or all three of the products, which are of one size
+    for (int which : {1, 3, 7}) {  // one, two or all three of the products, which are of one size
+      if (which > 1 && parts(rows) == 2) break;
       partial = most({partial, gemm16_plan(weight_grads(a, s, which), false).partial});
-    return 2 * round_up(2 * values) + sizeof(float) * static_cast<size_t>(partial);
+    }
+    return 2 * plane + sizeof(float) * static_cast<size_t>(partial);
   }
-  if (rows <= kFewRows) return round_up(4 * values);
+  if (rows <= kFewRows) return plane;  // h in FP32: the size of its two parts
   const int64_t partial = most({gemm16_plan(gate_up(a, s), true).partial, gemm16_plan(down(a, s), false).partial});
-  return round_up(2 * values) + sizeof(float) * static_cast<size_t>(partial);
+  return plane + sizeof(float) * static_cast<size_t>(partial);
 }
 
 hipError_t launch_gated(const GatedArgs& a, hipStream_t st) {
@@ -241,8 +267,9 @@ hipError_t launch_gated(const GatedArgs& a, hipStream_t st) {
 hipError_t launch_gated_backward(const GatedArgs& a, hipStream_t st) {
   const Space s = carve(a, true);
   const auto weights = [&](int which) {
+    if (which == 0) return hipSuccess;
     const Gemm16Args g = weight_grads(a, s, which);
-    return g.problems == 0 ? hipSuccess : gemm16<true, kColumn, kStore>(g, gemm16_plan(g, false), st);
+    return gemm16<true, kColumn, kStore>(g, gemm16_plan(g, false), st);
   };
   const int pair = (a.d_wg ? 1 : 0) | (a.d_wu ? 2 : 0), down = a.d_wd ? 4 : 0;
   if (a.dx != nullptr || pair != 0) {
@@ -252,6 +279,11 @@ hipError_t launch_gated_backward(const GatedArgs& a, hipStream_t st) {
   if (a.dx != nullptr) {
     const Gemm16Args x = input_grad(a, s);
     if (hipError_t e = gemm16<false, kColumn, kStore>(x, gemm16_plan(x, false), st); e != hipSuccess) return e;
+  }
+  if (parts(a.rows) == 2) {
+    for (int one : {1, 2, 4})
+      if (hipError_t e = weights((pair | down) & one); e != hipSuccess) return e;
+    return hipSuccess;
   }
   // The weights' gradients in one launch, or the down projection's apart, where
   // the numbers of tiles fill the chip's rounds better: 8,192 rows, 4096 x 2048

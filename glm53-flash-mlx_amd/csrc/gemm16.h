@@ -34,13 +34,13 @@ struct Gemm16Pair {
 };
 
 struct Gemm16Args {
-  Gemm16Pair pair[3];
+  Gemm16Pair pair[4];
   int64_t k;       // of each pair
   int problems;    // pairs that are products of their own
   int segments;    // pairs whose contractions are added into pair[0].out
   int splits;      // parts of the contraction, each to `partial`
   float* partial;  // of each problem [splits][planes][m][partial_ld(n)], at partial_at floats
-  int64_t partial_at[3];
+  int64_t partial_at[4];
   int64_t tiles;   // output tiles of all problems; tiles * splits below 2^31
   int group_m;     // tile rows that one XCD's neighbouring workgroups share
   // SwiGLU: pair[0].b gate and pair[1].b up rows, out = h; gate/up (f32
@@ -51,6 +51,7 @@ struct Gemm16Args {
   float* up;
   uint16_t* d_gate;
   uint16_t* d_up;
+  int64_t low;  // 0, or values from d_gate and d_up to the low parts that are written there too
   // 4-bit b: codes [n, k / 2], scales and offsets [n, k / group], bias [n]
   const uint8_t* codes;
   const void* scales;
@@ -75,6 +76,16 @@ __device__ __forceinline__ float clamp_up(float u, float limit) { return u > lim
 __device__ __forceinline__ u32x2 pack_bf16x4(f32x4 v) {
   return (u32x2){f32_to_bf16(v[0]) | static_cast<uint32_t>(f32_to_bf16(v[1])) << 16,
                  f32_to_bf16(v[2]) | static_cast<uint32_t>(f32_to_bf16(v[3])) << 16};
+}
+
+// What `high` (bf16) leaves of f; an infinity or NaN is in the high part alone.
+__device__ __forceinline__ float low_part(float f, uint16_t high) {
+  const float h = bf16_to_f32(high);
+  return fabsf(h) < INFINITY ? f - h : 0.0f;
+}
+__device__ __forceinline__ u32x2 low_bf16x4(f32x4 v, u32x2 high) {
+  return pack_bf16x4((f32x4){low_part(v[0], high[0] & 0xFFFF), low_part(v[1], high[0] >> 16),
+                             low_part(v[2], high[1] & 0xFFFF), low_part(v[3], high[1] >> 16)});
 }
 
 __device__ __forceinline__ float table_value(const void* t, bool f32, int64_t i) {
@@ -136,8 +147,13 @@ __device__ __forceinline__ void store_swiglu_grad(const Gemm16Args& g, const Gem
     du[i] = fabsf(up[i]) > g.limit ? 0.0f : dh[i] * (c * s);
     dg[i] = gate[i] > g.limit ? 0.0f : dh[i] * u * (s * (1.0f + c * (1.0f - s)));
   }
-  *reinterpret_cast<u32x2*>(g.d_gate + at) = pack_bf16x4(dg);
-  *reinterpret_cast<u32x2*>(g.d_up + at) = pack_bf16x4(du);
+  const u32x2 high_g = pack_bf16x4(dg), high_u = pack_bf16x4(du);
+  *reinterpret_cast<u32x2*>(g.d_gate + at) = high_g;
+  *reinterpret_cast<u32x2*>(g.d_up + at) = high_u;
+  if (g.low != 0) {
+    *reinterpret_cast<u32x2*>(g.d_gate + g.low + at) = low_bf16x4(dg, high_g);
+    *reinterpret_cast<u32x2*>(g.d_up + g.low + at) = low_bf16x4(du, high_u);
+  }
 }
 
 // ------------------------------------------------------------- staging ---

@@ -21,6 +21,9 @@ from . import _native as N
 from . import ops as _ops
 
 
+FEW_ROWS = 16  # up to here what is rounded as an operand is carried in two bf16 parts
+
+
 def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor, down_weight: torch.Tensor,
               limit: float | None = None) -> torch.Tensor:
     """``down(silu(min(gate(x), limit)) * clip(up(x), -limit, limit))``.
@@ -64,7 +67,7 @@ def native_gated_mlp(x, gate_weight, up_weight, down_weight, limit: float, keep:
     if keep:
         gate = x.new_empty((rows, inter), dtype=torch.float32)
         up = torch.empty_like(gate)
-        h = x.new_empty((rows, inter))
+        h = x.new_empty((2, rows, inter) if rows <= FEW_ROWS else (rows, inter))
         p_gate, p_up, p_h = gate.data_ptr(), up.data_ptr(), h.data_ptr()
     if rows:
         lib = N.lib()

@@ -239,10 +239,12 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
 
 @gated_mlp.register_fake
 def _(x, gate_weight, up_weight, down_weight, limit, keep):
+    from .gated import FEW_ROWS
+
     rows = x.numel() // x.shape[-1]
     kept = (rows, gate_weight.shape[0]) if keep else (0,)
     return (x.new_empty(x.shape), x.new_empty(kept, dtype=torch.float32), x.new_empty(kept, dtype=torch.float32),
-            x.new_empty(kept))
+            x.new_empty((2, *kept) if keep and rows <= FEW_ROWS else kept))
 
 
 @torch.library.custom_op("glm53::gated_mlp_backward", mutates_args=())

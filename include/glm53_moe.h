@@ -587,7 +587,8 @@ int glm53_residual_norm_backward(const glm53_norm* norm, void* stream);
  * multiples of 8; limit L > 0, INFINITY for none.  Sums, G, U and the
  * activation are FP32, h and y are rounded once (up to 16 rows h not at all).
  * gate, up (f32) and h (BF16) [rows, intermediate]: all NULL, or where G, U
- * and h are kept for the gradients. */
+ * and h are kept for the gradients; up to 16 rows h has two planes, [2, rows,
+ * intermediate], what BF16 leaves of h in the second. */
 typedef struct glm53_gated_mlp_desc {
   int64_t rows, hidden, intermediate;
   const void* x;           /* [rows, hidden] */
@@ -613,8 +614,8 @@ int glm53_gated_mlp(const glm53_gated_mlp_desc* desc, void* stream);
 /* dh = d_y Wd; dU = dh silu(min(G, L)) where |U| <= L, else 0; dG = dh
  * clip(U) silu'(min(G, L)) where G <= L, else 0; d_x = dG Wg + dU Wu, d_gate_weight
  * = dG^T x, d_up_weight = dU^T x, d_down_weight = d_y^T h.  dG, dU and h are
- * rounded to BF16 as operands of these products, sums are FP32 in a fixed
- * order.  rows > 0.  Results may not overlap inputs. */
+ * rounded to BF16 as operands of these products (up to 16 rows to two BF16
+ * parts), sums are FP32 in a fixed order.  rows > 0.  Results may not overlap inputs. */
 size_t glm53_gated_mlp_backward_workspace_bytes(int64_t rows, int64_t hidden, int64_t intermediate);
 int glm53_gated_mlp_backward(const glm53_gated_mlp_desc* desc, void* stream);
 

@@ -2,8 +2,8 @@
 
 Tolerances: an FP32 sum of K exact products of bf16 values is off by at most
 K 2^-24 of the sum of their magnitudes; h, dG and dU are rounded to bf16 once
-(half a step, 2^-8 of the value) before they enter a sum; a result is rounded
-once more.  sigmoid and exp in FP32 add a few steps of 2^-24, covered by 32.
+(half a step, 2^-8 of the value) before they enter a sum, or over at most 16
+rows twice, in a high and a low part (2^-16); a result is rounded once more.  sigmoid and exp in FP32 add a few steps of 2^-24, covered by 32.
 The magnitudes are summed in 64 bits beside the values.
 """
 
@@ -42,6 +42,7 @@ def _formulas(i, limit):
     hidden, inter = d["down"].shape
     x, dy = d["x"].reshape(-1, hidden), d["dy"].reshape(-1, hidden)
     rows = x.shape[0]
+    op = 2.0**-16 if rows <= 16 else HALF  # rounding of an operand
     limit = math.inf if limit is None else limit
     g, u = x @ d["gate"].t(), x @ d["up"].t()
     eg, eu = (STEP * hidden * (x.abs() @ d[n].abs().t()) for n in ("gate", "up"))
@@ -51,7 +52,7 @@ def _formulas(i, limit):
     h = silu * uc
     # |silu'| <= 1.1, |silu''| <= 0.5
     eh = 1.1 * eg * uc.abs() + silu.abs() * eu + 1.1 * eg * eu + 32 * STEP * h.abs()
-    rh = HALF * (h.abs() + eh) + eh  # of h as an operand
+    rh = op * (h.abs() + eh) + eh  # of h as an operand
     y = h @ d["down"].t()
     ey = rh @ d["down"].abs().t() + STEP * inter * (h.abs() @ d["down"].abs().t())
     dh = dy @ d["down"]
@@ -64,7 +65,7 @@ def _formulas(i, limit):
     if limit < math.inf:
         edg = torch.where((g - limit).abs() <= eg, (dh * uc).abs() * 1.1 + edg, edg)
         edu = torch.where((u.abs() - limit).abs() <= eu, (dh * silu).abs() + edu, edu)
-    rg, ru = HALF * (dg.abs() + edg) + edg, HALF * (du.abs() + edu) + edu
+    rg, ru = op * (dg.abs() + edg) + edg, op * (du.abs() + edu) + edu
     dx = dg @ d["gate"] + du @ d["up"]
     edx = rg @ d["gate"].abs() + ru @ d["up"].abs() + STEP * 2 * inter * (
         dg.abs() @ d["gate"].abs() + du.abs() @ d["up"].abs())
