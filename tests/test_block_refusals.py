@@ -159,6 +159,28 @@ def test_quantize_int4_gives_the_nearest_codes():
             bad()
 
 
+def test_struct_layouts(N, tmp_path):
+    """Sizes and offsets of the block's structs in the header, compiled as C,
+    are those of the Python binding."""
+    import subprocess
+
+    from conftest import ROOT
+
+    structs = {"glm53_norm": N.Norm, "glm53_gated_mlp_desc": N.GatedMLP, "glm53_int4_weight": N.Int4Weight}
+    lines = ["#include <glm53_moe.h>", "#include <stdio.h>", "int main(void) {"]
+    want = {}
+    for name, py in structs.items():
+        lines.append(f'  printf("{name} %zu\\n", sizeof({name}));')
+        want[name] = ctypes.sizeof(py)
+        for field, _ in py._fields_:
+            lines.append(f'  printf("{name}.{field} %zu\\n", offsetof({name}, {field}));')
+            want[f"{name}.{field}"] = getattr(py, field).offset
+    (tmp_path / "s.c").write_text("\n".join([*lines, "  return 0;", "}"]))
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(tmp_path / "s.c"), "-o", str(tmp_path / "s")], check=True)
+    out = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout
+    assert {a: int(b) for a, b in (line.split() for line in out.splitlines())} == want
+
+
 def test_python_functions_refuse_cpu_tensors():
     import torch
 

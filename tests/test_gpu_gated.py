@@ -311,3 +311,61 @@ def test_refusals(dev):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {k} was not refused")
+
+
+def test_offsets_past_32_bits(dev):
+    """G, U and h of more than 2^32 bytes, and the widest operand the kernels
+    address from one tile: the last rows are those of a call of their own."""
+    import torch
+
+    M = pkg()
+    rows, hidden, inter, tail = 270_000, 64, 8192, 40
+    i = _weights(hidden, inter, tail, std=0.05)
+    x = torch.randn(tail, hidden, device=dev).to(torch.bfloat16).repeat(rows // tail, 1)
+    x[-tail:] = i["x"]
+    dy = torch.zeros(rows, hidden, device=dev, dtype=torch.bfloat16)
+    dy[-tail:] = i["dy"]
+    leaves = [x.requires_grad_(), *(i[n].clone().requires_grad_() for n in ("gate", "up", "down"))]
+    y = M.gated_mlp(*leaves, 4.0)
+    grads = torch.autograd.grad(y, leaves, dy)
+    want = _formulas(i, 4.0)
+    _near("y", y[-tail:], want["y"])
+    _near("x", grads[0][-tail:], want["x"])
+    assert (grads[0][:-tail] == 0).all()
+    # rows without a gradient add zeros: the sums are the last rows', in other parts
+    for n, g in zip(("gate", "up", "down"), grads[1:]):
+        _near(n, g, want[n])
+    wide = 1 << 17
+    j = _weights(wide, 8, 300, std=0.003)
+    y = M.gated_mlp(j["x"], j["gate"], j["up"], j["down"])
+    _near("y", y, _formulas(j, None)["y"])
+
+
+def test_no_second_derivative_is_claimed(dev):
+    import torch
+
+    i = _weights(64, 32, 4)
+    x = i["x"].requires_grad_()
+    g, = torch.autograd.grad(pkg().gated_mlp(x, i["gate"], i["up"], i["down"]).float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
+
+
+def test_two_streams_at_once(dev):
+    """Calls that overlap on two streams have their own workspaces."""
+    import torch
+
+    M = pkg()
+    problems = [_weights(512, 256, rows, seed=rows) for rows in (90, 700)]
+    want = [_train(i, 2.0) for i in problems]
+    streams = [torch.cuda.Stream() for _ in problems]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, i in zip(streams, problems):
+            with torch.cuda.stream(s):
+                got.append(_train(i, 2.0))
+    torch.cuda.synchronize()
+    for k, (y, grads) in enumerate(got):
+        wy, wg = want[k % 2]
+        assert torch.equal(y, wy) and all(torch.equal(grads[n], wg[n]) for n in wg), k

@@ -230,3 +230,33 @@ def test_refusals(dev):
             pytest.fail(f"call {k} was not refused")
     with pytest.raises(RuntimeError):  # no gradient is claimed where there is none
         M.int4_linear(x.requires_grad_(), c, s).sum().backward()
+
+
+@pytest.mark.parametrize("rows", [1, 16, 40, 200])
+def test_offsets_past_32_bits(dev, rows):
+    """More than 2^32 codes: the last output columns are those of a call on
+    their rows alone."""
+    import torch
+
+    M = pkg()
+    n, k, tail = 70_000, 1 << 16, 24
+    assert n * k > 2**32
+    p = _problem(rows, tail, k, 128, bias=True)
+    codes = torch.zeros(n, k // 2, device=dev, dtype=torch.uint8)
+    scales = torch.ones(n, k // 128, device=dev, dtype=torch.bfloat16)
+    off, bias = torch.zeros_like(scales), torch.zeros(n, device=dev, dtype=torch.bfloat16)
+    for big, small in ((codes, p[1]), (scales, p[2]), (off, p[3]), (bias, p[4])):
+        big[-tail:] = small
+    y = M.int4_linear(p[0], codes, scales, off, bias)
+    assert (y[:, :-tail] == 0).all()
+    _check(p, y[:, -tail:].contiguous())
+
+
+def test_mlp_without_a_limit(dev):
+    import torch
+
+    M, fp8 = pkg(), submodule("fp8")
+    small = M.GatedMLP(128, 64, device=dev).to_int4(group_size=32, symmetric=True)
+    x = (8 * torch.randn(7, 128, device=dev)).to(torch.bfloat16)
+    joined = small.gate_up_proj(x)
+    assert torch.equal(small(x), small.down_proj(fp8.swiglu(joined[:, :64], joined[:, 64:], float("inf"))))

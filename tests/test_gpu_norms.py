@@ -417,3 +417,77 @@ def test_in_place(dev, width, post_norm):
                    post_norm=int(post is not None), scale=0.5, eps=1e-6)
         N.run(d.get_device(), N.lib().glm53_residual_norm_backward, ctypes.byref(n))
         assert torch.equal(d, want[0]) and torch.equal(d_out, want[1])
+
+
+def test_offsets_past_32_bits(dev):
+    """Tensors of more than 2^31 elements: the last rows are those of a call of
+    their own, forward and backward."""
+    import torch
+
+    M = pkg()
+    rows, width, tail = 140_000, 16384, 3
+    assert rows * width > 2**31
+    i = _inputs(tail, width, "bbb", "channel", seed=2)
+    big = {n: torch.zeros(rows, width, device=dev, dtype=torch.bfloat16) for n in ("residual", "out", "d_new", "d_y")}
+    for n in big:
+        big[n][-tail:] = i[n]
+    big["out"][:-tail, 0] = 1  # rows that are not all zero
+    big["residual"].requires_grad_()
+    big["out"].requires_grad_()
+    w = {n: i[n].clone().requires_grad_() for n in ("post", "gate", "next")}
+    x, y = M.residual_norm(big["residual"], big["out"], post_weight=w["post"], gate=w["gate"], scale=0.5,
+                           next_weight=w["next"])
+    grads = torch.autograd.grad([x, y], [big["residual"], big["out"], *w.values()], [big["d_new"], big["d_y"]])
+    want = _formulas(i, 0.5, 1e-6)
+    _near(x[-tail:], *want["new"])
+    _near(y[-tail:], *want["y"])
+    _near(grads[0][-tail:], *want["residual"])
+    _near(grads[1][-tail:], *want["out"])
+    for n, g in zip(("post", "gate", "next"), grads[2:]):
+        _near(g, *want[n], steps=200)
+
+
+def test_no_second_derivative_is_claimed(dev):
+    import torch
+
+    x = torch.randn(3, 16, device=dev, requires_grad=True)
+    g, = torch.autograd.grad(pkg().rms_norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_one_gradient_given_or_wanted(dev):
+    """Only the new residual's, or only y's gradient comes; each subset of
+    leaves gets what all of them get."""
+    import itertools
+
+    import torch
+
+    M = pkg()
+    i = _inputs(21, 72, "fbf", "token", seed=4)
+    names = ("residual", "out", "post", "gate", "next")
+
+    def run(need, given):
+        t = [i[n].detach().clone().requires_grad_(r) for n, r in zip(names, need)]
+        x, y = M.residual_norm(t[0], t[1], post_weight=t[2], gate=t[3], scale=0.5, next_weight=t[4])
+        pairs = [p for p, g in zip(((x, i["d_new"]), (y, i["d_y"])), given) if g]
+        wanted = [v for v in t if v.requires_grad]
+        got = torch.autograd.grad([p[0] for p in pairs], wanted, [p[1] for p in pairs], allow_unused=True)
+        return dict(zip([n for n, r in zip(names, need) if r], got))
+
+    for given in ((True, True), (True, False), (False, True)):
+        j = dict(i)
+        for n, g in zip(("d_new", "d_y"), given):
+            if not g:
+                j[n] = torch.zeros_like(i[n])
+        want = _formulas(j, 0.5, 1e-6)
+        every = run([True] * 5, given)
+        for n, g in every.items():
+            if g is None:
+                assert n == "next" and not given[1]
+            else:
+                _near(g, *want[n], steps=200)
+        for need in itertools.product([False, True], repeat=5):
+            if any(need) and not (need == (False,) * 4 + (True,) and not given[1]):
+                got = run(need, given)
+                assert all((g is None and every[n] is None) or torch.equal(g, every[n]) for n, g in got.items()), need
