@@ -136,6 +136,7 @@ int gated_args(const glm53_gated_mlp_desc* d, GatedArgs& a) {
   a.d_wu = static_cast<uint16_t*>(d->d_up_weight);
   a.d_wd = static_cast<uint16_t*>(d->d_down_weight);
   a.space = d->workspace;
+  a.space_bytes = d->workspace_bytes;
   const void* every[] = {a.x, a.wg, a.wu, a.wd, a.y, a.gate, a.up, a.h, a.dy, a.dx, a.d_wg, a.d_wu, a.d_wd};
   for (const void* p : every) CHECK_ARG(aligned(p, 16), "gated MLP tensors must be 16-byte aligned");
   CHECK_ARG((a.gate == nullptr) == (a.up == nullptr) && (a.gate == nullptr) == (a.h == nullptr),
@@ -220,6 +221,7 @@ int glm53_int4_linear(const glm53_int4_weight* w, const void* x, int64_t rows, v
   a.K = K;
   a.y = static_cast<uint16_t*>(y);
   a.space = workspace;
+  a.space_bytes = workspace_bytes;
   HIP_TRY(launch_int4(a, S(stream)), "4-bit linear launch");
   return GLM53_OK;
 }

@@ -24,7 +24,8 @@ struct GatedArgs {
   uint16_t* d_wg;
   uint16_t* d_wu;
   uint16_t* d_wd;
-  void* space;            // workspace of gated_space bytes, 256-byte aligned
+  void* space;            // workspace of gated_space bytes or more, 256-byte aligned
+  size_t space_bytes;
 };
 
 size_t gated_space(int64_t rows, int64_t hidden, int64_t inter, bool backward);

@@ -179,6 +179,7 @@ size_t plane_bytes(int64_t rows, int64_t inter) {
 struct Space {
   uint16_t *h, *dg, *du;
   float* partial;
+  int64_t room;  // floats at partial
 };
 Space carve(const GatedArgs& a, bool backward) {
   uint8_t* p = static_cast<uint8_t*>(a.space);
@@ -191,7 +192,9 @@ Space carve(const GatedArgs& a, bool backward) {
   } else if (s.h == nullptr) {
     s.h = reinterpret_cast<uint16_t*>(p);
   }
-  s.partial = reinterpret_cast<float*>(p + (backward ? 2 : 1) * plane);
+  const size_t before = (backward ? 2 : s.h == a.h ? 0 : 1) * plane;
+  s.partial = reinterpret_cast<float*>(p + before);
+  s.room = static_cast<int64_t>((a.space_bytes - before) / sizeof(float));
   return s;
 }
 
@@ -204,12 +207,14 @@ Gemm16Args gate_up(const GatedArgs& a, const Space& s) {
   g.gate = a.gate;
   g.up = a.up;
   g.partial = s.partial;
+  g.room = s.room;
   return g;
 }
 Gemm16Args down(const GatedArgs& a, const Space& s) {
   Gemm16Args g = product(a.inter);
   g.pair[0] = pair(s.h, a.inter, a.wd, a.inter, a.y, a.rows, a.hidden);
   g.partial = s.partial;
+  g.room = s.room;
   return g;
 }
 Gemm16Args hidden_grad(const GatedArgs& a, const Space& s) {
@@ -222,6 +227,7 @@ Gemm16Args hidden_grad(const GatedArgs& a, const Space& s) {
   g.d_up = s.du;
   g.low = parts(a.rows) == 2 ? a.rows * a.inter : 0;
   g.partial = s.partial;
+  g.room = s.room;
   return g;
 }
 Gemm16Args input_grad(const GatedArgs& a, const Space& s) {
@@ -233,6 +239,7 @@ Gemm16Args input_grad(const GatedArgs& a, const Space& s) {
     g.pair[g.segments++] = pair(s.du + at, a.inter, a.wu, a.hidden, a.dx, a.rows, a.hidden);
   }
   g.partial = s.partial;
+  g.room = s.room;
   return g;
 }
 Gemm16Pair weight_grad(const GatedArgs& a, const Space& s, int which, int part) {
@@ -246,6 +253,7 @@ Gemm16Pair weight_grad(const GatedArgs& a, const Space& s, int which, int part) 
 Gemm16Args weight_grads(const GatedArgs& a, const Space& s, int which) {
   Gemm16Args g = product(a.rows);
   g.partial = s.partial;
+  g.room = s.room;
   if (parts(a.rows) == 2) {
     g.segments = 2;
     for (int part = 0; part < 2; ++part) g.pair[part] = weight_grad(a, s, which, part);
@@ -270,8 +278,8 @@ size_t gated_space(int64_t rows, int64_t hidden, int64_t inter, bool backward) {
   const Space s{};
   if (backward) {
     int64_t partial = most({gemm16_plan(hidden_grad(a, s), false).partial, gemm16_plan(input_grad(a, s), false).partial});
-    for (int which : {1, 3, 7}) {  // one, two or all three of the products, which are of one size
-      if (which > 1 && parts(rows) == 2) break;
+    for (int which = 1; which < 8; ++which) {  // dWd is [hidden, inter], the others [inter, hidden]: their tiles differ
+      if (parts(rows) == 2 && (which & (which - 1)) != 0) continue;
       partial = most({partial, gemm16_plan(weight_grads(a, s, which), false).partial});
     }
     return 2 * plane + sizeof(float) * static_cast<size_t>(partial);

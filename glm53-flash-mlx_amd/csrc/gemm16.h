@@ -40,6 +40,7 @@ struct Gemm16Args {
   int segments;    // pairs whose contractions are added into pair[0].out
   int splits;      // parts of the contraction, each to `partial`
   float* partial;  // of each problem [splits][planes][m][partial_ld(n)], at partial_at floats
+  int64_t room;    // floats at partial
   int64_t partial_at[4];
   int64_t tiles;   // output tiles of all problems; tiles * splits below 2^31
   int group_m;     // tile rows that one XCD's neighbouring workgroups share
@@ -642,7 +643,9 @@ hipError_t gemm16_launch(Gemm16Args g, hipStream_t st) {
     at += plane * g.splits * (EPI == kSwiglu ? 2 : 1);
     most = most > plane ? most : plane;
   }
-  if (g.tiles * g.splits >= (int64_t{1} << 31) || most / 1024 >= (int64_t{1} << 31)) return hipErrorInvalidValue;
+  // a grid has fewer than 2^32 threads
+  if (g.tiles * g.splits * G::kThreads >= (int64_t{1} << 32) || (most / 1024 + 1) * 256 >= (int64_t{1} << 32)) return hipErrorInvalidValue;
+  if (g.splits > 1 && at > g.room) return hipErrorInvalidValue;
   gemm16_kernel<G><<<static_cast<uint32_t>(g.tiles * g.splits), G::kThreads, G::kLds, st>>>(g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || g.splits == 1) return e;
   const dim3 grid(static_cast<uint32_t>((most + 1023) / 1024), static_cast<uint32_t>(g.problems));
@@ -650,7 +653,7 @@ hipError_t gemm16_launch(Gemm16Args g, hipStream_t st) {
   return hipGetLastError();
 }
 
-// g's products in the plan's shape; g.partial has the plan's room.
+// g's products in the plan's shape.
 template <bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI>
 hipError_t gemm16(Gemm16Args g, const Gemm16Plan& plan, hipStream_t st) {
   g.splits = plan.splits;

@@ -17,7 +17,8 @@ struct Int4Args {
   int group_log2;         // 5, 6 or 7
   int64_t rows, N, K;
   uint16_t* y;            // [rows, N]
-  void* space;            // int4_space bytes
+  void* space;            // int4_space bytes or more
+  size_t space_bytes;
 };
 
 size_t int4_space(int64_t rows, int64_t N, int64_t K);

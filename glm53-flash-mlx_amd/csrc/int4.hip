@@ -347,12 +347,14 @@ hipError_t launch_int4(const Int4Args& a, hipStream_t st) {
     const Gemm16Plan plan = staged_plan(a);
     g.splits = plan.splits;
     g.partial = static_cast<float*>(a.space);
+    g.room = static_cast<int64_t>(a.space_bytes / sizeof(float));
     if (a.tables_f32) return gemm16_launch<Gemm16<1, 4, 4, 2, 2, false, kCodesF32, kBias>, kBias>(g, st);
     return gemm16_launch<Gemm16<1, 4, 4, 2, 2, false, kCodes, kBias>, kBias>(g, st);
   }
   uint16_t* w = static_cast<uint16_t*>(a.space);
   g.pair[0].b = w;
   g.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.space) + weight_bytes(a.N, a.K));
+  g.room = static_cast<int64_t>((a.space_bytes - weight_bytes(a.N, a.K)) / sizeof(float));
   const int64_t pieces = cdiv(a.N * (a.K >> 3), 256 * kExpand);
   if (pieces >= (int64_t{1} << 31)) return hipErrorInvalidValue;
   const uint32_t blocks = static_cast<uint32_t>(pieces);

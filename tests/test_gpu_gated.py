@@ -156,6 +156,36 @@ def test_wanted_gradients_alone(dev):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), need
 
 
+# Sizes at which dWd's product, whose sides are the other two's exchanged, is cut into more parts
+@pytest.mark.parametrize("rows, hidden, inter", [(3707, 1808, 16), (1436, 16, 1712), (1433, 3976, 32), (900, 64, 4000)])
+def test_wanted_gradients_stay_in_their_workspace(dev, monkeypatch, rows, hidden, inter):
+    import itertools
+
+    import torch
+
+    i = _weights(hidden, inter, rows)
+    native = submodule("_native")
+    guards = []
+
+    def workspace(nbytes, device):
+        room = torch.full((nbytes + 65536,), 165, dtype=torch.uint8, device=device)
+        guards.append(room[nbytes:])
+        return room[:nbytes]
+
+    monkeypatch.setattr(native, "workspace", workspace)
+    want = _formulas(i, 2.0)
+    names = ("x", "gate", "up", "down")
+    for need in itertools.product([False, True], repeat=4):
+        if not any(need):
+            continue
+        leaves = [i[n].detach().clone().requires_grad_(r) for n, r in zip(names, need)]
+        y = pkg().gated_mlp(*leaves, 2.0)
+        got = torch.autograd.grad(y, [t for t in leaves if t.requires_grad], i["dy"])
+        for n, g in zip([n for n, r in zip(names, need) if r], got):
+            _near(n, g, want[n])
+    assert all((g == 165).all() for g in guards)
+
+
 def test_gradients_against_differences(dev):
     """The slope along a direction in gate, up, down and x against the 64-bit
     formula's difference quotient: what the kernel's gradients are off by is
