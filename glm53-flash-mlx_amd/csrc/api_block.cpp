@@ -55,6 +55,11 @@ int norm_args(const glm53_norm* n, bool backward, NormArgs& a) {
     a.y = tensor(n->y, GLM53_NORM_F32_Y);
     CHECK_ARG(n->rows == 0 || (a.residual.p && (n->out == nullptr || a.new_residual.p)), "null pointer argument");
     CHECK_ARG(n->out != nullptr || n->y != nullptr, "nothing to compute: neither a block output nor y");
+    const auto over = [](const Tensor& result, const Tensor& input) {
+      return result.p != nullptr && result.p == input.p && result.f32 != input.f32;
+    };
+    CHECK_ARG(!over(a.new_residual, a.out) && !over(a.y, a.out) && !over(a.y, a.residual),
+              "a result in an input's place must have its type");
   } else {
     a.d_new = tensor(n->d_new_residual, GLM53_NORM_F32_RESIDUAL);
     a.d_y = tensor(n->d_y, GLM53_NORM_F32_Y);
@@ -201,7 +206,7 @@ int glm53_int4_linear(const glm53_int4_weight* w, const void* x, int64_t rows, v
             (long long)rows, (long long)N, (long long)K);
   CHECK_ARG(w->group == 32 || w->group == 64 || w->group == 128, "group must be 32, 64 or 128, got %d", w->group);
   CHECK_ARG(K % w->group == 0, "in_features %lld is not a multiple of the group %d", (long long)K, w->group);
-  CHECK_ARG(K <= kGatedMaxWidth && N < (int64_t{1} << 31), "weight too large");
+  CHECK_ARG(K <= kGatedMaxWidth && N <= kGatedMaxWidth, "weight too large: widths above %lld", (long long)kGatedMaxWidth);
   if (rows == 0) return GLM53_OK;
   CHECK_ARG(w->codes && w->scales && x && y, "null pointer argument");
   CHECK_ARG(aligned(w->codes, 16) && aligned(x, 16) && aligned(y, 16), "codes, x and y must be 16-byte aligned");

@@ -212,13 +212,13 @@ __device__ __forceinline__ void gate_values(const NormArgs& a, int64_t row, floa
 }
 
 template <int T, int C, Ends E, bool POST>
-__global__ __launch_bounds__(T) void norm_forward_kernel(NormArgs a) {
+__global__ __launch_bounds__(T) void norm_forward_kernel(NormArgs a, int64_t first) {
   using R = Row<T, C, E>;
   constexpr int N = R::kN;
   __shared__ float words[2][T / kWave];
   int turn = 0;
   const float inv_width = 1.0f / static_cast<float>(a.width);
-  const int64_t row = blockIdx.x, base = row * a.width;
+  const int64_t row = first + blockIdx.x, base = row * a.width;
   Raw rx[C], ro[C];
   R::raw(a.residual, base, a.width, rx);
   if (POST) R::raw(a.out, base, a.width, ro);
@@ -399,11 +399,14 @@ template <int T, int C, Ends E>
 hipError_t launch_shape(const NormArgs& a, bool backward, int64_t groups, int64_t slices, hipStream_t st) {
   const bool post = a.out.p != nullptr;
   if (!backward) {
-    const dim3 grid(static_cast<uint32_t>(a.rows));
-    if (post)
-      norm_forward_kernel<T, C, E, true><<<grid, T, 0, st>>>(a);
-    else
-      norm_forward_kernel<T, C, E, false><<<grid, T, 0, st>>>(a);
+    constexpr int64_t kMost = (int64_t{1} << 31) / T;  // a grid has fewer than 2^32 threads
+    for (int64_t first = 0; first < a.rows; first += kMost) {
+      const dim3 grid(static_cast<uint32_t>(a.rows - first < kMost ? a.rows - first : kMost));
+      if (post)
+        norm_forward_kernel<T, C, E, true><<<grid, T, 0, st>>>(a, first);
+      else
+        norm_forward_kernel<T, C, E, false><<<grid, T, 0, st>>>(a, first);
+    }
   } else {
     const dim3 grid(static_cast<uint32_t>(slices));
     if (post)

@@ -540,11 +540,11 @@ int glm53_prefill_plan_scratch(glm53_prefill_plan* plan, int32_t which, void** p
  *   new_residual = residual + scale * gate * s
  *   y = new_residual / rms(new_residual) * next_weight
  * with rms(v) = sqrt(mean(v^2) + eps), over contiguous rows of `width`
- * elements (at most 16384), aligned to their elements.  FP32 throughout, each output rounded once; y is made of
- * the new residual before it is rounded.  NULL: out (then y is the norm of
+ * elements (at most 16384), aligned to their elements.  FP32 throughout, each
+ * output rounded once; y is made of the new residual before it is rounded.  NULL: out (then y is the norm of
  * `residual` alone), post_weight and next_weight (ones), gate (one), y (not
  * computed), stats.  new_residual may be `residual` or `out` itself, y may be
- * `out` or (without out) `residual`.  stats f32 [rows, 2] keeps 1 / rms(out)
+ * `out` or (without out) `residual`, each where the types are the same.  stats f32 [rows, 2] keeps 1 / rms(out)
  * and 1 / rms(new_residual) for the backward call. */
 typedef struct glm53_norm {
   int64_t rows, width, rows_per_gate;
@@ -584,7 +584,7 @@ int glm53_residual_norm_backward(const glm53_norm* norm, void* stream);
  * ---------------------------------------------------------------------- */
 /*   G = x Wg^T, U = x Wu^T, h = silu(min(G, L)) clip(U, -L, L), y = h Wd^T
  * over contiguous BF16 tensors, 16-byte aligned; hidden and intermediate
- * multiples of 8; limit L > 0, INFINITY for none.  Sums, G, U and the
+ * multiples of 8 up to 2^22; limit L > 0, INFINITY for none.  Sums, G, U and the
  * activation are FP32, h and y are rounded once (up to 16 rows h not at all).
  * gate, up (f32) and h (BF16) [rows, intermediate]: all NULL, or where G, U
  * and h are kept for the gradients; up to 16 rows h has two planes, [2, rows,
@@ -627,7 +627,8 @@ int glm53_gated_mlp_backward(const glm53_gated_mlp_desc* desc, void* stream);
  * codes u8 [out, in / 2], column 2 j in the low half of byte j and 2 j + 1 in
  * the high half; scales and offsets [out, in / group], bias [out], all BF16 or
  * (tables_f32) all FP32; offsets NULL: -8 scale; bias NULL: none.  group 32,
- * 64 or 128, dividing in_features.  codes 16-byte aligned. */
+ * 64 or 128, dividing in_features; both widths up to 2^22.  codes 16-byte
+ * aligned. */
 typedef struct glm53_int4_weight {
   const uint8_t* codes;
   const void* scales;

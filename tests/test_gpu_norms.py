@@ -447,6 +447,24 @@ def test_offsets_past_32_bits(dev):
         _near(g, *want[n], steps=200)
 
 
+def test_more_rows_than_one_grid(dev):
+    """2^26 rows of 64 threads are the 2^32 that a grid may not have."""
+    import torch
+
+    M = pkg()
+    rows, width = 2**26 + 1025, 8
+    x = torch.randn(rows // 64 + 1, width, device=dev).to(torch.bfloat16).repeat(64, 1)[:rows]
+    period = x[:rows // 64 + 1]
+    got = M.rms_norm(x)
+    want = M.rms_norm(period)
+    d = period.double()
+    value = d / (d.square().mean(1, keepdim=True) + 1e-6).sqrt()
+    _near(want, value, value.abs(), steps=width + 8)
+    for first in range(0, rows, len(period)):
+        part = got[first:first + len(period)]
+        assert torch.equal(part, want[:len(part)]), first
+
+
 def test_no_second_derivative_is_claimed(dev):
     import torch
 
