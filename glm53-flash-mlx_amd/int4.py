@@ -98,6 +98,8 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 64, symmetric: bool = 
     scales = torch.where(scales == 0, torch.ones_like(scales), scales)
     offsets = None if symmetric else low.to(dtype)
     base = -8 * scales.float() if symmetric else offsets.float()
+    if not bool(torch.isfinite(base).all()) or not bool(torch.isfinite(base + 15 * scales.float()).all()):
+        raise ValueError(f"the weight's range does not fit {dtype} scales and offsets")
     q = ((v - base[:, :, None]) / scales.float()[:, :, None]).round_().clamp_(0, 15).to(torch.uint8).view(rows, cols)
     return (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous(), scales, offsets
 

@@ -39,6 +39,9 @@ def _norm(N, **changes):
     (dict(rows_per_gate=0), "rows_per_gate"), (dict(rows_per_gate=3), "rows_per_gate"),
     (dict(out=None), "without a block output"), (dict(post_norm=0), "post_weight"),
     (dict(residual=None), "null"), (dict(new_residual=None), "null"),
+    # rows of another type over rows that are still to be read
+    (dict(new_residual=FAKE, f32_mask=1), "type"), (dict(y=FAKE, f32_mask=32, new_residual=2 * FAKE), "type"),
+    (dict(out=None, gate=None, gate_kind=0, post_weight=None, post_norm=0, f32_mask=1), "type"),
     (dict(out=None, gate=None, gate_kind=0, post_weight=None, post_norm=0, y=None), "nothing to compute"),
 ])
 def test_norm_refusals(N, libso, changes, message):
@@ -112,6 +115,7 @@ def _int4(N, **changes):
     (dict(out_features=0), "invalid shape"), (dict(in_features=0), "invalid shape"), (dict(group=16), "group"),
     (dict(group=0), "group"), (dict(in_features=96), "multiple of the group"), (dict(codes=None), "null"),
     (dict(scales=None), "null"), (dict(codes=FAKE + 8), "aligned"), (dict(in_features=1 << 23), "too large"),
+    (dict(out_features=(1 << 22) + 1), "too large"),
 ])
 def test_int4_refusals(N, libso, changes, message):
     assert libso.glm53_int4_linear(_int4(N, **changes), FAKE, 4, FAKE, FAKE, 1 << 30, None) == N.INVALID_ARGUMENT
@@ -152,7 +156,8 @@ def test_quantize_int4_gives_the_nearest_codes():
             assert ((q * s + o)[0, 0] == 0).all()
     for bad in (lambda: M.quantize_int4(w, 48), lambda: M.quantize_int4(w[:, :96], 64), lambda: M.quantize_int4(w[0], 64),
                 lambda: M.quantize_int4(w.int(), 64), lambda: M.quantize_int4(w, 64, dtype=torch.float16),
-                lambda: M.quantize_int4(w / 0, 64), lambda: M.Int4Linear(96, 8, group_size=64),
+                lambda: M.quantize_int4(w / 0, 64), lambda: M.quantize_int4(w.sign() * 3e38, 64),
+                lambda: M.quantize_int4(w.sign() * 3.4e38, 64, True), lambda: M.Int4Linear(96, 8, group_size=64),
                 lambda: M.Int4MLP(M.Int4Linear(64, 64), M.Int4Linear(64, 64)),
                 lambda: M.Int4MLP.from_weights(w, w[:3], w.t())):
         with pytest.raises(ValueError):
