@@ -75,8 +75,8 @@ __device__ __forceinline__ float clamp_gate(float g, float limit) { return g > l
 __device__ __forceinline__ float clamp_up(float u, float limit) { return u > limit ? limit : u < -limit ? -limit : u; }
 
 __device__ __forceinline__ u32x2 pack_bf16x4(f32x4 v) {
-  return (u32x2){f32_to_bf16(v[0]) | static_cast<uint32_t>(f32_to_bf16(v[1])) << 16,
-                 f32_to_bf16(v[2]) | static_cast<uint32_t>(f32_to_bf16(v[3])) << 16};
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4));
 }
 
 // What `high` (bf16) leaves of f; an infinity or NaN is in the high part alone.
@@ -248,6 +248,25 @@ struct Stager {
   }
 };
 
+// The bf16 weights scale q + offset of 8 codes.  Each half's codes as bytes,
+// which one instruction turns into a float (the compiler, seeing that the
+// bytes are below 16, would take them out one by one first), and one rounding
+// instruction a pair: 23 instructions for 8 weights.
+__device__ __forceinline__ u32x4 weights_of(uint32_t v, float scale, float offset) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  uint32_t even = v & 0x0F0F0F0Fu, odd = (v >> 4) & 0x0F0F0F0Fu;
+  asm("" : "+v"(even), "+v"(odd));
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x2 p = {fmaf(static_cast<float>((even >> (8 * i)) & 0xFFu), scale, offset),
+                     fmaf(static_cast<float>((odd >> (8 * i)) & 0xFFu), scale, offset)};
+    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
+  }
+  return w;
+}
+
 // 4-bit rows into a row-form stage of R rows by T threads: a thread takes 32
 // codes (16 bytes, within one group) of a row, fetched a step ahead, and
 // writes them as bf16 w = scale q + offset.  That rounding, half a step of
@@ -290,17 +309,8 @@ struct CodeStager {
   __device__ __forceinline__ void write(uint8_t* stage, bool offsets) const {
     const float base = offsets ? offset : -8.0f * offset;
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const uint32_t even = codes[d] & 0x0F0F0F0Fu, odd = (codes[d] >> 4) & 0x0F0F0F0Fu;
-      u32x4 w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = fmaf(static_cast<float>((even >> (8 * i)) & 0xFFu), scale, base);
-        const float b = fmaf(static_cast<float>((odd >> (8 * i)) & 0xFFu), scale, base);
-        w[i] = f32_to_bf16(a) | static_cast<uint32_t>(f32_to_bf16(b)) << 16;
-      }
-      *reinterpret_cast<u32x4*>(stage + at + 16 * ((4 * half + d) ^ mix)) = w;
-    }
+    for (int d = 0; d < 4; ++d)
+      *reinterpret_cast<u32x4*>(stage + at + 16 * ((4 * half + d) ^ mix)) = weights_of(codes[d], scale, base);
   }
 };
 

@@ -85,7 +85,11 @@ __device__ __forceinline__ float table_load(const void* base, uint32_t off) {
   return bf16_to_f32(load_at<uint16_t>(base, off));
 }
 
-constexpr int64_t kFewXBytes = 32768;  // x of a phase in LDS
+// x of a phase that is put in LDS: more where several workgroups of a CU are
+// under way, one loading while another computes (8 x 4096 x 4096, one a CU, 64
+// KB: 7.6 us, and 7.0 from L2; 12 x 8192 x 2048, two, 48 KB: 7.3 and 8.1; 8 x
+// 8192 x 4096, 64 KB: 11.1 and 10.7).
+constexpr int64_t kFewXBytes = 32768, kFewXBytesMany = 49152;
 constexpr int kPhase = 8192;  // columns whose tables (and x) a workgroup has in LDS at a time
 
 // Table entries (scale, offset - 128 scale) of an output column and phase in
@@ -249,9 +253,21 @@ hipError_t launch_few_group(const Int4Args& a, hipStream_t st) {
   return launch_few<W, U, 7, XLDS>(a, st);
 }
 
+// Wavefronts a workgroup: 16 while the chip's 256 CUs have a workgroup or two
+// each, which 16 wavefronts keep in loads; with more workgroups fewer, whose
+// parts of the contraction are longer (x in LDS: 448 workgroups 8.3 us by 16,
+// 8.6 by 8; 896: 14.6, 13.2, by 4 14.0; 2,048: 18.6, 16.7, 14.1.  x from L2:
+// 256: 8.1, 8.7; 448: 11.2, 9.4, 10.8; 896: 27.0, 23.0, 23.3; 2,048: 39, 29, 26).
 hipError_t launch_few_rows(const Int4Args& a, hipStream_t st) {
-  if (2 * a.rows * (a.K < kPhase ? a.K : kPhase) <= kFewXBytes) return launch_few_group<16, 1, true>(a, st);
-  return launch_few_group<16, 1, false>(a, st);
+  const int64_t blocks = cdiv(a.N, 16);
+  if (2 * a.rows * (a.K < kPhase ? a.K : kPhase) <= (blocks <= 256 ? kFewXBytes : kFewXBytesMany)) {
+    if (blocks <= 512) return launch_few_group<16, 1, true>(a, st);
+    if (blocks <= 1024) return launch_few_group<8, 1, true>(a, st);
+    return launch_few_group<4, 1, true>(a, st);
+  }
+  if (blocks <= 256) return launch_few_group<16, 1, false>(a, st);
+  if (blocks <= 1024) return launch_few_group<8, 1, false>(a, st);
+  return launch_few_group<4, 1, false>(a, st);
 }
 
 }  // namespace
@@ -287,14 +303,7 @@ __global__ __launch_bounds__(256) void int4_expand_kernel(Int4Args a, uint16_t* 
     const int64_t at = first + u * 256 + threadIdx.x;
     if (at >= all) break;
     const float offset = a.offsets != nullptr ? second[u] : -8.0f * second[u];
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = fmaf(static_cast<float>((codes[u] >> (8 * i)) & 15u), scale[u], offset);
-      const float y = fmaf(static_cast<float>((codes[u] >> (8 * i + 4)) & 15u), scale[u], offset);
-      v[i] = f32_to_bf16(x) | static_cast<uint32_t>(f32_to_bf16(y)) << 16;
-    }
-    *reinterpret_cast<u32x4*>(w + 8 * at) = v;
+    *reinterpret_cast<u32x4*>(w + 8 * at) = weights_of(codes[u], scale[u], offset);
   }
 }
 

@@ -94,6 +94,14 @@ def test_larger(dev, rows, n, k, group):
     _check(_problem(rows, n, k, group))
 
 
+# 256, 512 and 1,024 workgroups, x of 32 and 48 KB and past it, tables of every kind
+@pytest.mark.parametrize("n", [4097, 8190, 8193, 16383, 16385])
+@pytest.mark.parametrize("rows, k, group", [(1, 1056, 32), (9, 2560, 128), (16, 1600, 64), (16, 2048, 32), (2, 8320, 64)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_many_workgroups(dev, n, rows, k, group, f32):
+    _check(_problem(rows, n, k, group, offsets=n % 2 == 1, f32=f32))
+
+
 def test_every_code_in_every_place(dev):
     """One-hot rows read each weight of a matrix that holds each code in each
     column: q, scale and offset chosen exact in bf16."""
