@@ -12,7 +12,7 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------- few rows ---
 //
-// Up to 16 rows: the call costs the codes' bytes.  A workgroup makes 16
+// Few rows: the call costs the codes' bytes.  A workgroup makes 16
 // output columns, its wavefronts taking parts of the contraction, joined in
 // LDS in their order; no code passes through LDS.  A lane loads 32 codes of
 // one row (16 bytes; a wavefront 64 bytes of each of 16 rows), the four
@@ -23,7 +23,16 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // is scaled once, sum x coming from an MFMA with ones: no weight is rounded.
 // Operands: rows of x as the MFMA's rows, so that a lane's four results have
 // one output column, one scale and one offset.
-constexpr int kFewRows = 16;
+//
+// 1 x 4096 x 4096, groups of 64: 5.9 us, 9 MB at 1.5 TB/s: a call this small is
+// bound by the launch and the first loads' way (8 wavefronts a workgroup 6.5
+// us, 4 8.9).  16 x 4096 x 7168: 12 us, x coming to every CU from L2.
+//
+// From 17 to 32 rows two MFMA rows share the codes, over at most 8,192
+// columns; wider outputs have enough tiles for the staged product below (32 x
+// 4096 x 4096 12.4 us here, 19.0 staged; 32 x 8192 x 2048 15.2, 16.8; 32 x
+// 14336 x 4096 44.8, 42.2).
+bool few(int64_t rows, int64_t N) { return rows <= 16 || (rows <= 32 && N <= 8192); }
 
 // Quarter q's dword s of four becomes quarter s's dword q.
 __device__ __forceinline__ void exchange_quarters(u32x4& v) {
@@ -93,10 +102,8 @@ constexpr int64_t kFewXBytes = 32768, kFewXBytesMany = 49152;
 constexpr int kPhase = 8192;  // columns whose tables (and x) a workgroup has in LDS at a time
 
 // Table entries (scale, offset - 128 scale) of an output column and phase in
-// LDS: its groups, then zeros for a block's groups.
-__host__ __device__ constexpr int few_table_groups(int columns, int group_log2) {
-  return ((columns + 127) / 128 << (7 - group_log2)) + (128 >> group_log2);
-}
+// LDS: its groups, zeros in the last block's place past them.
+__host__ __device__ constexpr int few_table_groups(int columns, int group_log2) { return (columns + 127) / 128 << (7 - group_log2); }
 
 // Entries from one column to the next: odd, so that the 16 columns' entries of a
 // group, which 16 lanes read at once, lie on different banks.
@@ -106,7 +113,7 @@ __host__ __device__ constexpr int few_table_ld(int columns, int group_log2) {
 
 // XLDS: x lies in LDS, [columns / 8][rows] pieces of 8 in the codes' order (few
 // rows, whose x fits); otherwise each wavefront reads its part from L2.
-template <int W, int U, int GROUP_LOG2, bool F32, bool OFFSETS, bool XLDS>
+template <int W, int MT, int GROUP_LOG2, bool F32, bool OFFSETS, bool XLDS>
 __global__ __launch_bounds__(64 * W) void int4_few_kernel(Int4Args a) {
   constexpr int kGroups = 128 >> GROUP_LOG2;     // groups of a block
   constexpr int kSteps = 1 << (GROUP_LOG2 - 5);  // MFMAs of a group
@@ -117,41 +124,47 @@ __global__ __launch_bounds__(64 * W) void int4_few_kernel(Int4Args a) {
   const int r = lane & 15, q = lane >> 4, K = static_cast<int>(a.K), rows = static_cast<int>(a.rows);
   const int64_t n0 = 16 * static_cast<int64_t>(blockIdx.x);
   const int cols = a.N - n0 < 16 ? static_cast<int>(a.N - n0) : 16;
-  const int nr = r < cols ? r : cols - 1, mr = r < rows ? r : rows - 1;
+  const int nr = r < cols ? r : cols - 1;
   const int groups = K >> GROUP_LOG2;
   // bases of the workgroup and a lane's byte offsets from them
   const uint8_t* codes = a.codes + n0 * (a.K >> 1);
   const uint8_t* scales = static_cast<const uint8_t*>(a.scales) + n0 * groups * kTable;
   const uint8_t* offsets = OFFSETS ? static_cast<const uint8_t*>(a.offsets) + n0 * groups * kTable : nullptr;
   const uint32_t code_off = static_cast<uint32_t>(nr) * (K >> 1);
-  const uint32_t x_off = static_cast<uint32_t>(mr) * (2 * K) + 16 * q;
+  int mr[MT];
+  uint32_t x_off[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    mr[i] = 16 * i + r < rows ? 16 * i + r : rows - 1;
+    x_off[i] = static_cast<uint32_t>(mr[i]) * (2 * K) + 16 * q;
+  }
   const int phase_columns = K < kPhase ? K : kPhase;
   f32x2* tables = reinterpret_cast<f32x2*>(lds);
   const int table_ld = few_table_ld(phase_columns, GROUP_LOG2);
   uint8_t* x_lds = lds + 128 * table_ld;
 
-  f32x4 total = {0, 0, 0, 0};
+  f32x4 total[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) total[i] = (f32x4){0, 0, 0, 0};
   const u32x4 one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
   const bf16x8 ones = __builtin_bit_cast(bf16x8, one);
   for (int k0 = 0; k0 < K; k0 += kPhase) {
     const int columns = K - k0 < kPhase ? K - k0 : kPhase;
     const int blocks = (columns + 127) / 128, each = (blocks + W - 1) / W;
     const int first = wave * each, last = first + each < blocks ? first + each : blocks;
-    // Codes and x of U blocks, without a branch: what lies past the
-    // wavefront's blocks or past K reads an address that is there and meets
-    // scale 0.  Branches around the steps would have the compiler move each
-    // step's loads behind them.
-    u32x4 code[2][U], xs[2][XLDS ? 1 : U][4];
+    // Codes and x of a block, without a branch: what lies past K reads an
+    // address that is there and meets scale 0.  Branches around the steps would
+    // have the compiler move each step's loads behind them.
+    u32x4 code[2], xs[2][XLDS ? 1 : MT][4];
     const auto load = [&](int b, int to) {
+      const int k = k0 + 128 * b;
+      const uint32_t piece = k + 128 <= K || k + 32 * q < K ? 16 * q : 0;
+      code[to] = load_at<u32x4>(codes, code_off + (k >> 1) + piece);
+      if constexpr (!XLDS) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int bb = b + u < last ? b + u : last - 1, k = k0 + 128 * bb;
-        const uint32_t piece = k + 128 <= K || k + 32 * q < K ? 16 * q : 0;
-        code[to][u] = load_at<u32x4>(codes, code_off + (k >> 1) + piece);
-        if constexpr (!XLDS) {
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int s = 0; s < 4; ++s) xs[to][u][s] = load_at<u32x4>(a.x, x_off + 2 * (k + 32 * s < K ? k + 32 * s : k));
-        }
+          for (int s = 0; s < 4; ++s) xs[to][i][s] = load_at<u32x4>(a.x, x_off[i] + 2 * (k + 32 * s < K ? k + 32 * s : k));
       }
     };
     if (first < last) load(first, 0);
@@ -173,84 +186,90 @@ __global__ __launch_bounds__(64 * W) void int4_few_kernel(Int4Args a) {
           *reinterpret_cast<bf16x8*>(x_lds + 16 * (c * rows + m)) = codes_order(load_at<u32x4>(a.x, 2 * (m * K + k0) + 16 * c));
     }
     __syncthreads();
-    const int zeros = entries - kGroups;
     const auto compute = [&](int b, int from) {
+      u32x4 cd = code[from];
+      exchange_quarters(cd);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool in = b + u < last;
-        u32x4 cd = code[from][u];
-        exchange_quarters(cd);
+      for (int g = 0; g < kGroups; ++g) {
+        const f32x2 t = tables[r * table_ld + b * kGroups + g];
+        f32x4 d[MT], sum[MT];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const f32x2 t = tables[r * table_ld + (in ? (b + u) * kGroups : zeros) + g];
-          f32x4 d = {0, 0, 0, 0}, sum = {0, 0, 0, 0};
+        for (int i = 0; i < MT; ++i) d[i] = sum[i] = (f32x4){0, 0, 0, 0};
 #pragma unroll
-          for (int s = g * kSteps; s < (g + 1) * kSteps; ++s) {
+        for (int s = g * kSteps; s < (g + 1) * kSteps; ++s) {
+          const bf16x8 w = codes_operand(cd[s]);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
             bf16x8 v;
             if constexpr (XLDS) {
-              const int at = in && 128 * (b + u) + 32 * s < columns ? 16 * (b + u) + 4 * s : 0;
-              v = *reinterpret_cast<const bf16x8*>(x_lds + 16 * ((at + q) * rows + mr));
+              const int at = 128 * b + 32 * s < columns ? 16 * b + 4 * s : 0;
+              v = *reinterpret_cast<const bf16x8*>(x_lds + 16 * ((at + q) * rows + mr[i]));
             } else {
-              v = codes_order(xs[from][u][s]);
+              v = codes_order(xs[from][i][s]);
             }
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, codes_operand(cd[s]), d, 0, 0, 0);
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ones, sum, 0, 0, 0);
+            d[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, w, d[i], 0, 0, 0);
+            sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ones, sum[i], 0, 0, 0);
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) total[i] += t[0] * d[i] + t[1] * sum[i];
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) total[i][e] += t[0] * d[i][e] + t[1] * sum[i][e];
       }
     };
-    for (int b = first; b < last; b += 2 * U) {
-      if (b + U < last) load(b + U, 1);
+    for (int b = first; b < last; b += 2) {
+      if (b + 1 < last) load(b + 1, 1);
       compute(b, 0);
-      if (b + 2 * U < last) load(b + 2 * U, 0);
-      if (b + U < last) compute(b + U, 1);
+      if (b + 2 < last) load(b + 2, 0);
+      if (b + 1 < last) compute(b + 1, 1);
     }
   }
   __syncthreads();  // the last phase is read; its place holds the partial sums
-  float(*part)[kFewRows][16] = reinterpret_cast<float(*)[kFewRows][16]>(lds);
+  float(*part)[16 * MT][16] = reinterpret_cast<float(*)[16 * MT][16]>(lds);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][4 * q + i][r] = total[i];
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave][16 * i + 4 * q + e][r] = total[i][e];
   __syncthreads();
-  if (threadIdx.x >= 16 * kFewRows) return;
-  const int col = threadIdx.x & 15, m = threadIdx.x >> 4;
-  if (m >= rows || col >= cols) return;
-  float y = part[0][m][col];
+  for (int at = threadIdx.x; at < 256 * MT; at += 64 * W) {
+    const int col = at & 15, m = at >> 4;
+    if (m >= rows || col >= cols) continue;
+    float y = part[0][m][col];
 #pragma unroll
-  for (int w = 1; w < W; ++w) y += part[w][m][col];
-  if (!(fabsf(y) < INFINITY))
-    y = one_output(a.x + m * a.K, codes + static_cast<int64_t>(col) * (K >> 1), scales + int64_t{col} * groups * kTable,
-                   OFFSETS ? offsets + int64_t{col} * groups * kTable : nullptr, F32, GROUP_LOG2, K);
-  if (a.bias != nullptr) y += table_value(a.bias, a.tables_f32, n0 + col);
-  a.y[m * a.N + n0 + col] = f32_to_bf16(y);
+    for (int w = 1; w < W; ++w) y += part[w][m][col];
+    if (!(fabsf(y) < INFINITY))
+      y = one_output(a.x + m * a.K, codes + static_cast<int64_t>(col) * (K >> 1), scales + int64_t{col} * groups * kTable,
+                     OFFSETS ? offsets + int64_t{col} * groups * kTable : nullptr, F32, GROUP_LOG2, K);
+    if (a.bias != nullptr) y += table_value(a.bias, a.tables_f32, n0 + col);
+    a.y[m * a.N + n0 + col] = f32_to_bf16(y);
+  }
 }
 
-template <int W, int U, int GROUP_LOG2, bool XLDS>
+template <int W, int MT, int GROUP_LOG2, bool XLDS>
 hipError_t launch_few(const Int4Args& a, hipStream_t st) {
   const dim3 grid(static_cast<uint32_t>(cdiv(a.N, 16))), block(64 * W);
   const int columns = static_cast<int>(a.K < kPhase ? a.K : kPhase);
   const size_t staged = 128 * few_table_ld(columns, GROUP_LOG2) + (XLDS ? 2 * static_cast<size_t>(a.rows * columns) : 0);
-  const size_t lds = staged > 1024 * W ? staged : 1024 * W;
+  const size_t lds = staged > 1024 * W * MT ? staged : 1024 * W * MT;
   if (a.tables_f32) {
     if (a.offsets != nullptr)
-      int4_few_kernel<W, U, GROUP_LOG2, true, true, XLDS><<<grid, block, lds, st>>>(a);
+      int4_few_kernel<W, MT, GROUP_LOG2, true, true, XLDS><<<grid, block, lds, st>>>(a);
     else
-      int4_few_kernel<W, U, GROUP_LOG2, true, false, XLDS><<<grid, block, lds, st>>>(a);
+      int4_few_kernel<W, MT, GROUP_LOG2, true, false, XLDS><<<grid, block, lds, st>>>(a);
   } else {
     if (a.offsets != nullptr)
-      int4_few_kernel<W, U, GROUP_LOG2, false, true, XLDS><<<grid, block, lds, st>>>(a);
+      int4_few_kernel<W, MT, GROUP_LOG2, false, true, XLDS><<<grid, block, lds, st>>>(a);
     else
-      int4_few_kernel<W, U, GROUP_LOG2, false, false, XLDS><<<grid, block, lds, st>>>(a);
+      int4_few_kernel<W, MT, GROUP_LOG2, false, false, XLDS><<<grid, block, lds, st>>>(a);
   }
   return hipGetLastError();
 }
 
-template <int W, int U, bool XLDS>
+template <int W, int MT, bool XLDS>
 hipError_t launch_few_group(const Int4Args& a, hipStream_t st) {
-  if (a.group_log2 == 5) return launch_few<W, U, 5, XLDS>(a, st);
-  if (a.group_log2 == 6) return launch_few<W, U, 6, XLDS>(a, st);
-  return launch_few<W, U, 7, XLDS>(a, st);
+  if (a.group_log2 == 5) return launch_few<W, MT, 5, XLDS>(a, st);
+  if (a.group_log2 == 6) return launch_few<W, MT, 6, XLDS>(a, st);
+  return launch_few<W, MT, 7, XLDS>(a, st);
 }
 
 // Wavefronts a workgroup: 16 while the chip's 256 CUs have a workgroup or two
@@ -260,6 +279,7 @@ hipError_t launch_few_group(const Int4Args& a, hipStream_t st) {
 // 256: 8.1, 8.7; 448: 11.2, 9.4, 10.8; 896: 27.0, 23.0, 23.3; 2,048: 39, 29, 26).
 hipError_t launch_few_rows(const Int4Args& a, hipStream_t st) {
   const int64_t blocks = cdiv(a.N, 16);
+  if (a.rows > 16) return launch_few_group<8, 2, false>(a, st);
   if (2 * a.rows * (a.K < kPhase ? a.K : kPhase) <= (blocks <= 256 ? kFewXBytes : kFewXBytesMany)) {
     if (blocks <= 512) return launch_few_group<16, 1, true>(a, st);
     if (blocks <= 1024) return launch_few_group<8, 1, true>(a, st);
@@ -307,11 +327,11 @@ __global__ __launch_bounds__(256) void int4_expand_kernel(Int4Args a, uint16_t* 
   }
 }
 
-// From 17 to this many rows the codes become weights in the tiled product's own
+// Up to this many rows the codes become weights in the tiled product's own
 // stage, tile row by tile row; beyond, in memory once, for the product of bf16
 // weights, whose larger tiles the conversion would hold up (4096 x 4096: 64
-// rows 23 us staged, 32 expanded; 128 rows 35 and 38; 300 rows 66 and 45;
-// 2,048 rows 110 and 81).
+// rows 21 us staged, 27 expanded; 128 rows 29 and 30; 200 rows 44 and 33; 300
+// rows 75 and 39).
 constexpr int64_t kStagedRows = 128;
 
 Gemm16Args product(const Int4Args& a) {
@@ -340,7 +360,7 @@ size_t weight_bytes(int64_t N, int64_t K) { return (2 * static_cast<size_t>(N) *
 }  // namespace
 
 size_t int4_space(int64_t rows, int64_t N, int64_t K) {
-  if (rows <= kFewRows) return 0;
+  if (few(rows, N)) return 0;
   Int4Args a{};
   a.rows = rows;
   a.N = N;
@@ -350,7 +370,7 @@ size_t int4_space(int64_t rows, int64_t N, int64_t K) {
 }
 
 hipError_t launch_int4(const Int4Args& a, hipStream_t st) {
-  if (a.rows <= kFewRows) return launch_few_rows(a, st);
+  if (few(a.rows, a.N)) return launch_few_rows(a, st);
   Gemm16Args g = product(a);
   if (a.rows <= kStagedRows) {
     const Gemm16Plan plan = staged_plan(a);

@@ -19,7 +19,7 @@ from . import _native as N
 from . import ops as _ops
 
 GROUP_SIZES = (32, 64, 128)
-FEW_ROWS = 16  # up to here the codes are multiplied as they are, and no workspace is taken
+FEW_ROWS = 16  # up to here no call takes a workspace
 
 
 def int4_linear(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor | None = None,
@@ -66,7 +66,7 @@ def native_int4_linear(x, weight, scales, offsets, bias):
         return y
     lib = N.lib()
     ws, ws_bytes = None, 0
-    if rows > FEW_ROWS:  # fewer take no workspace
+    if rows > FEW_ROWS:
         ws_bytes = lib.glm53_int4_linear_workspace_bytes(rows, out_features, in_features)
         ws = N.workspace(ws_bytes, x.device)
     w = N.Int4Weight(weight.data_ptr(), scales.data_ptr(), None if offsets is None else offsets.data_ptr(),

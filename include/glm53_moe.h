@@ -639,9 +639,9 @@ typedef struct glm53_int4_weight {
   int32_t tables_f32;
 } glm53_int4_weight;
 /* y[m] = T(x[m] . W^T + bias), x BF16 [rows, in], y BF16 [rows, out], both
- * contiguous and 16-byte aligned; FP32 sums.  Up to 16 rows multiply by the
- * codes themselves and scale the group sums in FP32; more rows multiply by W
- * rounded to BF16.  Workspace (256-byte aligned; NULL where 0 bytes) needs no
+ * contiguous and 16-byte aligned; FP32 sums.  Up to 16 rows, and up to 32
+ * over at most 8192 outputs, multiply by the codes themselves and scale the
+ * group sums in FP32; others multiply by W rounded to BF16.  Workspace (256-byte aligned; NULL where 0 bytes) needs no
  * initialisation. */
 size_t glm53_int4_linear_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features);
 int glm53_int4_linear(const glm53_int4_weight* weight, const void* x, int64_t rows, void* y, void* workspace,
