@@ -24,11 +24,13 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // ------------------------------------------------------------- few rows ---
 //
-// Up to 16 rows: the call costs the weights' bytes.  A workgroup makes 16
+// Few rows: the call costs the weights' bytes.  A workgroup makes 16
 // weight rows' results, its wavefronts taking parts of the contraction, joined
 // in LDS in their order; weights go from memory to the MFMA through registers
 // alone, a wavefront's loads all under way at once.  Rows of x are the MFMA's
-// rows, so a lane's four results belong to one weight row.
+// rows, so a lane's four results belong to one weight row.  1 x 4096 x 2048:
+// 8.8 us for gate and up, 5.6 for down, 50 MB at 3.5 TB/s; 1 x 7168 x 18432: 153
+// us, 5.2 TB/s.
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 16;
 // K steps of 32 that a wavefront has in flight (1 x 4096 x 2048 by 16 wavefronts: 2
@@ -43,18 +45,22 @@ struct Int {
 // y[m, n] = sum_k x[m, k] w(n)[k] of the 16 rows that row(n) gives, per wavefront
 // into part.  X: float rows are split into two bf16 operands, whose products
 // are added: no rounding of x.
-template <class X>
-__device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w_row, int K, float (*part)[16][16]) {
+template <int MT, class X>
+__device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w_row, int K, float (*part)[16 * MT][16]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int steps = (K + 31) / 32, each = (steps + kFewWaves - 1) / kFewWaves;
   const int first = wave * each, last = first + each < steps ? first + each : steps;
-  const X* x_row = x + static_cast<int64_t>(r < rows ? r : rows - 1) * K + 8 * q;
+  const X* x_row[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) x_row[i] = x + static_cast<int64_t>(16 * i + r < rows ? 16 * i + r : rows - 1) * K + 8 * q;
   w_row += 8 * q;
-  f32x4 acc = {0, 0, 0, 0};
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = (f32x4){0, 0, 0, 0};
   constexpr bool kFloat = sizeof(X) == 4;
   constexpr int kHalves = kFloat ? 2 : 1;
-  const auto multiply = [&](const u32x4 (&v)[kHalves], const u32x4& w, bool in) {
+  const auto multiply = [&](f32x4& acc, const u32x4 (&v)[kHalves], const u32x4& w, bool in) {
     const u32x4 zero = {0, 0, 0, 0};
     const bf16x8 b = __builtin_bit_cast(bf16x8, in ? w : zero);
     if constexpr (kFloat) {
@@ -75,17 +81,20 @@ __device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w
   // U whole steps, every load on its way before the first is used
   const auto batch = [&](int s, auto count) {
     constexpr int U = decltype(count)::value;
-    u32x4 w[U], v[U][kHalves];
+    u32x4 w[U], v[U][MT][kHalves];
     const uint16_t* wb = w_row + 32 * s;
-    const X* xb = x_row + 32 * s;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       w[u] = *reinterpret_cast<const u32x4*>(wb + 32 * u);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) v[u][h] = *reinterpret_cast<const u32x4*>(xb + 32 * u + 4 * h);
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) v[u][i][h] = *reinterpret_cast<const u32x4*>(x_row[i] + 32 * s + 32 * u + 4 * h);
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) multiply(v[u], w[u], true);
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) multiply(acc[i], v[u][i], w[u], true);
   };
   int s = first;
   const int whole_last = last < K / 32 ? last : K / 32;
@@ -94,18 +103,24 @@ __device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w
   if (s < last) {  // the end of K: what lies past it reads the step's first columns and is left out
     const bool in = 32 * s + 8 * q < K;
     const int at = in ? 32 * s : 32 * s - 8 * q;
-    u32x4 v[kHalves];
     const u32x4 w = *reinterpret_cast<const u32x4*>(w_row + at);
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) v[h] = *reinterpret_cast<const u32x4*>(x_row + at + 4 * h);
-    multiply(v, w, in);
+    for (int i = 0; i < MT; ++i) {
+      u32x4 v[kHalves];
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) v[h] = *reinterpret_cast<const u32x4*>(x_row[i] + at + 4 * h);
+      multiply(acc[i], v, w, in);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][4 * q + i][r] = acc[i];
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[wave][16 * i + 4 * q + e][r] = acc[i][e];
   __syncthreads();
 }
 
-__device__ __forceinline__ float few_sum(const float (*part)[16][16], int m, int n) {
+template <int MT>
+__device__ __forceinline__ float few_sum(const float (*part)[16 * MT][16], int m, int n) {
   float v = part[0][m][n];
 #pragma unroll
   for (int w = 1; w < kFewWaves; ++w) v += part[w][m][n];
@@ -113,16 +128,17 @@ __device__ __forceinline__ float few_sum(const float (*part)[16][16], int m, int
 }
 
 // 8 gate and the 8 up rows of the same outputs a workgroup; h stays FP32.
+template <int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_gate_up_kernel(GatedArgs a, float* h) {
-  __shared__ float part[kFewWaves][16][16];
+  __shared__ float part[kFewWaves][16 * MT][16];
   const int r = threadIdx.x & 15;
   const int64_t n0 = 8 * static_cast<int64_t>(blockIdx.x);
   const uint16_t* w = (r < 8 ? a.wg : a.wu) + (n0 + (r & 7)) * a.hidden;
-  few_rows(a.x, static_cast<int>(a.rows), w, static_cast<int>(a.hidden), part);
-  if (threadIdx.x >= 128) return;
+  few_rows<MT>(a.x, static_cast<int>(a.rows), w, static_cast<int>(a.hidden), part);
+  if (threadIdx.x >= 128 * MT) return;
   const int n = threadIdx.x & 7, m = threadIdx.x >> 3;
   if (m >= a.rows) return;
-  const float gate = few_sum(part, m, n), up = few_sum(part, m, 8 + n);
+  const float gate = few_sum<MT>(part, m, n), up = few_sum<MT>(part, m, 8 + n);
   const int64_t at = m * a.inter + n0 + n;
   if (a.gate != nullptr) {
     a.gate[at] = gate;
@@ -133,26 +149,37 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_gate_up_kernel(GatedArgs a
   if (a.h != nullptr) {
     const uint16_t high = f32_to_bf16(v);
     a.h[at] = high;
-    a.h[a.rows * a.inter + at] = f32_to_bf16(low_part(v, high));
+    if (MT == 1) a.h[a.rows * a.inter + at] = f32_to_bf16(low_part(v, high));
   }
 }
 
+template <int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_down_kernel(GatedArgs a, const float* h) {
-  __shared__ float part[kFewWaves][16][16];
+  __shared__ float part[kFewWaves][16 * MT][16];
   const int64_t n0 = 16 * static_cast<int64_t>(blockIdx.x);
   const int r = threadIdx.x & 15, cols = a.hidden - n0 < 16 ? 8 : 16;  // hidden is a multiple of 8
-  few_rows(h, static_cast<int>(a.rows), a.wd + (n0 + (r < cols ? r : cols - 1)) * a.inter, static_cast<int>(a.inter), part);
-  if (threadIdx.x >= 256) return;
+  few_rows<MT>(h, static_cast<int>(a.rows), a.wd + (n0 + (r < cols ? r : cols - 1)) * a.inter, static_cast<int>(a.inter), part);
+  if (threadIdx.x >= 256 * MT) return;
   const int n = threadIdx.x & 15, m = threadIdx.x >> 4;
-  if (m < a.rows && n < cols) a.y[m * a.hidden + n0 + n] = f32_to_bf16(few_sum(part, m, n));
+  if (m < a.rows && n < cols) a.y[m * a.hidden + n0 + n] = f32_to_bf16(few_sum<MT>(part, m, n));
 }
 
+template <int MT>
 hipError_t launch_few(const GatedArgs& a, hipStream_t st) {
   float* h = static_cast<float*>(a.space);
-  few_gate_up_kernel<<<static_cast<uint32_t>(a.inter / 8), 64 * kFewWaves, 0, st>>>(a, h);
+  few_gate_up_kernel<MT><<<static_cast<uint32_t>(a.inter / 8), 64 * kFewWaves, 0, st>>>(a, h);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  few_down_kernel<<<static_cast<uint32_t>(cdiv(a.hidden, 16)), 64 * kFewWaves, 0, st>>>(a, h);
+  few_down_kernel<MT><<<static_cast<uint32_t>(cdiv(a.hidden, 16)), 64 * kFewWaves, 0, st>>>(a, h);
   return hipGetLastError();
+}
+
+// From 17 to 32 rows two MFMA rows share the weights, while no kernel has more
+// than a workgroup a CU; x and h, which come to every workgroup from L2, then
+// cost more than the tiled product's partial results (17 and 32 rows, 4096 x
+// 2048: 21 and 27 us here, 28 and 30 tiled; 4096 x 4096: 37 and 48, 36 and 37;
+// 24 rows, 7168 x 2048: 42, 36).
+bool few(int64_t rows, int64_t hidden, int64_t inter) {
+  return rows <= kFewRows || (rows <= 32 && hidden <= 4096 && inter <= 2048);
 }
 
 Gemm16Pair pair(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb, uint16_t* out, int64_t m, int64_t n) {
@@ -284,13 +311,13 @@ size_t gated_space(int64_t rows, int64_t hidden, int64_t inter, bool backward) {
     }
     return 2 * plane + sizeof(float) * static_cast<size_t>(partial);
   }
-  if (rows <= kFewRows) return plane;  // h in FP32: the size of its two parts
+  if (few(rows, hidden, inter)) return round_up(4 * static_cast<size_t>(rows) * static_cast<size_t>(inter));  // h in FP32
   const int64_t partial = most({gemm16_plan(gate_up(a, s), true).partial, gemm16_plan(down(a, s), false).partial});
   return plane + sizeof(float) * static_cast<size_t>(partial);
 }
 
 hipError_t launch_gated(const GatedArgs& a, hipStream_t st) {
-  if (a.rows <= kFewRows) return launch_few(a, st);
+  if (few(a.rows, a.hidden, a.inter)) return a.rows <= kFewRows ? launch_few<1>(a, st) : launch_few<2>(a, st);
   const Space s = carve(a, false);
   const Gemm16Args g = gate_up(a, s), d = down(a, s);
   if (hipError_t e = gemm16<false, kRow, kSwiglu>(g, gemm16_plan(g, true), st); e != hipSuccess) return e;

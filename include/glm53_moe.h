@@ -585,7 +585,8 @@ int glm53_residual_norm_backward(const glm53_norm* norm, void* stream);
 /*   G = x Wg^T, U = x Wu^T, h = silu(min(G, L)) clip(U, -L, L), y = h Wd^T
  * over contiguous BF16 tensors, 16-byte aligned; hidden and intermediate
  * multiples of 8 up to 2^22; limit L > 0, INFINITY for none.  Sums, G, U and the
- * activation are FP32, h and y are rounded once (up to 16 rows h not at all).
+ * activation are FP32, h and y are rounded once (h not at all up to 16
+ * rows, and up to 32 where hidden is at most 4096 and intermediate 2048).
  * gate, up (f32) and h (BF16) [rows, intermediate]: all NULL, or where G, U
  * and h are kept for the gradients; up to 16 rows h has two planes, [2, rows,
  * intermediate], what BF16 leaves of h in the second. */

@@ -138,6 +138,12 @@ def test_larger(dev, hidden, inter, rows):
     _check(_weights(hidden, inter, rows, std=0.02), 10.0)
 
 
+@pytest.mark.parametrize("hidden, inter", [(4096, 2048), (4104, 2048), (4096, 2056), (8, 2048), (4096, 8), (104, 1000)])
+@pytest.mark.parametrize("rows", [17, 24, 32])
+def test_rows_of_two_mfma_tiles(dev, hidden, inter, rows):
+    _check(_weights(hidden, inter, rows, seed=rows, std=0.02), 2.0)
+
+
 def test_wanted_gradients_alone(dev):
     """Each subset of leaves gets the gradients that all of them get."""
     import itertools
