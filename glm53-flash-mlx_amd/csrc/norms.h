@@ -34,7 +34,7 @@ struct NormArgs {
   // backward: gradients given (null: zero) and wanted (null: not written)
   Tensor d_new, d_y;
   Tensor d_residual, d_out, d_post, d_gate, d_next;
-  float* partial;       // [slices(), sums(), width]
+  float* partial;       // [norm_slices, kNormSums, width]
 };
 
 constexpr int64_t kNormMaxWidth = 16384;  // rows whose values a workgroup holds in registers

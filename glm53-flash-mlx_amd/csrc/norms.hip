@@ -30,7 +30,8 @@ struct Raw {
 // How a row's last elements are taken where the width is no multiple of kVec.
 // kWhole: it is one.  kOverlap: the last load is the row's last kVec elements,
 // whose first ones another thread has too: both compute and store the same
-// values for them, and one of the two leaves them out of the row's sums.
+// values for them, and one of the two leaves them out of the row's sums (8,192
+// x 2,050 forward: 52 us, 108 with single elements).
 // kSingly (rows shorter than kVec): one by one.
 enum Ends { kWhole, kOverlap, kSingly };
 
@@ -211,6 +212,10 @@ __device__ __forceinline__ void gate_values(const NormArgs& a, int64_t row, floa
   }
 }
 
+// One row a workgroup.  Bound by its bytes from about 1,000 rows on: 2,048 x
+// 4096, FP32 in and bf16 out, 10.9 us, 4.6 TB/s; 8,192 x 4096 bf16 behind a block
+// 57 to 63 us, 4.3 to 4.7 TB/s (a 4 GiB copy: 4.7).  One row costs a launch and
+// the way of two dependent sums, 5.2 us.
 template <int T, int C, Ends E, bool POST>
 __global__ __launch_bounds__(T) void norm_forward_kernel(NormArgs a, int64_t first) {
   using R = Row<T, C, E>;
@@ -266,7 +271,8 @@ __device__ __forceinline__ Slice slice_rows(int64_t rows, int64_t groups, int64_
 // Each workgroup takes a run of rows and keeps the column sums of d_post,
 // d_gate (kGateColumns) and d_next in registers, written once as one row of
 // fp32 partial sums: 3 width floats against 16 rows or more of five tensors.
-// The order of the sums is the rows', whatever runs when.
+// The order of the sums is the rows', whatever runs when.  8,192 x 4096 bf16 with
+// all gradients: 85 to 94 us, 403 MB at 4.3 to 4.7 TB/s.
 template <int T, int C, Ends E, bool POST>
 __global__ __launch_bounds__(T) void norm_backward_kernel(NormArgs a, int64_t groups, int64_t slices) {
   using R = Row<T, C, E>;
@@ -371,7 +377,8 @@ __global__ __launch_bounds__(T) void norm_backward_kernel(NormArgs a, int64_t gr
 
 // Adds the partial rows: out[v][column] = sum over rows first_v .. of sum v,
 // blockIdx.y = 0 d_next, 1 d_post, 2 + g d_gate of gate group g.  16 row
-// slices of 64 columns a workgroup, joined in LDS in their order.
+// slices of 64 columns a workgroup, joined in LDS in their order.  512 slices of
+// 4096 columns: 5.4 us.
 constexpr int kJoin = 16;
 __global__ __launch_bounds__(kWave* kJoin) void norm_join_kernel(NormArgs a, int64_t groups, int64_t slices) {
   __shared__ float part[kJoin][kWave];
@@ -417,7 +424,10 @@ hipError_t launch_shape(const NormArgs& a, bool backward, int64_t groups, int64_
   return hipGetLastError();
 }
 
-// Threads a row, so that each holds one or two loads of every tensor.
+// Threads a row, so that each holds one or two loads of every tensor: more
+// threads leave lanes without elements, more loads a thread take the registers
+// of half the wavefronts.  Narrow rows on 64 and 128 threads, the next row read
+// ahead, against 256 threads: 8,192 x 256 backward 46 -> 25 us, x 1,024 59 -> 38.
 int row_threads(int64_t width) { return width <= 512 ? 64 : width <= 1024 ? 128 : width <= 4096 ? 256 : width <= 8192 ? 512 : 1024; }
 
 template <Ends E>
