@@ -5,7 +5,7 @@
 //
 // A workgroup computes a BM x BN tile, its wavefronts a grid of them.  Each K
 // step of 64 stages both operands in LDS while the step before is
-// multiplied (two stages, one barrier a step).  An operand is stored either
+// multiplied (two or three stages, one barrier a step).  An operand is stored either
 // with k contiguous (rows of 64 k: "row" form) or with m or n contiguous
 // ("column" form, the contraction over rows: gradients), which is read from
 // LDS by the transposing ds_read_b64_tr_b16, so no operand is ever
@@ -199,10 +199,11 @@ __device__ __forceinline__ void load_lds16(const void* base, uint32_t off, uint3
                : "memory", "m0");
 }
 
-// All of this wavefront's loads and LDS accesses are done, and every
-// wavefront of the workgroup is here.
+// All of this wavefront's LDS accesses and all but its last LEFT loads are done
+// (loads return in their order), and every wavefront of the workgroup is here.
+template <int LEFT>
 __device__ __forceinline__ void stage_wait() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
 // The share of one wavefront in staging an operand tile of R rows (row form)
@@ -382,7 +383,13 @@ struct Gemm16 {
   static constexpr bool kPairB = EPI == kSwiglu;           // half the tile gate columns, half up
   static constexpr int kColumns = kPairB ? BN / 2 : BN;    // output columns of a tile
   static constexpr int kStageA = BM * 128, kBlock = kStageA + BN * 128, kStage = SUB * kBlock;
-  static constexpr int kLds = 2 * kStage;
+  // Small tiles multiply a stage in less than its loads' way, and one workgroup
+  // fills a CU's LDS anyway: a third stage, loaded two steps ahead.  Codes, which
+  // pass through registers, are one step ahead.
+  static constexpr int kStages = SUB == 2 && !kFromCodes ? 3 : 2;
+  static constexpr int kLds = kStages * kStage;
+  // direct loads of a wavefront and stage
+  static constexpr int kStageLoads = SUB * (BM + BN) / 8 / W;
 
   static constexpr int kReadA = A_COLUMN ? 2 : 1, kReadB = B_COLUMN ? 2 : 1;  // LDS reads of an operand
   static constexpr int kAhead = 2;
@@ -466,6 +473,9 @@ struct Gemm16 {
     const int64_t next_a = A_COLUMN ? kStepK * p.lda : kStepK, next_b = B_COLUMN ? kStepK * p.ldb : kStepK;
     const auto issue = [&](int slot) {
       const bool partial = tail != 0 && left == 1;
+      // the count that stage_wait leaves open is of direct loads: none older than
+      // a partial stage, of which a wavefront may have no load at all
+      if (kStages > 2 && partial) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
         const uint32_t at = slot * kStage + u * kBlock;
@@ -510,14 +520,20 @@ struct Gemm16 {
         if (first + 1 < last) fetch_codes(first + 1);
       }
     }
-    if (first < last) issue(0);
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s)
+      if (first + s < last) issue(s);
     int slot = 0;
-    for (int step = first; step < last; ++step, slot ^= 1) {
-      stage_wait();
+    for (int step = first; step < last; ++step, slot = slot + 1 < kStages ? slot + 1 : 0) {
+      // the stage after this one may still be on its way
+      if (kStages == 3 && step + 1 < last)
+        stage_wait<kStages == 3 ? kStageLoads : 0>();
+      else
+        stage_wait<0>();
       if constexpr (kFromCodes) {  // codes before the direct loads: the compiler's wait for them drains both
         if (step + 1 < last) write_codes(slot ^ 1);
       }
-      if (step + 1 < last) issue(slot ^ 1);
+      if (step + kStages - 1 < last) issue(slot > 0 ? slot - 1 : kStages - 1);  // the stage read a step ago
       if constexpr (kFromCodes) {
         if (step + 2 < last) fetch_codes(step + 2);
       }
