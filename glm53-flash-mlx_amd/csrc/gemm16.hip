@@ -12,7 +12,7 @@ struct Shape {
   int64_t slots;
   float step_us, step_full_us, fixed_us;
 };
-constexpr Shape kShapes[] = {{kTile64, 64, 128, 128, 256, 1.3f, 1.3f, 4.0f},
+constexpr Shape kShapes[] = {{kTile64, 64, 128, 128, 256, 1.1f, 1.1f, 4.0f},
                              {kTile128, 128, 128, 64, 512, 0.95f, 1.05f, 6.0f},
                              {kTile256, 256, 256, 64, 256, 1.6f, 1.6f, 12.0f}};
 
@@ -30,7 +30,7 @@ int64_t tiles_of(const Gemm16Args& g, const Shape& s, int planes) {
 // measured over 16 to 8,192 rows, 1,000 to 8,192 columns and contractions of
 // 1,000 to 8,192 (bf16, row form):
 //   tile        a step    workgroups at once   and, once a round
-//   64 x 128    1.3 us of 128 k   256 (1 a CU)   4 us
+//   64 x 128    1.1 us of 128 k   256 (1 a CU)   4 us
 //   128 x 128   0.95 to 1.05 of 64   512 (2 a CU)   6 us
 //   256 x 256   1.6 us of 64      256 (1 a CU)   12 us
 // The large tile has the best rate (1.35 PFLOP/s between its start and end)
