@@ -14,9 +14,9 @@
 // Bound by the matrix pipes where the tiles fill the chip: a step of a 256 x 256
 // tile takes 1.45 to 1.6 us on every CU, 1.35 to 1.48 PFLOP/s (the library's
 // product of 8192^3: 1.35), and ~12 us a tile go to its first loads and its
-// epilogue.  8,192 rows, 4096 x 2048: gate and up with SwiGLU 253 us, 1.09
-// PFLOP/s, down 127, SwiGLU's gradient 160, x's gradient over both segments
-// 238, 1.15 PFLOP/s, dWg and dWu together 233, 1.18.
+// epilogue.  8,192 rows, 4096 x 2048: gate and up with SwiGLU 247 us, 1.11
+// PFLOP/s, down 123, SwiGLU's gradient 160, x's gradient over both segments
+// 232, 1.18 PFLOP/s, dWg and dWu together 226, 1.22.
 #pragma once
 
 #include "common.h"
