@@ -630,15 +630,32 @@ __global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
   const int64_t ldp = partial_ld(p.n), plane = p.m * ldp, at = 4 * (blockIdx.x * int64_t{256} + threadIdx.x);
   if (at >= plane) return;
   constexpr int kPlanes = EPI == kSwiglu ? 2 : 1;
-  f32x4 v[kPlanes];
-#pragma unroll
-  for (int h = 0; h < kPlanes; ++h) {
-    v[h] = *reinterpret_cast<const f32x4*>(partial + h * plane + at);
-    for (int s = 1; s < g.splits; ++s)
-      v[h] += *reinterpret_cast<const f32x4*>(partial + (s * kPlanes + h) * plane + at);
-  }
   const int64_t m = at / ldp, n = at % ldp;
   if (n >= p.n) return;
+  f32x4 gate, up;
+  if constexpr (EPI == kSwigluGrad) {
+    gate = *reinterpret_cast<const f32x4*>(g.gate + m * p.n + n);
+    up = *reinterpret_cast<const f32x4*>(g.up + m * p.n + n);
+  }
+  // four splits' loads on their way at once, past the last one it again
+  f32x4 v[kPlanes];
+#pragma unroll
+  for (int h = 0; h < kPlanes; ++h) v[h] = (f32x4){0, 0, 0, 0};
+  for (int s = 0; s < g.splits; s += 4) {
+    f32x4 t[4][kPlanes];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < kPlanes; ++h) {
+        const int one = s + i < g.splits ? s + i : g.splits - 1;
+        t[i][h] = *reinterpret_cast<const f32x4*>(partial + (one * kPlanes + h) * plane + at);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < kPlanes; ++h)
+        if (s + i < g.splits) v[h] += t[i][h];
+  }
   if constexpr (EPI == kStore)
     store_plain(g, p, m, n, v[0]);
   else if constexpr (EPI == kBias)
@@ -646,8 +663,7 @@ __global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
   else if constexpr (EPI == kSwiglu)
     store_swiglu(g, p, m, n, v[0], v[1]);
   else
-    store_swiglu_grad(g, p, m, n, v[0], *reinterpret_cast<const f32x4*>(g.gate + m * p.n + n),
-                      *reinterpret_cast<const f32x4*>(g.up + m * p.n + n));
+    store_swiglu_grad(g, p, m, n, v[0], gate, up);
 }
 
 // ---------------------------------------------------------------- host ---
