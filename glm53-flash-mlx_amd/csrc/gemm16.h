@@ -14,9 +14,9 @@
 // Bound by the matrix pipes where the tiles fill the chip: a step of a 256 x 256
 // tile takes 1.45 to 1.6 us on every CU, 1.35 to 1.48 PFLOP/s (the library's
 // product of 8192^3: 1.35), and ~12 us a tile go to its first loads and its
-// epilogue.  8,192 rows, 4096 x 2048: gate and up with SwiGLU 247 us, 1.11
-// PFLOP/s, down 123, SwiGLU's gradient 160, x's gradient over both segments
-// 232, 1.18 PFLOP/s, dWg and dWu together 226, 1.22.
+// epilogue.  8,192 rows, 4096 x 2048: gate and up with SwiGLU 250 us, 1.10
+// PFLOP/s, down 126, SwiGLU's gradient 161, x's gradient over both segments
+// 234, 1.17 PFLOP/s, dWg and dWu together 231, 1.19.
 #pragma once
 
 #include "common.h"
