@@ -45,7 +45,7 @@ struct Gemm16Args {
   int64_t k;       // of each pair
   int problems;    // pairs that are products of their own
   int segments;    // pairs whose contractions are added into pair[0].out
-  int splits;      // parts of the contraction, each to `partial`
+  int splits;      // parts of the contraction, each to `partial` and none without a K step (used_splits)
   float* partial;  // of each problem [splits][planes][m][partial_ld(n)], at partial_at floats
   int64_t room;    // floats at partial
   int64_t partial_at[4];
@@ -675,6 +675,12 @@ struct Gemm16Plan {
   int64_t partial;  // floats of the splits' partial results
   float us;         // expected time
 };
+// `steps` K steps in at most `splits` parts of the same number of steps, the
+// last one's rest: the parts that have one.
+inline int used_splits(int64_t steps, int64_t splits) {
+  const int64_t each = (steps + splits - 1) / splits;
+  return static_cast<int>((steps + each - 1) / each);
+}
 // The tile and the number of splits for g's products; pair_b: gate and up
 // columns in one product.
 Gemm16Plan gemm16_plan(const Gemm16Args& g, bool pair_b);

@@ -46,8 +46,9 @@ Gemm16Plan gemm16_plan(const Gemm16Args& g, bool pair_b) {
   Gemm16Plan best{};
   for (const Shape& s : kShapes) {
     const int64_t tiles = tiles_of(g, s, planes), steps = cdiv(g.k, s.step) * g.segments;
-    for (int splits : {1, 2, 3, 4, 6, 8, 12, 16}) {
-      if (splits > 1 && steps < 2 * splits) break;
+    for (int most : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (most > 1 && steps < 2 * most) break;
+      const int splits = used_splits(steps, most);
       const int64_t units = tiles * splits, rounds = cdiv(units, s.slots);
       float us = static_cast<float>(rounds * cdiv(steps, splits)) * (units > 256 ? s.step_full_us : s.step_us);
       us += s.tile == kTile256 ? static_cast<float>(rounds) * s.fixed_us : s.fixed_us;

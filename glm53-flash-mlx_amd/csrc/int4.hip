@@ -351,7 +351,7 @@ Gemm16Args product(const Int4Args& a) {
 // 64 x 128 tiles; as many parts of the contraction as fill the chip once.
 Gemm16Plan staged_plan(const Int4Args& a) {
   const int64_t tiles = cdiv(a.rows, 64) * cdiv(a.N, 128), steps = cdiv(a.K, 128);
-  const int splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({16, 256 / tiles, steps / 2})));
+  const int splits = used_splits(steps, std::max<int64_t>(1, std::min<int64_t>({16, 256 / tiles, steps / 2})));
   return {kTile64, splits, splits > 1 ? splits * a.rows * partial_ld(a.N) : 0, 0.0f};
 }
 
