@@ -67,10 +67,13 @@ struct Gemm16Args {
   const void* bias;     // or null
   bool scales_f32;
   int group_log2;
+  const float* tables;  // with kCodeValues: [k / group][tiles of 128 columns][scale, base][128]
 };
 
 enum Gemm16Epilogue { kStore, kSwiglu, kSwigluGrad, kBias };
-enum OperandForm { kRow, kColumn, kCodes, kCodesF32 };  // 4-bit codes with bf16 or FP32 tables
+// b as 4-bit codes with bf16 or FP32 tables, or (kCodeValues) as the bf16 values
+// 128 + q of the codes, [n, k], with `tables`: the products of kBias.
+enum OperandForm { kRow, kColumn, kCodes, kCodesF32, kCodeValues };
 
 // Row length of the partial results: whole groups of four.
 __host__ __device__ __forceinline__ int64_t partial_ld(int64_t n) { return (n + 3) & ~int64_t{3}; }
@@ -105,9 +108,34 @@ __device__ __forceinline__ void store_plain(const Gemm16Args& g, const Gemm16Pai
   *reinterpret_cast<u32x2*>(p.out + m * p.ldo + n) = pack_bf16x4(v);
 }
 
-// The same plus a bias, for any number of columns: outputs past the last one
-// are left out, and rows whose length is no multiple of 4 have no aligned
-// group of four.
+// One output of a 4-bit product in the formula's own order: for results that
+// the sums of x times codes cannot tell from inf - inf.  Its pointers come one
+// by one: with an argument block's address taken, every load of a kernel would
+// go by flat addresses and wait for the one before.  2,048 x 4096 x 4096 with an
+// infinity in every row's last column: 15 ms.
+__device__ __forceinline__ float one_output(const uint16_t* x, const uint8_t* codes, const void* scales,
+                                            const void* offsets, bool f32, int group_log2, int64_t k_all) {
+  float y = 0.0f;
+  for (int64_t k = 0; k < k_all && y == y; k += 8) {  // a NaN stays one
+    const float scale = table_value(scales, f32, k >> group_log2);
+    const float offset = offsets != nullptr ? table_value(offsets, f32, k >> group_log2) : -8.0f * scale;
+    const uint32_t q = *reinterpret_cast<const uint32_t*>(codes + (k >> 1));
+    const u32x4 v = *reinterpret_cast<const u32x4*>(x + k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      y += bf16_to_f32(static_cast<uint16_t>(v[i >> 1] >> (16 * (i & 1)))) *
+           fmaf(static_cast<float>((q >> (4 * i)) & 15), scale, offset);
+  }
+  return y;
+}
+
+__device__ __forceinline__ bool finite(f32x4 v) {
+  return fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY;
+}
+
+// Outputs of a 4-bit product plus its bias, for any number of columns: outputs
+// past the last one are left out, and rows whose length is no multiple of 4
+// have no aligned group of four.
 __device__ __forceinline__ void store_bias(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n, f32x4 v) {
   uint16_t* out = p.out + m * p.ldo + n;
   if (g.bias != nullptr) {
@@ -122,6 +150,21 @@ __device__ __forceinline__ void store_bias(const Gemm16Args& g, const Gemm16Pair
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (n + i < p.n) out[i] = f32_to_bf16(v[i]);
+}
+
+// Those of the four outputs stored that are not finite, once more by the formula.
+__device__ __forceinline__ void store_bias_again(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n) {
+#pragma unroll 1
+  for (const int64_t last = n + 4 < p.n ? n + 4 : p.n; n < last; ++n) {
+    uint16_t* out = p.out + m * p.ldo + n;
+    if ((*out & 0x7F80) != 0x7F80) continue;
+    const int64_t table = n * (g.k >> g.group_log2) * (g.scales_f32 ? 4 : 2);
+    float y = one_output(p.a + m * p.lda, g.codes + n * (g.k >> 1), static_cast<const uint8_t*>(g.scales) + table,
+                         g.offsets != nullptr ? static_cast<const uint8_t*>(g.offsets) + table : nullptr, g.scales_f32,
+                         g.group_log2, g.k);
+    if (g.bias != nullptr) y += table_value(g.bias, g.scales_f32, n);
+    *out = f32_to_bf16(y);
+  }
 }
 
 // h = silu(min(g, L)) clip(u, -L, L).  G and U themselves are kept in FP32
@@ -256,32 +299,28 @@ struct Stager {
   }
 };
 
-// The bf16 weights scale q + offset of 8 codes.  Each half's codes as bytes,
-// which one instruction turns into a float (the compiler, seeing that the
-// bytes are below 16, would take them out one by one first), and one rounding
-// instruction a pair: 23 instructions for 8 weights.
-__device__ __forceinline__ u32x4 weights_of(uint32_t v, float scale, float offset) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  uint32_t even = v & 0x0F0F0F0Fu, odd = (v >> 4) & 0x0F0F0F0Fu;
-  asm("" : "+v"(even), "+v"(odd));
+// The bf16 values 128 + q of 8 codes, or-ed into the mantissa of 128 and so
+// exact: 11 instructions.
+__device__ __forceinline__ u32x4 code_values(uint32_t v) {
+  const uint32_t even = v & 0x0F0F0F0Fu, odd = (v >> 4) & 0x0F0F0F0Fu;
+  constexpr uint32_t kPair[4] = {0x0C040C00u, 0x0C050C01u, 0x0C060C02u, 0x0C070C03u};  // bytes i of both, zeros between
   u32x4 w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f32x2 p = {fmaf(static_cast<float>((even >> (8 * i)) & 0xFFu), scale, offset),
-                     fmaf(static_cast<float>((odd >> (8 * i)) & 0xFFu), scale, offset)};
-    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
-  }
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(odd, even, kPair[i]) | 0x43004300u;
   return w;
+}
+
+// What a group's sum x (128 + q) and sum x are multiplied by: scale and base,
+//   sum x (scale q + offset) = scale (sum x (128 + q)) + base (sum x).
+__device__ __forceinline__ float code_base(float scale, bool offsets, float offset) {
+  return offsets ? offset - 128.0f * scale : -136.0f * scale;
 }
 
 // 4-bit rows into a row-form stage of R rows by T threads: a thread takes 32
 // codes (16 bytes, within one group) of a row, fetched a step ahead, and
-// writes them as bf16 w = scale q + offset.  That rounding, half a step of
-// bf16 as the activations carry, makes the weights an MFMA operand; over the
-// rows this form is used for, sums of scaled group products in FP32 instead
-// would cost the vector units as many cycles as the product.
-template <int R, int T, bool F32>
+// writes their values, and beside the stage the scale and base of their group,
+// [group of GROUP columns][scale, base][R].
+template <int R, int T, int GROUP, bool F32>
 struct CodeStager {
   static_assert(R * 2 == T, "32 codes a thread");
   u32x4 codes;
@@ -289,10 +328,10 @@ struct CodeStager {
   const uint8_t* row;
   int64_t table;
   int at;  // byte of the row's piece 0 in the stage, without the slot
-  int mix, half;
+  int mix, half, r;
 
   __device__ __forceinline__ void init(const Gemm16Args& g, int64_t n0, int64_t n, int64_t k) {
-    const int r = threadIdx.x >> 1;
+    r = threadIdx.x >> 1;
     half = threadIdx.x & 1;
     const int64_t nr = n0 + r < n ? n0 + r : n - 1;
     row = g.codes + nr * (k >> 1);
@@ -314,24 +353,30 @@ struct CodeStager {
     // way before either is waited for
     offset = table_value(g.offsets != nullptr ? g.offsets : g.scales, F32, t);
   }
-  __device__ __forceinline__ void write(uint8_t* stage, bool offsets) const {
-    const float base = offsets ? offset : -8.0f * offset;
+  __device__ __forceinline__ void write(uint8_t* stage, float* tables, bool offsets) const {
 #pragma unroll
     for (int d = 0; d < 4; ++d)
-      *reinterpret_cast<u32x4*>(stage + at + 16 * ((4 * half + d) ^ mix)) = weights_of(codes[d], scale, base);
+      *reinterpret_cast<u32x4*>(stage + at + 16 * ((4 * half + d) ^ mix)) = code_values(codes[d]);
+    if (GROUP == 32 || half == 0) {
+      float* t = tables + (GROUP == 32 ? half : 0) * 2 * R + r;
+      t[0] = scale;
+      t[R] = code_base(scale, offsets, offset);
+    }
   }
 };
 
-// MFMA operand j (0, 1) of 16-row or 16-column tile t of a stage.
-template <int R, bool COLUMN>
+// MFMA operand j (0, 1) of 16-row or 16-column tile t of a stage.  HALVES (row
+// form): j contracts k = 32 j + 8 (l / 16) + 0..7, a half of the step's columns,
+// instead of the pieces that the staging comment names.
+template <int R, bool COLUMN, bool HALVES = false>
 struct Reader {
   uint32_t lo, hi;  // row form: a tile's two pieces; column form: row base and swizzle
   __device__ __forceinline__ Reader(int lane) {
     const int r = lane & 15, kq = lane >> 4;
     if (!COLUMN) {
       const int g = (r & 7) ^ (r >> 3);
-      lo = 128 * r + 16 * ((2 * kq) ^ g);
-      hi = 128 * r + 16 * ((2 * kq + 1) ^ g);
+      lo = 128 * r + 16 * ((HALVES ? kq : 2 * kq) ^ g);
+      hi = 128 * r + 16 * ((HALVES ? 4 + kq : 2 * kq + 1) ^ g);
     } else {
       lo = (16 * kq + (r >> 2)) * (2 * R) + 8 * (r & 3);
       hi = ((r >> 2) | ((kq & 1) << 2)) & (R / 16 - 1);
@@ -374,8 +419,9 @@ __device__ __forceinline__ int tiles_of(int64_t n, int size) {
 
 // WM x WN wavefronts, each MT x NT MFMA tiles of 16 x 16; SUB blocks of 64 k a
 // step and stage: small tiles multiply a block faster than its loads return, so
-// they take two blocks between barriers.
-template <int WM, int WN, int MT, int NT, int SUB, bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI>
+// they take two blocks between barriers.  GROUP (4-bit products): columns whose
+// sums are scaled at once, 32 or 64.
+template <int WM, int WN, int MT, int NT, int SUB, bool A_COLUMN, OperandForm B, Gemm16Epilogue EPI, int GROUP = 64>
 struct Gemm16 {
   static constexpr int W = WM * WN, kThreads = 64 * W;
   static constexpr int BM = 16 * WM * MT, BN = 16 * WN * NT;
@@ -387,7 +433,12 @@ struct Gemm16 {
   // fills a CU's LDS anyway: a third stage, loaded two steps ahead.  Codes, which
   // pass through registers, are one step ahead.
   static constexpr int kStages = SUB == 2 && !kFromCodes ? 3 : 2;
-  static constexpr int kLds = kStages * kStage;
+  // 4-bit products: scales and bases of a stage's groups, behind all stages
+  static constexpr bool kScaled = EPI == kBias;
+  static_assert(!kScaled || kFromCodes || (B == kCodeValues && BN == 128 && kStages == 2), "tables of 128 columns");
+  static constexpr int kParts = SUB * 64 / GROUP, kTable = 2 * BN;
+  static constexpr int kTableStage = kScaled ? kParts * kTable * 4 : 0;
+  static constexpr int kLds = kStages * (kStage + kTableStage);
   // direct loads of a wavefront and stage
   static constexpr int kStageLoads = SUB * (BM + BN) / 8 / W;
 
@@ -408,6 +459,56 @@ struct Gemm16 {
           __builtin_amdgcn_sched_group_barrier(kLdsRead, NT * kReadB + kAhead * kReadA, 0);
         __builtin_amdgcn_sched_group_barrier(kMfma, kAhead * NT, 0);
       }
+    }
+  }
+
+  // A step of a 4-bit product: acc += scale (sum x (128 + q)) + base (sum x) for
+  // each group's part of it, sums of x by an MFMA with ones.  The codes' values
+  // are exact, scales and bases FP32: no weight is rounded.  A weight rounded to
+  // bf16 would be off by half a step of the offset, which a group whose range is
+  // small against it does not get back; the price is a quarter more MFMAs and two
+  // FMAs a result and part: 2,048 x 4096 x 4096 in groups of 64 102 us instead of
+  // 74, in groups of 32 129 instead of 75, 64 rows 21 instead of 20.
+  template <class RA, class RB>
+  __device__ static __forceinline__ void multiply_scaled(f32x4 (&acc)[MT][NT], const uint8_t* stage, const float* tables,
+                                                         const RA& ra, const RB& rb, int wm, int wn, int lane) {
+    constexpr int J = GROUP / 32;  // MFMAs of a part
+    const u32x4 one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+    const bf16x8 ones = __builtin_bit_cast(bf16x8, one);
+    const f32x4 zero = {0, 0, 0, 0};
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const uint8_t* block = stage + part * GROUP / 64 * kBlock;
+      const int j0 = J == 2 ? 0 : part & 1;
+      bf16x8 a[MT][J], b[NT][J];
+      f32x4 scale[NT], base[NT], sum[MT];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        const float* t = tables + part * kTable + 16 * (wn * NT + c) + 4 * (lane >> 4);
+        scale[c] = *reinterpret_cast<const f32x4*>(t);
+        base[c] = *reinterpret_cast<const f32x4*>(t + BN);
+#pragma unroll
+        for (int j = 0; j < J; ++j) b[c][j] = rb(block + kStageA, wn * NT + c, j0 + j);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        sum[i] = zero;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          a[i][j] = ra(block, wm * MT + i, j0 + j);
+          sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, a[i][j], sum[i], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int c = 0; c < NT; ++c) {
+          f32x4 d = zero;
+#pragma unroll
+          for (int j = 0; j < J; ++j) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[c][j], a[i][j], d, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][c][e] = fmaf(scale[c][e], d[e], fmaf(base[c][e], sum[i][e], acc[i][c][e]));
+        }
     }
   }
 
@@ -443,7 +544,7 @@ struct Gemm16 {
     Stager<BN / kHalves, W, B_COLUMN> sb;
     sb.init(wave, lane, p.ldb, p.n - n0);
     const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    CodeStager<kFromCodes ? BN : kThreads / 2, kThreads, B == kCodesF32> sq[SUB];
+    CodeStager<kFromCodes ? BN : kThreads / 2, kThreads, GROUP, B == kCodesF32> sq[SUB];
     if constexpr (kFromCodes) {
 #pragma unroll
       for (int u = 0; u < SUB; ++u) sq[u].init(g, n0, p.n, g.k);
@@ -452,9 +553,12 @@ struct Gemm16 {
 #pragma unroll
       for (int u = 0; u < SUB; ++u) sq[u].fetch(g, static_cast<int64_t>(step) * kStep + u * kStepK);
     };
+    float* const tables = reinterpret_cast<float*>(lds + kStages * kStage);
+    const auto table_at = [&](int slot, int part) { return (slot * kParts + part) * kTable; };
     const auto write_codes = [&](int slot) {
 #pragma unroll
-      for (int u = 0; u < SUB; ++u) sq[u].write(lds + slot * kStage + u * kBlock + kStageA, g.offsets != nullptr);
+      for (int u = 0; u < SUB; ++u)
+        sq[u].write(lds + slot * kStage + u * kBlock + kStageA, tables + table_at(slot, u * (64 / GROUP)), g.offsets != nullptr);
     };
     // Where the next step's operands start; a step on costs two additions.
     const uint16_t *pa, *pb[kHalves];
@@ -468,6 +572,8 @@ struct Gemm16 {
       for (int h = 0; h < kHalves; ++h) pb[h] = (kPairB ? g.pair[h].b : o.b) + b_at;
       left = steps - step;
     };
+    // the column whose group's table this wavefront loads for the next step, if one
+    int64_t table_k = static_cast<int64_t>(first) * kStep + wave * GROUP;
     int segment = first / steps;
     seek(segment, first - segment * steps);
     const int64_t next_a = A_COLUMN ? kStepK * p.lda : kStepK, next_b = B_COLUMN ? kStepK * p.ldb : kStepK;
@@ -497,6 +603,13 @@ struct Gemm16 {
           }
         }
       }
+      if constexpr (B == kCodeValues) {
+        const int64_t k = table_k < g.k ? table_k : g.k - 1;  // past the last column: any group, whose sums are zero
+        if (wave < kParts)
+          load_lds16(g.tables + ((k >> g.group_log2) * cols + tn) * kTable, 16 * lane,
+                     lds_at + kStages * kStage + 4 * table_at(slot, wave));
+        table_k += kStep;
+      }
       if (--left == 0 && ++segment < g.segments) seek(segment, 0);
     };
 
@@ -505,8 +618,8 @@ struct Gemm16 {
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int c = 0; c < NT; ++c) acc[i][c] = (f32x4){0, 0, 0, 0};
-    const Reader<BM, A_COLUMN> ra(lane);
-    const Reader<BN / kHalves, B_COLUMN> rb(lane);
+    const Reader<BM, A_COLUMN, GROUP == 32> ra(lane);
+    const Reader<BN / kHalves, B_COLUMN, GROUP == 32> rb(lane);
     // LDS tile of the wavefront's column tile c: in a pair, the first half of
     // its tiles are gate columns, the others the up columns of the same outputs
     const auto b_tile = [&](int c) {
@@ -538,6 +651,10 @@ struct Gemm16 {
         if (step + 2 < last) fetch_codes(step + 2);
       }
       const uint8_t* stage = lds + slot * kStage;
+if constexpr (kScaled) {
+        multiply_scaled(acc, stage, tables + table_at(slot, 0), ra, rb, wm, wn, lane);
+        continue;
+      }
 #pragma unroll
       for (int j = 0; j < 2 * SUB; ++j) {
         bf16x8 a[MT], b[NT];
@@ -592,6 +709,7 @@ struct Gemm16 {
         return;
       }
     }
+    bool all_finite = true;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int64_t m = row(i);
@@ -607,9 +725,18 @@ struct Gemm16 {
           store_plain(g, p, m, n, acc[i][c]);
         } else if constexpr (EPI == kBias) {
           store_bias(g, p, m, n, acc[i][c]);
+          all_finite = all_finite && finite(acc[i][c]);
         } else if constexpr (EPI == kSwiglu) {
           store_swiglu(g, p, m, n, acc[i][c], acc[i][c + NT / 2]);
         }
+      }
+    }
+    if constexpr (EPI == kBias) {
+      if (all_finite) return;
+#pragma unroll 1
+      for (int t = 0; t < MT * kOut; ++t) {
+        const int64_t m = row(t / kOut), n = col(t % kOut);
+        if (m < p.m && n < p.n) store_bias_again(g, p, m, n);
       }
     }
   }
@@ -658,9 +785,10 @@ __global__ __launch_bounds__(256) void gemm16_join_kernel(Gemm16Args g) {
   }
   if constexpr (EPI == kStore)
     store_plain(g, p, m, n, v[0]);
-  else if constexpr (EPI == kBias)
+  else if constexpr (EPI == kBias) {
     store_bias(g, p, m, n, v[0]);
-  else if constexpr (EPI == kSwiglu)
+    if (!finite(v[0])) store_bias_again(g, p, m, n);
+  } else if constexpr (EPI == kSwiglu)
     store_swiglu(g, p, m, n, v[0], v[1]);
   else
     store_swiglu_grad(g, p, m, n, v[0], gate, up);
@@ -684,6 +812,8 @@ inline int used_splits(int64_t steps, int64_t splits) {
 // The tile and the number of splits for g's products; pair_b: gate and up
 // columns in one product.
 Gemm16Plan gemm16_plan(const Gemm16Args& g, bool pair_b);
+// The same for a 4-bit product of code values and tables (kCodeValues).
+Gemm16Plan gemm16_plan_scaled(const Gemm16Args& g);
 
 template <class G, Gemm16Epilogue EPI>
 hipError_t gemm16_launch(Gemm16Args g, hipStream_t st) {

@@ -28,11 +28,10 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // bound by the launch and the first loads' way (8 wavefronts a workgroup 6.5
 // us, 4 8.9).  16 x 4096 x 7168: 12 us, x coming to every CU from L2.
 //
-// From 17 to 32 rows two MFMA rows share the codes, over at most 8,192
-// columns; wider outputs have enough tiles for the staged product below (32 x
-// 4096 x 4096 12.4 us here, 19.0 staged; 32 x 8192 x 2048 15.2, 16.8; 32 x
-// 14336 x 4096 44.8, 42.2).
-bool few(int64_t rows, int64_t N) { return rows <= 16 || (rows <= 32 && N <= 8192); }
+// From 17 to 32 rows two MFMA rows share the codes (32 x 4096 x 4096 12.3 us here,
+// 18.6 by the staged product below; 32 x 8192 x 2048 14.6, 17.7; 17 and 32 x 14336
+// x 4096 33 and 43.5, 44).
+bool few(int64_t rows) { return rows <= 32; }
 
 // Quarter q's dword s of four becomes quarter s's dword q.
 __device__ __forceinline__ void exchange_quarters(u32x4& v) {
@@ -66,22 +65,6 @@ __device__ __forceinline__ bf16x8 codes_order(u32x4 x) {
   const u32x4 r = {__builtin_amdgcn_perm(x[2], x[0], 0x05040100u), __builtin_amdgcn_perm(x[2], x[0], 0x07060302u),
                    __builtin_amdgcn_perm(x[3], x[1], 0x05040100u), __builtin_amdgcn_perm(x[3], x[1], 0x07060302u)};
   return __builtin_bit_cast(bf16x8, r);
-}
-
-// One output in the formula's own order: for results that the kernel below
-// cannot tell from inf - inf of its two sums.  Its pointers come one by one:
-// with the argument block's address taken, every load of the kernel would go
-// by flat addresses and wait for the one before.
-__device__ __forceinline__ float one_output(const uint16_t* x, const uint8_t* codes, const void* scales,
-                                                      const void* offsets, bool f32, int group_log2, int k_all) {
-  float y = 0.0f;
-  for (int k = 0; k < k_all; ++k) {
-    const float scale = table_value(scales, f32, k >> group_log2);
-    const float offset = offsets != nullptr ? table_value(offsets, f32, k >> group_log2) : -8.0f * scale;
-    const int q = (codes[k >> 1] >> (4 * (k & 1))) & 15;
-    y += bf16_to_f32(x[k]) * fmaf(static_cast<float>(q), scale, offset);
-  }
-  return y;
 }
 
 template <class T>
@@ -293,45 +276,68 @@ hipError_t launch_few_rows(const Int4Args& a, hipStream_t st) {
 }  // namespace
 
 namespace {
-// The weights as bf16, W = scale q + offset rounded once, [N, K].  A thread
-// takes kExpand pieces of 8 codes (4 bytes, within one group), 256 apart, so
-// that a wavefront reads 256 bytes and writes 1 KB in a row; bound by the
-// writes, 2 bytes a weight.  4096 x 4096: 9.6 us (32 codes a thread, its writes
-// 64 bytes apart: 15.8).
-constexpr int kExpand = 4;
+
+// ------------------------------------------------------------ many rows ---
+//
+// Tiled products of x by the codes' values 128 + q, whose group sums are scaled
+// in FP32 as above.
+
+// The values as bf16 [N, K], and scale and base of every group in the order
+// that the product's tiles load them, [K / group][tiles of 128 columns][scale,
+// base][128].  Tables: the first workgroups, 128 columns and kTurn groups each,
+// turned in LDS.  Values: a thread takes kExpand pieces of 8 codes (4 bytes), 256
+// apart, so that a wavefront reads 256 bytes and writes 1 KB in a row; bound by
+// the writes, 2 bytes a weight.  4096 x 4096: 9.4 us.
+constexpr int kExpand = 4, kTurn = 16;
+
+int64_t value_blocks(const Int4Args& a) { return cdiv(a.N * (a.K >> 3), 256 * kExpand); }
+int64_t table_blocks(const Int4Args& a) { return cdiv(a.N, 128) * cdiv(a.K >> a.group_log2, kTurn); }
+
 template <bool F32>
-__global__ __launch_bounds__(256) void int4_expand_kernel(Int4Args a, uint16_t* w) {
-  const uint32_t row = static_cast<uint32_t>(a.K >> 3);  // pieces of a row
-  const int64_t first = blockIdx.x * int64_t{256 * kExpand}, n0 = first / row, all = a.N * row;
-  const uint32_t in_row = static_cast<uint32_t>(first - n0 * row);
-  const int groups = static_cast<int>(a.K >> a.group_log2);
-  uint32_t codes[kExpand];
-  float scale[kExpand], second[kExpand];
+__global__ __launch_bounds__(256) void int4_expand_kernel(Int4Args a, int64_t table_blocks, uint16_t* w, float* tables) {
+  __shared__ float turn[2][kTurn][128 + 1];
+  if (blockIdx.x >= table_blocks) {
+    const int64_t first = (blockIdx.x - table_blocks) * int64_t{256 * kExpand}, all = a.N * (a.K >> 3);
+    uint32_t codes[kExpand];
 #pragma unroll
-  for (int u = 0; u < kExpand; ++u) {
-    const uint32_t local = u * 256 + threadIdx.x, at = in_row + local, down = at / row;
-    const bool in = first + local < all;
-    codes[u] = in ? reinterpret_cast<const uint32_t*>(a.codes)[first + local] : 0;
-    // without offsets: the scale, read again, so that both loads are on their
-    // way before either is waited for
-    const int64_t t = in ? (n0 + down) * groups + ((at - down * row) >> (a.group_log2 - 3)) : 0;
-    scale[u] = table_value(a.scales, F32, t);
-    second[u] = table_value(a.offsets != nullptr ? a.offsets : a.scales, F32, t);
+    for (int u = 0; u < kExpand; ++u) {
+      const int64_t at = first + u * 256 + threadIdx.x;
+      codes[u] = reinterpret_cast<const uint32_t*>(a.codes)[at < all ? at : all - 1];
+    }
+#pragma unroll
+    for (int u = 0; u < kExpand; ++u) {
+      const int64_t at = first + u * 256 + threadIdx.x;
+      if (at < all) *reinterpret_cast<u32x4*>(w + 8 * at) = code_values(codes[u]);
+    }
+    return;
+  }
+  const int64_t groups = a.K >> a.group_log2, bands = (groups + kTurn - 1) / kTurn, tiles = (a.N + 127) / 128;
+  const int64_t tile = blockIdx.x / bands, g0 = (blockIdx.x - tile * bands) * kTurn;
+  constexpr int kEach = 128 * kTurn / 256;  // entries of a thread, all on their way before the first is used
+  const int g = threadIdx.x % kTurn, n0 = threadIdx.x / kTurn;
+  float scale[kEach], offset[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int64_t n = 128 * tile + n0 + 256 / kTurn * i;
+    const int64_t t = n < a.N && g0 + g < groups ? n * groups + g0 + g : 0;  // past the edges: never used
+    scale[i] = table_value(a.scales, F32, t);
+    offset[i] = table_value(a.offsets != nullptr ? a.offsets : a.scales, F32, t);
   }
 #pragma unroll
-  for (int u = 0; u < kExpand; ++u) {
-    const int64_t at = first + u * 256 + threadIdx.x;
-    if (at >= all) break;
-    const float offset = a.offsets != nullptr ? second[u] : -8.0f * second[u];
-    *reinterpret_cast<u32x4*>(w + 8 * at) = weights_of(codes[u], scale[u], offset);
+  for (int i = 0; i < kEach; ++i) {
+    turn[0][g][n0 + 256 / kTurn * i] = scale[i];
+    turn[1][g][n0 + 256 / kTurn * i] = code_base(scale[i], a.offsets != nullptr, offset[i]);
   }
+  __syncthreads();
+  for (int i = 0; i < kTurn && g0 + i < groups; ++i)
+    tables[((g0 + i) * tiles + tile) * 256 + threadIdx.x] = turn[threadIdx.x >> 7][i][threadIdx.x & 127];
 }
 
-// Up to this many rows the codes become weights in the tiled product's own
-// stage, tile row by tile row; beyond, in memory once, for the product of bf16
-// weights, whose larger tiles the conversion would hold up (4096 x 4096: 64
-// rows 21 us staged, 27 expanded; 128 rows 29 and 30; 200 rows 44 and 33; 300
-// rows 75 and 39).
+// Up to this many rows the codes become values in the tiled product's own
+// stage, tile row by tile row; beyond, in memory once, for products whose
+// larger tiles the conversion would hold up (64 rows, 4096 x 4096: 21 us staged;
+// 128: 29; 200: 45, 35 from memory; 300: 75, 39; 1536 x 4096 in groups of 32, 200
+// and 300 rows: 27 and 30, 31 and 32).
 constexpr int64_t kStagedRows = 128;
 
 Gemm16Args product(const Int4Args& a) {
@@ -355,44 +361,62 @@ Gemm16Plan staged_plan(const Int4Args& a) {
   return {kTile64, splits, splits > 1 ? splits * a.rows * partial_ld(a.N) : 0, 0.0f};
 }
 
-size_t weight_bytes(int64_t N, int64_t K) { return (2 * static_cast<size_t>(N) * static_cast<size_t>(K) + 255) & ~size_t{255}; }
+template <int GROUP>
+hipError_t launch_staged(const Gemm16Args& g, hipStream_t st) {
+  if (g.scales_f32) return gemm16_launch<Gemm16<1, 4, 4, 2, 2, false, kCodesF32, kBias, GROUP>, kBias>(g, st);
+  return gemm16_launch<Gemm16<1, 4, 4, 2, 2, false, kCodes, kBias, GROUP>, kBias>(g, st);
+}
+
+template <int GROUP>
+hipError_t launch_values(Gemm16Args g, const Gemm16Plan& plan, hipStream_t st) {
+  g.splits = plan.splits;
+  if (plan.tile == kTile64) return gemm16_launch<Gemm16<2, 2, 2, 4, 1, false, kCodeValues, kBias, GROUP>, kBias>(g, st);
+  return gemm16_launch<Gemm16<2, 2, 4, 4, 1, false, kCodeValues, kBias, GROUP>, kBias>(g, st);
+}
+
+size_t value_bytes(int64_t N, int64_t K) { return (2 * static_cast<size_t>(N) * static_cast<size_t>(K) + 255) & ~size_t{255}; }
+size_t table_bytes(int64_t N, int64_t K, int group_log2) {
+  return 1024 * static_cast<size_t>(cdiv(N, 128)) * static_cast<size_t>(K >> group_log2);
+}
 
 }  // namespace
 
 size_t int4_space(int64_t rows, int64_t N, int64_t K) {
-  if (few(rows, N)) return 0;
+  if (few(rows)) return 0;
   Int4Args a{};
   a.rows = rows;
   a.N = N;
   a.K = K;
   if (rows <= kStagedRows) return sizeof(float) * static_cast<size_t>(staged_plan(a).partial);
-  return weight_bytes(N, K) + sizeof(float) * static_cast<size_t>(gemm16_plan(product(a), false).partial);
+  return value_bytes(N, K) + table_bytes(N, K, 5) + sizeof(float) * static_cast<size_t>(gemm16_plan_scaled(product(a)).partial);
 }
 
 hipError_t launch_int4(const Int4Args& a, hipStream_t st) {
-  if (few(a.rows, a.N)) return launch_few_rows(a, st);
+  if (few(a.rows)) return launch_few_rows(a, st);
   Gemm16Args g = product(a);
   if (a.rows <= kStagedRows) {
     const Gemm16Plan plan = staged_plan(a);
     g.splits = plan.splits;
     g.partial = static_cast<float*>(a.space);
     g.room = static_cast<int64_t>(a.space_bytes / sizeof(float));
-    if (a.tables_f32) return gemm16_launch<Gemm16<1, 4, 4, 2, 2, false, kCodesF32, kBias>, kBias>(g, st);
-    return gemm16_launch<Gemm16<1, 4, 4, 2, 2, false, kCodes, kBias>, kBias>(g, st);
+    return a.group_log2 == 5 ? launch_staged<32>(g, st) : launch_staged<64>(g, st);
   }
   uint16_t* w = static_cast<uint16_t*>(a.space);
+  float* tables = reinterpret_cast<float*>(static_cast<uint8_t*>(a.space) + value_bytes(a.N, a.K));
+  const size_t before = value_bytes(a.N, a.K) + table_bytes(a.N, a.K, a.group_log2);
   g.pair[0].b = w;
-  g.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.space) + weight_bytes(a.N, a.K));
-  g.room = static_cast<int64_t>((a.space_bytes - weight_bytes(a.N, a.K)) / sizeof(float));
-  const int64_t pieces = cdiv(a.N * (a.K >> 3), 256 * kExpand);
-  if (pieces >= (int64_t{1} << 31)) return hipErrorInvalidValue;
-  const uint32_t blocks = static_cast<uint32_t>(pieces);
+  g.tables = tables;
+  g.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(a.space) + before);
+  g.room = static_cast<int64_t>((a.space_bytes - before) / sizeof(float));
+  const int64_t turns = table_blocks(a), blocks = turns + value_blocks(a);
+  if (blocks * 256 >= (int64_t{1} << 32)) return hipErrorInvalidValue;  // a grid has fewer than 2^32 threads
   if (a.tables_f32)
-    int4_expand_kernel<true><<<blocks, 256, 0, st>>>(a, w);
+    int4_expand_kernel<true><<<static_cast<uint32_t>(blocks), 256, 0, st>>>(a, turns, w, tables);
   else
-    int4_expand_kernel<false><<<blocks, 256, 0, st>>>(a, w);
+    int4_expand_kernel<false><<<static_cast<uint32_t>(blocks), 256, 0, st>>>(a, turns, w, tables);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  return gemm16<false, kRow, kBias>(g, gemm16_plan(g, false), st);
+  const Gemm16Plan plan = gemm16_plan_scaled(g);
+  return a.group_log2 == 5 ? launch_values<32>(g, plan, st) : launch_values<64>(g, plan, st);
 }
 
 }  // namespace glm53

@@ -6,6 +6,13 @@ block-FP8 weights, which is what a call over few tokens costs.  Codes lie two
 to a byte, the even column in the low half.  No gradients: the served form of
 trained weights (``GatedMLP.to_int4``).  The reference's weights are FP8 and
 have no counterpart.
+
+A product multiplies by the codes and scales the sums of each group in FP32,
+whatever the number of rows: the weights are those that codes and tables
+define, not their roundings to bf16, in decode and in prefill alike.  Above 128
+rows a call writes the codes' bf16 values into a workspace of 2.25 bytes a
+weight and more (4096 x 4096: 38 MB), which torch's allocator keeps for the next
+one.
 """
 
 from __future__ import annotations
@@ -19,7 +26,7 @@ from . import _native as N
 from . import ops as _ops
 
 GROUP_SIZES = (32, 64, 128)
-FEW_ROWS = 16  # up to here no call takes a workspace
+FEW_ROWS = 32  # up to here no call takes a workspace
 
 
 def int4_linear(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, offsets: torch.Tensor | None = None,
@@ -27,7 +34,8 @@ def int4_linear(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, off
     """``x @ W.T + bias`` with W as the module describes.
 
     x bfloat16 [..., in]; weight uint8 [out, in / 2]; scales and offsets [out,
-    in / g], bias [out], all bfloat16 or all float32; offsets None: -8 scales."""
+    in / g], bias [out], all bfloat16 or all float32; offsets None: -8 scales.
+    FP32 sums, rounded once; no weight is rounded."""
     N.same_device(x, weight, scales, offsets, bias)
     x_shape, w_shape, s_shape, table = x.shape, weight.shape, scales.shape, scales.dtype
     if x.dtype is not torch.bfloat16:

@@ -640,10 +640,11 @@ typedef struct glm53_int4_weight {
   int32_t tables_f32;
 } glm53_int4_weight;
 /* y[m] = T(x[m] . W^T + bias), x BF16 [rows, in], y BF16 [rows, out], both
- * contiguous and 16-byte aligned; FP32 sums.  Up to 16 rows, and up to 32
- * over at most 8192 outputs, multiply by the codes themselves and scale the
- * group sums in FP32; others multiply by W rounded to BF16.  Workspace (256-byte aligned; NULL where 0 bytes) needs no
- * initialisation. */
+ * contiguous and 16-byte aligned.  Every number of rows multiplies by the codes
+ * themselves and scales group sums in FP32: W is not rounded.  Workspace
+ * (256-byte aligned; NULL where 0 bytes) needs no initialisation: none up to 32
+ * rows, partial sums up to 128; above, the codes as BF16 values and the
+ * tables in FP32, 2.25 bytes a weight, and partial sums. */
 size_t glm53_int4_linear_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features);
 int glm53_int4_linear(const glm53_int4_weight* weight, const void* x, int64_t rows, void* y, void* workspace,
                       size_t workspace_bytes, void* stream);
