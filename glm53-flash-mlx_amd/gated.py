@@ -30,8 +30,9 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
 
     x bfloat16 [..., hidden], gate_weight and up_weight bfloat16
     [intermediate, hidden], down_weight bfloat16 [hidden, intermediate], both
-    widths multiples of 8; limit None: no clamp.  Differentiable (first order)
-    in all four tensors."""
+    widths multiples of 8; limit None: no clamp.  Differentiable (first order, in
+    reverse mode; forward mode and torch.func's grad, vjp and jvp raise) in all
+    four tensors."""
     N.same_device(x, gate_weight, up_weight, down_weight)
     weights = (gate_weight, up_weight, down_weight)
     x_shape, shape = x.shape, gate_weight.shape
@@ -53,6 +54,7 @@ def gated_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
         return native_gated_mlp(x, *weights, limit, False)[0]
     if _ops.eager(x, *weights):
         return _GatedMLP.apply(x, *weights, limit)
+    _ops.refuse_transforms("gated_mlp", x, *weights)
     keep = torch.is_grad_enabled() and any(t.requires_grad for t in (x, *weights))
     return torch.ops.glm53.gated_mlp(x, *weights, limit, keep)[0]
 

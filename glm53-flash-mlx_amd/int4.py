@@ -56,6 +56,7 @@ def int4_linear(x: torch.Tensor, weight: torch.Tensor, scales: torch.Tensor, off
         raise ValueError(f"bias must be {table} [{out_features}], got {tuple(bias.shape)} {bias.dtype}")
     if _ops.direct(x, weight, scales, offsets, bias):
         return native_int4_linear(x, weight, scales, offsets, bias)
+    _ops.refuse_transforms("int4_linear", x, scales, offsets, bias)
     return torch.ops.glm53.int4_linear(x, weight, scales, offsets, bias)
 
 
@@ -181,4 +182,5 @@ class Int4MLP(torch.nn.Module):
         limit = math.inf if self.limit is None else float(self.limit)
         if _ops.direct(joined):
             return self.down_proj(native_joined_swiglu(joined, limit))
+        _ops.refuse_transforms("Int4MLP", joined)
         return self.down_proj(torch.ops.glm53.joined_swiglu(joined, limit))

@@ -11,7 +11,8 @@ still to be added to the residual stream; ``rms_norm`` makes that input and
 with rms(v) = sqrt(mean(v^2) + eps) over the last axis.  Everything between
 the loads and the stores is FP32 and each result is rounded once; ``normed``
 is made of the new residual before it is rounded.  Both have gradients (first
-order), and both are torch custom ops where a call is traced or transformed.
+order, in reverse mode; forward mode and torch.func's grad, vjp and jvp raise),
+and both are torch custom ops where a call is traced.
 The reference takes its norms from mlx-vlm's layers and has no counterpart.
 """
 
@@ -122,6 +123,7 @@ def _call(residual, out, post_weight, gate, next_weight, form):
         return x, y
     if _ops.eager(*tensors):
         return _ResidualNorm.apply(*tensors, form)
+    _ops.refuse_transforms("rms_norm" if out is None else "residual_norm", *tensors)
     return torch.ops.glm53.residual_norm(*tensors, *form)[:2]
 
 

@@ -100,6 +100,43 @@ def eager(*tensors) -> bool:
     return not _dispatch_acts() and all(t is None or type(t) in _PLAIN_TENSORS for t in tensors)
 
 
+def _carries_derivative(t: torch.Tensor) -> bool:
+    """Whether `t` carries a tangent or a gradient of torch.func at any of the
+    levels that are active: asked level by level from the innermost one, below
+    which its wrapper is taken off and the level left."""
+    functorch = torch._C._functorch
+    top = functorch.peek_interpreter_stack()
+    if top is None or torch.compiler.is_compiling():
+        return torch.autograd.forward_ad._current_level >= 0 and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+    if functorch.is_functorch_wrapped_tensor(t) and functorch.maybe_get_level(t) == top.level():
+        if functorch.is_gradtrackingtensor(t):
+            if top.key() == functorch.TransformType.Jvp:
+                carries = torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+            else:
+                carries = t.requires_grad
+            if carries:
+                return True
+        t = functorch.get_unwrapped(t)
+    from torch._functorch import pyfunctorch
+
+    with pyfunctorch.temporarily_pop_interpreter_stack():
+        return _carries_derivative(t)
+
+
+def refuse_transforms(what: str, *tensors) -> None:
+    """An error where one of `tensors` carries a derivative that a custom op
+    would drop or cannot give: a forward-mode tangent (dropped below autograd,
+    the result's tangent would be zero), or torch.func's own differentiation.
+    Before a call that ``direct`` and ``eager`` leave to the op."""
+    if torch.autograd.forward_ad._current_level < 0 and (torch.compiler.is_compiling()
+                                                         or torch._C._functorch.peek_interpreter_stack() is None):
+        return
+    for t in tensors:
+        if t is not None and _carries_derivative(t):
+            raise RuntimeError(f"{what} has no derivative in forward mode or under torch.func: "
+                               "use torch.autograd in reverse mode")
+
+
 def _owner(key: int):
     ref = _OWNERS.get(int(key))
     module = ref() if ref is not None else None
