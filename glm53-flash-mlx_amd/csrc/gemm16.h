@@ -19,6 +19,8 @@
 // 234, 1.17 PFLOP/s, dWg and dWu together 231, 1.19.
 #pragma once
 
+#include <initializer_list>
+
 #include "common.h"
 
 namespace glm53 {
@@ -425,7 +427,7 @@ template <int WM, int WN, int MT, int NT, int SUB, bool A_COLUMN, OperandForm B,
 struct Gemm16 {
   static constexpr int W = WM * WN, kThreads = 64 * W;
   static constexpr int BM = 16 * WM * MT, BN = 16 * WN * NT;
-  static constexpr bool B_COLUMN = B == kColumn, kFromCodes = B == kCodes || B == kCodesF32;
+  static constexpr bool kAColumn = A_COLUMN, B_COLUMN = B == kColumn, kFromCodes = B == kCodes || B == kCodesF32;
   static constexpr bool kPairB = EPI == kSwiglu;           // half the tile gate columns, half up
   static constexpr int kColumns = kPairB ? BN / 2 : BN;    // output columns of a tile
   static constexpr int kStageA = BM * 128, kBlock = kStageA + BN * 128, kStage = SUB * kBlock;
@@ -817,20 +819,42 @@ Gemm16Plan gemm16_plan_scaled(const Gemm16Args& g);
 
 template <class G, Gemm16Epilogue EPI>
 hipError_t gemm16_launch(Gemm16Args g, hipStream_t st) {
+  constexpr int64_t kMostTiles = ((int64_t{1} << 32) - 1) / G::kThreads;  // a grid has fewer than 2^32 threads
   g.tiles = 0;
   g.group_m = 8;
   int64_t most = 0, at = 0;
+  const auto tile_columns = [](const Gemm16Pair& p) { return (p.n + G::kColumns - 1) / G::kColumns; };
   for (int q = 0; q < g.problems; ++q) {
     const Gemm16Pair& p = g.pair[q];
-    g.tiles += ((p.m + G::BM - 1) / G::BM) * ((p.n + G::kColumns - 1) / G::kColumns);
+    g.tiles += ((p.m + G::BM - 1) / G::BM) * tile_columns(p);
     const int64_t plane = p.m * partial_ld(p.n);
     g.partial_at[q] = at;
     at += plane * g.splits * (EPI == kSwiglu ? 2 : 1);
     most = most > plane ? most : plane;
   }
-  // a grid has fewer than 2^32 threads
-  if (g.tiles * g.splits * G::kThreads >= (int64_t{1} << 32) || (most / 1024 + 1) * 256 >= (int64_t{1} << 32)) return hipErrorInvalidValue;
-  if (g.splits > 1 && at > g.room) return hipErrorInvalidValue;
+  if (g.splits > 1 && (at > g.room || (most + 1023) / 1024 * 256 >= (int64_t{1} << 32))) return hipErrorInvalidValue;
+  if (g.tiles * g.splits > kMostTiles) {
+    // One product over very many rows, whole: a launch for each band of rows.
+    const int64_t columns = tile_columns(g.pair[0]), rows = g.pair[0].m, band = kMostTiles / columns * G::BM;
+    if (g.problems != 1 || g.splits != 1 || band == 0) return hipErrorInvalidValue;
+    for (int64_t first = 0; first < rows; first += band) {
+      Gemm16Args part = g;
+      for (Gemm16Pair& p : part.pair) {
+        if (p.a != nullptr) p.a += G::kAColumn ? first : first * p.lda;
+        if (p.out != nullptr) p.out += first * p.ldo;
+        p.m = rows - first < band ? rows - first : band;
+      }
+      const int64_t values = first * g.pair[0].n;
+      for (float** p : {&part.gate, &part.up})
+        if (*p != nullptr) *p += values;
+      for (uint16_t** p : {&part.d_gate, &part.d_up})
+        if (*p != nullptr) *p += values;
+      part.tiles = (part.pair[0].m + G::BM - 1) / G::BM * columns;
+      gemm16_kernel<G><<<static_cast<uint32_t>(part.tiles), G::kThreads, G::kLds, st>>>(part);
+      if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   gemm16_kernel<G><<<static_cast<uint32_t>(g.tiles * g.splits), G::kThreads, G::kLds, st>>>(g);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || g.splits == 1) return e;
   const dim3 grid(static_cast<uint32_t>((most + 1023) / 1024), static_cast<uint32_t>(g.problems));
