@@ -13,8 +13,8 @@ class FeedForwardBlock(torch.nn.Module):
     """``residual + scale * gate * post_norm(mlp(norm(residual)))``.
 
     mlp: any module that takes normalised bfloat16 [..., hidden] (GatedMLP,
-    Int4MLP, ClampedMLP, PackedFP8MoE, SortedGroupedFP8MoE, ...).  The residual
-    stream may be bfloat16 or float32.  gate: a learned value a channel;
+    Int4MLP, ClampedMLP, PackedFP8MoE, SortedGroupedFP8MoE, ...) and returns
+    bfloat16 or float32.  The residual stream may be bfloat16 or float32.  gate: a learned value a channel;
     forward's own `gate` (a token's, a sequence's: see residual_norm) stands in
     for it."""
 
@@ -38,6 +38,8 @@ class FeedForwardBlock(torch.nn.Module):
         returned `normed` is made with (None: no such norm, returns None)."""
         if normed is None:
             normed = rms_norm(residual, self.norm_weight, self.eps, dtype=torch.bfloat16)
+        elif normed.dtype is not torch.bfloat16:  # the block before returned another type
+            normed = normed.to(torch.bfloat16)
         return residual_norm(residual, self.mlp(normed), post_weight=self.post_weight,
                              gate=self.gate if gate is None else gate, scale=self.residual_scale,
                              next_weight=next_weight, eps=self.eps)
