@@ -43,8 +43,9 @@ struct Int {
 };
 
 // y[m, n] = sum_k x[m, k] w(n)[k] of the 16 rows that row(n) gives, per wavefront
-// into part.  X: float rows are split into two bf16 operands, whose products
-// are added: no rounding of x.
+// into part.  X: float rows are split into two bf16 operands, which keep 16 of
+// their 24 bits, and whose products are added at the end: an infinite weight
+// times a low part, of either sign or zero, is left out.
 template <int MT, class X>
 __device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w_row, int K, float (*part)[16 * MT][16]) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -55,12 +56,12 @@ __device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w
 #pragma unroll
   for (int i = 0; i < MT; ++i) x_row[i] = x + static_cast<int64_t>(16 * i + r < rows ? 16 * i + r : rows - 1) * K + 8 * q;
   w_row += 8 * q;
-  f32x4 acc[MT];
+  f32x4 acc[MT], low[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = (f32x4){0, 0, 0, 0};
+  for (int i = 0; i < MT; ++i) acc[i] = low[i] = (f32x4){0, 0, 0, 0};
   constexpr bool kFloat = sizeof(X) == 4;
   constexpr int kHalves = kFloat ? 2 : 1;
-  const auto multiply = [&](f32x4& acc, const u32x4 (&v)[kHalves], const u32x4& w, bool in) {
+  const auto multiply = [&](f32x4& acc, f32x4& low, const u32x4 (&v)[kHalves], const u32x4& w, bool in) {
     const u32x4 zero = {0, 0, 0, 0};
     const bf16x8 b = __builtin_bit_cast(bf16x8, in ? w : zero);
     if constexpr (kFloat) {
@@ -73,7 +74,7 @@ __device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w
         lo[i] = f32_to_bf16(low_part(f0, h0)) | static_cast<uint32_t>(f32_to_bf16(low_part(f1, h1))) << 16;
       }
       acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, in ? hi : zero), b, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, in ? lo : zero), b, acc, 0, 0, 0);
+      low = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, in ? lo : zero), b, low, 0, 0, 0);
     } else {
       acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, in ? v[0] : zero), b, acc, 0, 0, 0);
     }
@@ -94,7 +95,7 @@ __device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) multiply(acc[i], v[u][i], w[u], true);
+      for (int i = 0; i < MT; ++i) multiply(acc[i], low[i], v[u][i], w[u], true);
   };
   int s = first;
   const int whole_last = last < K / 32 ? last : K / 32;
@@ -109,13 +110,14 @@ __device__ __forceinline__ void few_rows(const X* x, int rows, const uint16_t* w
       u32x4 v[kHalves];
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) v[h] = *reinterpret_cast<const u32x4*>(x_row[i] + at + 4 * h);
-      multiply(acc[i], v, w, in);
+      multiply(acc[i], low[i], v, w, in);
     }
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[wave][16 * i + 4 * q + e][r] = acc[i][e];
+    for (int e = 0; e < 4; ++e)
+      part[wave][16 * i + 4 * q + e][r] = kFloat && fabsf(low[i][e]) < INFINITY ? acc[i][e] + low[i][e] : acc[i][e];
   __syncthreads();
 }
 

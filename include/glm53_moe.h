@@ -616,7 +616,9 @@ int glm53_gated_mlp(const glm53_gated_mlp_desc* desc, void* stream);
  * clip(U) silu'(min(G, L)) where G <= L, else 0; d_x = dG Wg + dU Wu, d_gate_weight
  * = dG^T x, d_up_weight = dU^T x, d_down_weight = d_y^T h.  dG, dU and h are
  * rounded to BF16 as operands of these products (up to 16 rows to two BF16
- * parts), sums are FP32 in a fixed order.  rows > 0.  Results may not overlap inputs. */
+ * parts: a gradient that an infinity in x, d_y or a weight makes infinite may
+ * then be NaN), sums are FP32 in a fixed order.  rows > 0.  Results may not
+ * overlap inputs. */
 size_t glm53_gated_mlp_backward_workspace_bytes(int64_t rows, int64_t hidden, int64_t intermediate);
 int glm53_gated_mlp_backward(const glm53_gated_mlp_desc* desc, void* stream);
 
