@@ -178,8 +178,10 @@ class Int4MLP(torch.nn.Module):
                    Int4Linear.from_weight(down, **options), limit)
 
     def forward(self, x):
-        joined = self.gate_up_proj(x)
         limit = math.inf if self.limit is None else float(self.limit)
+        if not limit > 0:
+            raise ValueError(f"limit must be positive, got {limit}")
+        joined = self.gate_up_proj(x)
         if _ops.direct(joined):
             return self.down_proj(native_joined_swiglu(joined, limit))
         _ops.refuse_transforms("Int4MLP", joined)

@@ -196,3 +196,13 @@ def test_python_functions_refuse_cpu_tensors():
                  lambda: M.int4_linear(x, torch.zeros(8, 32, dtype=torch.uint8), torch.ones(8, 1))):
         with pytest.raises((RuntimeError, ValueError)):
             call()
+
+
+@pytest.mark.parametrize("limit", [0.0, -1.0, float("nan")])
+def test_the_mlp_in_4_bits_refuses_the_limits_that_gated_mlp_refuses(limit):
+    import torch
+
+    M = pkg()
+    mlp = M.Int4MLP.from_weights(torch.randn(32, 64), torch.randn(32, 64), torch.randn(64, 32), limit, group_size=32)
+    with pytest.raises(ValueError, match="limit must be positive"):
+        mlp(torch.zeros(2, 64, dtype=torch.bfloat16))
