@@ -80,6 +80,14 @@ def test_offsets_and_tables(dev, offset, rows, k, group):
     _check(_problem(rows, 264, k, group, offset, seed=k))
 
 
+@pytest.mark.parametrize("k", [32, 64, 96, 160, 224])
+@pytest.mark.parametrize("rows", [33, 128, 129, 300])
+@pytest.mark.parametrize("n", [3, 130])
+def test_short_contractions(dev, k, rows, n):
+    """Less than a step of columns, and steps that end in a group of 32."""
+    _check(_problem(rows, n, k, 32, 1.0, seed=k))
+
+
 @pytest.mark.parametrize("n", [100, 1000, 8200])
 def test_a_row_among_any_number_of_rows(dev, n):
     """A row's results with 1, 17, 33 and 129 rows differ by the rounding of
