@@ -104,14 +104,14 @@ def _carries_derivative(t: torch.Tensor) -> bool:
     """Whether `t` carries a tangent or a gradient of torch.func at any of the
     levels that are active: asked level by level from the innermost one, below
     which its wrapper is taken off and the level left."""
-    functorch = torch._C._functorch
+    functorch, forward_ad = torch._C._functorch, torch.autograd.forward_ad
     top = functorch.peek_interpreter_stack()
     if top is None or torch.compiler.is_compiling():
-        return torch.autograd.forward_ad._current_level >= 0 and torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+        return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
     if functorch.is_functorch_wrapped_tensor(t) and functorch.maybe_get_level(t) == top.level():
         if functorch.is_gradtrackingtensor(t):
             if top.key() == functorch.TransformType.Jvp:
-                carries = torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+                carries = forward_ad.unpack_dual(t).tangent is not None
             else:
                 carries = t.requires_grad
             if carries:
