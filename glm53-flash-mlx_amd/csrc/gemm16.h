@@ -156,6 +156,7 @@ __device__ __forceinline__ void store_bias(const Gemm16Args& g, const Gemm16Pair
 
 // Those of the four outputs stored that are not finite, once more by the formula.
 __device__ __forceinline__ void store_bias_again(const Gemm16Args& g, const Gemm16Pair& p, int64_t m, int64_t n) {
+  asm volatile("" ::: "memory");  // read as stored, whatever type they were stored as
 #pragma unroll 1
   for (const int64_t last = n + 4 < p.n ? n + 4 : p.n; n < last; ++n) {
     uint16_t* out = p.out + m * p.ldo + n;
