@@ -29,8 +29,8 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // in LDS in their order; weights go from memory to the MFMA through registers
 // alone, a wavefront's loads all under way at once.  Rows of x are the MFMA's
 // rows, so a lane's four results belong to one weight row.  1 x 4096 x 2048:
-// 8.8 us for gate and up, 5.6 for down, 50 MB at 3.5 TB/s; 1 x 7168 x 18432: 153
-// us, 5.2 TB/s.
+// 7.9 us for gate and up, 5.9 for down, 50 MB at 3.6 TB/s; 1 x 7168 x 18432: 145
+// us, 5.5 TB/s.
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 16;
 // K steps of 32 that a wavefront has in flight (1 x 4096 x 2048 by 16 wavefronts: 2
@@ -129,7 +129,8 @@ __device__ __forceinline__ float few_sum(const float (*part)[16 * MT][16], int m
   return v;
 }
 
-// 8 gate and the 8 up rows of the same outputs a workgroup; h stays FP32.
+// 8 gate and the 8 up rows of the same outputs a workgroup; h goes on in FP32,
+// for few_rows to split.
 template <int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_gate_up_kernel(GatedArgs a, float* h) {
   __shared__ float part[kFewWaves][16 * MT][16];

@@ -5,10 +5,13 @@
 //   x' = x + a g s
 //   y = x' r' w,  r' = (mean x'^2 + eps)^-1/2
 //
-// One workgroup holds a row in registers from its load to its store, so each
-// tensor crosses HBM once: the kernels are bound by those bytes.  All values
-// between load and store are fp32; y is made of the x' that has not been
-// rounded yet.
+// One workgroup holds a row in registers from its load to its store, so that
+// each tensor crosses HBM once in a pass: over many rows the kernels are bound by
+// those bytes.  Beside them the gradients write and read partial column sums, which
+// over few rows are as many (norm_backward_kernel), and past 8,192 columns
+// their registers spill.  All values between load and store are fp32; y is made
+// of the x' that has not been rounded yet.  Squares are summed as they are: rows
+// of values past 2^63 sum to infinity, and their norm is 0.
 #include "common.h"
 #include "norms.h"
 
@@ -270,9 +273,17 @@ __device__ __forceinline__ Slice slice_rows(int64_t rows, int64_t groups, int64_
 
 // Each workgroup takes a run of rows and keeps the column sums of d_post,
 // d_gate (kGateColumns) and d_next in registers, written once as one row of
-// fp32 partial sums: 3 width floats against 16 rows or more of five tensors.
-// The order of the sums is the rows', whatever runs when.  8,192 x 4096 bf16 with
-// all gradients: 85 to 94 us, 403 MB at 4.3 to 4.7 TB/s.
+// fp32 partial sums: 3 width floats beside the six bf16 or fp32 rows of each row
+// that it has, 16 of 8,192 x 4096 and one of 512 x 4096, where the sums, written
+// and read again, are twice the tensors' bytes; a workgroup whose run begins past
+// its group's last row writes zeros.  The order of the sums is the rows',
+// whatever runs when.
+// bf16 with all gradients, us without the join: 8,192 x 4096 85 to 96, 403 MB at
+// 4.2 to 4.7 TB/s; 4,096 x 4096 49; 2,048 29; 512 17.  4,096 x 8192 120, 3.4 TB/s.
+// Odd widths above 2,048 take 256 registers, one workgroup a CU: x 3001 72, x 5000
+// 82.  Past 8,192 columns 1,024 threads have 128 registers each, and 178 (220
+// in odd rows) of a thread's values spill: x 9001 602, x 12288 551, 1.1 TB/s, x
+// 16384 637.
 template <int T, int C, Ends E, bool POST>
 __global__ __launch_bounds__(T) void norm_backward_kernel(NormArgs a, int64_t groups, int64_t slices) {
   using R = Row<T, C, E>;
@@ -448,7 +459,10 @@ hipError_t launch(const NormArgs& a, bool backward, int64_t groups, int64_t slic
   return a.width % kVec ? launch_any<kOverlap>(a, backward, groups, slices, st) : launch_any<kWhole>(a, backward, groups, slices, st);
 }
 
-constexpr int64_t kNormSlices = 512;  // workgroups of 256 threads or more, two a CU
+// Workgroups of 256 threads or more: two a CU, where 256 threads have 218
+// registers each; odd rows, and the 512 and 1,024 threads of wider ones, are one
+// a CU at a time.
+constexpr int64_t kNormSlices = 512;
 
 int64_t gate_groups(const NormArgs& a) {
   return a.gate_kind == kGateColumns && a.rows > 0 ? a.rows / a.rows_per_gate : 1;

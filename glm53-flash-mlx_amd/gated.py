@@ -5,7 +5,11 @@ weights (patch.py:114-129 of the reference).
 
 Gate and up projections, activation and product are one kernel; sums, G, U
 and the activation are FP32, h and y are rounded to bf16 once each (the FP8
-path keeps the reference's rounding after every step instead).  A call that
+path keeps the reference's rounding after every step instead).  Over few rows,
+16, or 32 of at most 4,096 hidden and 2,048 intermediate columns, h enters the
+down projection in two bf16 parts, 16 bits, so a token's result beside few
+others differs from its result in a batch by that rounding (2^-8 of h at most);
+so do dG, dU and h in the gradients, up to 16 rows.  A call that
 may be differentiated keeps G and U in FP32 and h, 10 bytes an intermediate
 value, for the backward pass.
 """

@@ -10,7 +10,8 @@ still to be added to the residual stream; ``rms_norm`` makes that input and
 
 with rms(v) = sqrt(mean(v^2) + eps) over the last axis.  Everything between
 the loads and the stores is FP32 and each result is rounded once; ``normed``
-is made of the new residual before it is rounded.  Both have gradients (first
+is made of the new residual before it is rounded.  Squares are FP32 too: rows of
+values past 2^63 have an infinite rms, and norm to 0.  Both have gradients (first
 order, in reverse mode; forward mode and torch.func's grad, vjp and jvp raise),
 and both are torch custom ops where a call is traced.
 The reference takes its norms from mlx-vlm's layers and has no counterpart.

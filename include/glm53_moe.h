@@ -541,7 +541,8 @@ int glm53_prefill_plan_scratch(glm53_prefill_plan* plan, int32_t which, void** p
  *   y = new_residual / rms(new_residual) * next_weight
  * with rms(v) = sqrt(mean(v^2) + eps), over contiguous rows of `width`
  * elements (at most 16384), aligned to their elements.  FP32 throughout, each
- * output rounded once; y is made of the new residual before it is rounded.  NULL: out (then y is the norm of
+ * output rounded once; y is made of the new residual before it is rounded
+ * (squares are summed in FP32: rows of values past 2^63 norm to 0).  NULL: out (then y is the norm of
  * `residual` alone), post_weight and next_weight (ones), gate (one), y (not
  * computed), stats.  new_residual may be `residual` or `out` itself, y may be
  * `out` or (without out) `residual`, each where the types are the same.  stats f32 [rows, 2] keeps 1 / rms(out)
@@ -585,8 +586,9 @@ int glm53_residual_norm_backward(const glm53_norm* norm, void* stream);
 /*   G = x Wg^T, U = x Wu^T, h = silu(min(G, L)) clip(U, -L, L), y = h Wd^T
  * over contiguous BF16 tensors, 16-byte aligned; hidden and intermediate
  * multiples of 8 up to 2^22; limit L > 0, INFINITY for none.  Sums, G, U and the
- * activation are FP32, h and y are rounded once (h not at all up to 16
- * rows, and up to 32 where hidden is at most 4096 and intermediate 2048).
+ * activation are FP32, h and y are rounded once (h to two BF16 parts, 16 bits
+ * together, up to 16 rows, and up to 32 where hidden is at most 4096 and
+ * intermediate 2048).
  * gate, up (f32) and h (BF16) [rows, intermediate]: all NULL, or where G, U
  * and h are kept for the gradients; up to 16 rows h has two planes, [2, rows,
  * intermediate], what BF16 leaves of h in the second. */
