@@ -15,6 +15,7 @@ from .abi import (
     PACKED_DECODE_KERNEL_ABI,
     PACKED_EXPERT_BANK_ABI,
 )
+from .attention import packed_attention
 from .block import FeedForwardBlock, run_blocks
 from .checkpoint import CheckpointError, load_moe_layer
 from .fp8 import (
@@ -39,6 +40,7 @@ from .grouped_fp8 import (
     restore_and_reduce,
 )
 from .int4 import Int4Linear, Int4MLP, int4_linear, quantize_int4
+from .kv_cache import append_kv, paged_attention, read_kv
 from .loader import install_packed_decode_moe, install_packed_grouped_moe, install_packed_moe
 from .norms import residual_norm, rms_norm
 from .ownership import (

@@ -157,6 +157,54 @@ class Int4Weight(ctypes.Structure):
     ]
 
 
+class HeadRows(ctypes.Structure):
+    _fields_ = [("data", P), ("token_stride", I64), ("head_stride", I64)]
+
+
+class Attention(ctypes.Structure):
+    _fields_ = [
+        ("tokens", I64),
+        ("keys", I64),
+        ("sequences", I64),
+        ("heads", I64),
+        ("kv_heads", I64),
+        ("head_dim", I64),
+        ("q", HeadRows),
+        ("k", HeadRows),
+        ("v", HeadRows),
+        ("offsets", P),
+        ("key_offsets", P),
+        ("out", P),
+        ("lse", P),
+        ("d_out", HeadRows),
+        ("d_q", P),
+        ("d_k", P),
+        ("d_v", P),
+        ("workspace", P),
+        ("workspace_bytes", SZ),
+        ("causal", I32),
+        ("scale", F32),
+    ]
+
+
+class KVCache(ctypes.Structure):
+    _fields_ = [
+        ("k_pages", P),
+        ("v_pages", P),
+        ("k_scales", P),
+        ("v_scales", P),
+        ("page_table", P),
+        ("pages", I64),
+        ("page_size", I64),
+        ("kv_heads", I64),
+        ("head_dim", I64),
+        ("sequences", I64),
+        ("max_pages", I64),
+        ("table_stride", I64),
+        ("e4m3", I32),
+    ]
+
+
 _SIGNATURES = {
     "glm53_last_error": (ctypes.c_char_p, []),
     "glm53_abi_version": (ctypes.c_int, []),
@@ -219,6 +267,13 @@ _SIGNATURES = {
     "glm53_gated_mlp_backward": (ctypes.c_int, [P, P]),
     "glm53_int4_linear_workspace_bytes": (SZ, [I64, I64, I64]),
     "glm53_int4_linear": (ctypes.c_int, [P, P, I64, P, P, SZ, P]),
+    "glm53_packed_attention": (ctypes.c_int, [P, P]),
+    "glm53_packed_attention_backward_workspace_bytes": (SZ, [I64, I64]),
+    "glm53_packed_attention_backward": (ctypes.c_int, [P, P]),
+    "glm53_kv_append": (ctypes.c_int, [P, P, P, I64, P, P, P]),
+    "glm53_kv_read": (ctypes.c_int, [P, P, I64, P, P, P]),
+    "glm53_paged_attention_workspace_bytes": (SZ, [I64, I64, I64, I64]),
+    "glm53_paged_attention": (ctypes.c_int, [P, P, I64, P, F32, P, P, SZ, P]),
     "glm53_synth_fp8": (ctypes.c_int, [P, P, I64, I64, ctypes.c_uint64, F32, P]),
     "glm53_synth_f32": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, F32, F32, I32, P]),
     "glm53_synth_bf16": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, P]),

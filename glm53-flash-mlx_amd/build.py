@@ -20,7 +20,7 @@ CSRC = PKG / "csrc"
 OUT = PKG / "libglm53_moe.so"
 BUILD = PKG / "_build"
 SOURCES = ["decode.hip", "step.hip", "grouped.hip", "dense.hip", "router.hip", "layout.hip", "synth.hip", "norms.hip",
-           "gemm16.hip", "gated.hip", "int4.hip", "api.cpp", "api_block.cpp"]
+           "gemm16.hip", "gated.hip", "int4.hip", "attention.hip", "kv_cache.hip", "api.cpp", "api_block.cpp", "api_attention.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

@@ -1,0 +1,639 @@
+// The paged key-value cache: rows written (and quantised), rows read back,
+// and the attention of one token a sequence over its pages.
+#include "attention_tile.h"
+#include "kv_cache.h"
+
+namespace glm53 {
+
+namespace {
+
+// ---------------------------------------------------- writing and reading ---
+
+// Which sequence row `row` of packed rows belongs to, or -1; a wavefront asks
+// for one row.
+__device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences, int row) {
+  const int lane = threadIdx.x & 63;
+  int count = 0;
+  for (int i = 0; i <= sequences; i += 64)
+    count += __popcll(__ballot(i + lane <= sequences && offsets[i + lane] <= row));
+  count = __builtin_amdgcn_readfirstlane(count);
+  return count >= 1 && count <= sequences ? count - 1 : -1;
+}
+
+// Number of the cache row of a sequence's position, without its head: page *
+// kv_heads << page_log2 and the token in the page; -1 where it has no page.
+struct Place {
+  int64_t page;
+  int token;
+};
+__device__ __forceinline__ Place place_of(const CacheArgs& c, int sequence, int64_t position) {
+  const int64_t n = position >> c.page_log2;
+  if (position < 0 || n >= c.max_pages) return Place{-1, 0};
+  const int page = c.table[sequence * c.table_stride + n];
+  return Place{page >= 0 && page < c.pages ? page : -1, static_cast<int>(position & ((1 << c.page_log2) - 1))};
+}
+
+__device__ __forceinline__ int64_t cache_row(const CacheArgs& c, const Place& p, int head) {
+  return ((p.page * c.kv_heads + head) << c.page_log2) + p.token;
+}
+
+// The power of two that a row whose largest finite |x| is `top` is divided by:
+// the smallest 2^e with top <= 448 * 2^e, 2^-117 or more, so that the smallest
+// code times it is still a normal number.
+__device__ __forceinline__ int row_exponent(float top) {
+  const uint32_t bits = __float_as_uint(top);
+  const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return e < -117 ? -117 : e;
+}
+
+// A wavefront writes one token: its rows of keys and values by groups of LANES
+// lanes, 8 values a lane.  Every code is one conversion of x * 2^-e, whose
+// product is exact or far below the smallest code; |x| * 2^-e <= 448, so nothing
+// saturates.
+template <bool E4M3, int LANES>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+  const CacheArgs& c = a.cache;
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= a.tokens) return;
+  int sequence = row, place = 0;
+  if (a.offsets != nullptr) {
+    sequence = sequence_of(a.offsets, c.sequences, row);
+    if (sequence < 0) return;
+    place = row - a.offsets[sequence];
+  }
+  const Place at = place_of(c, sequence, static_cast<int64_t>(a.lengths[sequence]) + place);
+  if (at.page < 0) return;
+  const int piece = lane % LANES;
+  for (int i = lane / LANES; i < 2 * c.kv_heads; i += 64 / LANES) {
+    const bool values = i >= c.kv_heads;
+    const int head = values ? i - c.kv_heads : i;
+    const Rows16& x = values ? a.rows_v : a.rows_k;
+    const bool in = 8 * piece < c.dim;
+    u32x4 w = {0, 0, 0, 0};
+    if (in) w = *reinterpret_cast<const u32x4*>(x.p + row * x.token + head * x.head + 8 * piece);
+    const int64_t to = cache_row(c, at, head);
+    if constexpr (!E4M3) {
+      if (in) *reinterpret_cast<u32x4*>((values ? c.v : c.k) + (to * c.dim + 8 * piece) * 2) = w;
+    } else {
+      float f[8], top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[j] = bf16_to_f32(static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1))));
+        if (fabsf(f[j]) < INFINITY) top = fmaxf(top, fabsf(f[j]));
+        else f[j] = NAN;
+      }
+#pragma unroll
+      for (int s = LANES / 2; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, LANES));
+      const int e = row_exponent(top);
+      const float by = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      u32x2 codes = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        codes[j] = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j] * by, f[4 * j + 1] * by, codes[j], false);
+        codes[j] = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j + 2] * by, f[4 * j + 3] * by, codes[j], true);
+      }
+      if (in) *reinterpret_cast<u32x2*>((values ? c.v : c.k) + to * c.dim + 8 * piece) = codes;
+      if (piece == 0) (values ? c.v_scales : c.k_scales)[to] = static_cast<uint8_t>(e + 127);
+    }
+  }
+}
+
+// Four E4M3 codes times 2^(scale - 127) as bf16, exact.
+__device__ __forceinline__ u32x2 codes_to_bf16(uint32_t codes, float scale) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false);
+  const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true);
+  return (u32x2){__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
+__device__ __forceinline__ float scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// A wavefront reads one token.
+template <bool E4M3, int LANES>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+  const CacheArgs& c = a.cache;
+  const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const int sequence = sequence_of(a.offsets, c.sequences, row);
+  Place at{-1, 0};
+  if (sequence >= 0) at = place_of(c, sequence, row - a.offsets[sequence]);
+  const uint32_t none = sequence >= 0 ? 0x7FC07FC0u : 0u;
+  const int piece = lane % LANES;
+  if (8 * piece >= c.dim) return;
+  for (int i = lane / LANES; i < 2 * c.kv_heads; i += 64 / LANES) {
+    const bool values = i >= c.kv_heads;
+    const int head = values ? i - c.kv_heads : i;
+    uint16_t* to = values ? a.v : a.k;
+    if (to == nullptr) continue;
+    u32x4 w = {none, none, none, none};
+    if (at.page >= 0) {
+      const int64_t from = cache_row(c, at, head);
+      const uint8_t* p = values ? c.v : c.k;
+      if constexpr (!E4M3) {
+        w = *reinterpret_cast<const u32x4*>(p + (from * c.dim + 8 * piece) * 2);
+      } else {
+        const u32x2 codes = *reinterpret_cast<const u32x2*>(p + from * c.dim + 8 * piece);
+        const float scale = scale_value((values ? c.v_scales : c.k_scales)[from]);
+        const u32x2 lo = codes_to_bf16(codes[0], scale), hi = codes_to_bf16(codes[1], scale);
+        w = (u32x4){lo[0], lo[1], hi[0], hi[1]};
+      }
+    }
+    *reinterpret_cast<u32x4*>(to + (static_cast<int64_t>(row) * c.kv_heads + head) * c.dim + 8 * piece) = w;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_append(const AppendArgs& a, hipStream_t st) {
+  const int dim = a.cache.dim;
+  const uint32_t grid = static_cast<uint32_t>((a.tokens + 3) / 4);
+  if (a.cache.e4m3) {
+    if (dim <= 64) append_kernel<true, 8><<<grid, 256, 0, st>>>(a);
+    else if (dim <= 128) append_kernel<true, 16><<<grid, 256, 0, st>>>(a);
+    else append_kernel<true, 32><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (dim <= 64) append_kernel<false, 8><<<grid, 256, 0, st>>>(a);
+    else if (dim <= 128) append_kernel<false, 16><<<grid, 256, 0, st>>>(a);
+    else append_kernel<false, 32><<<grid, 256, 0, st>>>(a);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_read(const ReadArgs& a, hipStream_t st) {
+  const int dim = a.cache.dim;
+  const uint32_t grid = static_cast<uint32_t>((a.rows + 3) / 4);
+  if (a.cache.e4m3) {
+    if (dim <= 64) read_kernel<true, 8><<<grid, 256, 0, st>>>(a);
+    else if (dim <= 128) read_kernel<true, 16><<<grid, 256, 0, st>>>(a);
+    else read_kernel<true, 32><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (dim <= 64) read_kernel<false, 8><<<grid, 256, 0, st>>>(a);
+    else if (dim <= 128) read_kernel<false, 16><<<grid, 256, 0, st>>>(a);
+    else read_kernel<false, 32><<<grid, 256, 0, st>>>(a);
+  }
+  return hipGetLastError();
+}
+
+namespace {
+
+// ------------------------------------------------------- one token's attention ---
+//
+// Bound by the cache's bytes.  A wavefront streams TS tokens of keys and values
+// at a time into its own part of LDS by direct loads, the next TS on their way
+// while it multiplies: S^T = k q^T (16 tokens x 16 heads, the heads of one key
+// head beside each other) and out^T += v^T P^T, P straight from the registers
+// that S is in, values read across by the transposing LDS read.  No barrier and
+// no exchange between wavefronts until a sequence ends.
+//
+// A sequence's positions in chunks of W * TS tokens, one after the other for
+// every sequence and head, are dealt to kWorkers workgroups in equal
+// contiguous runs, whatever the lengths.  A run holds the end of one (sequence,
+// head), whole ones, which it finishes, and the start of another: two partial results
+// at most, joined by a second launch in their order.
+
+constexpr int kWorkers = 256;  // one workgroup a CU: its stages fill the LDS
+constexpr int kHeads = 16;     // columns of the MFMA
+
+typedef __attribute__((address_space(3))) uint8_t* lds_bytes;
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// Over the four lanes of a column.
+__device__ __forceinline__ float quarter_max(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return both_max(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return both_sum(__uint_as_float(x[0]) + __uint_as_float(x[1]));
+}
+
+// Sequence `s`'s tokens: 0 .. what its table holds; `whole` false where its
+// length says more.
+__device__ __forceinline__ int64_t tokens_of(const DecodeArgs& a, int s, bool& whole) {
+  const int64_t n = a.lengths[s], most = static_cast<int64_t>(a.cache.max_pages) << a.cache.page_log2;
+  whole = n <= most;
+  return n < 0 ? 0 : n > most ? most : n;
+}
+
+// Units (chunks of all heads) of the sequences before `before`; a wavefront
+// asks, every lane gets it.
+__device__ __forceinline__ int64_t units_before(const DecodeArgs& a, int before, int chunk, int parts) {
+  int64_t sum = 0;
+  for (int s = threadIdx.x & 63; s < before; s += 64) {
+    bool whole;
+    sum += (tokens_of(a, s, whole) + chunk - 1) / chunk;
+  }
+#pragma unroll
+  for (int w = 32; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
+  return sum * parts;
+}
+
+__device__ __forceinline__ int64_t run_start(int64_t units, int worker) { return units * worker / kWorkers; }
+// The worker that has unit u.
+__device__ __forceinline__ int run_of(int64_t units, int64_t u) {
+  return static_cast<int>(((u + 1) * kWorkers - 1) / units);
+}
+
+template <int DP_, bool E4M3_>
+struct Decode {
+  static constexpr int DP = DP_;
+  static constexpr bool E4M3 = E4M3_;
+  static constexpr int kRowBytes = E4M3 ? DP : 2 * DP;
+  static constexpr int kPitch = kRowBytes < 128 ? 128 : kRowBytes;
+  static constexpr int kSlots = kPitch / 16, kLoadRows = 64 / kSlots;
+  static constexpr int TS = kPitch >= 256 ? 32 : 64;     // tokens of a stage
+  static constexpr int W = kPitch >= 512 ? 2 : 4;        // wavefronts
+  static constexpr int kThreads = 64 * W, kChunk = W * TS, kSub = TS / 16;
+  static constexpr int kTile = TS * kPitch;
+  static constexpr int kStage = 2 * kTile + (E4M3 ? 512 : 0);
+  static constexpr int kLds = 2 * W * kStage;
+  static constexpr int kLoads = 2 * (TS / kLoadRows) + (E4M3 ? 2 * kSub : 0);  // of a whole stage
+  static_assert(W * kHeads * (DP + 2) * 4 <= kLds, "the wavefronts' results fit where the stages were");
+
+  __device__ static __forceinline__ int swizzle(int row) {
+    return kPitch == 128 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+  }
+
+  static __device__ void run(const DecodeArgs& a, uint8_t* lds) {
+    const CacheArgs& c = a.cache;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quarter = lane >> 4;
+    const int head_parts = (a.group + kHeads - 1) / kHeads, parts = c.kv_heads * head_parts;
+    const int64_t units = units_before(a, c.sequences, kChunk, parts);
+    if (units == 0) return;
+    const int worker = blockIdx.x;
+    int64_t unit = run_start(units, worker);
+    const int64_t end = run_start(units, worker + 1);
+    if (unit >= end) return;
+    // the sequence of the first unit
+    int sequence = 0;
+    int64_t base = 0;  // units before it
+    for (;; sequence += 64) {
+      int64_t own = 0;
+      if (sequence + lane < c.sequences) {
+        bool whole;
+        own = (tokens_of(a, sequence + lane, whole) + kChunk - 1) / kChunk * parts;
+      }
+      int64_t upto = own;
+#pragma unroll
+      for (int w = 1; w < 64; w <<= 1) {
+        const int64_t left = __shfl_up(upto, w);
+        if (lane >= w) upto += left;
+      }
+      const uint64_t past = __ballot(base + upto > unit);
+      if (past != 0) {
+        const int first = __builtin_ctzll(past);
+        sequence += first;
+        base += __shfl(upto, first) - __shfl(own, first);
+        break;
+      }
+      base += __shfl(upto, 63);
+    }
+
+    uint8_t* const mine = lds + 2 * wave * kStage;
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_bytes)mine));
+    const float sc = a.scale * 1.44269504088896340736f;
+    const int row_bytes = E4M3 ? c.dim : 2 * c.dim;
+    const auto clear = [&] {  // pads, where no load writes
+      if (row_bytes == kPitch) return;
+      for (int i = lane; i < 2 * kStage / 16; i += 64) *reinterpret_cast<u32x4*>(mine + 16 * i) = (u32x4){0, 0, 0, 0};
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    clear();
+
+    while (unit < end) {
+      sequence = __builtin_amdgcn_readfirstlane(sequence);
+      bool whole;
+      const int64_t tokens = tokens_of(a, sequence, whole), chunks = (tokens + kChunk - 1) / kChunk;
+      if (chunks == 0 || unit >= base + chunks * parts) {
+        base += chunks * parts;
+        ++sequence;
+        continue;
+      }
+      const int part = static_cast<int>((unit - base) / chunks);
+      const int64_t seg = base + part * chunks;  // its first unit
+      const int head = part / head_parts, first_head = (part - head * head_parts) * kHeads;
+      const int64_t from = unit - seg, to = (end - seg < chunks ? end - seg : chunks);
+
+      // q of 16 heads as the second operand
+      bf16x8 q[DP / 32];
+      const int g = first_head + col;
+      const uint16_t* qp = a.q.p + sequence * a.q.token + (head * a.group + (g < a.group ? g : 0)) * a.q.head;
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) {
+        // dims of operand j: as the keys' 16-byte pieces bring them
+        const int d = E4M3 ? 64 * (j >> 1) + 16 * quarter + 8 * (j & 1) : 32 * j + 8 * quarter;
+        u32x4 v = {0, 0, 0, 0};
+        if (g < a.group && d < c.dim) v = *reinterpret_cast<const u32x4*>(qp + d);
+        q[j] = __builtin_bit_cast(bf16x8, v);
+      }
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) arrived(q[j]);
+      bool bad = !whole;
+      const int32_t* table = c.table + sequence * c.table_stride;
+      const int64_t stages = (tokens + TS - 1) / TS, last = stages < to * W ? stages : to * W;
+      int64_t stage = from * W + wave;
+
+      // The pages of this wavefront's next 64 16-token parts, one a lane.
+      int pages = 0;
+      const auto look_up = [&](int64_t next) {
+        const int64_t first = (next + lane / kSub * W) * TS + lane % kSub * 16;
+        pages = 0;
+        if (first < tokens) {
+          pages = table[first >> c.page_log2];
+          if (pages < 0 || pages >= c.pages) {
+            bad = true;
+            pages = 0;
+          }
+        }
+        arrived(pages);
+      };
+      const auto issue = [&](int64_t next, int slot, int ahead) {
+        const int64_t first = next * TS;
+        const uint32_t at = lds_at + slot * kStage;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read here last
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+          if (first + 16 * u >= tokens) break;
+          const int page = __builtin_amdgcn_readlane(pages, ahead * kSub + u);
+          const int64_t row0 = ((static_cast<int64_t>(page) * c.kv_heads + head) << c.page_log2) +
+                               ((first + 16 * u) & ((1 << c.page_log2) - 1));
+#pragma unroll
+          for (int i = 0; i < 16 / kLoadRows; ++i) {
+            const int row = i * kLoadRows + lane / kSlots, piece = (lane % kSlots) ^ swizzle(row);
+            const uint32_t off = row * row_bytes + 16 * piece;
+            const uint32_t to_lds = at + (16 * u + i * kLoadRows) * kPitch;
+            if (16 * piece < row_bytes) {
+              load_to_lds(c.k + row0 * row_bytes, off, to_lds);
+              load_to_lds(c.v + row0 * row_bytes, off, to_lds + kTile);
+            }
+          }
+          if constexpr (E4M3) {
+            if (lane < 4) {
+              load_to_lds<4>(c.k_scales + row0, 4 * lane, at + 2 * kTile + 16 * u);
+              load_to_lds<4>(c.v_scales + row0, 4 * lane, at + 2 * kTile + 256 + 16 * u);
+            }
+          }
+        }
+      };
+
+      float m = -INFINITY, l = 0.0f;
+      f32x4 out[DP / 16];
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) out[t] = (f32x4){0, 0, 0, 0};
+
+      const auto compute = [&](int64_t stage, int slot) {
+        const uint8_t* kt = mine + slot * kStage;
+        const uint8_t* vt = kt + kTile;
+        const int64_t left64 = tokens - stage * TS;
+        const int left = left64 < TS ? static_cast<int>(left64) : TS;
+#pragma unroll
+        for (int u = 0; u < kSub; u += 2) {  // 32 tokens
+          f32x4 s[2], vs[2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            s[b] = (f32x4){0, 0, 0, 0};
+            const uint8_t* row = kt + (16 * (u + b) + col) * kPitch;
+            if constexpr (!E4M3) {
+#pragma unroll
+              for (int j = 0; j < DP / 32; ++j)
+                s[b] = mfma16(*reinterpret_cast<const bf16x8*>(row + 16 * ((4 * j + quarter) ^ swizzle(col))), q[j], s[b]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < DP / 64; ++j) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(row + 16 * ((4 * j + quarter) ^ swizzle(col)));
+                const u32x2 x0 = codes_to_bf16(w[0], 1.0f), x1 = codes_to_bf16(w[1], 1.0f);
+                const u32x2 x2 = codes_to_bf16(w[2], 1.0f), x3 = codes_to_bf16(w[3], 1.0f);
+                s[b] = mfma16(__builtin_bit_cast(bf16x8, (u32x4){x0[0], x0[1], x1[0], x1[1]}), q[2 * j], s[b]);
+                s[b] = mfma16(__builtin_bit_cast(bf16x8, (u32x4){x2[0], x2[1], x3[0], x3[1]}), q[2 * j + 1], s[b]);
+              }
+              const uint32_t ks = *reinterpret_cast<const uint32_t*>(vt + kTile + 16 * (u + b) + 4 * quarter);
+              const uint32_t ws = *reinterpret_cast<const uint32_t*>(vt + kTile + 256 + 16 * (u + b) + 4 * quarter);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                s[b][r] *= scale_value((ks >> (8 * r)) & 255);
+                vs[b][r] = scale_value((ws >> (8 * r)) & 255);
+              }
+            }
+          }
+          const int here = left - 16 * u - 4 * quarter;  // tokens of this lane's part that exist
+          if (left < TS) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (16 * b + r >= here) s[b][r] = -INFINITY;
+          }
+          const float top = quarter_max(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                              fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
+          if (__any(top * sc > m * sc + 8.0f)) {  // see the packed form: weights reach 2^8
+            const float next = fmaxf(m, top), alpha = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - next) * sc);
+            m = next;
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) out[t][r] *= alpha;
+          }
+          const float mc = m == -INFINITY ? 0.0f : m * sc;
+          bf16x8 p;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float w = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc, -mc));
+              l += w;
+              p[4 * b + r] = static_cast<__bf16>(!E4M3 ? w : left < TS && 16 * b + r >= here ? 0.0f : w * vs[b][r]);
+            }
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) {
+            bf16x8 v = values(vt, u, t, lane);
+            if (left < TS) {  // what lies behind the last token is no value
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (16 * (e >> 2) + (e & 3) >= here) v[e] = static_cast<__bf16>(0.0f);
+            }
+            out[t] = mfma16(v, p, out[t]);
+          }
+        }
+      };
+
+      constexpr int kAhead = 64 / kSub;  // stages of a look-up
+      int slot = 0, ahead = 0;
+      if (stage < last) {
+        look_up(stage);
+        issue(stage, 0, 0);
+      }
+      for (; stage < last; stage += W, slot ^= 1) {
+        if (stage + W < last) {
+          if (++ahead == kAhead) {
+            ahead = 0;
+            look_up(stage + W);
+          }
+          issue(stage + W, slot ^ 1, ahead);
+          if ((stage + W + 1) * TS <= tokens)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+          else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        compute(stage, slot);
+      }
+
+      // the wavefronts' results, where their stages were
+      l = quarter_sum(l);
+      if (__any(bad)) l = NAN;
+      __syncthreads();
+      float* const sums = reinterpret_cast<float*>(lds);  // [W][16][DP], then [W][16][2]
+      float* const stats = sums + W * kHeads * DP;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t)
+        *reinterpret_cast<f32x4*>(sums + (wave * kHeads + col) * DP + 16 * t + 4 * quarter) = out[t];
+      if (quarter == 0) {
+        stats[(wave * kHeads + col) * 2] = m;
+        stats[(wave * kHeads + col) * 2 + 1] = l;
+      }
+      __syncthreads();
+      const bool finished = from == 0 && to == chunks;
+      float* const to_sums = a.partial + static_cast<int64_t>(2 * worker + (from == 0 ? 1 : 0)) * kHeads * (DP + 2);
+      for (int i = threadIdx.x; i < kHeads * DP / 4; i += kThreads) {
+        const int hd = i / (DP / 4), d = 4 * (i % (DP / 4));
+        if (first_head + hd >= a.group || d >= c.dim) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < W; ++w) top = fmaxf(top, stats[(w * kHeads + hd) * 2]);
+        float total = 0.0f;
+        f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float mw = stats[(w * kHeads + hd) * 2];
+          const float by = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - top) * sc);
+          const float lw = stats[(w * kHeads + hd) * 2 + 1];
+          total += lw != lw ? lw : by * lw;
+          const f32x4 x = *reinterpret_cast<const f32x4*>(sums + (w * kHeads + hd) * DP + d);
+          if (by != 0.0f) sum += by * x;
+        }
+        if (finished) {
+          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+          uint16_t* o = a.out + (static_cast<int64_t>(sequence) * c.kv_heads * a.group + head * a.group + first_head + hd) * c.dim + d;
+          *reinterpret_cast<u32x2*>(o) = pack4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
+        } else {
+          *reinterpret_cast<f32x4*>(to_sums + hd * DP + d) = sum;
+          if (d == 0) {
+            to_sums[kHeads * DP + 2 * hd] = top;
+            to_sums[kHeads * DP + 2 * hd + 1] = total;
+          }
+        }
+      }
+      __syncthreads();
+      clear();
+      unit = seg + to;
+    }
+  }
+
+  // Dims 16 t .. + 15 of 32 tokens from part u on, as a first operand whose
+  // contraction is in the order of P's registers.
+  __device__ static __forceinline__ bf16x8 values(const uint8_t* vt, int u, int t, int lane) {
+    const int a = lane & 15, quarter = lane >> 4;
+    if constexpr (!E4M3) {
+      typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+      s16x4 v[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int row = 16 * (u + b) + 4 * quarter + (a >> 2), piece = 2 * t + ((a & 3) >> 1);
+        v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(vt + row * kPitch + 16 * (piece ^ swizzle(row)) + 8 * (a & 1)));
+      }
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      // eight rows of 16 codes: lane a of 16 reads row a / 2, codes 8 (a % 2) .. + 7
+      typedef int i32x2 __attribute__((vector_size(8)));
+      typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
+      const int i = a >> 1, row = 16 * (u + (i >> 2)) + 4 * quarter + (i & 3);
+      const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(
+          vt + row * kPitch + 16 * (t ^ swizzle(row)) + 8 * (a & 1)));
+      const u32x2 lo = codes_to_bf16(static_cast<uint32_t>(w[0]), 1.0f), hi = codes_to_bf16(static_cast<uint32_t>(w[1]), 1.0f);
+      return __builtin_bit_cast(bf16x8, (u32x4){lo[0], lo[1], hi[0], hi[1]});
+    }
+  }
+};
+
+template <class D>
+__global__ __launch_bounds__(D::kThreads) void decode_kernel(DecodeArgs a) {
+  extern __shared__ __align__(1024) uint8_t lds[];
+  D::run(a, lds);
+}
+
+// One (sequence, key head, 16 heads) a workgroup: adds its parts where there
+// are several, and writes 0 where the sequence has no token.
+template <class D>
+__global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
+  constexpr int DP = D::DP;
+  const CacheArgs& c = a.cache;
+  const int head_parts = (a.group + kHeads - 1) / kHeads, parts = c.kv_heads * head_parts;
+  const int sequence = blockIdx.x / parts, part = blockIdx.x - sequence * parts;
+  const int head = part / head_parts, first_head = (part - head * head_parts) * kHeads;
+  bool whole;
+  const int64_t tokens = tokens_of(a, sequence, whole), chunks = (tokens + D::kChunk - 1) / D::kChunk;
+  int first = 0, last = -1;
+  if (chunks > 0) {
+    const int64_t units = units_before(a, c.sequences, D::kChunk, parts);
+    const int64_t seg = units_before(a, sequence, D::kChunk, parts) + part * chunks;
+    first = run_of(units, seg);
+    last = run_of(units, seg + chunks - 1);
+    if (first == last) return;
+  }
+  const float sc = a.scale * 1.44269504088896340736f;
+  for (int i = threadIdx.x; i < kHeads * DP / 4; i += 256) {
+    const int hd = i / (DP / 4), d = 4 * (i % (DP / 4));
+    if (first_head + hd >= a.group || d >= c.dim) continue;
+    float top = -INFINITY, total = whole ? 0.0f : NAN;
+    f32x4 sum = {0, 0, 0, 0};
+    for (int w = first; w <= last; ++w) {
+      const float* p = a.partial + static_cast<int64_t>(2 * w + (w == first ? 1 : 0)) * kHeads * (DP + 2);
+      const float mw = p[kHeads * DP + 2 * hd], lw = p[kHeads * DP + 2 * hd + 1];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + hd * DP + d);
+      const float next = fmaxf(top, mw);
+      const float old = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - next) * sc);
+      const float by = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - next) * sc);
+      total = (total != total ? total : old * total) + (lw != lw ? lw : by * lw);
+      if (old != 0.0f) sum *= old; else sum = (f32x4){0, 0, 0, 0};
+      if (by != 0.0f) sum += by * x;
+      top = next;
+    }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    uint16_t* o = a.out + (static_cast<int64_t>(sequence) * c.kv_heads * a.group + head * a.group + first_head + hd) * c.dim + d;
+    *reinterpret_cast<u32x2*>(o) = pack4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
+  }
+}
+
+template <class D>
+hipError_t decode(const DecodeArgs& a, hipStream_t st) {
+  decode_kernel<D><<<kWorkers, D::kThreads, D::kLds, st>>>(a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  const int64_t grid = static_cast<int64_t>(a.cache.sequences) * a.cache.kv_heads * ((a.group + kHeads - 1) / kHeads);
+  decode_join_kernel<D><<<static_cast<uint32_t>(grid), 256, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+}  // namespace
+
+size_t decode_space(int dim) { return sizeof(float) * 2 * kWorkers * kHeads * (padded(dim) + 2); }
+
+hipError_t launch_decode(const DecodeArgs& a, hipStream_t st) {
+  if (a.cache.e4m3) {
+    if (a.cache.dim <= 64) return decode<Decode<64, true>>(a, st);
+    if (a.cache.dim <= 128) return decode<Decode<128, true>>(a, st);
+    return decode<Decode<256, true>>(a, st);
+  }
+  if (a.cache.dim <= 64) return decode<Decode<64, false>>(a, st);
+  if (a.cache.dim <= 128) return decode<Decode<128, false>>(a, st);
+  return decode<Decode<256, false>>(a, st);
+}
+
+}  // namespace glm53

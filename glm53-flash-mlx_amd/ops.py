@@ -342,3 +342,95 @@ def joined_swiglu(joined: torch.Tensor, limit: float) -> torch.Tensor:
 @joined_swiglu.register_fake
 def _(joined, limit):
     return joined.new_empty((*joined.shape[:-1], joined.shape[-1] // 2))
+
+
+@torch.library.custom_op("glm53::packed_attention", mutates_args=())
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Optional[torch.Tensor],
+                     key_offsets: Optional[torch.Tensor], causal: bool, scale: float,
+                     keep: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    from .attention import native_packed_attention
+
+    out, lse = native_packed_attention(q, k, v, offsets, key_offsets, causal, scale, keep)
+    return out, q.new_empty(0, dtype=torch.float32) if lse is None else lse
+
+
+@packed_attention.register_fake
+def _(q, k, v, offsets, key_offsets, causal, scale, keep):
+    kept = (k.shape[1], q.shape[0] * (q.shape[1] // k.shape[1])) if keep else (0,)
+    return q.new_empty(q.shape), q.new_empty(kept, dtype=torch.float32)
+
+
+@torch.library.custom_op("glm53::packed_attention_backward", mutates_args=())
+def packed_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Optional[torch.Tensor],
+                              key_offsets: Optional[torch.Tensor], out: torch.Tensor, lse: torch.Tensor,
+                              d_out: torch.Tensor, causal: bool, scale: float, wanted: list[bool]) -> list[torch.Tensor]:
+    from .attention import native_packed_attention_backward
+
+    grads = native_packed_attention_backward(q, k, v, offsets, key_offsets, out, lse, d_out, causal, scale, wanted)
+    return [q.new_empty(0) if g is None else g for g in grads]
+
+
+@packed_attention_backward.register_fake
+def _(q, k, v, offsets, key_offsets, out, lse, d_out, causal, scale, wanted):
+    return [t.new_empty(t.shape) if w else q.new_empty(0) for t, w in zip((q, k, v), wanted)]
+
+
+def _packed_attention_context(ctx, inputs, output):
+    if not inputs[7]:
+        raise RuntimeError("glm53::packed_attention without keep has no gradient")
+    ctx.save_for_backward(*inputs[:5], *output)
+    ctx.causal, ctx.scale = inputs[5:7]
+    ctx.set_materialize_grads(False)
+
+
+def _packed_attention_backward(ctx, d_out, _):
+    if d_out is None:
+        return (None,) * 8
+    wanted = [bool(w) for w in ctx.needs_input_grad[:3]]
+    grads = torch.ops.glm53.packed_attention_backward(*ctx.saved_tensors, d_out, ctx.causal, ctx.scale, wanted)
+    return (*(g if w else None for g, w in zip(grads, wanted)), None, None, None, None, None)
+
+
+packed_attention.register_autograd(_packed_attention_backward, setup_context=_packed_attention_context)
+
+
+@torch.library.custom_op("glm53::append_kv", mutates_args=("k_pages", "v_pages", "k_scales", "v_scales"))
+def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+              lengths: torch.Tensor, offsets: Optional[torch.Tensor], k_scales: Optional[torch.Tensor],
+              v_scales: Optional[torch.Tensor]) -> None:
+    from .kv_cache import native_append_kv
+
+    native_append_kv(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scales, v_scales)
+
+
+@append_kv.register_fake
+def _(k, v, k_pages, v_pages, page_table, lengths, offsets, k_scales, v_scales):
+    return None
+
+
+@torch.library.custom_op("glm53::read_kv", mutates_args=())
+def read_kv(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, offsets: torch.Tensor, rows: int,
+            k_scales: Optional[torch.Tensor], v_scales: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    from .kv_cache import native_read_kv
+
+    return native_read_kv(k_pages, v_pages, page_table, offsets, rows, k_scales, v_scales)
+
+
+@read_kv.register_fake
+def _(k_pages, v_pages, page_table, offsets, rows, k_scales, v_scales):
+    shape = (rows, k_pages.shape[1], k_pages.shape[3])
+    return tuple(k_pages.new_empty(shape, dtype=torch.bfloat16) for _ in range(2))
+
+
+@torch.library.custom_op("glm53::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, k_scales: Optional[torch.Tensor], v_scales: Optional[torch.Tensor],
+                    scale: float) -> torch.Tensor:
+    from .kv_cache import native_paged_attention
+
+    return native_paged_attention(q, k_pages, v_pages, page_table, lengths, k_scales, v_scales, scale)
+
+
+@paged_attention.register_fake
+def _(q, k_pages, v_pages, page_table, lengths, k_scales, v_scales, scale):
+    return q.new_empty(q.shape)

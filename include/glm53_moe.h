@@ -654,6 +654,92 @@ int glm53_int4_linear(const glm53_int4_weight* weight, const void* x, int64_t ro
                       size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Attention over packed sequences, with its gradients, and over a paged
+ * key-value cache (no reference counterpart: its attention is sparse and
+ * recurrent, over caches of its own).
+ * ---------------------------------------------------------------------- */
+/* Rows of one head each in BF16: element d of head h of token t at data + t *
+ * token_stride + h * head_stride + d.  16-byte aligned, strides multiples of 8
+ * elements up to 2^22. */
+typedef struct glm53_head_rows {
+  const void* data;
+  int64_t token_stride, head_stride;
+} glm53_head_rows;
+/*   S = scale q k^T over the keys that a query sees, P = softmax(S), out = P v
+ * Sequence s has queries offsets[s] .. offsets[s + 1] - 1 of `tokens` and keys
+ * key_offsets[s] .. key_offsets[s + 1] - 1 of `keys` (int32 [sequences + 1],
+ * ascending; key_offsets NULL: offsets; offsets NULL: one sequence of all, key_offsets
+ * NULL too).  causal: query i of n sees keys 0 .. i + (the sequence's keys) -
+ * n, so that the last query sees them all.  A query that sees no key, and rows of
+ * no sequence, are 0.  Query head h reads key head h / (heads / kv_heads).
+ * head_dim a multiple of 8 up to 256; tokens * heads and keys * heads below 2^30.
+ * Scores, softmax and sums are FP32; P is rounded to BF16 as an operand, out once. */
+typedef struct glm53_attention {
+  int64_t tokens, keys, sequences, heads, kv_heads, head_dim;
+  glm53_head_rows q; /* [tokens, heads] */
+  glm53_head_rows k; /* [keys, kv_heads] */
+  glm53_head_rows v;
+  const int32_t* offsets;
+  const int32_t* key_offsets;
+  void* out;  /* [tokens, heads, head_dim] contiguous, 16-byte aligned; forward: written, backward: read */
+  float* lse; /* [kv_heads, tokens * heads / kv_heads]: what the gradients need; forward: NULL where not kept */
+  /* backward only; results contiguous and 16-byte aligned, NULL: not wanted */
+  glm53_head_rows d_out; /* [tokens, heads] */
+  void* d_q;             /* [tokens, heads, head_dim] */
+  void* d_k;             /* [keys, kv_heads, head_dim] */
+  void* d_v;
+  void* workspace; /* 256-byte aligned, needs no initialisation */
+  size_t workspace_bytes;
+  int32_t causal;
+  float scale; /* above 0 */
+} glm53_attention;
+int glm53_packed_attention(const glm53_attention* attention, void* stream);
+/* delta = sum(d_out out), dP = d_out v^T, dS = P (dP - delta); d_q = scale dS
+ * k, d_k = scale dS^T q and d_v = P^T d_out, summed over a key head's query heads,
+ * in FP32 in a fixed order.  P and dS are rounded to BF16 as operands.  Rows
+ * of no sequence get 0.  Results may not overlap inputs. */
+size_t glm53_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t heads);
+int glm53_packed_attention_backward(const glm53_attention* attention, void* stream);
+
+/* A cache of keys and values: `pages` pages of page_size tokens (a power of two
+ * from 16 to 2^16), row (page, head, token) of head_dim values, contiguous and
+ * 16-byte aligned.  BF16 as they were given, or (e4m3) E4M3 codes and the byte
+ * 127 + e of each row, [pages, kv_heads, page_size]: values code * 2^e, e the
+ * smallest with |x| <= 448 * 2^e for the row's finite x, -117 or more.  An
+ * infinity or NaN is stored as NaN.  Every stored value is a BF16 value.
+ * Token `position` of sequence s lies in page_table[s, position / page_size]
+ * (int32 [sequences, table_stride], of which max_pages are a sequence's). */
+typedef struct glm53_kv_cache {
+  void* k_pages;
+  void* v_pages;
+  uint8_t* k_scales; /* e4m3 only */
+  uint8_t* v_scales;
+  const int32_t* page_table;
+  int64_t pages, page_size, kv_heads, head_dim;
+  int64_t sequences, max_pages, table_stride;
+  int32_t e4m3;
+} glm53_kv_cache;
+/* Writes `tokens` new rows of each head: sequence s's, offsets[s] ..
+ * offsets[s + 1] - 1 (NULL: one each), at its positions lengths[s] on.  Rows whose
+ * position has no page, or one outside the cache, are not written.  Two
+ * sequences that share the page they write to overwrite each other. */
+int glm53_kv_append(const glm53_kv_cache* cache, const glm53_head_rows* k, const glm53_head_rows* v, int64_t tokens,
+                    const int32_t* offsets, const int32_t* lengths, void* stream);
+/* Reads sequence s's positions 0 .. offsets[s + 1] - offsets[s] - 1 into rows
+ * offsets[s] on of k and v, BF16 [rows, kv_heads, head_dim] contiguous (either may be
+ * NULL).  Rows of no sequence are 0, positions without a page in the cache NaN. */
+int glm53_kv_read(const glm53_kv_cache* cache, const int32_t* offsets, int64_t rows, void* k, void* v, void* stream);
+/* One query a sequence, q [sequences, heads], over its positions 0 ..
+ * lengths[s] - 1; out BF16 [sequences, heads, head_dim] contiguous.  A sequence
+ * without a token gives 0, one with a position that has no page in the cache
+ * NaN.  The work is split evenly over the card whatever the lengths; parts
+ * are joined in their order.  Workspace (256-byte aligned) needs no
+ * initialisation. */
+size_t glm53_paged_attention_workspace_bytes(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim);
+int glm53_paged_attention(const glm53_kv_cache* cache, const glm53_head_rows* q, int64_t heads, const int32_t* lengths,
+                          float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
  * Seeded synthetic inputs (no reference counterpart: the reference loads a
  * checkpoint).  Element i of stream `seed` is N(0, std) (or U(lo, hi)). */
 int glm53_synth_fp8(uint8_t* codes, float* scale_inv, int64_t rows, int64_t cols, uint64_t seed,
