@@ -20,7 +20,7 @@ CSRC = PKG / "csrc"
 OUT = PKG / "libglm53_moe.so"
 BUILD = PKG / "_build"
 SOURCES = ["decode.hip", "step.hip", "grouped.hip", "dense.hip", "router.hip", "layout.hip", "synth.hip", "norms.hip",
-           "gemm16.hip", "gated.hip", "int4.hip", "attention.hip", "kv_cache.hip", "api.cpp", "api_block.cpp", "api_attention.cpp"]
+           "gemm16.hip", "gated.hip", "int4.hip", "attention.hip", "attention_wide.hip", "kv_cache.hip", "api.cpp", "api_block.cpp", "api_attention.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
@@ -38,7 +38,7 @@ COMMON = [
 # Per-source additions.  The matrix kernels: MFMA results in ordinary VGPRs (the
 # compiler otherwise parks the chained hi/lo results of the narrow GEMM in
 # accumulation registers and copies every element out before folding it).
-EXTRA = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("grouped.hip", "dense.hip", "gemm16.hip", "gated.hip", "int4.hip")}
+EXTRA = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("grouped.hip", "dense.hip", "gemm16.hip", "gated.hip", "int4.hip", "attention.hip")}
 
 
 def _compile(src: str) -> Path:

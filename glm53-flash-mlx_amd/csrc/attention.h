@@ -40,5 +40,8 @@ struct AttentionArgs {
 
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t st);
 hipError_t launch_attention_backward(const AttentionArgs& a, hipStream_t st);
+// The same for heads of more than 128 values.
+hipError_t launch_attention_wide(const AttentionArgs& a, hipStream_t st);
+hipError_t launch_attention_backward_wide(const AttentionArgs& a, hipStream_t st);
 
 }  // namespace glm53

@@ -1,672 +1,27 @@
-// Attention within packed sequences, forward and backward.
-//
-//   S = scale q k^T over the keys a query sees, P = softmax(S), out = P v
-//
-// A row is one query of one head.  The `group` heads of a key head are rows
-// of the same tile, token by token, so that a tile's keys and values serve all
-// of them, and a key head's gradients are one contraction over its rows.
-#include <type_traits>
-
-#include "attention.h"
-#include "attention_tile.h"
+// Attention over heads of up to 128 values.
+#include "attention_kernels.h"
 
 namespace glm53 {
-
-namespace {
 
 #ifndef ATT_RB
 #define ATT_RB 1
 #define ATT_W 4
 #endif
-constexpr float kLog2e = 1.44269504088896340736f;
-// A row's maximum is kept until a new one is this many powers of two above it:
-// the weights 2^(s - m) then reach 2^8, which changes no relative rounding, and
-// few tiles after the first rescale their sums.
-constexpr float kSlack = 8.0f;
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Keys of sequence `number`: first and how many.
-__device__ __forceinline__ void sequence_keys(const AttentionArgs& a, int number, int& first, int& count) {
-  const int32_t* offsets = a.key_offsets != nullptr ? a.key_offsets : a.offsets;
-  if (offsets == nullptr) {
-    first = 0;
-    count = static_cast<int>(a.keys);
-    return;
-  }
-  const int most = static_cast<int>(a.keys);
-  int lo = offsets[number], hi = offsets[number + 1];
-  lo = lo < 0 ? 0 : lo > most ? most : lo;
-  hi = hi < lo ? lo : hi > most ? most : hi;
-  first = __builtin_amdgcn_readfirstlane(lo);
-  count = __builtin_amdgcn_readfirstlane(hi - lo);
-}
-
-// Tile numbers of `rows` rows in `sequences` sequences (see find_segment).
-int64_t tile_numbers(int64_t rows, bool packed, int sequences, int size) {
-  return packed ? rows / size + sequences + 2 : (rows + size - 1) / size;
-}
-
-// ------------------------------------------------------------- forward ---
-//
-// W wavefronts of RB x 32 rows; a tile of 64 keys is multiplied while the next
-// one is loaded.  Scores are computed as S^T (keys the result's rows), so a
-// lane holds 32 of its row's 64 scores, a row's maximum and sum are within a
-// lane and its counterpart 32 lanes away, and the weights go into the second
-// product (out^T = v^T P^T) from the registers they are in.
-
-template <int DP_, bool EXACT, int RB_, int W_>
-struct Forward {
-  static constexpr int DP = DP_, RB = RB_, W = W_;
-  static constexpr int kRows = 32 * RB * W, kThreads = 64 * W, kKeys = 64;
-  using Tile = HeadTile<DP, kKeys, W>;
-  static constexpr int kLds = 4 * Tile::kBytes;  // two stages of keys and values
-
-  static __device__ __forceinline__ void run(const AttentionArgs& a, const Divisor& group, int tiles, uint8_t* lds) {
-    const int dim = EXACT ? DP : a.dim;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = blockIdx.x % a.kv_heads, number = tiles - 1 - blockIdx.x / a.kv_heads;
-    const Segment seg = find_segment(a.offsets, a.sequences, a.tokens, a.group, kRows, number);
-    const int row0 = seg.first + seg.tile * kRows;
-    if (seg.tile < 0 || row0 >= seg.last) return;
-
-    int key0 = 0, keys = 0;
-    if (seg.number >= 0) sequence_keys(a, seg.number, key0, keys);
-    // keys that the query of row r sees: a prefix
-    const int shift = keys - group.quotient(seg.last - seg.first);
-    const auto limit = [&](int row) {
-      if (!a.causal) return keys;
-      const int n = group.quotient(row - seg.first) + shift + 1;
-      return n < 0 ? 0 : n > keys ? keys : n;
-    };
-    const int last_row = row0 + kRows < seg.last ? row0 + kRows - 1 : seg.last - 1;
-    const int steps = (__builtin_amdgcn_readfirstlane(limit(last_row)) + kKeys - 1) / kKeys;
-
-    const int h = lane >> 5;
-    int row[RB], lim[RB];
-    bf16x8 q[RB][DP / 16];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      row[b] = row0 + 32 * (RB * wave + b) + (lane & 31);
-      const int r = row[b] < seg.last ? row[b] : seg.last - 1;  // rows past the last repeat it
-      lim[b] = limit(r);
-      const int token = group.quotient(r);
-      const uint16_t* p = a.q.p + token * a.q.token + (head * a.group + r - token * a.group) * a.q.head;
-#pragma unroll
-      for (int j = 0; j < DP / 16; ++j) {
-        u32x4 v = {0, 0, 0, 0};
-        if (16 * j + 8 * h < dim) v = *reinterpret_cast<const u32x4*>(p + 16 * j + 8 * h);
-        q[b][j] = __builtin_bit_cast(bf16x8, v);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int j = 0; j < DP / 16; ++j) arrived(q[b][j]);
-    const int all_see = __builtin_amdgcn_readfirstlane(lim[0]);                  // every row of the wavefront
-    const int some_see = __builtin_amdgcn_readlane(lim[RB - 1], 31);             // its last row
-
-    if (dim < DP) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) Tile::clear(lds + s * Tile::kBytes, dim, kThreads);
-    }
-    const uint16_t* kp = a.k.p + static_cast<int64_t>(key0) * a.k.token + static_cast<int64_t>(head) * a.k.head;
-    const uint16_t* vp = a.v.p + static_cast<int64_t>(key0) * a.v.token + static_cast<int64_t>(head) * a.v.head;
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    const auto issue = [&](int step) {
-      const uint32_t at = lds_at + (step & 1) * 2 * Tile::kBytes;
-      const int64_t first = static_cast<int64_t>(step) * kKeys;
-      const int left = keys - step * kKeys;
-      const auto rows = [](int64_t pitch) {
-        return [p = static_cast<uint32_t>(2 * pitch)](int row) { return static_cast<uint32_t>(row) * p; };
-      };
-      Tile::load(kp + first * a.k.token, rows(a.k.token), left, dim, wave, lane, at);
-      Tile::load(vp + first * a.v.token, rows(a.v.token), left, dim, wave, lane, at + Tile::kBytes);
-    };
-
-    const float c = a.scale * kLog2e;
-    f32x16 out[RB][DP / 32];
-    float m[RB], l[RB];  // m in units of scores; l: this lane's part
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      m[b] = -INFINITY;
-      l[b] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < DP / 32; ++t) out[b][t] = zero16();
-    }
-
-    uint32_t dirty = 0;
-    const auto compute = [&](int step, auto masked) {
-      constexpr bool kMasked = decltype(masked)::value;
-      const uint8_t* kt = lds + (step & 1) * 2 * Tile::kBytes;
-      const uint8_t* vt = kt + Tile::kBytes;
-      f32x16 s[RB][2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-        for (int b = 0; b < RB; ++b) s[b][kb] = zero16();
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-          const bf16x8 f = Tile::along(kt, kb, j, lane);
-#pragma unroll
-          for (int b = 0; b < RB; ++b) s[b][kb] = mfma32(f, q[b][j], s[b][kb]);
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        if constexpr (kMasked) {
-          const int left = lim[b] - step * kKeys - 4 * h;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (32 * kb + result_row(r, 0) >= left) s[b][kb][r] = -INFINITY;
-        }
-        float top = s[b][0][0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[b][0][r]);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][1][r]);
-        top = both_max(top);
-        if (__any(top * c > m[b] * c + kSlack)) {
-          const float next = fmaxf(m[b], top);
-          const float alpha = next == -INFINITY ? 1.0f : exp2_fast((m[b] - next) * c);
-          m[b] = next;
-          l[b] *= alpha;
-#pragma unroll
-          for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) out[b][t][r] *= alpha;
-        }
-        const float mc = m[b] == -INFINITY ? 0.0f : m[b] * c;
-        float sum = 0.0f;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[b][kb][r] = exp2_fast(fmaf(s[b][kb][r], c, -mc));
-            sum += s[b][kb][r];
-          }
-        l[b] += sum;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        bf16x8 p[RB];
-#pragma unroll
-        for (int b = 0; b < RB; ++b) p[b] = operand8(s[b][i >> 1], i & 1);
-#pragma unroll
-        for (int t = 0; t < DP / 32; ++t) {
-          bf16x8 f = Tile::across(vt, i, t, lane);
-          if constexpr (kMasked) f = finite_part(f, dirty);
-#pragma unroll
-          for (int b = 0; b < RB; ++b) out[b][t] = mfma32(f, p[b], out[b][t]);
-        }
-      }
-    };
-
-    if (steps > 0) issue(0);
-    for (int step = 0; step < steps; ++step) {
-      loads_done();
-      if (step + 1 < steps) issue(step + 1);
-      if ((step + 1) * kKeys <= all_see)
-        compute(step, std::false_type{});
-      else if (step * kKeys < some_see)
-        compute(step, std::true_type{});
-    }
-
-    if (__any(dirty != 0)) {
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-        add_nonfinite<DP>(out[b], all_see / kKeys * kKeys, some_see, dim, h,
-                          [&](int key) { return vp + key * a.v.token; }, [&](int key) { return key < lim[b]; });
-    }
-    const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const float total = both_sum(l[b]);
-      const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-      if (row[b] >= seg.last) continue;
-      const int token = group.quotient(row[b]);
-      uint16_t* o = a.out + (token * heads + head * a.group + row[b] - token * a.group) * dim;
-#pragma unroll
-      for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const int d = 32 * t + result_row(r, h);
-          if (d < dim)
-            *reinterpret_cast<u32x2*>(o + d) = pack4(out[b][t][r] * inverse, out[b][t][r + 1] * inverse,
-                                                     out[b][t][r + 2] * inverse, out[b][t][r + 3] * inverse);
-        }
-      if (a.lse != nullptr && h == 0)
-        a.lse[static_cast<int64_t>(head) * a.tokens * a.group + row[b]] =
-            total == 0.0f ? 0.0f : m[b] * c + __builtin_amdgcn_logf(total);
-    }
-  }
-};
-
-template <class F>
-__global__ __launch_bounds__(F::kThreads, F::DP == 256 || F::RB == 2 ? 1 : F::W == 8 ? 1 : 2) void attention_kernel(AttentionArgs a, Divisor group, int tiles) {
-  extern __shared__ __align__(1024) uint8_t lds[];
-  F::run(a, group, tiles, lds);
-}
-
-// ------------------------------------------------------------ backward ---
-//
-//   P = 2^(S log2 e - lse), dP = d_out v^T, dS = P (dP - delta), delta = sum(d_out out)
-//   d_q = scale dS k,  d_k = scale dS^T q,  d_v = P^T d_out
-//
-// Two kernels, each with one side of the scores for its own and a loop over the other:
-// no sum is shared, so every gradient is added in a fixed order, for seven
-// products instead of five.
-
-// delta of each row, 16 lanes a row.
-__global__ __launch_bounds__(256) void attention_delta_kernel(AttentionArgs a, Divisor group, int64_t rows) {
-  const int64_t at = blockIdx.x * int64_t{16} + (threadIdx.x >> 4);
-  const int i = threadIdx.x & 15, heads = a.kv_heads * a.group;
-  if (at >= rows * a.kv_heads) return;
-  const int head = static_cast<int>(at / rows), row = static_cast<int>(at - head * rows);
-  const int token = group.quotient(row), query_head = head * a.group + row - token * a.group;
-  const uint16_t* o = a.out + (static_cast<int64_t>(token) * heads + query_head) * a.dim;
-  const uint16_t* d = a.d_out.p + token * a.d_out.token + query_head * a.d_out.head;
-  float sum = 0.0f;
-  for (int p = 8 * i; p < a.dim; p += 128) {
-    const u32x4 x = *reinterpret_cast<const u32x4*>(o + p), y = *reinterpret_cast<const u32x4*>(d + p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      sum = fmaf(__uint_as_float(x[e] << 16), __uint_as_float(y[e] << 16), sum);
-      sum = fmaf(__uint_as_float(x[e] & 0xFFFF0000u), __uint_as_float(y[e] & 0xFFFF0000u), sum);
-    }
-  }
-#pragma unroll
-  for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
-  if (i == 0) a.delta[at] = sum;
-}
-
-// d_q: a lane's row as in the forward pass, a tile of 64 keys at a time.
-template <int DP_, bool EXACT, int W_>
-struct QueryGradient {
-  static constexpr int DP = DP_, W = W_;
-  static constexpr int kRows = 32 * W, kThreads = 64 * W, kKeys = 64;
-  using Tile = HeadTile<DP, kKeys, W>;
-  static constexpr int kLds = 4 * Tile::kBytes;
-
-  static __device__ __forceinline__ void run(const AttentionArgs& a, const Divisor& group, int tiles, uint8_t* lds) {
-    const int dim = EXACT ? DP : a.dim;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = blockIdx.x % a.kv_heads, number = tiles - 1 - blockIdx.x / a.kv_heads;
-    const Segment seg = find_segment(a.offsets, a.sequences, a.tokens, a.group, kRows, number);
-    const int row0 = seg.first + seg.tile * kRows;
-    if (seg.tile < 0 || row0 >= seg.last) return;
-    int key0 = 0, keys = 0;
-    if (seg.number >= 0) sequence_keys(a, seg.number, key0, keys);
-    const int shift = keys - group.quotient(seg.last - seg.first);
-    const auto limit = [&](int row) {
-      if (!a.causal) return keys;
-      const int n = group.quotient(row - seg.first) + shift + 1;
-      return n < 0 ? 0 : n > keys ? keys : n;
-    };
-    const int last_row = row0 + kRows < seg.last ? row0 + kRows - 1 : seg.last - 1;
-    const int steps = (__builtin_amdgcn_readfirstlane(limit(last_row)) + kKeys - 1) / kKeys;
-
-    const int h = lane >> 5, row = row0 + 32 * wave + (lane & 31);
-    const int r = row < seg.last ? row : seg.last - 1, token = group.quotient(r), query_head = head * a.group + r - token * a.group;
-    const int lim = limit(r);
-    bf16x8 q[DP / 16], d_out[DP / 16];
-    const uint16_t* qp = a.q.p + token * a.q.token + query_head * a.q.head;
-    const uint16_t* dp = a.d_out.p + token * a.d_out.token + query_head * a.d_out.head;
-#pragma unroll
-    for (int j = 0; j < DP / 16; ++j) {
-      u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-      if (16 * j + 8 * h < dim) {
-        x = *reinterpret_cast<const u32x4*>(qp + 16 * j + 8 * h);
-        y = *reinterpret_cast<const u32x4*>(dp + 16 * j + 8 * h);
-      }
-      q[j] = __builtin_bit_cast(bf16x8, x);
-      d_out[j] = __builtin_bit_cast(bf16x8, y);
-    }
-    const int64_t stat = static_cast<int64_t>(head) * a.tokens * a.group + r;
-    float lse = a.lse[stat], delta = a.delta[stat];
-    arrived(lse);
-    arrived(delta);
-#pragma unroll
-    for (int j = 0; j < DP / 16; ++j) {
-      arrived(q[j]);
-      arrived(d_out[j]);
-    }
-    const int all_see = __builtin_amdgcn_readfirstlane(lim), some_see = __builtin_amdgcn_readlane(lim, 31);
-
-    if (dim < DP) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) Tile::clear(lds + s * Tile::kBytes, dim, kThreads);
-    }
-    const uint16_t* kp = a.k.p + key0 * a.k.token + head * a.k.head;
-    const uint16_t* vp = a.v.p + key0 * a.v.token + head * a.v.head;
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    const auto issue = [&](int step) {
-      const uint32_t at = lds_at + (step & 1) * 2 * Tile::kBytes;
-      const int64_t first = static_cast<int64_t>(step) * kKeys;
-      const int left = keys - step * kKeys;
-      Tile::load(kp + first * a.k.token, [&](int n) { return static_cast<uint32_t>(n) * static_cast<uint32_t>(2 * a.k.token); },
-                 left, dim, wave, lane, at);
-      Tile::load(vp + first * a.v.token, [&](int n) { return static_cast<uint32_t>(n) * static_cast<uint32_t>(2 * a.v.token); },
-                 left, dim, wave, lane, at + Tile::kBytes);
-    };
-
-    const float c = a.scale * kLog2e;
-    f32x16 d_q[DP / 32];
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t) d_q[t] = zero16();
-    const auto compute = [&](int step, auto masked) {
-      constexpr bool kMasked = decltype(masked)::value;
-      const uint8_t* kt = lds + (step & 1) * 2 * Tile::kBytes;
-      const uint8_t* vt = kt + Tile::kBytes;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        f32x16 s = zero16(), p = zero16();
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-          s = mfma32(Tile::along(kt, kb, j, lane), q[j], s);
-          p = mfma32(Tile::along(vt, kb, j, lane), d_out[j], p);
-        }
-        const int left = lim - step * kKeys - 32 * kb - 4 * h;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[e] = exp2_fast(fmaf(s[e], c, -lse)) * (p[e] - delta);
-          if (kMasked && result_row(e, 0) >= left) s[e] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bf16x8 ds = operand8(s, i);
-#pragma unroll
-          for (int t = 0; t < DP / 32; ++t) {
-            bf16x8 f = Tile::across(kt, 2 * kb + i, t, lane);
-            // a key that holds an infinity or NaN gives them to the dS of the rows that see it
-            uint32_t unused = 0;
-            if constexpr (kMasked) f = finite_part(f, unused);
-            d_q[t] = mfma32(f, ds, d_q[t]);
-          }
-        }
-      }
-    };
-    if (steps > 0) issue(0);
-    for (int step = 0; step < steps; ++step) {
-      loads_done();
-      if (step + 1 < steps) issue(step + 1);
-      if ((step + 1) * kKeys <= all_see)
-        compute(step, std::false_type{});
-      else if (step * kKeys < some_see)
-        compute(step, std::true_type{});
-    }
-    if (row >= seg.last) return;
-    const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
-    uint16_t* o = a.d_q + (token * heads + query_head) * dim;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int d = 32 * t + result_row(e, h);
-        if (d < dim)
-          *reinterpret_cast<u32x2*>(o + d) =
-              pack4(d_q[t][e] * a.scale, d_q[t][e + 1] * a.scale, d_q[t][e + 2] * a.scale, d_q[t][e + 3] * a.scale);
-      }
-  }
-};
-
-// d_k and d_v: a lane's key and a tile of RT rows at a time.  Scores are
-// computed with rows the result's rows, so that P and dS are the second
-// operands of d_v^T += d_out^T P and d_k^T += q^T dS as they are.
-template <int DP_, bool EXACT, int W_, int RT_, bool DK, bool DV>
-struct KeyGradient {
-  static constexpr int DP = DP_, W = W_, RT = RT_;
-  static constexpr int kKeys = 32 * W, kThreads = 64 * W;
-  using Tile = HeadTile<DP, RT, W>;
-  static constexpr int kStage = 2 * Tile::kBytes + 512;  // q, d_out, 64 values of lse and of delta
-  static constexpr int kLds = 2 * kStage;
-  static_assert(RT <= 64, "one load of lse and delta");
-
-  static __device__ __forceinline__ void run(const AttentionArgs& a, const Divisor& group, uint8_t* lds) {
-    const int dim = EXACT ? DP : a.dim;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
-    const Segment seg = find_segment(a.key_offsets != nullptr ? a.key_offsets : a.offsets, a.sequences, a.keys, 1, kKeys, number);
-    const int key0 = seg.first + seg.tile * kKeys;
-    if (seg.tile < 0 || key0 >= seg.last) return;
-    // the sequence's rows
-    int first_row = 0, last_row = 0;
-    if (seg.number >= 0) {
-      if (a.offsets == nullptr) {
-        last_row = static_cast<int>(a.tokens) * a.group;
-      } else {
-        const int most = static_cast<int>(a.tokens);
-        int lo = a.offsets[seg.number], hi = a.offsets[seg.number + 1];
-        lo = lo < 0 ? 0 : lo > most ? most : lo;
-        hi = hi < lo ? lo : hi > most ? most : hi;
-        first_row = __builtin_amdgcn_readfirstlane(lo) * a.group;
-        last_row = __builtin_amdgcn_readfirstlane(hi) * a.group;
-      }
-    }
-    const int shift = seg.last - seg.first - group.quotient(last_row - first_row);
-    // the first row that sees a key
-    const auto sees = [&](int key) {
-      const int n = a.causal ? key - seg.first - shift : 0;
-      return n <= 0 ? first_row : first_row + n * a.group;
-    };
-    const int h = lane >> 5, key = key0 + 32 * wave + (lane & 31), k = key < seg.last ? key : seg.last - 1;
-    const int from = sees(k), from_all = __builtin_amdgcn_readlane(from, 31), from_some = __builtin_amdgcn_readfirstlane(from);
-    const int start = __builtin_amdgcn_readfirstlane(sees(key0));
-    const int steps = start < last_row ? (last_row - start + RT - 1) / RT : 0;
-
-    bf16x8 kf[DP / 16], vf[DP / 16];
-    const uint16_t* kp = a.k.p + k * a.k.token + head * a.k.head;
-    const uint16_t* vp = a.v.p + k * a.v.token + head * a.v.head;
-#pragma unroll
-    for (int j = 0; j < DP / 16; ++j) {
-      u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-      if (16 * j + 8 * h < dim) {
-        x = *reinterpret_cast<const u32x4*>(kp + 16 * j + 8 * h);
-        if (DK) y = *reinterpret_cast<const u32x4*>(vp + 16 * j + 8 * h);
-      }
-      kf[j] = __builtin_bit_cast(bf16x8, x);
-      vf[j] = __builtin_bit_cast(bf16x8, y);
-    }
-#pragma unroll
-    for (int j = 0; j < DP / 16; ++j) {
-      arrived(kf[j]);
-      if (DK) arrived(vf[j]);
-    }
-    if (dim < DP) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) Tile::clear(lds + (s >> 1) * kStage + (s & 1) * Tile::kBytes, dim, kThreads);
-    }
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    const float* lse = a.lse + static_cast<int64_t>(head) * a.tokens * a.group;
-    const float* delta = a.delta + static_cast<int64_t>(head) * a.tokens * a.group;
-    const auto issue = [&](int step) {
-      const uint32_t at = lds_at + (step & 1) * kStage;
-      const int row0 = start + step * RT, left = last_row - row0;
-      const int token0 = group.quotient(row0);
-      const auto rows = [&](const Rows16& x) {
-        return [&](int n) {
-          const int token = group.quotient(row0 + n), g = row0 + n - token * a.group;
-          return static_cast<uint32_t>(token - token0) * static_cast<uint32_t>(2 * x.token) + static_cast<uint32_t>(g) * static_cast<uint32_t>(2 * x.head);
-        };
-      };
-      const int64_t q_at = token0 * a.q.token + head * a.group * a.q.head;
-      const int64_t d_at = token0 * a.d_out.token + head * a.group * a.d_out.head;
-      Tile::load(a.q.p + q_at, rows(a.q), left, dim, wave, lane, at);
-      Tile::load(a.d_out.p + d_at, rows(a.d_out), left, dim, wave, lane, at + Tile::kBytes);
-      if (wave == 0) {
-        const uint32_t off = 4 * (lane < left ? lane : left - 1);
-        load_to_lds<4>(lse + row0, off, at + 2 * Tile::kBytes);
-        load_to_lds<4>(delta + row0, off, at + 2 * Tile::kBytes + 256);
-      }
-    };
-
-    const float c = a.scale * kLog2e;
-    f32x16 d_k[DP / 32], d_v[DP / 32];
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t) d_k[t] = d_v[t] = zero16();
-    uint32_t dirty = 0;
-    const auto compute = [&](int step, auto masked) {
-      constexpr bool kMasked = decltype(masked)::value;
-      const uint8_t* qt = lds + (step & 1) * kStage;
-      const uint8_t* ot = qt + Tile::kBytes;
-      const float* stats = reinterpret_cast<const float*>(qt + 2 * Tile::kBytes);
-#pragma unroll
-      for (int b = 0; b < RT / 32; ++b) {
-        f32x16 s = zero16(), p = zero16();
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-          s = mfma32(Tile::along(qt, b, j, lane), kf[j], s);
-          if (DK) p = mfma32(Tile::along(ot, b, j, lane), vf[j], p);
-        }
-        const int base = start + step * RT + 32 * b + 4 * h;
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const f32x4 l = *reinterpret_cast<const f32x4*>(stats + 32 * b + result_row(e, h));
-          const f32x4 d = *reinterpret_cast<const f32x4*>(stats + 64 + 32 * b + result_row(e, h));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float w = exp2_fast(fmaf(s[e + i], c, -l[i]));
-            s[e + i] = w;
-            p[e + i] = w * (p[e + i] - d[i]);
-            if constexpr (kMasked) {
-              const int row = base + result_row(e + i, 0);
-              if (row < from || row >= last_row) s[e + i] = p[e + i] = 0.0f;
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bf16x8 w = operand8(s, i), ds = operand8(p, i);
-#pragma unroll
-          for (int t = 0; t < DP / 32; ++t) {
-            if constexpr (DV) {
-              bf16x8 f = Tile::across(ot, 2 * b + i, t, lane);
-              if constexpr (kMasked) f = finite_part(f, dirty);
-              d_v[t] = mfma32(f, w, d_v[t]);
-            }
-            if constexpr (DK) {
-              bf16x8 f = Tile::across(qt, 2 * b + i, t, lane);
-              // a query that holds an infinity or NaN gives them to the dS of the keys it sees
-              uint32_t unused = 0;
-              if constexpr (kMasked) f = finite_part(f, unused);
-              d_k[t] = mfma32(f, ds, d_k[t]);
-            }
-          }
-        }
-      }
-    };
-    if (steps > 0) issue(0);
-    for (int step = 0; step < steps; ++step) {
-      loads_done();
-      if (step + 1 < steps) issue(step + 1);
-      const int row0 = start + step * RT;
-      if (row0 >= from_all && row0 + RT <= last_row)
-        compute(step, std::false_type{});
-      else if (row0 + RT > from_some)
-        compute(step, std::true_type{});
-    }
-    if (DV && __any(dirty != 0)) {
-      const auto at = [&](int row) {
-        const int token = group.quotient(row);
-        return a.d_out.p + token * a.d_out.token + (head * a.group + row - token * a.group) * a.d_out.head;
-      };
-      const auto seen = [&](int row) { return row >= from; };
-      const int cut = from_all + RT < last_row ? from_all + RT : last_row, tail = last_row - RT > cut ? last_row - RT : cut;
-      add_nonfinite<DP>(d_v, from_some, cut, dim, h, at, seen);
-      add_nonfinite<DP>(d_v, tail, last_row, dim, h, at, seen);
-    }
-    if (key >= seg.last) return;
-    const int64_t o = (static_cast<int64_t>(key) * a.kv_heads + head) * dim;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int d = 32 * t + result_row(e, h);
-        if (d >= dim) continue;
-        if (DK)
-          *reinterpret_cast<u32x2*>(a.d_k + o + d) =
-              pack4(d_k[t][e] * a.scale, d_k[t][e + 1] * a.scale, d_k[t][e + 2] * a.scale, d_k[t][e + 3] * a.scale);
-        if (DV) *reinterpret_cast<u32x2*>(a.d_v + o + d) = pack4(d_v[t][e], d_v[t][e + 1], d_v[t][e + 2], d_v[t][e + 3]);
-      }
-  }
-};
-
-template <class F>
-__global__ __launch_bounds__(F::kThreads, F::DP == 256 ? 1 : 2) void query_gradient_kernel(AttentionArgs a, Divisor group, int tiles) {
-  extern __shared__ __align__(1024) uint8_t lds[];
-  F::run(a, group, tiles, lds);
-}
-template <class F>
-__global__ __launch_bounds__(F::kThreads, F::DP == 64 ? 2 : 1) void key_gradient_kernel(AttentionArgs a, Divisor group) {
-  extern __shared__ __align__(1024) uint8_t lds[];
-  F::run(a, group, lds);
-}
-
-template <class F>
-hipError_t launch_query_gradient(const AttentionArgs& a, hipStream_t st) {
-  if (a.d_q == nullptr || a.tokens == 0) return hipSuccess;
-  const int64_t tiles = tile_numbers(a.tokens * a.group, a.offsets != nullptr, a.sequences, F::kRows);
-  query_gradient_kernel<F><<<static_cast<uint32_t>(tiles * a.kv_heads), F::kThreads, F::kLds, st>>>(a, Divisor(a.group), static_cast<int>(tiles));
-  return hipGetLastError();
-}
-template <class F>
-hipError_t launch_key_gradient(const AttentionArgs& a, hipStream_t st) {
-  if (a.keys == 0) return hipSuccess;
-  const int64_t tiles = tile_numbers(a.keys, a.offsets != nullptr, a.sequences, F::kKeys);
-  key_gradient_kernel<F><<<static_cast<uint32_t>(tiles * a.kv_heads), F::kThreads, F::kLds, st>>>(a, Divisor(a.group));
-  return hipGetLastError();
-}
-
-template <int DP, bool EXACT, int RT>
-hipError_t backward(const AttentionArgs& a, hipStream_t st) {
-  if (hipError_t e = launch_query_gradient<QueryGradient<DP, EXACT, 4>>(a, st); e != hipSuccess) return e;
-  // both gradients of 256 columns at once would not leave a lane registers for the scores
-  if (DP < 256 && a.d_k != nullptr && a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, 4, RT, DP < 256, true>>(a, st);
-  if (a.d_k != nullptr)
-    if (hipError_t e = launch_key_gradient<KeyGradient<DP, EXACT, 4, RT, true, false>>(a, st); e != hipSuccess) return e;
-  if (a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, 4, RT, false, true>>(a, st);
-  return hipSuccess;
-}
-
-template <class F>
-hipError_t launch_forward(const AttentionArgs& a, hipStream_t st) {
-  const int64_t tiles = tile_numbers(a.tokens * a.group, a.offsets != nullptr, a.sequences, F::kRows);
-  attention_kernel<F><<<static_cast<uint32_t>(tiles * a.kv_heads), F::kThreads, F::kLds, st>>>(a, Divisor(a.group), static_cast<int>(tiles));
-  return hipGetLastError();
-}
-
-template <bool EXACT>
-hipError_t forward(const AttentionArgs& a, hipStream_t st) {
-  if (a.dim <= 64) return launch_forward<Forward<64, EXACT, ATT_RB, ATT_W>>(a, st);
-  if (a.dim <= 128) return launch_forward<Forward<128, EXACT, ATT_RB, ATT_W>>(a, st);
-  return launch_forward<Forward<256, EXACT, 1, 4>>(a, st);
-}
-
-template <bool EXACT>
-hipError_t gradients(const AttentionArgs& a, hipStream_t st) {
-  if (a.dim <= 64) return backward<64, EXACT, 64>(a, st);
-  if (a.dim <= 128) return backward<128, EXACT, 64>(a, st);
-  return backward<256, EXACT, 32>(a, st);
-}
-
-// Head widths without padding, whose loads need no test.
-bool exact_width(int dim) { return dim == 64 || dim == 128 || dim == 256; }
-
-}  // namespace
 
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t st) {
-  return exact_width(a.dim) ? forward<true>(a, st) : forward<false>(a, st);
+  if (a.dim > 128) return launch_attention_wide(a, st);
+  if (a.dim == 128) return launch_forward<Forward<128, true, ATT_RB, ATT_W>>(a, st);
+  if (a.dim == 64) return launch_forward<Forward<64, true, ATT_RB, ATT_W>>(a, st);
+  if (a.dim > 64) return launch_forward<Forward<128, false, ATT_RB, ATT_W>>(a, st);
+  return launch_forward<Forward<64, false, ATT_RB, ATT_W>>(a, st);
 }
 
 hipError_t launch_attention_backward(const AttentionArgs& a, hipStream_t st) {
-  if (a.tokens > 0) {
-    const int64_t rows = a.tokens * a.group;
-    attention_delta_kernel<<<static_cast<uint32_t>((rows * a.kv_heads + 15) / 16), 256, 0, st>>>(a, Divisor(a.group), rows);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  }
-  return exact_width(a.dim) ? gradients<true>(a, st) : gradients<false>(a, st);
+  if (a.dim > 128) return launch_attention_backward_wide(a, st);
+  if (a.dim == 128) return backward<128, true, 64>(a, st);
+  if (a.dim == 64) return backward<64, true, 64>(a, st);
+  if (a.dim > 64) return backward<128, false, 64>(a, st);
+  return backward<64, false, 64>(a, st);
 }
 
 }  // namespace glm53

@@ -48,18 +48,30 @@ __device__ __forceinline__ float both_sum(float v) {
   return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
-// Eight results as an operand, rounded to nearest even.
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+// Eight results as an operand, rounded to nearest even, and what that leaves of them.
 __device__ __forceinline__ bf16x8 operand8(const f32x16& v, int i) {
-  bf16x8 o;
+  u32x4 o;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = static_cast<__bf16>(v[8 * i + e]);
-  return o;
+  for (int e = 0; e < 4; ++e) o[e] = pack2(v[8 * i + 2 * e], v[8 * i + 2 * e + 1]);
+  return __builtin_bit_cast(bf16x8, o);
+}
+__device__ __forceinline__ bf16x8 low_operand8(const f32x16& v, int i, bf16x8 high) {
+  const u32x4 w = __builtin_bit_cast(u32x4, high);
+  u32x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    o[e] = pack2(v[8 * i + 2 * e] - __uint_as_float(w[e] << 16), v[8 * i + 2 * e + 1] - __uint_as_float(w[e] & 0xFFFF0000u));
+  return __builtin_bit_cast(bf16x8, o);
 }
 
 __device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) {
-  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-  const bf16x4 v = {static_cast<__bf16>(a), static_cast<__bf16>(b), static_cast<__bf16>(c), static_cast<__bf16>(d)};
-  return __builtin_bit_cast(u32x2, v);
+  return (u32x2){pack2(a, b), pack2(c, d)};
 }
 
 __device__ __forceinline__ const void* uniform_address(const void* p) {
@@ -123,6 +135,25 @@ struct HeadTile {
       const int piece = (lane % kSlots) ^ swizzle(row);
       const uint32_t off = offset(row < left ? row : left - 1) + 16 * piece;
       if (8 * piece < dim) load_to_lds(base, off, lds + first * kPitch);
+    }
+  }
+
+  // The same of rows `pitch` bytes apart.  Whole tiles go by one offset a lane:
+  // its rows are a multiple of 16 apart, which have one swizzle, so the rest is uniform.
+  __device__ static __forceinline__ void load(const uint16_t* base, uint32_t pitch, int left, int dim, int wave, int lane,
+                                              uint32_t lds) {
+    constexpr int kApart = W * kLoadRows;
+    if (kApart % 16 != 0 || left < ROWS) {
+      load(base, [&](int row) { return static_cast<uint32_t>(row) * pitch; }, left, dim, wave, lane, lds);
+      return;
+    }
+    const int row = wave * kLoadRows + lane / kSlots, piece = (lane % kSlots) ^ swizzle(row);
+    const uint32_t off = static_cast<uint32_t>(row) * pitch + 16 * piece;
+    const uint8_t* at = reinterpret_cast<const uint8_t*>(base);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if (8 * piece < dim) load_to_lds(at, off, lds + (wave + W * i) * kLoadRows * kPitch);
+      at += static_cast<uint64_t>(kApart) * pitch;
     }
   }
 

@@ -1,0 +1,17 @@
+// Attention over heads of more than 128 values: a translation unit of its own, as its
+// kernels need accumulation registers, which the other ones are compiled without.
+#include "attention_kernels.h"
+
+namespace glm53 {
+
+hipError_t launch_attention_wide(const AttentionArgs& a, hipStream_t st) {
+  if (a.dim == 256) return launch_forward<Forward<256, true, 1, 4>>(a, st);
+  return launch_forward<Forward<256, false, 1, 4>>(a, st);
+}
+
+hipError_t launch_attention_backward_wide(const AttentionArgs& a, hipStream_t st) {
+  if (a.dim == 256) return backward<256, true, 32>(a, st);
+  return backward<256, false, 32>(a, st);
+}
+
+}  // namespace glm53
