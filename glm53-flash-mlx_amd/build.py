@@ -38,7 +38,7 @@ COMMON = [
 # Per-source additions.  The matrix kernels: MFMA results in ordinary VGPRs (the
 # compiler otherwise parks the chained hi/lo results of the narrow GEMM in
 # accumulation registers and copies every element out before folding it).
-EXTRA = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("grouped.hip", "dense.hip", "gemm16.hip", "gated.hip", "int4.hip", "attention.hip")}
+EXTRA = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("grouped.hip", "dense.hip", "gemm16.hip", "gated.hip", "int4.hip")}
 
 
 def _compile(src: str) -> Path:

@@ -82,7 +82,7 @@ int attention_args(const glm53_attention* d, bool backward, AttentionArgs& a) {
   const size_t need = glm53_packed_attention_backward_workspace_bytes(d->tokens, d->heads);
   CHECK_ARG(need == 0 || (d->workspace && d->workspace_bytes >= need && aligned(d->workspace, 256)),
             "attention's gradients need a 256-byte aligned workspace of %zu bytes", need);
-  a.delta = static_cast<float*>(d->workspace);
+  a.starts = static_cast<float*>(d->workspace);
   return GLM53_OK;
 }
 
@@ -135,7 +135,7 @@ int glm53_packed_attention(const glm53_attention* attention, void* stream) {
 
 size_t glm53_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t heads) {
   if (tokens <= 0 || heads <= 0 || tokens >= kMaxRows / heads) return 0;
-  return round_up(sizeof(float) * static_cast<size_t>(tokens * heads));
+  return round_up(2 * sizeof(float) * static_cast<size_t>(tokens * heads));
 }
 
 int glm53_packed_attention_backward(const glm53_attention* attention, void* stream) {

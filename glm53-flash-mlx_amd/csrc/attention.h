@@ -35,7 +35,7 @@ struct AttentionArgs {
   // backward
   Rows16 d_out;
   uint16_t *d_q, *d_k, *d_v;   // contiguous; null: not wanted
-  float* delta;                // [kv_heads, tokens * group]
+  float* starts;               // [2, kv_heads, tokens * group]: -lse / (scale log2 e), -delta
 };
 
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t st);

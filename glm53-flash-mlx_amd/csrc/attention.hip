@@ -18,10 +18,10 @@ hipError_t launch_attention(const AttentionArgs& a, hipStream_t st) {
 
 hipError_t launch_attention_backward(const AttentionArgs& a, hipStream_t st) {
   if (a.dim > 128) return launch_attention_backward_wide(a, st);
-  if (a.dim == 128) return backward<128, true, 64>(a, st);
-  if (a.dim == 64) return backward<64, true, 64>(a, st);
-  if (a.dim > 64) return backward<128, false, 64>(a, st);
-  return backward<64, false, 64>(a, st);
+  if (a.dim == 128) return backward<128, true, 2>(a, st);
+  if (a.dim == 64) return backward<64, true, 2>(a, st);
+  if (a.dim > 64) return backward<128, false, 2>(a, st);
+  return backward<64, false, 2>(a, st);
 }
 
 }  // namespace glm53

@@ -16,6 +16,27 @@ namespace glm53 {
 
 namespace {
 
+#ifndef QAHEAD
+#define QAHEAD 1
+#endif
+#ifndef KAHEAD64
+#define KAHEAD64 2
+#endif
+// Keeps what is in front of it in front and what is behind it behind, when the
+// compiler orders instructions: left alone it puts each LDS read directly
+// before the product that waits for it.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// Around a run of products: its wavefront goes first on its SIMD, so that the
+// other one there comes to its weights while this one multiplies (16,384 causal
+// tokens, 8 heads of 128: 505 us, without 560).
+__device__ __forceinline__ void products(bool begin) {
+  if (begin)
+    __builtin_amdgcn_s_setprio(1);
+  else
+    __builtin_amdgcn_s_setprio(0);
+}
+
 constexpr float kLog2e = 1.44269504088896340736f;
 // A row's maximum is kept until a new one is this many powers of two above it:
 // the weights 2^(s - m) then reach 2^8, which changes no relative rounding, and
@@ -24,14 +45,17 @@ constexpr float kSlack = 8.0f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Keys of sequence `number`: first and how many.
-__device__ __forceinline__ void sequence_keys(const AttentionArgs& a, int number, int& first, int& count) {
-  const int32_t* offsets = a.key_offsets != nullptr ? a.key_offsets : a.offsets;
-  if (offsets == nullptr) {
-    first = 0;
-    count = static_cast<int>(a.keys);
+// Keys of the sequence that `seg` is of: first and how many.
+__device__ __forceinline__ void sequence_keys(const AttentionArgs& a, const Divisor& group, const Segment& seg, int& first, int& count) {
+  first = count = 0;
+  if (seg.number < 0) return;
+  if (a.key_offsets == nullptr) {  // the queries' own
+    first = group.quotient(seg.first);
+    count = group.quotient(seg.last - seg.first);
     return;
   }
+  const int32_t* offsets = a.key_offsets;
+  const int number = seg.number;
   const int most = static_cast<int>(a.keys);
   int lo = offsets[number], hi = offsets[number + 1];
   lo = lo < 0 ? 0 : lo > most ? most : lo;
@@ -56,7 +80,7 @@ int64_t tile_numbers(int64_t rows, bool packed, int sequences, int size) {
 template <int DP_, bool EXACT, int RB_, int W_>
 struct Forward {
   static constexpr int DP = DP_, RB = RB_, W = W_;
-  static constexpr int kRows = 32 * RB * W, kThreads = 64 * W, kKeys = 64;
+  static constexpr int kRows = 32 * RB * W, kThreads = 64 * W, kKeys = 64, T = DP / 32;
   using Tile = HeadTile<DP, kKeys, W>;
   static constexpr int kLds = 4 * Tile::kBytes;  // two stages of keys and values
 
@@ -68,8 +92,8 @@ struct Forward {
     const int row0 = seg.first + seg.tile * kRows;
     if (seg.tile < 0 || row0 >= seg.last) return;
 
-    int key0 = 0, keys = 0;
-    if (seg.number >= 0) sequence_keys(a, seg.number, key0, keys);
+    int key0, keys;
+    sequence_keys(a, group, seg, key0, keys);
     // keys that the query of row r sees: a prefix
     const int shift = keys - group.quotient(seg.last - seg.first);
     const auto limit = [&](int row) {
@@ -81,6 +105,22 @@ struct Forward {
     const int steps = (__builtin_amdgcn_readfirstlane(limit(last_row)) + kKeys - 1) / kKeys;
 
     const int h = lane >> 5;
+    if (dim < DP) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) Tile::clear(lds + s * Tile::kBytes, dim, kThreads);
+    }
+    const uint16_t* kp = a.k.p + static_cast<int64_t>(key0) * a.k.token + static_cast<int64_t>(head) * a.k.head;
+    const uint16_t* vp = a.v.p + static_cast<int64_t>(key0) * a.v.token + static_cast<int64_t>(head) * a.v.head;
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    const auto issue = [&](int step) {
+      const uint32_t at = lds_at + (step & 1) * 2 * Tile::kBytes;
+      const int64_t first = static_cast<int64_t>(step) * kKeys;
+      const int left = keys - step * kKeys;
+      Tile::load(kp + first * a.k.token, static_cast<uint32_t>(2 * a.k.token), left, dim, wave, lane, at);
+      Tile::load(vp + first * a.v.token, static_cast<uint32_t>(2 * a.v.token), left, dim, wave, lane, at + Tile::kBytes);
+    };
+
+    if (steps > 0) issue(0);
     int row[RB], lim[RB];
     bf16x8 q[RB][DP / 16];
 #pragma unroll
@@ -104,21 +144,7 @@ struct Forward {
     const int all_see = __builtin_amdgcn_readfirstlane(lim[0]);                  // every row of the wavefront
     const int some_see = __builtin_amdgcn_readlane(lim[RB - 1], 31);             // its last row
 
-    if (dim < DP) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) Tile::clear(lds + s * Tile::kBytes, dim, kThreads);
-    }
-    const uint16_t* kp = a.k.p + static_cast<int64_t>(key0) * a.k.token + static_cast<int64_t>(head) * a.k.head;
-    const uint16_t* vp = a.v.p + static_cast<int64_t>(key0) * a.v.token + static_cast<int64_t>(head) * a.v.head;
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    const auto issue = [&](int step) {
-      const uint32_t at = lds_at + (step & 1) * 2 * Tile::kBytes;
-      const int64_t first = static_cast<int64_t>(step) * kKeys;
-      const int left = keys - step * kKeys;
-      Tile::load(kp + first * a.k.token, static_cast<uint32_t>(2 * a.k.token), left, dim, wave, lane, at);
-      Tile::load(vp + first * a.v.token, static_cast<uint32_t>(2 * a.v.token), left, dim, wave, lane, at + Tile::kBytes);
-    };
-
+    const typename Tile::Places at(lds_at, lane);
     const float c = a.scale * kLog2e;
     f32x16 out[RB][DP / 32];
     float m[RB], l[RB];  // m in units of scores; l: this lane's part
@@ -133,20 +159,37 @@ struct Forward {
     uint32_t dirty = 0;
     const auto compute = [&](int step, auto stage, auto masked) {
       constexpr bool kMasked = decltype(masked)::value;
-      const uint8_t* kt = lds + stage * 2 * Tile::kBytes;
-      const uint8_t* vt = kt + Tile::kBytes;
+      const int kt = stage * 2 * Tile::kBytes, vt = kt + Tile::kBytes;
       f32x16 s[RB][2];
+      // groups of operands: the keys' in kb and 64 columns, the values' in 16 keys
+      constexpr int kGroups = DP / 64, kMost = T > 4 ? T : 4;
+      bf16x8 f[3][kMost];
+      const auto read = [&](int n) {
+        bf16x8 (&x)[kMost] = f[n % 3];
+        if (n < 2 * kGroups) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+          for (int j = 0; j < 4; ++j) x[j] = at.along(kt, n / kGroups, 4 * (n % kGroups) + j);
+        } else if (n < 2 * kGroups + 4) {
 #pragma unroll
-        for (int b = 0; b < RB; ++b) s[b][kb] = zero16();
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-          const bf16x8 f = Tile::along(kt, kb, j, lane);
-#pragma unroll
-          for (int b = 0; b < RB; ++b) s[b][kb] = mfma32(f, q[b][j], s[b][kb]);
+          for (int t = 0; t < T; ++t) x[t] = at.across(vt, n - 2 * kGroups, t);
         }
+      };
+      read(0);
+      read(1);
+      products(true);
+#pragma unroll
+      for (int n = 0; n < 2 * kGroups; ++n) {
+        fence();
+        read(n + 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+            s[b][n / kGroups] = mfma32(f[n % 3][j], q[b][4 * (n % kGroups) + j], n % kGroups + j == 0 ? zero16() : s[b][n / kGroups]);
       }
+      fence();
+      products(false);
+      float mc[RB];
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
         if constexpr (kMasked) {
@@ -169,37 +212,47 @@ struct Forward {
           m[b] = next;
           l[b] *= alpha;
 #pragma unroll
-          for (int t = 0; t < DP / 32; ++t)
+          for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) out[b][t][r] *= alpha;
         }
-        const float mc = m[b] == -INFINITY ? 0.0f : m[b] * c;
-        float sum = 0.0f;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            s[b][kb][r] = exp2_fast(fmaf(s[b][kb][r], c, -mc));
-            sum += s[b][kb][r];
-          }
-        l[b] += sum;
+        mc[b] = m[b] == -INFINITY ? 0.0f : m[b] * c;
       }
+      bf16x8 p[RB], next[RB];
+      const auto weigh = [&](int i) {  // 8 of a lane's scores
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            s[b][i >> 1][8 * (i & 1) + e] = exp2_fast(fmaf(s[b][i >> 1][8 * (i & 1) + e], c, -mc[b]));
+          float sum = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum += s[b][i >> 1][8 * (i & 1) + e];
+          l[b] += sum;
+          next[b] = operand8(s[b][i >> 1], i & 1);
+        }
+      };
+      weigh(0);
+      products(true);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        bf16x8 p[RB];
+        fence();
+        const int n = 2 * kGroups + i;
+        read(n + 2);
 #pragma unroll
-        for (int b = 0; b < RB; ++b) p[b] = operand8(s[b][i >> 1], i & 1);
+        for (int b = 0; b < RB; ++b) p[b] = next[b];
 #pragma unroll
-        for (int t = 0; t < DP / 32; ++t) {
-          bf16x8 f = Tile::across(vt, i, t, lane);
-          if constexpr (kMasked) f = finite_part(f, dirty);
+        for (int t = 0; t < T; ++t) {
+          if constexpr (kMasked) f[n % 3][t] = finite_part(f[n % 3][t], dirty);
 #pragma unroll
-          for (int b = 0; b < RB; ++b) out[b][t] = mfma32(f, p[b], out[b][t]);
+          for (int b = 0; b < RB; ++b) out[b][t] = mfma32(f[n % 3][t], p[b], out[b][t]);
         }
+        if (i < 3) weigh(i + 1);
       }
+      fence();
+      products(false);
     };
 
-    if (steps > 0) issue(0);
     // whole tiles two at a time: their places in LDS are constants then
     const int whole = all_see / kKeys & ~1;
     int step = 0;
@@ -220,7 +273,7 @@ struct Forward {
     if (__any(dirty != 0)) {
 #pragma unroll
       for (int b = 0; b < RB; ++b)
-        add_nonfinite<DP>(out[b], all_see / kKeys * kKeys, some_see, dim, h,
+        add_nonfinite<DP>(out[b], whole * kKeys, some_see, dim, h,
                           [&](int key) { return vp + key * a.v.token; }, [&](int key) { return key < lim[b]; });
     }
     const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
@@ -272,7 +325,7 @@ __global__ __launch_bounds__(F::kThreads, F::DP == 256 || F::RB == 2 ? 1 : F::W 
 template <int DP_, bool EXACT, int W_, bool DQ>
 struct QueryGradient {
   static constexpr int DP = DP_, W = W_;
-  static constexpr int kRows = 32 * W, kThreads = 64 * W, kKeys = 64;
+  static constexpr int kRows = 32 * W, kThreads = 64 * W, kKeys = 64, T = DP / 32;
   using Tile = HeadTile<DP, kKeys, W>;
   static constexpr int kLds = 4 * Tile::kBytes;
 
@@ -283,8 +336,8 @@ struct QueryGradient {
     const Segment seg = find_segment(a.offsets, a.sequences, a.tokens, a.group, kRows, number);
     const int row0 = seg.first + seg.tile * kRows;
     if (seg.tile < 0 || row0 >= seg.last) return;
-    int key0 = 0, keys = 0;
-    if (seg.number >= 0) sequence_keys(a, seg.number, key0, keys);
+    int key0, keys;
+    sequence_keys(a, group, seg, key0, keys);
     const int shift = keys - group.quotient(seg.last - seg.first);
     const auto limit = [&](int row) {
       if (!a.causal) return keys;
@@ -297,6 +350,22 @@ struct QueryGradient {
     const int h = lane >> 5, row = row0 + 32 * wave + (lane & 31);
     const int r = row < seg.last ? row : seg.last - 1, token = group.quotient(r), query_head = head * a.group + r - token * a.group;
     const int lim = limit(r);
+    if (dim < DP) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) Tile::clear(lds + s * Tile::kBytes, dim, kThreads);
+    }
+    const uint16_t* kp = a.k.p + key0 * a.k.token + head * a.k.head;
+    const uint16_t* vp = a.v.p + key0 * a.v.token + head * a.v.head;
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    const auto issue = [&](int step) {
+      const uint32_t at = lds_at + (step & 1) * 2 * Tile::kBytes;
+      const int64_t first = static_cast<int64_t>(step) * kKeys;
+      const int left = keys - step * kKeys;
+      Tile::load(kp + first * a.k.token, static_cast<uint32_t>(2 * a.k.token), left, dim, wave, lane, at);
+      Tile::load(vp + first * a.v.token, static_cast<uint32_t>(2 * a.v.token), left, dim, wave, lane, at + Tile::kBytes);
+    };
+
+    if (steps > 0) issue(0);
     bf16x8 q[DP / 16], d_out[DP / 16];
     const uint16_t* qp = a.q.p + token * a.q.token + query_head * a.q.head;
     const uint16_t* dp = a.d_out.p + token * a.d_out.token + query_head * a.d_out.head;
@@ -329,21 +398,7 @@ struct QueryGradient {
     }
     const int all_see = __builtin_amdgcn_readfirstlane(lim), some_see = __builtin_amdgcn_readlane(lim, 31);
 
-    if (dim < DP) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) Tile::clear(lds + s * Tile::kBytes, dim, kThreads);
-    }
-    const uint16_t* kp = a.k.p + key0 * a.k.token + head * a.k.head;
-    const uint16_t* vp = a.v.p + key0 * a.v.token + head * a.v.head;
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    const auto issue = [&](int step) {
-      const uint32_t at = lds_at + (step & 1) * 2 * Tile::kBytes;
-      const int64_t first = static_cast<int64_t>(step) * kKeys;
-      const int left = keys - step * kKeys;
-      Tile::load(kp + first * a.k.token, static_cast<uint32_t>(2 * a.k.token), left, dim, wave, lane, at);
-      Tile::load(vp + first * a.v.token, static_cast<uint32_t>(2 * a.v.token), left, dim, wave, lane, at + Tile::kBytes);
-    };
-
+    const typename Tile::Places at(lds_at, lane);
     const float c = a.scale * kLog2e;
     float sum = 0.0f;  // of dS
     f32x16 d_q[DP / 32];
@@ -351,40 +406,74 @@ struct QueryGradient {
     for (int t = 0; t < DP / 32; ++t) d_q[t] = zero16();
     const auto compute = [&](int step, auto stage, auto masked) {
       constexpr bool kMasked = decltype(masked)::value;
-      const uint8_t* kt = lds + stage * 2 * Tile::kBytes;
-      const uint8_t* vt = kt + Tile::kBytes;
+      const int kt = stage * 2 * Tile::kBytes, vt = kt + Tile::kBytes;
+      // groups of operands, read ahead of the products that take them: of 32 keys
+      // those of 32 columns of scores at a time, then those of 16 keys
+      constexpr int kGroups = DP / 32, kAhead = QAHEAD, kPart = kGroups + (DQ ? 2 : 0), kAll = 2 * kPart, kMost = T > 4 ? T : 4;
+      bf16x8 f[kAhead + 1][kMost];
+      const auto read = [&](int n) {
+        if (n >= kAll) return;
+        bf16x8 (&x)[kMost] = f[n % (kAhead + 1)];
+        const int kb = n / kPart, g = n % kPart;
+        if (g < kGroups) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        f32x16 s = zero16(), p = zero16();
+          for (int j = 0; j < 2; ++j) {
+            x[2 * j] = at.along(kt, kb, 2 * g + j);
+            x[2 * j + 1] = at.along(vt, kb, 2 * g + j);
+          }
+        } else {
 #pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-          s = mfma32(Tile::along(kt, kb, j, lane), q[j], s);
-          p = mfma32(Tile::along(vt, kb, j, lane), d_out[j], p);
+          for (int t = 0; t < T; ++t) x[t] = at.across(kt, 2 * kb + g - kGroups, t);
         }
-        const int left = lim - step * kKeys - 32 * kb - 4 * h;
+      };
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          s[e] = exp2_fast(fmaf(s[e], c, -lse)) * (p[e] - delta);
-          if (kMasked && result_row(e, 0) >= left) s[e] = 0.0f;
-          sum += s[e];
+      for (int n = 0; n < kAhead; ++n) read(n);
+      f32x16 s, p;
+      products(true);
+#pragma unroll
+      for (int n = 0; n < kAll; ++n) {
+        const int kb = n / kPart, g = n % kPart;
+        fence();
+        read(n + kAhead);
+        bf16x8 (&x)[kMost] = f[n % (kAhead + 1)];
+        if (g == 0) {
+          s = zero16();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) p[e] = -delta;
         }
-        if constexpr (!DQ) continue;
+        if (g < kGroups) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bf16x8 ds = operand8(s, i), low = low_operand8(s, i, ds);
+          for (int j = 0; j < 2; ++j) {
+            s = mfma32(x[2 * j], q[2 * g + j], s);
+            p = mfma32(x[2 * j + 1], d_out[2 * g + j], p);
+          }
+        } else {
+          const bf16x8 ds = operand8(s, g - kGroups), low = low_operand8(s, g - kGroups, ds);
 #pragma unroll
-          for (int t = 0; t < DP / 32; ++t) {
-            bf16x8 f = Tile::across(kt, 2 * kb + i, t, lane);
+          for (int t = 0; t < T; ++t) {
             // a key that holds an infinity or NaN gives them to the dS of the rows that see it
             uint32_t unused = 0;
-            if constexpr (kMasked) f = finite_part(f, unused);
-            d_q[t] = mfma32(f, ds, d_q[t]);
-            d_q[t] = mfma32(f, low, d_q[t]);
+            if constexpr (kMasked) x[t] = finite_part(x[t], unused);
+            d_q[t] = mfma32(x[t], ds, d_q[t]);
+            d_q[t] = mfma32(x[t], low, d_q[t]);
           }
         }
+        if (g == kGroups - 1) {
+          fence();
+          products(false);
+          const int left = lim - step * kKeys - 32 * kb - 4 * h;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[e] = exp2_fast(fmaf(s[e], c, -lse)) * p[e];
+            if (kMasked && result_row(e, 0) >= left) s[e] = 0.0f;
+            sum += s[e];
+          }
+          products(true);
+        }
       }
+      fence();
+      products(false);
     };
-    if (steps > 0) issue(0);
     // whole tiles two at a time: their places in LDS are constants then
     const int whole = all_see / kKeys & ~1;
     int step = 0;
@@ -403,7 +492,10 @@ struct QueryGradient {
     }
     sum = both_sum(sum);
     if (row >= seg.last) return;
-    if (h == 0) a.delta[stat] = delta + sum;
+    if (h == 0) {  // where the second kernel's products start
+      a.starts[stat] = -lse / c;
+      a.starts[stat + heads * a.tokens] = -(delta + sum);
+    }
     if (!DQ) return;
     uint16_t* o = a.d_q + own;
 #pragma unroll
@@ -418,21 +510,28 @@ struct QueryGradient {
   }
 };
 
-// d_k and d_v: a lane's key and a tile of RT rows at a time.  Scores are
-// computed with rows the result's rows, so that P and dS are the second
-// operands of d_v^T += d_out^T P and d_k^T += q^T dS as they are.
-template <int DP_, bool EXACT, int W_, int RT_, bool DK, bool DV>
+// d_k and d_v: a lane's key and a tile of rows at a time.  Scores are computed
+// with rows the result's rows, so that P and dS are the second operands of
+// d_v^T += d_out^T P and d_k^T += q^T dS as they are.  Of the four wavefronts two
+// and two share 32 keys, each with half of a tile's rows, and add up at the end: a
+// workgroup has 64 keys and half as many turns, so that the first keys of a
+// causal sequence, which all rows see, take no longer than the card takes for the
+// rest (8,192 tokens in three sequences, 8 key heads: DKDV us; 128 keys a
+// workgroup: 777).
+template <int DP_, bool EXACT, int NB_, bool DK, bool DV>
 struct KeyGradient {
-  static constexpr int DP = DP_, W = W_, RT = RT_;
-  static constexpr int kKeys = 32 * W, kThreads = 64 * W;
+  static constexpr int DP = DP_, NB = NB_;  // NB blocks of 32 rows a wavefront and turn
+  static constexpr int W = 4, kKeys = 64, kThreads = 64 * W, RT = 2 * NB * 32, T = DP / 32;
   using Tile = HeadTile<DP, RT, W>;
-  static constexpr int kStage = 2 * Tile::kBytes + 512;  // q, d_out, 64 values of lse and of delta
-  static constexpr int kLds = 2 * kStage;
-  static_assert(RT <= 64, "one load of lse and delta");
+  static constexpr int kStats = 4 * 64 * ((RT + 63) / 64);      // bytes of lse, and of delta
+  static constexpr int kStage = 2 * Tile::kBytes + 2 * kStats;  // q, d_out, lse, delta
+  static constexpr int kSums = (DK + DV) * T / 2 * 4096;        // of one wavefront, exchanged at the end
+  static constexpr int kLds = 2 * kStage > 4 * kSums ? 2 * kStage : 4 * kSums;
 
   static __device__ __forceinline__ void run(const AttentionArgs& a, const Divisor& group, uint8_t* lds) {
     const int dim = EXACT ? DP : a.dim;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = wave >> 1;  // of a tile's rows
     const int head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
     const Segment seg = find_segment(a.key_offsets != nullptr ? a.key_offsets : a.offsets, a.sequences, a.keys, 1, kKeys, number);
     const int key0 = seg.first + seg.tile * kKeys;
@@ -440,8 +539,9 @@ struct KeyGradient {
     // the sequence's rows
     int first_row = 0, last_row = 0;
     if (seg.number >= 0) {
-      if (a.offsets == nullptr) {
-        last_row = static_cast<int>(a.tokens) * a.group;
+      if (a.key_offsets == nullptr) {  // the keys' own
+        first_row = seg.first * a.group;
+        last_row = seg.last * a.group;
       } else {
         const int most = static_cast<int>(a.tokens);
         int lo = a.offsets[seg.number], hi = a.offsets[seg.number + 1];
@@ -457,11 +557,57 @@ struct KeyGradient {
       const int n = a.causal ? key - seg.first - shift : 0;
       return n <= 0 ? first_row : first_row + n * a.group;
     };
-    const int h = lane >> 5, key = key0 + 32 * wave + (lane & 31), k = key < seg.last ? key : seg.last - 1;
+    const int h = lane >> 5, key = key0 + 32 * (wave & 1) + (lane & 31), k = key < seg.last ? key : seg.last - 1;
     const int from = sees(k), from_all = __builtin_amdgcn_readlane(from, 31), from_some = __builtin_amdgcn_readfirstlane(from);
     const int start = __builtin_amdgcn_readfirstlane(sees(key0));
     const int steps = start < last_row ? (last_row - start + RT - 1) / RT : 0;
 
+    if (dim < DP) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) Tile::clear(lds + (s >> 1) * kStage + (s & 1) * Tile::kBytes, dim, kThreads);
+    }
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    const int64_t stat = static_cast<int64_t>(head) * a.tokens * a.group, heads = static_cast<int64_t>(a.kv_heads) * a.group;
+    const float* lse = (DK ? a.starts : a.lse) + stat;
+    const float* delta = a.starts + heads * a.tokens + stat;
+    const bool even = 16 % a.group == 0;  // rows 16 apart are whole tokens apart
+    const int own = Tile::row_of(wave, lane), own_token = group.quotient(own), own_head = own - own_token * a.group;
+    const uint32_t q_off = static_cast<uint32_t>(2 * (own_token * a.q.token + own_head * a.q.head)) + Tile::piece_of(wave, lane);
+    const uint32_t o_off = static_cast<uint32_t>(2 * (own_token * a.d_out.token + own_head * a.d_out.head)) + Tile::piece_of(wave, lane);
+    const auto issue = [&](int step) {
+      const uint32_t at = lds_at + (step & 1) * kStage;
+      const int row0 = start + step * RT, left = last_row - row0;
+      const int token0 = group.quotient(row0);
+      const uint16_t* qp = a.q.p + token0 * a.q.token + head * a.group * a.q.head;
+      const uint16_t* op = a.d_out.p + token0 * a.d_out.token + head * a.group * a.d_out.head;
+      const auto offset = [&](const Rows16& x) {  // start, and so row0, is a token's first row
+        return [&](int n) {
+          const int token = group.quotient(row0 + n), g = row0 + n - token * a.group;
+          return static_cast<uint32_t>(token - token0) * static_cast<uint32_t>(2 * x.token) + static_cast<uint32_t>(g) * static_cast<uint32_t>(2 * x.head);
+        };
+      };
+      bool done = false;
+      if constexpr (Tile::kEven) {
+        if (even && left >= RT) {
+          const uint64_t apart = 16 / a.group;
+          Tile::load_even(qp, q_off, 2 * apart * a.q.token, dim, wave, lane, at);
+          Tile::load_even(op, o_off, 2 * apart * a.d_out.token, dim, wave, lane, at + Tile::kBytes);
+          done = true;
+        }
+      }
+      if (!done) {
+        Tile::load(qp, offset(a.q), left, dim, wave, lane, at);
+        Tile::load(op, offset(a.d_out), left, dim, wave, lane, at + Tile::kBytes);
+      }
+      if (wave < kStats / 256) {
+        const int n = 64 * wave + lane;
+        const uint32_t off = 4 * (n < left ? n : left - 1), to = at + 2 * Tile::kBytes + 256 * wave;
+        load_to_lds<4>(lse + row0, off, to);
+        if (DK) load_to_lds<4>(delta + row0, off, to + kStats);
+      }
+    };
+
+    if (steps > 0) issue(0);
     bf16x8 kf[DP / 16], vf[DP / 16];
     const uint16_t* kp = a.k.p + k * a.k.token + head * a.k.head;
     const uint16_t* vp = a.v.p + k * a.v.token + head * a.v.head;
@@ -480,80 +626,125 @@ struct KeyGradient {
       arrived(kf[j]);
       if (DK) arrived(vf[j]);
     }
-    if (dim < DP) {
+    const typename Tile::Places at(lds_at + half * (NB * 32 * Tile::kPitch), lane);
+    const float c = a.scale * kLog2e, start_scale = -1.0f / c;
+    f32x16 d_k[T], d_v[T];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) Tile::clear(lds + (s >> 1) * kStage + (s & 1) * Tile::kBytes, dim, kThreads);
-    }
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
-    const float* lse = a.lse + static_cast<int64_t>(head) * a.tokens * a.group;
-    const float* delta = a.delta + static_cast<int64_t>(head) * a.tokens * a.group;
-    const auto issue = [&](int step) {
-      const uint32_t at = lds_at + (step & 1) * kStage;
-      const int row0 = start + step * RT, left = last_row - row0;
-      const int token0 = group.quotient(row0);
-      const auto rows = [&](const Rows16& x) {
-        return [&](int n) {
-          const int token = group.quotient(row0 + n), g = row0 + n - token * a.group;
-          return static_cast<uint32_t>(token - token0) * static_cast<uint32_t>(2 * x.token) + static_cast<uint32_t>(g) * static_cast<uint32_t>(2 * x.head);
-        };
-      };
-      const int64_t q_at = token0 * a.q.token + head * a.group * a.q.head;
-      const int64_t d_at = token0 * a.d_out.token + head * a.group * a.d_out.head;
-      Tile::load(a.q.p + q_at, rows(a.q), left, dim, wave, lane, at);
-      Tile::load(a.d_out.p + d_at, rows(a.d_out), left, dim, wave, lane, at + Tile::kBytes);
-      if (wave == 0) {
-        const uint32_t off = 4 * (lane < left ? lane : left - 1);
-        load_to_lds<4>(lse + row0, off, at + 2 * Tile::kBytes);
-        load_to_lds<4>(delta + row0, off, at + 2 * Tile::kBytes + 256);
-      }
-    };
-
-    const float c = a.scale * kLog2e;
-    f32x16 d_k[DP / 32], d_v[DP / 32];
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t) d_k[t] = d_v[t] = zero16();
+    for (int t = 0; t < T; ++t) d_k[t] = d_v[t] = zero16();
     uint32_t dirty = 0;
     const auto compute = [&](int step, auto stage, auto masked) {
       constexpr bool kMasked = decltype(masked)::value;
-      const uint8_t* qt = lds + stage * kStage;
-      const uint8_t* ot = qt + Tile::kBytes;
-      const float* stats = reinterpret_cast<const float*>(qt + 2 * Tile::kBytes);
-#pragma unroll
-      for (int b = 0; b < RT / 32; ++b) {
-        f32x16 s = zero16(), p = zero16();
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-          s = mfma32(Tile::along(qt, b, j, lane), kf[j], s);
-          if (DK) p = mfma32(Tile::along(ot, b, j, lane), vf[j], p);
-        }
-        const int base = start + step * RT + 32 * b + 4 * h;
+      const int qt = stage * kStage, ot = qt + Tile::kBytes;
+      const float* stats = reinterpret_cast<const float*>(lds + stage * kStage + 2 * Tile::kBytes) + half * (NB * 32);
+      f32x16 s[NB], p[NB];
+      const auto begin = [&](int b) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const f32x4 l = *reinterpret_cast<const f32x4*>(stats + 32 * b + result_row(e, h));
-          const f32x4 d = *reinterpret_cast<const f32x4*>(stats + 64 + 32 * b + result_row(e, h));
+          const f32x4 d = *reinterpret_cast<const f32x4*>(stats + (DK ? kStats / 4 : 0) + 32 * b + result_row(e, h));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float w = exp2_fast(fmaf(s[e + i], c, -l[i]));
-            s[e + i] = w;
-            p[e + i] = w * (p[e + i] - d[i]);
-            if constexpr (kMasked) {
-              const int row = base + result_row(e + i, 0);
-              if (row < from || row >= last_row) s[e + i] = p[e + i] = 0.0f;
-            }
+            s[b][e + i] = DK ? l[i] : l[i] * start_scale;
+            p[b][e + i] = d[i];
           }
         }
+      };
+      // w = P, p = dS of results first .. first + 7 of a block
+      const auto weigh = [&](int b, int first) {
+#pragma unroll
+        for (int e = first; e < first + 8; ++e) {
+          const float w = exp2_fast(s[b][e] * c);
+          s[b][e] = w;
+          p[b][e] *= w;
+          if constexpr (kMasked) {
+            const int row = start + step * RT + half * (NB * 32) + 32 * b + 4 * h + result_row(e, 0);
+            if (row < from || row >= last_row) s[b][e] = p[b][e] = 0.0f;
+          }
+        }
+      };
+      if constexpr (DK && DV && NB == 2 && !kMasked) {
+        // Operands are read two groups ahead of the products that take them, and the weights
+        // of a block are made beside the products of the other one.
+        constexpr int kGroups = DP / 64;  // of a block's scores
+        constexpr int kAhead = DP == 64 ? KAHEAD64 : 2;
+        bf16x8 f[kAhead + 1][8];
+        const auto read_scores = [&](bf16x8 (&x)[8], int n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[2 * j] = at.along(qt, n / kGroups, 4 * (n % kGroups) + j);
+            x[2 * j + 1] = at.along(ot, n / kGroups, 4 * (n % kGroups) + j);
+          }
+        };
+        const auto scores = [&](const bf16x8 (&x)[8], int n) {
+          const int b = n / kGroups;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[b] = mfma32(x[2 * j], kf[4 * (n % kGroups) + j], s[b]);
+            p[b] = mfma32(x[2 * j + 1], vf[4 * (n % kGroups) + j], p[b]);
+          }
+        };
+        const auto read_across = [&](bf16x8 (&x)[8], int n) {
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            x[2 * t] = at.across(ot, n, t);
+            x[2 * t + 1] = at.across(qt, n, t);
+          }
+        };
+        const auto add = [&](const bf16x8 (&x)[8], int n) {
+          const bf16x8 w = operand8(s[n >> 1], n & 1), ds = operand8(p[n >> 1], n & 1);
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            d_v[t] = mfma32(x[2 * t], w, d_v[t]);
+            d_k[t] = mfma32(x[2 * t + 1], ds, d_k[t]);
+          }
+        };
+        constexpr int kAll = 2 * kGroups + 4;
+        const auto read = [&](int n) { n < 2 * kGroups ? read_scores(f[n % (kAhead + 1)], n) : read_across(f[n % (kAhead + 1)], n - 2 * kGroups); };
+        begin(0);
+        begin(1);
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) read(n);
+#pragma unroll
+        for (int n = 0; n < kAll; ++n) {
+          fence();
+          if (n + kAhead < kAll) read(n + kAhead);
+          if (n < 2 * kGroups) scores(f[n % (kAhead + 1)], n);
+          else add(f[n % (kAhead + 1)], n - 2 * kGroups);
+          // block 0's weights beside block 1's scores, block 1's beside block 0's sums
+          if (n >= kGroups && n < 2 * kGroups) {
+            weigh(0, kGroups == 2 ? 8 * (n - kGroups) : 0);
+            if (kGroups == 1) weigh(0, 8);
+          }
+          if (n >= 2 * kGroups && n < 2 * kGroups + 2) weigh(1, 8 * (n - 2 * kGroups));
+        }
+        fence();
+        return;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        begin(b);
+#pragma unroll
+        for (int j = 0; j < DP / 16; ++j) {
+          s[b] = mfma32(at.along(qt, b, j), kf[j], s[b]);
+          if (DK) p[b] = mfma32(at.along(ot, b, j), vf[j], p[b]);
+        }
+        weigh(b, 0);
+        weigh(b, 8);
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const bf16x8 w = operand8(s, i), ds = operand8(p, i);
+          const bf16x8 w = operand8(s[b], i), ds = operand8(p[b], i);
 #pragma unroll
-          for (int t = 0; t < DP / 32; ++t) {
+          for (int t = 0; t < T; ++t) {
             if constexpr (DV) {
-              bf16x8 f = Tile::across(ot, 2 * b + i, t, lane);
+              bf16x8 f = at.across(ot, 2 * b + i, t);
               if constexpr (kMasked) f = finite_part(f, dirty);
               d_v[t] = mfma32(f, w, d_v[t]);
             }
             if constexpr (DK) {
-              bf16x8 f = Tile::across(qt, 2 * b + i, t, lane);
+              bf16x8 f = at.across(qt, 2 * b + i, t);
               // a query that holds an infinity or NaN gives them to the dS of the keys it sees
               uint32_t unused = 0;
               if constexpr (kMasked) f = finite_part(f, unused);
@@ -561,19 +752,19 @@ struct KeyGradient {
             }
           }
         }
-      }
     };
-    if (steps > 0) issue(0);
+    const int first_own = start + half * (NB * 32);  // this wavefront's first row
     const auto masked = [&](int step) {
       loads_done();
       if (step + 1 < steps) issue(step + 1);
-      if (start + (step + 1) * RT > from_some) compute(step, step & 1, std::true_type{});
+      if (first_own + step * RT + NB * 32 > from_some && first_own + step * RT < last_row) compute(step, step & 1, std::true_type{});
     };
-    // steps whose rows all exist and see every key of the wavefront, two at a time
-    int first = from_all > start ? (from_all - start + RT - 1) / RT : 0, end = (last_row - start) / RT;
-    first += first & 1;
+    // turns whose rows all exist and see every key of the wavefront, two at a time
+    int lead = from_all > start ? (from_all - start + RT - 1) / RT : 0;
+    lead += lead & 1;
+    const int end = (last_row - start) / RT;
     int step = 0;
-    for (; step < (first < steps ? first : steps); ++step) masked(step);
+    for (; step < (lead < steps ? lead : steps); ++step) masked(step);
     for (; step + 2 <= end; step += 2) {
       loads_done();
       issue(step + 1);
@@ -582,30 +773,49 @@ struct KeyGradient {
       if (step + 2 < steps) issue(step + 2);
       compute(step + 1, std::integral_constant<int, 1>{}, std::false_type{});
     }
+    const int tail = start + step * RT;
     for (; step < steps; ++step) masked(step);
     if (DV && __any(dirty != 0)) {
-      const auto at = [&](int row) {
+      const auto place = [&](int row) {
         const int token = group.quotient(row);
         return a.d_out.p + token * a.d_out.token + (head * a.group + row - token * a.group) * a.d_out.head;
       };
       const auto seen = [&](int row) { return row >= from; };
-      const int cut = from_all + RT < last_row ? from_all + RT : last_row, tail = last_row - RT > cut ? last_row - RT : cut;
-      add_nonfinite<DP>(d_v, from_some, cut, dim, h, at, seen);
-      add_nonfinite<DP>(d_v, tail, last_row, dim, h, at, seen);
+      const int until = start + lead * RT < last_row ? start + lead * RT : last_row;
+      add_nonfinite<DP>(d_v, start, until, dim, h, place, seen);
+      add_nonfinite<DP>(d_v, tail > until ? tail : until, last_row, dim, h, place, seen);
     }
+
+    // Each of two wavefronts finishes half of the columns that both have sums of.
+    __syncthreads();
+    const auto sums = [&](int of, int n) { return reinterpret_cast<f32x4*>(lds + of * kSums + n * 4096) + 4 * lane; };
+    const auto give = [&](const f32x16 (&x)[T], int slot) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+        if ((t >= T / 2) == (half == 0))
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sums(wave, slot + t % (T / 2))[e] = (f32x4){x[t][4 * e], x[t][4 * e + 1], x[t][4 * e + 2], x[t][4 * e + 3]};
+    };
+    if (DK) give(d_k, 0);
+    if (DV) give(d_v, DK ? T / 2 : 0);
+    __syncthreads();
     if (key >= seg.last) return;
     const int64_t o = (static_cast<int64_t>(key) * a.kv_heads + head) * dim;
+    const auto finish = [&](const f32x16 (&x)[T], int slot, float scale, uint16_t* to) {
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+      for (int t = 0; t < T; ++t)
+        if ((t < T / 2) == (half == 0))
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int d = 32 * t + result_row(e, h);
-        if (d >= dim) continue;
-        if (DK)
-          *reinterpret_cast<u32x2*>(a.d_k + o + d) =
-              pack4(d_k[t][e] * a.scale, d_k[t][e + 1] * a.scale, d_k[t][e + 2] * a.scale, d_k[t][e + 3] * a.scale);
-        if (DV) *reinterpret_cast<u32x2*>(a.d_v + o + d) = pack4(d_v[t][e], d_v[t][e + 1], d_v[t][e + 2], d_v[t][e + 3]);
-      }
+          for (int e = 0; e < 4; ++e) {
+            const f32x4 y = sums(wave ^ 2, slot + t % (T / 2))[e];
+            const int d = 32 * t + result_row(4 * e, h);
+            if (d < dim)
+              *reinterpret_cast<u32x2*>(to + o + d) = pack4((x[t][4 * e] + y[0]) * scale, (x[t][4 * e + 1] + y[1]) * scale,
+                                                            (x[t][4 * e + 2] + y[2]) * scale, (x[t][4 * e + 3] + y[3]) * scale);
+          }
+    };
+    if (DK) finish(d_k, 0, a.scale, a.d_k);
+    if (DV) finish(d_v, DK ? T / 2 : 0, 1.0f, a.d_v);
   }
 };
 
@@ -635,7 +845,7 @@ hipError_t launch_key_gradient(const AttentionArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int DP, bool EXACT, int RT>
+template <int DP, bool EXACT, int NB>
 hipError_t backward(const AttentionArgs& a, hipStream_t st) {
   hipError_t e = hipSuccess;
   if (a.d_q != nullptr)
@@ -644,10 +854,10 @@ hipError_t backward(const AttentionArgs& a, hipStream_t st) {
     e = launch_query_gradient<QueryGradient<DP, EXACT, 4, false>>(a, st);  // for delta
   if (e != hipSuccess) return e;
   // both gradients of 256 columns at once would not leave a lane registers for the scores
-  if (DP < 256 && a.d_k != nullptr && a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, 4, RT, DP < 256, true>>(a, st);
+  if (DP < 256 && a.d_k != nullptr && a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, NB, DP < 256, true>>(a, st);
   if (a.d_k != nullptr)
-    if (e = launch_key_gradient<KeyGradient<DP, EXACT, 4, RT, true, false>>(a, st); e != hipSuccess) return e;
-  if (a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, 4, RT, false, true>>(a, st);
+    if (e = launch_key_gradient<KeyGradient<DP, EXACT, NB, true, false>>(a, st); e != hipSuccess) return e;
+  if (a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, NB, false, true>>(a, st);
   return hipSuccess;
 }
 

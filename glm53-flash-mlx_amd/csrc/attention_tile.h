@@ -110,6 +110,7 @@ struct HeadTile {
   static constexpr int kSlots = kPitch / 16;     // 16-byte pieces a row
   static constexpr int kLoadRows = 64 / kSlots;  // rows of one load instruction
   static constexpr int kLoads = ROWS / kLoadRows / W;
+  static constexpr bool kEven = W * kLoadRows % 16 == 0;  // a lane's rows are a multiple of 16 apart, and have one swizzle
   static_assert(ROWS % (kLoadRows * W) == 0 && ROWS % 16 == 0, "whole loads a wavefront");
 
   __device__ static __forceinline__ int swizzle(int row) {
@@ -138,45 +139,75 @@ struct HeadTile {
     }
   }
 
-  // The same of rows `pitch` bytes apart.  Whole tiles go by one offset a lane:
-  // its rows are a multiple of 16 apart, which have one swizzle, so the rest is uniform.
+  // The same of rows `pitch` bytes apart.
   __device__ static __forceinline__ void load(const uint16_t* base, uint32_t pitch, int left, int dim, int wave, int lane,
                                               uint32_t lds) {
-    constexpr int kApart = W * kLoadRows;
-    if (kApart % 16 != 0 || left < ROWS) {
-      load(base, [&](int row) { return static_cast<uint32_t>(row) * pitch; }, left, dim, wave, lane, lds);
-      return;
+    if constexpr (kEven) {
+      if (left >= ROWS) {
+        load_even(base, static_cast<uint32_t>(row_of(wave, lane)) * pitch + piece_of(wave, lane), uint64_t{16} * pitch, dim,
+                  wave, lane, lds);
+        return;
+      }
     }
-    const int row = wave * kLoadRows + lane / kSlots, piece = (lane % kSlots) ^ swizzle(row);
-    const uint32_t off = static_cast<uint32_t>(row) * pitch + 16 * piece;
+    load(base, [&](int row) { return static_cast<uint32_t>(row) * pitch; }, left, dim, wave, lane, lds);
+  }
+
+  // A lane's row of a wavefront's first load, and the byte of its piece.
+  __device__ static __forceinline__ int row_of(int wave, int lane) { return wave * kLoadRows + lane / kSlots; }
+  __device__ static __forceinline__ int piece_of(int wave, int lane) {
+    return 16 * ((lane % kSlots) ^ swizzle(row_of(wave, lane)));
+  }
+  // A whole tile whose rows 16 apart lie `apart` bytes apart, by one offset a lane, of its
+  // first row: the rest is uniform.
+  __device__ static __forceinline__ void load_even(const uint16_t* base, uint32_t off, uint64_t apart, int dim, int wave,
+                                                   int lane, uint32_t lds) {
+    static_assert(kEven, "rows of one lane have one swizzle");
     const uint8_t* at = reinterpret_cast<const uint8_t*>(base);
+    const bool in = piece_of(wave, lane) < 2 * dim;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      if (8 * piece < dim) load_to_lds(at, off, lds + (wave + W * i) * kLoadRows * kPitch);
-      at += static_cast<uint64_t>(kApart) * pitch;
+      if (in) load_to_lds(at, off, lds + (wave + W * i) * kLoadRows * kPitch);
+      at += W * kLoadRows / 16 * apart;
     }
   }
 
-  // Operand j of rows 32 b .. 32 b + 31: values 16 j .. 16 j + 15.
-  __device__ static __forceinline__ bf16x8 along(const uint8_t* tile, int b, int j, int lane) {
-    const int row = 32 * b + (lane & 31), piece = 2 * j + (lane >> 5);
-    return *reinterpret_cast<const bf16x8*>(tile + row * kPitch + 16 * (piece ^ swizzle(row)));
-  }
+  // Where a lane reads a tile's operands, from the tile at LDS address `base`: the rest of an
+  // address is a constant of the read.
+  struct Places {
+    uint32_t row[DP / 16];       // operand j of rows 0 .. 31
+    uint32_t column[DP / 32][2];  // columns 32 t .. of rows 0 .. 15, its two halves
 
-  // Values 32 t .. 32 t + 31 as the operand's rows, rows 16 i .. 16 i + 15 as its
-  // contraction, in the order of a result's registers (above).
-  __device__ static __forceinline__ bf16x8 across(const uint8_t* tile, int i, int t, int lane) {
-    typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-    const int a = lane & 15, piece = 4 * t + 2 * ((lane >> 4) & 1) + ((a & 3) >> 1);
-    s16x4 v[2];
+    __device__ __forceinline__ Places(uint32_t base, int lane) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int row = 16 * i + 8 * half + 4 * (lane >> 5) + (a >> 2);
-      v[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_s16x4)(tile + row * kPitch + 16 * (piece ^ swizzle(row)) + 8 * (a & 1)));
+      for (int j = 0; j < DP / 16; ++j) {
+        const int r = lane & 31, piece = 2 * j + (lane >> 5);
+        row[j] = base + r * kPitch + 16 * (piece ^ swizzle(r));
+        arrived(row[j]);
+      }
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int a = lane & 15, piece = 4 * t + 2 * ((lane >> 4) & 1) + ((a & 3) >> 1);
+          const int r = 8 * half + 4 * (lane >> 5) + (a >> 2);
+          column[t][half] = base + r * kPitch + 16 * (piece ^ swizzle(r)) + 8 * (a & 1);
+          arrived(column[t][half]);
+        }
     }
-    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
-  }
+    // Operand j of rows 32 b .. 32 b + 31, values 16 j .. 16 j + 15, of the tile `tile` bytes on.
+    __device__ __forceinline__ bf16x8 along(int tile, int b, int j) const {
+      typedef __attribute__((address_space(3))) const bf16x8* lds;
+      return *reinterpret_cast<lds>(row[j] + (tile + 32 * b * kPitch));
+    }
+    // Values 32 t .. 32 t + 31 as the operand's rows, rows 16 i .. 16 i + 15 as its
+    // contraction, in the order of a result's registers (above).
+    __device__ __forceinline__ bf16x8 across(int tile, int i, int t) const {
+      typedef __attribute__((address_space(3))) s16x4* lds;
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds>(column[t][0] + (tile + 16 * i * kPitch)));
+      const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds>(column[t][1] + (tile + 16 * i * kPitch)));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
 };
 
 // Tiles that a mask cuts: a weight that is 0 because its place is masked must
@@ -252,13 +283,20 @@ __device__ __forceinline__ Segment find_segment(const int32_t* offsets, int sequ
     v = v < 0 ? 0 : v > most ? most : v;
     return v * times;
   };
-  int count = 0;
-  for (int i = 0; i < sequences + 2; i += 64)
-    count += __popcll(__ballot(i + lane < sequences + 2 && boundary(i + lane) / size + i + lane <= t));
+  int count = 0, mine = 0;
+  for (int i = 0; i < sequences + 2; i += 64) {
+    mine = boundary(i + lane);
+    count += __popcll(__ballot(i + lane < sequences + 2 && mine / size + i + lane <= t));
+  }
   const int s = __builtin_amdgcn_readfirstlane(count) - 1;  // boundary 0 counts for every t
   Segment g;
-  g.first = __builtin_amdgcn_readfirstlane(boundary(s));
-  g.last = __builtin_amdgcn_readfirstlane(boundary(s + 1));
+  if (sequences + 2 < 64) {
+    g.first = __builtin_amdgcn_readlane(mine, s);
+    g.last = __builtin_amdgcn_readlane(mine, s + 1);
+  } else {
+    g.first = __builtin_amdgcn_readfirstlane(boundary(s));
+    g.last = __builtin_amdgcn_readfirstlane(boundary(s + 1));
+  }
   g.number = s >= 1 && s <= sequences ? s - 1 : -1;
   g.tile = t - g.first / size - s;
   return g;

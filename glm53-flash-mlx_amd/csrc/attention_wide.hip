@@ -10,8 +10,8 @@ hipError_t launch_attention_wide(const AttentionArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_attention_backward_wide(const AttentionArgs& a, hipStream_t st) {
-  if (a.dim == 256) return backward<256, true, 32>(a, st);
-  return backward<256, false, 32>(a, st);
+  if (a.dim == 256) return backward<256, true, 1>(a, st);
+  return backward<256, false, 1>(a, st);
 }
 
 }  // namespace glm53
