@@ -3,17 +3,12 @@
 
 namespace glm53 {
 
-#ifndef ATT_RB
-#define ATT_RB 1
-#define ATT_W 4
-#endif
-
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t st) {
   if (a.dim > 128) return launch_attention_wide(a, st);
-  if (a.dim == 128) return launch_forward<Forward<128, true, ATT_RB, ATT_W>>(a, st);
-  if (a.dim == 64) return launch_forward<Forward<64, true, ATT_RB, ATT_W>>(a, st);
-  if (a.dim > 64) return launch_forward<Forward<128, false, ATT_RB, ATT_W>>(a, st);
-  return launch_forward<Forward<64, false, ATT_RB, ATT_W>>(a, st);
+  if (a.dim == 128) return launch_forward<Forward<128, true, 4>>(a, st);
+  if (a.dim == 64) return launch_forward<Forward<64, true, 4>>(a, st);
+  if (a.dim > 64) return launch_forward<Forward<128, false, 4>>(a, st);
+  return launch_forward<Forward<64, false, 4>>(a, st);
 }
 
 hipError_t launch_attention_backward(const AttentionArgs& a, hipStream_t st) {

@@ -8,6 +8,7 @@
 #pragma once
 
 #include <type_traits>
+#include <utility>
 
 #include "attention.h"
 #include "attention_tile.h"
@@ -16,12 +17,20 @@ namespace glm53 {
 
 namespace {
 
-#ifndef QAHEAD
-#define QAHEAD 1
-#endif
-#ifndef KAHEAD64
-#define KAHEAD64 2
-#endif
+// How a tile is multiplied: every place of it seen; some masked; or masked,
+// with infinities and NaNs in masked places kept from the results.  The last is the price
+// of a kernel's second pass, which follows where the first one's results are
+// not all finite: they may be what 0 x NaN made of a masked place.
+enum How { kPlain, kMasked, kCareful };
+template <int N>
+using Constant = std::integral_constant<int, N>;
+
+// f(0), ..., f(N - 1) with constants: a loop that is unrolled whatever its length.
+template <class F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) { (f(Constant<I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void each(F f) { each(f, std::make_integer_sequence<int, N>{}); }
+
 // Keeps what is in front of it in front and what is behind it behind, when the
 // compiler orders instructions: left alone it puts each LDS read directly
 // before the product that waits for it.
@@ -64,6 +73,77 @@ __device__ __forceinline__ void sequence_keys(const AttentionArgs& a, const Divi
   count = __builtin_amdgcn_readfirstlane(hi - lo);
 }
 
+// Whether a causal pass over row tiles of `size` starts with those that see the most keys
+// whatever their sequence, which pays for its search where sequences are long (8,192
+// tokens in two, 16 heads of 64: 84 us for 94; in eleven, 32 / 8 heads of 128: 105 for 99).
+__device__ __forceinline__ bool longest_first(const AttentionArgs& a, int size) {
+  return a.causal && a.tokens * a.group >= int64_t{32} * size * a.sequences;
+}
+
+// Keys that the query of a row sees: a prefix of its sequence's.
+struct Prefix {
+  const Divisor& group;
+  int first, shift, keys;
+  bool causal;
+  __device__ __forceinline__ Prefix(const AttentionArgs& a, const Divisor& group, const Segment& seg, int keys)
+      : group(group), first(seg.first), shift(keys - group.quotient(seg.last - seg.first)), keys(keys), causal(a.causal) {}
+  __device__ __forceinline__ int operator()(int row) const {
+    if (!causal) return keys;
+    const int n = group.quotient(row - first) + shift + 1;
+    return n < 0 ? 0 : n > keys ? keys : n;
+  }
+};
+
+// A row of memory as the operands that a lane of it holds, zeros from `dim` on, and
+// a result's column as a row of memory.
+template <int DP>
+__device__ __forceinline__ void load_operand(bf16x8 (&x)[DP / 16], const uint16_t* p, int dim, int h) {
+#pragma unroll
+  for (int j = 0; j < DP / 16; ++j) {
+    u32x4 v = {0, 0, 0, 0};
+    if (16 * j + 8 * h < dim) v = *reinterpret_cast<const u32x4*>(p + 16 * j + 8 * h);
+    x[j] = __builtin_bit_cast(bf16x8, v);
+  }
+}
+template <int DP>
+__device__ __forceinline__ void store_operand(uint16_t* p, const f32x16 (&x)[DP / 32], float by, int dim, int h) {
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int d = 32 * t + result_row(e, h);
+      if (d < dim)
+        *reinterpret_cast<u32x2*>(p + d) = pack4(x[t][e] * by, x[t][e + 1] * by, x[t][e + 2] * by, x[t][e + 3] * by);
+    }
+}
+
+template <int T>
+__device__ __forceinline__ bool nonfinite(const f32x16 (&x)[T]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum = fmaf(x[t][e], 0.0f, sum);
+  return sum != 0.0f;
+}
+
+// Whether any of the workgroup's threads says so, asked when all are through with
+// LDS, whose first words it takes.
+template <int W>
+__device__ __forceinline__ bool voted(bool mine, uint8_t* lds, int wave) {
+  int* votes = reinterpret_cast<int*>(lds);
+  const int own = __any(mine);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) votes[wave] = own;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) all |= votes[w];
+  if (!__builtin_amdgcn_readfirstlane(all)) return false;
+  __syncthreads();
+  return true;
+}
+
 // Tile numbers of `rows` rows in `sequences` sequences (see find_segment).
 int64_t tile_numbers(int64_t rows, bool packed, int sequences, int size) {
   return packed ? rows / size + sequences + 2 : (rows + size - 1) / size;
@@ -77,91 +157,65 @@ int64_t tile_numbers(int64_t rows, bool packed, int sequences, int size) {
 // lane and its counterpart 32 lanes away, and the weights go into the second
 // product (out^T = v^T P^T) from the registers they are in.
 
-template <int DP_, bool EXACT, int RB_, int W_>
+template <int DP_, bool EXACT, int W_>
 struct Forward {
-  static constexpr int DP = DP_, RB = RB_, W = W_;
-  static constexpr int kRows = 32 * RB * W, kThreads = 64 * W, kKeys = 64, T = DP / 32;
+  static constexpr int DP = DP_, W = W_;
+  static constexpr int kRows = 32 * W, kThreads = 64 * W, kKeys = 64, T = DP / 32;
   using Tile = HeadTile<DP, kKeys, W>;
   static constexpr int kLds = 4 * Tile::kBytes;  // two stages of keys and values
 
   static __device__ __forceinline__ void run(const AttentionArgs& a, const Divisor& group, int tiles, uint8_t* lds) {
     const int dim = EXACT ? DP : a.dim;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = blockIdx.x % a.kv_heads, number = tiles - 1 - blockIdx.x / a.kv_heads;
-    const Segment seg = find_segment(a.offsets, a.sequences, a.tokens, a.group, kRows, number);
+    const int head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
+    const Segment seg = find_segment(a.offsets, a.sequences, a.tokens, a.group, kRows, number, tiles,
+                                     longest_first(a, kRows) ? kLastFirst : kReversed);
     const int row0 = seg.first + seg.tile * kRows;
     if (seg.tile < 0 || row0 >= seg.last) return;
-
     int key0, keys;
     sequence_keys(a, group, seg, key0, keys);
-    // keys that the query of row r sees: a prefix
-    const int shift = keys - group.quotient(seg.last - seg.first);
-    const auto limit = [&](int row) {
-      if (!a.causal) return keys;
-      const int n = group.quotient(row - seg.first) + shift + 1;
-      return n < 0 ? 0 : n > keys ? keys : n;
-    };
+    const Prefix prefix(a, group, seg, keys);
     const int last_row = row0 + kRows < seg.last ? row0 + kRows - 1 : seg.last - 1;
-    const int steps = (__builtin_amdgcn_readfirstlane(limit(last_row)) + kKeys - 1) / kKeys;
+    const int steps = (__builtin_amdgcn_readfirstlane(prefix(last_row)) + kKeys - 1) / kKeys;
 
     const int h = lane >> 5;
     if (dim < DP) {
 #pragma unroll
       for (int s = 0; s < 4; ++s) Tile::clear(lds + s * Tile::kBytes, dim, kThreads);
     }
-    const uint16_t* kp = a.k.p + static_cast<int64_t>(key0) * a.k.token + static_cast<int64_t>(head) * a.k.head;
-    const uint16_t* vp = a.v.p + static_cast<int64_t>(key0) * a.v.token + static_cast<int64_t>(head) * a.v.head;
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    const uint16_t* kp = a.k.p + key0 * a.k.token + head * a.k.head;
+    const uint16_t* vp = a.v.p + key0 * a.v.token + head * a.v.head;
+    const uint32_t lds_at = lds_address(lds);
     const auto issue = [&](int step) {
-      const uint32_t at = lds_at + (step & 1) * 2 * Tile::kBytes;
+      const uint32_t to = lds_at + (step & 1) * 2 * Tile::kBytes;
       const int64_t first = static_cast<int64_t>(step) * kKeys;
       const int left = keys - step * kKeys;
-      Tile::load(kp + first * a.k.token, static_cast<uint32_t>(2 * a.k.token), left, dim, wave, lane, at);
-      Tile::load(vp + first * a.v.token, static_cast<uint32_t>(2 * a.v.token), left, dim, wave, lane, at + Tile::kBytes);
+      Tile::load(kp + first * a.k.token, static_cast<uint32_t>(2 * a.k.token), left, dim, wave, lane, to);
+      Tile::load(vp + first * a.v.token, static_cast<uint32_t>(2 * a.v.token), left, dim, wave, lane, to + Tile::kBytes);
     };
-
     if (steps > 0) issue(0);
-    int row[RB], lim[RB];
-    bf16x8 q[RB][DP / 16];
+
+    const int row = row0 + 32 * wave + (lane & 31);
+    const int r = row < seg.last ? row : seg.last - 1;  // rows past the last repeat it
+    const int token = group.quotient(r), query_head = head * a.group + r - token * a.group;
+    const int lim = prefix(r);
+    bf16x8 q[DP / 16];
+    load_operand<DP>(q, a.q.p + token * a.q.token + query_head * a.q.head, dim, h);
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      row[b] = row0 + 32 * (RB * wave + b) + (lane & 31);
-      const int r = row[b] < seg.last ? row[b] : seg.last - 1;  // rows past the last repeat it
-      lim[b] = limit(r);
-      const int token = group.quotient(r);
-      const uint16_t* p = a.q.p + token * a.q.token + (head * a.group + r - token * a.group) * a.q.head;
-#pragma unroll
-      for (int j = 0; j < DP / 16; ++j) {
-        u32x4 v = {0, 0, 0, 0};
-        if (16 * j + 8 * h < dim) v = *reinterpret_cast<const u32x4*>(p + 16 * j + 8 * h);
-        q[b][j] = __builtin_bit_cast(bf16x8, v);
-      }
-    }
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int j = 0; j < DP / 16; ++j) arrived(q[b][j]);
-    const int all_see = __builtin_amdgcn_readfirstlane(lim[0]);                  // every row of the wavefront
-    const int some_see = __builtin_amdgcn_readlane(lim[RB - 1], 31);             // its last row
+    for (int j = 0; j < DP / 16; ++j) arrived(q[j]);
+    const int all_see = __builtin_amdgcn_readfirstlane(lim), some_see = __builtin_amdgcn_readlane(lim, 31);
 
     const typename Tile::Places at(lds_at, lane);
     const float c = a.scale * kLog2e;
-    f32x16 out[RB][DP / 32];
-    float m[RB], l[RB];  // m in units of scores; l: this lane's part
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      m[b] = -INFINITY;
-      l[b] = 0.0f;
-#pragma unroll
-      for (int t = 0; t < DP / 32; ++t) out[b][t] = zero16();
-    }
-
+    f32x16 out[T];
+    float m, l;  // m in units of scores; l: this lane's part
     uint32_t dirty = 0;
-    const auto compute = [&](int step, auto stage, auto masked) {
-      constexpr bool kMasked = decltype(masked)::value;
+    // How: kPlain, kMasked, or kCareful (see finite_part)
+    const auto compute = [&](int step, auto stage, auto how) {
+      constexpr int kHow = decltype(how)::value;
       const int kt = stage * 2 * Tile::kBytes, vt = kt + Tile::kBytes;
-      f32x16 s[RB][2];
-      // groups of operands: the keys' in kb and 64 columns, the values' in 16 keys
+      f32x16 s[2];
+      // groups of operands: the keys' in 32 keys and 64 columns, the values' in 16 keys
       constexpr int kGroups = DP / 64, kMost = T > 4 ? T : 4;
       bf16x8 f[3][kMost];
       const auto read = [&](int n) {
@@ -181,56 +235,48 @@ struct Forward {
       for (int n = 0; n < 2 * kGroups; ++n) {
         fence();
         read(n + 2);
+        f32x16& x = s[n / kGroups];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int b = 0; b < RB; ++b)
-            s[b][n / kGroups] = mfma32(f[n % 3][j], q[b][4 * (n % kGroups) + j], n % kGroups + j == 0 ? zero16() : s[b][n / kGroups]);
+        for (int j = 0; j < 4; ++j) x = mfma32(f[n % 3][j], q[4 * (n % kGroups) + j], n % kGroups + j == 0 ? zero16() : x);
       }
       fence();
       products(false);
-      float mc[RB];
+      if constexpr (kHow != kPlain) {
+        const int left = lim - step * kKeys - 4 * h;
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        if constexpr (kMasked) {
-          const int left = lim[b] - step * kKeys - 4 * h;
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (32 * kb + result_row(r, 0) >= left) s[b][kb][r] = -INFINITY;
-        }
-        float top = s[b][0][0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[b][0][r]);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][1][r]);
-        top = both_max(top);
-        if (__any(top * c > m[b] * c + kSlack)) {
-          const float next = fmaxf(m[b], top);
-          const float alpha = next == -INFINITY ? 1.0f : exp2_fast((m[b] - next) * c);
-          m[b] = next;
-          l[b] *= alpha;
-#pragma unroll
-          for (int t = 0; t < T; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) out[b][t][r] *= alpha;
-        }
-        mc[b] = m[b] == -INFINITY ? 0.0f : m[b] * c;
+          for (int e = 0; e < 16; ++e)
+            if (32 * kb + result_row(e, 0) >= left) s[kb][e] = -INFINITY;
       }
-      bf16x8 p[RB], next[RB];
+      float top = s[0][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[0][e]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, s[1][e]);
+      top = both_max(top);
+      if (__any(top * c > m * c + kSlack)) {
+        const float next = fmaxf(m, top);
+        const float alpha = next == -INFINITY ? 1.0f : exp2_fast((m - next) * c);
+        m = next;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) out[t][e] *= alpha;
+      }
+      const float mc = m == -INFINITY ? 0.0f : m * c;
+      bf16x8 next;
       const auto weigh = [&](int i) {  // 8 of a lane's scores
+        f32x16& x = s[i >> 1];
+        float sum = 0.0f;
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            s[b][i >> 1][8 * (i & 1) + e] = exp2_fast(fmaf(s[b][i >> 1][8 * (i & 1) + e], c, -mc[b]));
-          float sum = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sum += s[b][i >> 1][8 * (i & 1) + e];
-          l[b] += sum;
-          next[b] = operand8(s[b][i >> 1], i & 1);
+        for (int e = 8 * (i & 1); e < 8 * (i & 1) + 8; ++e) {
+          x[e] = exp2_fast(fmaf(x[e], c, -mc));
+          sum += x[e];
         }
+        l += sum;
+        next = operand8(x, i & 1);
       };
       weigh(0);
       products(true);
@@ -239,13 +285,11 @@ struct Forward {
         fence();
         const int n = 2 * kGroups + i;
         read(n + 2);
-#pragma unroll
-        for (int b = 0; b < RB; ++b) p[b] = next[b];
+        const bf16x8 p = next;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-          if constexpr (kMasked) f[n % 3][t] = finite_part(f[n % 3][t], dirty);
-#pragma unroll
-          for (int b = 0; b < RB; ++b) out[b][t] = mfma32(f[n % 3][t], p[b], out[b][t]);
+          if constexpr (kHow == kCareful) f[n % 3][t] = finite_part(f[n % 3][t], dirty);
+          out[t] = mfma32(f[n % 3][t], p, out[t]);
         }
         if (i < 3) weigh(i + 1);
       }
@@ -255,53 +299,46 @@ struct Forward {
 
     // whole tiles two at a time: their places in LDS are constants then
     const int whole = all_see / kKeys & ~1;
-    int step = 0;
-    for (; step < whole; step += 2) {
-      loads_done();
-      issue(step + 1);
-      compute(step, std::integral_constant<int, 0>{}, std::false_type{});
-      loads_done();
-      if (step + 2 < steps) issue(step + 2);
-      compute(step + 1, std::integral_constant<int, 1>{}, std::false_type{});
-    }
-    for (; step < steps; ++step) {
-      loads_done();
-      if (step + 1 < steps) issue(step + 1);
-      if (step * kKeys < some_see) compute(step, step & 1, std::true_type{});
+    const auto pass = [&](auto how) {
+      m = -INFINITY;
+      l = 0.0f;
+#pragma unroll
+      for (int t = 0; t < T; ++t) out[t] = zero16();
+      int step = 0;
+      for (; step < whole; step += 2) {
+        loads_done();
+        issue(step + 1);
+        compute(step, Constant<0>{}, Constant<kPlain>{});
+        loads_done();
+        if (step + 2 < steps) issue(step + 2);
+        compute(step + 1, Constant<1>{}, Constant<kPlain>{});
+      }
+      for (; step < steps; ++step) {
+        loads_done();
+        if (step + 1 < steps) issue(step + 1);
+        if (step * kKeys < some_see) compute(step, step & 1, how);
+      }
+    };
+    pass(Constant<kMasked>{});
+    if (voted<W>(nonfinite(out), lds, wave)) {
+      issue(0);
+      pass(Constant<kCareful>{});
+      if (__any(dirty != 0))
+        add_nonfinite<DP>(out, whole * kKeys, some_see, dim, h, [&](int key) { return vp + key * a.v.token; },
+                          [&](int key) { return key < lim; });
     }
 
-    if (__any(dirty != 0)) {
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-        add_nonfinite<DP>(out[b], whole * kKeys, some_see, dim, h,
-                          [&](int key) { return vp + key * a.v.token; }, [&](int key) { return key < lim[b]; });
-    }
+    const float total = both_sum(l), inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    if (row >= seg.last) return;
     const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const float total = both_sum(l[b]);
-      const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-      if (row[b] >= seg.last) continue;
-      const int token = group.quotient(row[b]);
-      uint16_t* o = a.out + (token * heads + head * a.group + row[b] - token * a.group) * dim;
-#pragma unroll
-      for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-          const int d = 32 * t + result_row(r, h);
-          if (d < dim)
-            *reinterpret_cast<u32x2*>(o + d) = pack4(out[b][t][r] * inverse, out[b][t][r + 1] * inverse,
-                                                     out[b][t][r + 2] * inverse, out[b][t][r + 3] * inverse);
-        }
-      if (a.lse != nullptr && h == 0)
-        a.lse[static_cast<int64_t>(head) * a.tokens * a.group + row[b]] =
-            total == 0.0f ? 0.0f : m[b] * c + __builtin_amdgcn_logf(total);
-    }
+    store_operand<DP>(a.out + (token * heads + query_head) * dim, out, inverse, dim, h);
+    if (a.lse != nullptr && h == 0)
+      a.lse[static_cast<int64_t>(head) * a.tokens * a.group + row] = total == 0.0f ? 0.0f : m * c + __builtin_amdgcn_logf(total);
   }
 };
 
 template <class F>
-__global__ __launch_bounds__(F::kThreads, F::DP == 256 || F::RB == 2 ? 1 : F::W == 8 ? 1 : 2) void attention_kernel(AttentionArgs a, Divisor group, int tiles) {
+__global__ __launch_bounds__(F::kThreads, F::DP == 256 ? 1 : 2) void attention_kernel(AttentionArgs a, Divisor group, int tiles) {
   extern __shared__ __align__(1024) uint8_t lds[];
   F::run(a, group, tiles, lds);
 }
@@ -326,37 +363,34 @@ template <int DP_, bool EXACT, int W_, bool DQ>
 struct QueryGradient {
   static constexpr int DP = DP_, W = W_;
   static constexpr int kRows = 32 * W, kThreads = 64 * W, kKeys = 64, T = DP / 32;
+  static constexpr int kAhead = DP >= 128 ? 1 : 2;  // the registers leave no more
   using Tile = HeadTile<DP, kKeys, W>;
   static constexpr int kLds = 4 * Tile::kBytes;
 
   static __device__ __forceinline__ void run(const AttentionArgs& a, const Divisor& group, int tiles, uint8_t* lds) {
     const int dim = EXACT ? DP : a.dim;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head = blockIdx.x % a.kv_heads, number = tiles - 1 - blockIdx.x / a.kv_heads;
-    const Segment seg = find_segment(a.offsets, a.sequences, a.tokens, a.group, kRows, number);
+    const int head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
+    const Segment seg = find_segment(a.offsets, a.sequences, a.tokens, a.group, kRows, number, tiles,
+                                     longest_first(a, kRows) ? kLastFirst : kReversed);
     const int row0 = seg.first + seg.tile * kRows;
     if (seg.tile < 0 || row0 >= seg.last) return;
     int key0, keys;
     sequence_keys(a, group, seg, key0, keys);
-    const int shift = keys - group.quotient(seg.last - seg.first);
-    const auto limit = [&](int row) {
-      if (!a.causal) return keys;
-      const int n = group.quotient(row - seg.first) + shift + 1;
-      return n < 0 ? 0 : n > keys ? keys : n;
-    };
+    const Prefix prefix(a, group, seg, keys);
     const int last_row = row0 + kRows < seg.last ? row0 + kRows - 1 : seg.last - 1;
-    const int steps = (__builtin_amdgcn_readfirstlane(limit(last_row)) + kKeys - 1) / kKeys;
+    const int steps = (__builtin_amdgcn_readfirstlane(prefix(last_row)) + kKeys - 1) / kKeys;
 
     const int h = lane >> 5, row = row0 + 32 * wave + (lane & 31);
     const int r = row < seg.last ? row : seg.last - 1, token = group.quotient(r), query_head = head * a.group + r - token * a.group;
-    const int lim = limit(r);
+    const int lim = prefix(r);
     if (dim < DP) {
 #pragma unroll
       for (int s = 0; s < 4; ++s) Tile::clear(lds + s * Tile::kBytes, dim, kThreads);
     }
     const uint16_t* kp = a.k.p + key0 * a.k.token + head * a.k.head;
     const uint16_t* vp = a.v.p + key0 * a.v.token + head * a.v.head;
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    const uint32_t lds_at = lds_address(lds);
     const auto issue = [&](int step) {
       const uint32_t at = lds_at + (step & 1) * 2 * Tile::kBytes;
       const int64_t first = static_cast<int64_t>(step) * kKeys;
@@ -369,16 +403,8 @@ struct QueryGradient {
     bf16x8 q[DP / 16], d_out[DP / 16];
     const uint16_t* qp = a.q.p + token * a.q.token + query_head * a.q.head;
     const uint16_t* dp = a.d_out.p + token * a.d_out.token + query_head * a.d_out.head;
-#pragma unroll
-    for (int j = 0; j < DP / 16; ++j) {
-      u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-      if (16 * j + 8 * h < dim) {
-        x = *reinterpret_cast<const u32x4*>(qp + 16 * j + 8 * h);
-        y = *reinterpret_cast<const u32x4*>(dp + 16 * j + 8 * h);
-      }
-      q[j] = __builtin_bit_cast(bf16x8, x);
-      d_out[j] = __builtin_bit_cast(bf16x8, y);
-    }
+    load_operand<DP>(q, qp, dim, h);
+    load_operand<DP>(d_out, dp, dim, h);
     const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
     const int64_t own = (token * heads + query_head) * dim, stat = static_cast<int64_t>(head) * a.tokens * a.group + r;
     float lse = a.lse[stat], delta = 0.0f;
@@ -400,95 +426,106 @@ struct QueryGradient {
 
     const typename Tile::Places at(lds_at, lane);
     const float c = a.scale * kLog2e;
-    float sum = 0.0f;  // of dS
-    f32x16 d_q[DP / 32];
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t) d_q[t] = zero16();
-    const auto compute = [&](int step, auto stage, auto masked) {
-      constexpr bool kMasked = decltype(masked)::value;
+    float sum;  // of dS
+    f32x16 d_q[T];
+    const auto compute = [&](int step, auto stage, auto how) {
+      constexpr int kHow = decltype(how)::value;
       const int kt = stage * 2 * Tile::kBytes, vt = kt + Tile::kBytes;
-      // groups of operands, read ahead of the products that take them: of 32 keys
-      // those of 32 columns of scores at a time, then those of 16 keys
-      constexpr int kGroups = DP / 32, kAhead = QAHEAD, kPart = kGroups + (DQ ? 2 : 0), kAll = 2 * kPart, kMost = T > 4 ? T : 4;
-      bf16x8 f[kAhead + 1][kMost];
+      // groups of operands, read ahead of the products that take them: of 32 keys those of
+      // scores, 16 columns and two operands at a time, then those of 16 keys, 32 columns each
+      constexpr int kOf = DP == 256 ? 4 : 2, kScores = DP / 8 / kOf, kAcross = T / kOf;
+      constexpr int kPart = kScores + (DQ ? 2 * kAcross : 0), kAll = 2 * kPart;
+      bf16x8 f[kAhead + 1][kOf];
       const auto read = [&](int n) {
         if (n >= kAll) return;
-        bf16x8 (&x)[kMost] = f[n % (kAhead + 1)];
-        const int kb = n / kPart, g = n % kPart;
-        if (g < kGroups) {
+        bf16x8 (&x)[kOf] = f[n % (kAhead + 1)];
+        const int kb = n / kPart, g = n % kPart, turn = g - kScores;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            x[2 * j] = at.along(kt, kb, 2 * g + j);
-            x[2 * j + 1] = at.along(vt, kb, 2 * g + j);
-          }
-        } else {
-#pragma unroll
-          for (int t = 0; t < T; ++t) x[t] = at.across(kt, 2 * kb + g - kGroups, t);
+        for (int i = 0; i < kOf; ++i) {
+          if (g >= kScores)
+            x[i] = at.across(kt, 2 * kb + turn / kAcross, kOf * (turn % kAcross) + i);
+          else
+            x[i] = at.along(i & 1 ? vt : kt, kb, kOf / 2 * g + i / 2);
         }
       };
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) read(n);
       f32x16 s, p;
+      bf16x8 ds, low;
       products(true);
-#pragma unroll
-      for (int n = 0; n < kAll; ++n) {
-        const int kb = n / kPart, g = n % kPart;
+      each<kAll>([&](auto number) {
+        constexpr int n = decltype(number)::value, kb = n / kPart, g = n % kPart, turn = g - kScores;
         fence();
         read(n + kAhead);
-        bf16x8 (&x)[kMost] = f[n % (kAhead + 1)];
+        bf16x8 (&x)[kOf] = f[n % (kAhead + 1)];
         if (g == 0) {
           s = zero16();
 #pragma unroll
           for (int e = 0; e < 16; ++e) p[e] = -delta;
         }
-        if (g < kGroups) {
+        if constexpr (g < kScores) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            s = mfma32(x[2 * j], q[2 * g + j], s);
-            p = mfma32(x[2 * j + 1], d_out[2 * g + j], p);
+          for (int i = 0; i < kOf; i += 2) {
+            s = mfma32(x[i], q[(kOf * g + i) / 2], s);
+            p = mfma32(x[i + 1], d_out[(kOf * g + i) / 2], p);
           }
         } else {
-          const bf16x8 ds = operand8(s, g - kGroups), low = low_operand8(s, g - kGroups, ds);
+          if (turn % kAcross == 0) {
+            ds = operand8(s, turn / kAcross);
+            low = low_operand8(s, turn / kAcross, ds);
+          }
 #pragma unroll
-          for (int t = 0; t < T; ++t) {
+          for (int i = 0; i < kOf; ++i) {
             // a key that holds an infinity or NaN gives them to the dS of the rows that see it
             uint32_t unused = 0;
-            if constexpr (kMasked) x[t] = finite_part(x[t], unused);
-            d_q[t] = mfma32(x[t], ds, d_q[t]);
-            d_q[t] = mfma32(x[t], low, d_q[t]);
+            if constexpr (kHow == kCareful) x[i] = finite_part(x[i], unused);
+            f32x16& sum_q = d_q[kOf * (turn % kAcross) + i];
+            sum_q = mfma32(x[i], ds, sum_q);
+            sum_q = mfma32(x[i], low, sum_q);
           }
         }
-        if (g == kGroups - 1) {
+        if constexpr (g == kScores - 1) {
           fence();
           products(false);
           const int left = lim - step * kKeys - 32 * kb - 4 * h;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             s[e] = exp2_fast(fmaf(s[e], c, -lse)) * p[e];
-            if (kMasked && result_row(e, 0) >= left) s[e] = 0.0f;
+            if (kHow != kPlain && result_row(e, 0) >= left) s[e] = 0.0f;
             sum += s[e];
           }
           products(true);
         }
-      }
+      });
       fence();
       products(false);
     };
-    // whole tiles two at a time: their places in LDS are constants then
     const int whole = all_see / kKeys & ~1;
-    int step = 0;
-    for (; step < whole; step += 2) {
-      loads_done();
-      issue(step + 1);
-      compute(step, std::integral_constant<int, 0>{}, std::false_type{});
-      loads_done();
-      if (step + 2 < steps) issue(step + 2);
-      compute(step + 1, std::integral_constant<int, 1>{}, std::false_type{});
-    }
-    for (; step < steps; ++step) {
-      loads_done();
-      if (step + 1 < steps) issue(step + 1);
-      if (step * kKeys < some_see) compute(step, step & 1, std::true_type{});
+    const auto pass = [&](auto how) {
+      sum = 0.0f;
+#pragma unroll
+      for (int t = 0; t < T; ++t) d_q[t] = zero16();
+      int step = 0;
+      for (; step < whole; step += 2) {
+        loads_done();
+        issue(step + 1);
+        compute(step, Constant<0>{}, Constant<kPlain>{});
+        loads_done();
+        if (step + 2 < steps) issue(step + 2);
+        compute(step + 1, Constant<1>{}, Constant<kPlain>{});
+      }
+      for (; step < steps; ++step) {
+        loads_done();
+        if (step + 1 < steps) issue(step + 1);
+        if (step * kKeys < some_see) compute(step, step & 1, how);
+      }
+    };
+    pass(Constant<kMasked>{});
+    if constexpr (DQ) {
+      if (voted<W>(nonfinite(d_q), lds, wave)) {
+        issue(0);
+        pass(Constant<kCareful>{});
+      }
     }
     sum = both_sum(sum);
     if (row >= seg.last) return;
@@ -496,17 +533,7 @@ struct QueryGradient {
       a.starts[stat] = -lse / c;
       a.starts[stat + heads * a.tokens] = -(delta + sum);
     }
-    if (!DQ) return;
-    uint16_t* o = a.d_q + own;
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        const int d = 32 * t + result_row(e, h);
-        if (d < dim)
-          *reinterpret_cast<u32x2*>(o + d) =
-              pack4(d_q[t][e] * a.scale, d_q[t][e + 1] * a.scale, d_q[t][e + 2] * a.scale, d_q[t][e + 3] * a.scale);
-      }
+    if constexpr (DQ) store_operand<DP>(a.d_q + own, d_q, a.scale, dim, h);
   }
 };
 
@@ -518,22 +545,23 @@ struct QueryGradient {
 // causal sequence, which all rows see, take no longer than the card takes for the
 // rest (8,192 tokens in three sequences, 8 key heads: DKDV us; 128 keys a
 // workgroup: 777).
-template <int DP_, bool EXACT, int NB_, bool DK, bool DV>
+template <int DP_, bool EXACT, int NB_, int RW_, bool DK, bool DV>
 struct KeyGradient {
-  static constexpr int DP = DP_, NB = NB_;  // NB blocks of 32 rows a wavefront and turn
-  static constexpr int W = 4, kKeys = 64, kThreads = 64 * W, RT = 2 * NB * 32, T = DP / 32;
+  static constexpr int DP = DP_, NB = NB_, RW = RW_;  // NB blocks of 32 rows a wavefront and turn, RW wavefronts' rows a tile
+  static constexpr int W = 4, KW = W / RW, kKeys = 32 * KW, kThreads = 64 * W, RT = RW * NB * 32, T = DP / 32;
   using Tile = HeadTile<DP, RT, W>;
   static constexpr int kStats = 4 * 64 * ((RT + 63) / 64);      // bytes of lse, and of delta
   static constexpr int kStage = 2 * Tile::kBytes + 2 * kStats;  // q, d_out, lse, delta
-  static constexpr int kSums = (DK + DV) * T / 2 * 4096;        // of one wavefront, exchanged at the end
+  static constexpr int kSums = RW == 2 ? (DK + DV) * T / 2 * 4096 : 0;  // of one wavefront, exchanged at the end
   static constexpr int kLds = 2 * kStage > 4 * kSums ? 2 * kStage : 4 * kSums;
 
-  static __device__ __forceinline__ void run(const AttentionArgs& a, const Divisor& group, uint8_t* lds) {
+  static __device__ __forceinline__ void run(const AttentionArgs& a, const Divisor& group, int tiles, uint8_t* lds) {
     const int dim = EXACT ? DP : a.dim;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int half = wave >> 1;  // of a tile's rows
+    const int half = wave / KW;  // whose rows of a tile
     const int head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
-    const Segment seg = find_segment(a.key_offsets != nullptr ? a.key_offsets : a.offsets, a.sequences, a.keys, 1, kKeys, number);
+    const Segment seg = find_segment(a.key_offsets != nullptr ? a.key_offsets : a.offsets, a.sequences, a.keys, 1, kKeys, number,
+                                     tiles, a.causal ? kFirstFirst : kInOrder);
     const int key0 = seg.first + seg.tile * kKeys;
     if (seg.tile < 0 || key0 >= seg.last) return;
     // the sequence's rows
@@ -557,7 +585,7 @@ struct KeyGradient {
       const int n = a.causal ? key - seg.first - shift : 0;
       return n <= 0 ? first_row : first_row + n * a.group;
     };
-    const int h = lane >> 5, key = key0 + 32 * (wave & 1) + (lane & 31), k = key < seg.last ? key : seg.last - 1;
+    const int h = lane >> 5, key = key0 + 32 * (wave % KW) + (lane & 31), k = key < seg.last ? key : seg.last - 1;
     const int from = sees(k), from_all = __builtin_amdgcn_readlane(from, 31), from_some = __builtin_amdgcn_readfirstlane(from);
     const int start = __builtin_amdgcn_readfirstlane(sees(key0));
     const int steps = start < last_row ? (last_row - start + RT - 1) / RT : 0;
@@ -566,7 +594,7 @@ struct KeyGradient {
 #pragma unroll
       for (int s = 0; s < 4; ++s) Tile::clear(lds + (s >> 1) * kStage + (s & 1) * Tile::kBytes, dim, kThreads);
     }
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds));
+    const uint32_t lds_at = lds_address(lds);
     const int64_t stat = static_cast<int64_t>(head) * a.tokens * a.group, heads = static_cast<int64_t>(a.kv_heads) * a.group;
     const float* lse = (DK ? a.starts : a.lse) + stat;
     const float* delta = a.starts + heads * a.tokens + stat;
@@ -611,16 +639,8 @@ struct KeyGradient {
     bf16x8 kf[DP / 16], vf[DP / 16];
     const uint16_t* kp = a.k.p + k * a.k.token + head * a.k.head;
     const uint16_t* vp = a.v.p + k * a.v.token + head * a.v.head;
-#pragma unroll
-    for (int j = 0; j < DP / 16; ++j) {
-      u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-      if (16 * j + 8 * h < dim) {
-        x = *reinterpret_cast<const u32x4*>(kp + 16 * j + 8 * h);
-        if (DK) y = *reinterpret_cast<const u32x4*>(vp + 16 * j + 8 * h);
-      }
-      kf[j] = __builtin_bit_cast(bf16x8, x);
-      vf[j] = __builtin_bit_cast(bf16x8, y);
-    }
+    load_operand<DP>(kf, kp, dim, h);
+    if (DK) load_operand<DP>(vf, vp, dim, h);
 #pragma unroll
     for (int j = 0; j < DP / 16; ++j) {
       arrived(kf[j]);
@@ -629,11 +649,9 @@ struct KeyGradient {
     const typename Tile::Places at(lds_at + half * (NB * 32 * Tile::kPitch), lane);
     const float c = a.scale * kLog2e, start_scale = -1.0f / c;
     f32x16 d_k[T], d_v[T];
-#pragma unroll
-    for (int t = 0; t < T; ++t) d_k[t] = d_v[t] = zero16();
     uint32_t dirty = 0;
-    const auto compute = [&](int step, auto stage, auto masked) {
-      constexpr bool kMasked = decltype(masked)::value;
+    const auto compute = [&](int step, auto stage, auto how) {
+      constexpr int kHow = decltype(how)::value;
       const int qt = stage * kStage, ot = qt + Tile::kBytes;
       const float* stats = reinterpret_cast<const float*>(lds + stage * kStage + 2 * Tile::kBytes) + half * (NB * 32);
       f32x16 s[NB], p[NB];
@@ -656,136 +674,138 @@ struct KeyGradient {
           const float w = exp2_fast(s[b][e] * c);
           s[b][e] = w;
           p[b][e] *= w;
-          if constexpr (kMasked) {
+          if constexpr (kHow != kPlain) {
             const int row = start + step * RT + half * (NB * 32) + 32 * b + 4 * h + result_row(e, 0);
             if (row < from || row >= last_row) s[b][e] = p[b][e] = 0.0f;
           }
         }
       };
-      if constexpr (DK && DV && NB == 2 && !kMasked) {
-        // Operands are read two groups ahead of the products that take them, and the weights
-        // of a block are made beside the products of the other one.
-        constexpr int kGroups = DP / 64;  // of a block's scores
-        constexpr int kAhead = DP == 64 ? KAHEAD64 : 2;
-        bf16x8 f[kAhead + 1][8];
-        const auto read_scores = [&](bf16x8 (&x)[8], int n) {
+      // Operands are read two groups ahead of the products that take them (a block's scores
+      // over 64 columns, the sums over 16 rows), and the weights of a block are made beside
+      // the products of the other one.
+      constexpr int kGroups = DP / 64, kScores = NB * kGroups, kAll = kScores + 2 * NB;
+      constexpr int kAhead = 2, kOf = DK + DV, kMost = kOf * T > 8 ? kOf * T : 8;
+      bf16x8 f[kAhead + 1][kMost];
+      const auto read = [&](int n) {
+        if (n >= kAll) return;
+        bf16x8 (&x)[kMost] = f[n % (kAhead + 1)];
+        if (n < kScores) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             x[2 * j] = at.along(qt, n / kGroups, 4 * (n % kGroups) + j);
-            x[2 * j + 1] = at.along(ot, n / kGroups, 4 * (n % kGroups) + j);
+            if (DK) x[2 * j + 1] = at.along(ot, n / kGroups, 4 * (n % kGroups) + j);
           }
-        };
-        const auto scores = [&](const bf16x8 (&x)[8], int n) {
-          const int b = n / kGroups;
+        } else {
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+            if (DV) x[kOf * t] = at.across(ot, n - kScores, t);
+            if (DK) x[kOf * t + DV] = at.across(qt, n - kScores, t);
+          }
+        }
+      };
+#pragma unroll
+      for (int b = 0; b < NB; ++b) begin(b);
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) read(n);
+      each<kAll>([&](auto number) {
+        constexpr int n = decltype(number)::value;
+        if constexpr (DP > 64) fence();
+        read(n + kAhead);
+        bf16x8 (&x)[kMost] = f[n % (kAhead + 1)];
+        if constexpr (n < kScores) {
+          constexpr int b = n / kGroups;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             s[b] = mfma32(x[2 * j], kf[4 * (n % kGroups) + j], s[b]);
-            p[b] = mfma32(x[2 * j + 1], vf[4 * (n % kGroups) + j], p[b]);
+            if (DK) p[b] = mfma32(x[2 * j + 1], vf[4 * (n % kGroups) + j], p[b]);
           }
-        };
-        const auto read_across = [&](bf16x8 (&x)[8], int n) {
-#pragma unroll
-          for (int t = 0; t < T; ++t) {
-            x[2 * t] = at.across(ot, n, t);
-            x[2 * t + 1] = at.across(qt, n, t);
-          }
-        };
-        const auto add = [&](const bf16x8 (&x)[8], int n) {
-          const bf16x8 w = operand8(s[n >> 1], n & 1), ds = operand8(p[n >> 1], n & 1);
-#pragma unroll
-          for (int t = 0; t < T; ++t) {
-            d_v[t] = mfma32(x[2 * t], w, d_v[t]);
-            d_k[t] = mfma32(x[2 * t + 1], ds, d_k[t]);
-          }
-        };
-        constexpr int kAll = 2 * kGroups + 4;
-        const auto read = [&](int n) { n < 2 * kGroups ? read_scores(f[n % (kAhead + 1)], n) : read_across(f[n % (kAhead + 1)], n - 2 * kGroups); };
-        begin(0);
-        begin(1);
-#pragma unroll
-        for (int n = 0; n < kAhead; ++n) read(n);
-#pragma unroll
-        for (int n = 0; n < kAll; ++n) {
-          fence();
-          if (n + kAhead < kAll) read(n + kAhead);
-          if (n < 2 * kGroups) scores(f[n % (kAhead + 1)], n);
-          else add(f[n % (kAhead + 1)], n - 2 * kGroups);
-          // block 0's weights beside block 1's scores, block 1's beside block 0's sums
-          if (n >= kGroups && n < 2 * kGroups) {
-            weigh(0, kGroups == 2 ? 8 * (n - kGroups) : 0);
-            if (kGroups == 1) weigh(0, 8);
-          }
-          if (n >= 2 * kGroups && n < 2 * kGroups + 2) weigh(1, 8 * (n - 2 * kGroups));
-        }
-        fence();
-        return;
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        begin(b);
-#pragma unroll
-        for (int j = 0; j < DP / 16; ++j) {
-          s[b] = mfma32(at.along(qt, b, j), kf[j], s[b]);
-          if (DK) p[b] = mfma32(at.along(ot, b, j), vf[j], p[b]);
-        }
-        weigh(b, 0);
-        weigh(b, 8);
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const bf16x8 w = operand8(s[b], i), ds = operand8(p[b], i);
+        } else {
+          constexpr int i = n - kScores;
+          const bf16x8 w = operand8(s[i >> 1], i & 1), ds = operand8(p[i >> 1], i & 1);
 #pragma unroll
           for (int t = 0; t < T; ++t) {
             if constexpr (DV) {
-              bf16x8 f = at.across(ot, 2 * b + i, t);
-              if constexpr (kMasked) f = finite_part(f, dirty);
-              d_v[t] = mfma32(f, w, d_v[t]);
+              if constexpr (kHow == kCareful) x[kOf * t] = finite_part(x[kOf * t], dirty);
+              d_v[t] = mfma32(x[kOf * t], w, d_v[t]);
             }
             if constexpr (DK) {
-              bf16x8 f = at.across(qt, 2 * b + i, t);
               // a query that holds an infinity or NaN gives them to the dS of the keys it sees
               uint32_t unused = 0;
-              if constexpr (kMasked) f = finite_part(f, unused);
-              d_k[t] = mfma32(f, ds, d_k[t]);
+              if constexpr (kHow == kCareful) x[kOf * t + DV] = finite_part(x[kOf * t + DV], unused);
+              d_k[t] = mfma32(x[kOf * t + DV], ds, d_k[t]);
             }
           }
         }
+        // block b's weights beside the products behind its scores
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const int from_group = (b + 1) * kGroups - (NB == 1 ? 1 : 0);
+          if (kGroups == 1 && b + 1 < NB) {
+            if (n == from_group) {
+              weigh(b, 0);
+              weigh(b, 8);
+            }
+          } else if (NB == 1) {
+            if (n == from_group) {
+              weigh(b, 0);
+              weigh(b, 8);
+            }
+          } else if (n == from_group || n == from_group + 1) {
+            weigh(b, 8 * (n - from_group));
+          }
+        }
+      });
+      if constexpr (DP > 64) fence();
     };
     const int first_own = start + half * (NB * 32);  // this wavefront's first row
-    const auto masked = [&](int step) {
-      loads_done();
-      if (step + 1 < steps) issue(step + 1);
-      if (first_own + step * RT + NB * 32 > from_some && first_own + step * RT < last_row) compute(step, step & 1, std::true_type{});
-    };
     // turns whose rows all exist and see every key of the wavefront, two at a time
     int lead = from_all > start ? (from_all - start + RT - 1) / RT : 0;
     lead += lead & 1;
-    const int end = (last_row - start) / RT;
-    int step = 0;
-    for (; step < (lead < steps ? lead : steps); ++step) masked(step);
-    for (; step + 2 <= end; step += 2) {
-      loads_done();
-      issue(step + 1);
-      compute(step, std::integral_constant<int, 0>{}, std::false_type{});
-      loads_done();
-      if (step + 2 < steps) issue(step + 2);
-      compute(step + 1, std::integral_constant<int, 1>{}, std::false_type{});
-    }
-    const int tail = start + step * RT;
-    for (; step < steps; ++step) masked(step);
-    if (DV && __any(dirty != 0)) {
-      const auto place = [&](int row) {
-        const int token = group.quotient(row);
-        return a.d_out.p + token * a.d_out.token + (head * a.group + row - token * a.group) * a.d_out.head;
+    lead = lead < steps ? lead : steps;
+    const int end = (last_row - start) / RT, tail = end > lead ? lead + ((end - lead) & ~1) : lead;
+    const auto pass = [&](auto how) {
+#pragma unroll
+      for (int t = 0; t < T; ++t) d_k[t] = d_v[t] = zero16();
+      const auto masked = [&](int step) {
+        loads_done();
+        if (step + 1 < steps) issue(step + 1);
+        if (first_own + step * RT + NB * 32 > from_some && first_own + step * RT < last_row) compute(step, step & 1, how);
       };
-      const auto seen = [&](int row) { return row >= from; };
-      const int until = start + lead * RT < last_row ? start + lead * RT : last_row;
-      add_nonfinite<DP>(d_v, start, until, dim, h, place, seen);
-      add_nonfinite<DP>(d_v, tail > until ? tail : until, last_row, dim, h, place, seen);
+      int step = 0;
+      for (; step < lead; ++step) masked(step);
+      for (; step < tail; step += 2) {
+        loads_done();
+        issue(step + 1);
+        compute(step, Constant<0>{}, Constant<kPlain>{});
+        loads_done();
+        if (step + 2 < steps) issue(step + 2);
+        compute(step + 1, Constant<1>{}, Constant<kPlain>{});
+      }
+      for (; step < steps; ++step) masked(step);
+    };
+    pass(Constant<kMasked>{});
+    if (voted<W>((DK && nonfinite(d_k)) || (DV && nonfinite(d_v)), lds, wave)) {
+      issue(0);
+      pass(Constant<kCareful>{});
+      if (DV && __any(dirty != 0)) {
+        const auto place = [&](int row) {
+          const int token = group.quotient(row);
+          return a.d_out.p + token * a.d_out.token + (head * a.group + row - token * a.group) * a.d_out.head;
+        };
+        const auto seen = [&](int row) { return row >= from; };
+        const int until = start + lead * RT < last_row ? start + lead * RT : last_row;
+        add_nonfinite<DP>(d_v, start, until, dim, h, place, seen);
+        add_nonfinite<DP>(d_v, start + tail * RT > until ? start + tail * RT : until, last_row, dim, h, place, seen);
+      }
     }
 
+    const int64_t o = (static_cast<int64_t>(key) * a.kv_heads + head) * dim;
+    if constexpr (RW == 1) {
+      if (key >= seg.last) return;
+      if (DK) store_operand<DP>(a.d_k + o, d_k, a.scale, dim, h);
+      if (DV) store_operand<DP>(a.d_v + o, d_v, 1.0f, dim, h);
+      return;
+    }
     // Each of two wavefronts finishes half of the columns that both have sums of.
     __syncthreads();
     const auto sums = [&](int of, int n) { return reinterpret_cast<f32x4*>(lds + of * kSums + n * 4096) + 4 * lane; };
@@ -800,14 +820,13 @@ struct KeyGradient {
     if (DV) give(d_v, DK ? T / 2 : 0);
     __syncthreads();
     if (key >= seg.last) return;
-    const int64_t o = (static_cast<int64_t>(key) * a.kv_heads + head) * dim;
     const auto finish = [&](const f32x16 (&x)[T], int slot, float scale, uint16_t* to) {
 #pragma unroll
       for (int t = 0; t < T; ++t)
         if ((t < T / 2) == (half == 0))
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const f32x4 y = sums(wave ^ 2, slot + t % (T / 2))[e];
+            const f32x4 y = sums(wave ^ KW, slot + t % (T / 2))[e];
             const int d = 32 * t + result_row(4 * e, h);
             if (d < dim)
               *reinterpret_cast<u32x2*>(to + o + d) = pack4((x[t][4 * e] + y[0]) * scale, (x[t][4 * e + 1] + y[1]) * scale,
@@ -825,9 +844,9 @@ __global__ __launch_bounds__(F::kThreads, F::DP == 256 ? 1 : 2) void query_gradi
   F::run(a, group, tiles, lds);
 }
 template <class F>
-__global__ __launch_bounds__(F::kThreads, F::DP == 64 ? 2 : 1) void key_gradient_kernel(AttentionArgs a, Divisor group) {
+__global__ __launch_bounds__(F::kThreads, F::DP == 64 ? 2 : 1) void key_gradient_kernel(AttentionArgs a, Divisor group, int tiles) {
   extern __shared__ __align__(1024) uint8_t lds[];
-  F::run(a, group, lds);
+  F::run(a, group, tiles, lds);
 }
 
 template <class F>
@@ -841,9 +860,15 @@ template <class F>
 hipError_t launch_key_gradient(const AttentionArgs& a, hipStream_t st) {
   if (a.keys == 0) return hipSuccess;
   const int64_t tiles = tile_numbers(a.keys, a.offsets != nullptr, a.sequences, F::kKeys);
-  key_gradient_kernel<F><<<static_cast<uint32_t>(tiles * a.kv_heads), F::kThreads, F::kLds, st>>>(a, Divisor(a.group));
+  key_gradient_kernel<F><<<static_cast<uint32_t>(tiles * a.kv_heads), F::kThreads, F::kLds, st>>>(a, Divisor(a.group), static_cast<int>(tiles));
   return hipGetLastError();
 }
+
+// Whether to take 128 keys a workgroup, which load each row half as often as 64: where
+// they are enough for every CU, and twice as many in causal sequences, whose tiles have
+// different amounts of work (8,192 tokens in two sequences, 16 / 4 heads, all seen: 927 us
+// with 128 keys, 1026 with 64; 4,096 causal tokens, 16 / 4 heads of 96: 556 and 401).
+bool wide_key_tiles(const AttentionArgs& a) { return a.keys * a.kv_heads / 128 >= (a.causal ? 512 : 256); }
 
 template <int DP, bool EXACT, int NB>
 hipError_t backward(const AttentionArgs& a, hipStream_t st) {
@@ -854,10 +879,13 @@ hipError_t backward(const AttentionArgs& a, hipStream_t st) {
     e = launch_query_gradient<QueryGradient<DP, EXACT, 4, false>>(a, st);  // for delta
   if (e != hipSuccess) return e;
   // both gradients of 256 columns at once would not leave a lane registers for the scores
-  if (DP < 256 && a.d_k != nullptr && a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, NB, DP < 256, true>>(a, st);
+  if (DP < 256 && a.d_k != nullptr && a.d_v != nullptr) {
+    if (wide_key_tiles(a)) return launch_key_gradient<KeyGradient<DP, EXACT, NB, 1, DP < 256, true>>(a, st);
+    return launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, DP < 256, true>>(a, st);
+  }
   if (a.d_k != nullptr)
-    if (e = launch_key_gradient<KeyGradient<DP, EXACT, NB, true, false>>(a, st); e != hipSuccess) return e;
-  if (a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, NB, false, true>>(a, st);
+    if (e = launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, true, false>>(a, st); e != hipSuccess) return e;
+  if (a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, false, true>>(a, st);
   return hipSuccess;
 }
 

@@ -74,6 +74,10 @@ __device__ __forceinline__ u32x2 pack4(float a, float b, float c, float d) {
   return (u32x2){pack2(a, b), pack2(c, d)};
 }
 
+__device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p));
+}
+
 __device__ __forceinline__ const void* uniform_address(const void* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
@@ -269,36 +273,68 @@ struct Segment {
   int tile;         // which of its tiles
 };
 
-// Tile number t of rows cut into sequences and then into tiles of `size`
-// (offsets and rows are multiplied by `times`).  Sequence i's tiles are numbered from
-// floor(first row / size) + i on, so every tile has a number below rows / size +
-// sequences + 2 and some numbers have no tile (`tile` behind the segment's last
-// row).  Rows before the first and behind the last sequence are segments too.
-__device__ __forceinline__ Segment find_segment(const int32_t* offsets, int sequences, int64_t rows, int times, int size, int t) {
+// Where work starts.  Rows are cut into sequences and these into tiles of `size`
+// (offsets and rows are multiplied by `times`); rows before the first and behind the
+// last sequence are segments too.  `t` counts the workgroups, of which there
+// are rows / size + sequences + 2 for packed rows; some get no tile (`tile` negative or
+// behind the segment's last row).
+//
+// kInOrder, kReversed: the tiles one after the other; segment i's are numbered from
+// floor(first row / size) + i on, so that every one has a number of its own.
+// kLastFirst, kFirstFirst: those with the most tiles of their sequence before (behind) them
+// first, which of a causal sequence's row (key) tiles have the most work, so that
+// the short ones fill the card's last turns.  Costs ~1.5 us a workgroup.
+enum TileOrder { kInOrder, kReversed, kLastFirst, kFirstFirst };
+__device__ __forceinline__ Segment find_segment(const int32_t* offsets, int sequences, int64_t rows, int times, int size, int t,
+                                                int tiles, TileOrder order) {
+  const int lane = threadIdx.x & 63, most = static_cast<int>(rows), segments = sequences + 2;
+  const bool ranked = order >= kLastFirst && offsets != nullptr && sequences > 1 && segments < 64;
+  if (order == kReversed || (order == kLastFirst && !ranked)) t = tiles - 1 - t;
   if (offsets == nullptr) return Segment{0, static_cast<int>(rows * times), 0, t};
-  const int lane = threadIdx.x & 63, most = static_cast<int>(rows);
   // boundary 0 is row 0, boundary i offsets[i - 1], boundary sequences + 2 the end
   const auto boundary = [&](int i) {
     int v = i <= 0 ? 0 : i > sequences + 1 ? most : offsets[i - 1];
     v = v < 0 ? 0 : v > most ? most : v;
     return v * times;
   };
-  int count = 0, mine = 0;
-  for (int i = 0; i < sequences + 2; i += 64) {
-    mine = boundary(i + lane);
-    count += __popcll(__ballot(i + lane < sequences + 2 && mine / size + i + lane <= t));
-  }
-  const int s = __builtin_amdgcn_readfirstlane(count) - 1;  // boundary 0 counts for every t
+  int s, mine = 0;
   Segment g;
-  if (sequences + 2 < 64) {
+  if (ranked) {
+    mine = boundary(lane);
+    const int next = __shfl_down(mine, 1);
+    const int own = lane < segments && next > mine ? (next - mine + size - 1) / size : 0;  // tiles of segment `lane`
+    // tiles with `place` or more before (behind) them; sums below 2^24 are exact
+    const auto from = [&](int place) { return static_cast<int>(wave_sum(static_cast<float>(own > place ? own - place : 0))); };
+    int low = 0, high = tiles;  // from(low) > t, from(high) <= t
+    if (from(0) <= t) return Segment{0, 0, -1, 0};
+    while (high - low > 1) {
+      const int mid = (low + high) >> 1;
+      if (from(mid) > t)
+        low = mid;
+      else
+        high = mid;
+    }
+    const int rank = t - from(low + 1);
+    const uint64_t have = __ballot(own > low);
+    s = __builtin_ctzll(__ballot(own > low && __popcll(have & ((uint64_t{1} << lane) - 1)) == rank));
+    g.tile = order == kLastFirst ? low : __builtin_amdgcn_readlane(own, s) - 1 - low;
+  } else {
+    int count = 0;
+    for (int i = 0; i < segments; i += 64) {
+      mine = boundary(i + lane);
+      count += __popcll(__ballot(i + lane < segments && mine / size + i + lane <= t));
+    }
+    s = __builtin_amdgcn_readfirstlane(count) - 1;  // boundary 0 counts for every t
+  }
+  if (segments < 64) {
     g.first = __builtin_amdgcn_readlane(mine, s);
     g.last = __builtin_amdgcn_readlane(mine, s + 1);
   } else {
     g.first = __builtin_amdgcn_readfirstlane(boundary(s));
     g.last = __builtin_amdgcn_readfirstlane(boundary(s + 1));
   }
+  if (!ranked) g.tile = t - g.first / size - s;
   g.number = s >= 1 && s <= sequences ? s - 1 : -1;
-  g.tile = t - g.first / size - s;
   return g;
 }
 
