@@ -272,7 +272,7 @@ _SIGNATURES = {
     "glm53_packed_attention_backward": (ctypes.c_int, [P, P]),
     "glm53_kv_append": (ctypes.c_int, [P, P, P, I64, P, P, P]),
     "glm53_kv_read": (ctypes.c_int, [P, P, I64, P, P, P]),
-    "glm53_paged_attention_workspace_bytes": (SZ, [I64, I64, I64, I64]),
+    "glm53_paged_attention_workspace_bytes": (SZ, [I64, I32]),
     "glm53_paged_attention": (ctypes.c_int, [P, P, I64, P, F32, P, P, SZ, P]),
     "glm53_synth_fp8": (ctypes.c_int, [P, P, I64, I64, ctypes.c_uint64, F32, P]),
     "glm53_synth_f32": (ctypes.c_int, [P, I64, ctypes.c_uint64, F32, F32, F32, I32, P]),

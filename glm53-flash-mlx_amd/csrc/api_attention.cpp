@@ -179,9 +179,9 @@ int glm53_kv_read(const glm53_kv_cache* cache, const int32_t* offsets, int64_t r
   return GLM53_OK;
 }
 
-size_t glm53_paged_attention_workspace_bytes(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim) {
-  if (sequences <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || head_dim > kMaxHeadDim) return 0;
-  return round_up(decode_space(static_cast<int>(head_dim)));
+size_t glm53_paged_attention_workspace_bytes(int64_t head_dim, int32_t e4m3) {
+  if (head_dim <= 0 || head_dim > kMaxHeadDim) return 0;
+  return round_up(decode_space(static_cast<int>(head_dim), e4m3 != 0));
 }
 
 int glm53_paged_attention(const glm53_kv_cache* cache, const glm53_head_rows* q, int64_t heads, const int32_t* lengths,
@@ -196,7 +196,7 @@ int glm53_paged_attention(const glm53_kv_cache* cache, const glm53_head_rows* q,
   CHECK_ARG(lengths && out, "null pointer argument");
   CHECK_ARG(aligned(out, 16), "out must be 16-byte aligned");
   CHECK_ARG(cache->sequences * heads < kMaxGrid, "sequences times heads reach %lld", (long long)kMaxGrid);
-  const size_t need = glm53_paged_attention_workspace_bytes(cache->sequences, heads, cache->kv_heads, cache->head_dim);
+  const size_t need = glm53_paged_attention_workspace_bytes(cache->head_dim, cache->e4m3);
   CHECK_ARG(workspace && workspace_bytes >= need && aligned(workspace, 256),
             "attention over a cache needs a 256-byte aligned workspace of %zu bytes", need);
   a.lengths = lengths;

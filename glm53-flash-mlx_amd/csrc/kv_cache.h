@@ -43,7 +43,7 @@ struct DecodeArgs {
 
 hipError_t launch_append(const AppendArgs& a, hipStream_t st);
 hipError_t launch_read(const ReadArgs& a, hipStream_t st);
-size_t decode_space(int dim);
+size_t decode_space(int dim, bool e4m3);
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t st);
 
 }  // namespace glm53

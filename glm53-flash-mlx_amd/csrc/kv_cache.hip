@@ -178,21 +178,20 @@ namespace {
 
 // ------------------------------------------------------- one token's attention ---
 //
-// Bound by the cache's bytes.  A wavefront streams TS tokens of keys and values
-// at a time into its own part of LDS by direct loads, the next TS on their way
-// while it multiplies: S^T = k q^T (16 tokens x 16 heads, the heads of one key
-// head beside each other) and out^T += v^T P^T, P straight from the registers
-// that S is in, values read across by the transposing LDS read.  No barrier and
-// no exchange between wavefronts until a sequence ends.
+// Bound by the cache's bytes.  A wavefront, which is a workgroup of its own, streams
+// TS tokens of keys and values at a time into LDS by direct loads, the next TS on
+// their way while it multiplies: S^T = k q^T (16 tokens x 16 heads, the heads
+// of one key head beside each other) and out^T += v^T P^T, P straight from the
+// registers that S is in, values read across by the transposing LDS read.  It
+// meets no barrier.
 //
-// A sequence's positions in chunks of W * TS tokens, one after the other for
-// every sequence and head, are dealt to kWorkers workgroups in equal
-// contiguous runs, whatever the lengths.  A run holds the end of one (sequence,
-// head), whole ones, which it finishes, and the start of another: two partial results
-// at most, joined by a second launch in their order.
+// The positions of every sequence and head, in chunks of TS tokens one after the
+// other, are dealt to the wavefronts in equal contiguous runs, whatever the
+// lengths.  A run holds the end of one (sequence, head), whole ones, which it
+// finishes, and the start of another: two partial results at most, joined by a second
+// launch in their order.  SHARES.
 
-constexpr int kWorkers = 256;  // one workgroup a CU: its stages fill the LDS
-constexpr int kHeads = 16;     // columns of the MFMA
+constexpr int kHeads = 16;  // columns of the MFMA
 
 typedef __attribute__((address_space(3))) uint8_t* lds_bytes;
 
@@ -218,23 +217,59 @@ __device__ __forceinline__ int64_t tokens_of(const DecodeArgs& a, int s, bool& w
   return n < 0 ? 0 : n > most ? most : n;
 }
 
-// Units (chunks of all heads) of the sequences before `before`; a wavefront
-// asks, every lane gets it.
-__device__ __forceinline__ int64_t units_before(const DecodeArgs& a, int before, int chunk, int parts) {
-  int64_t sum = 0;
-  for (int s = threadIdx.x & 63; s < before; s += 64) {
-    bool whole;
-    sum += (tokens_of(a, s, whole) + chunk - 1) / chunk;
-  }
-#pragma unroll
-  for (int w = 32; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
-  return sum * parts;
-}
+// How the work is dealt: units are chunks of all heads' parts of every sequence.
+// Wavefronts ask; 64 sequences' numbers lie in a wavefront's lanes at a time.
+template <int WORKERS, int CHUNK>
+struct Shares {
+  const DecodeArgs& a;
+  const int lane, head_parts, parts;  // groups of 16 heads of a key head, and of all of them
+  int64_t units;                      // of all sequences
+  int block;                          // sequences block .. block + 63 are in the lanes
+  int64_t tokens, before;             // of the lane's sequence, and the units before it
+  bool whole;
 
-__device__ __forceinline__ int64_t run_start(int64_t units, int worker) { return units * worker / kWorkers; }
-// The worker that has unit u.
-__device__ __forceinline__ int run_of(int64_t units, int64_t u) {
-  return static_cast<int>(((u + 1) * kWorkers - 1) / units);
+  __device__ __forceinline__ explicit Shares(const DecodeArgs& a)
+      : a(a), lane(threadIdx.x & 63), head_parts((a.group + kHeads - 1) / kHeads), parts(a.cache.kv_heads * head_parts) {
+    units = 0;
+    for (int s = 0; s < a.cache.sequences; s += 64) units = load(s, units);
+  }
+  __device__ __forceinline__ static int64_t chunks(int64_t tokens) { return (tokens + CHUNK - 1) / CHUNK; }
+  // Takes the 64 sequences from s on, `at` units behind the start; the units behind their end.
+  __device__ __forceinline__ int64_t load(int s, int64_t at) {
+    block = s;
+    tokens = 0;
+    whole = true;
+    if (s + lane < a.cache.sequences) tokens = tokens_of(a, s + lane, whole);
+    const int64_t own = chunks(tokens) * parts;
+    int64_t upto = own;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      const int64_t left = __shfl_up(upto, w);
+      if (lane >= w) upto += left;
+    }
+    before = at + upto - own;
+    return at + __shfl(upto, 63);
+  }
+  // The sequence of unit u.
+  __device__ __forceinline__ int find(int64_t u) {
+    int64_t end = units;
+    if (a.cache.sequences > 64) {
+      end = 0;
+      for (int s = 0; s < a.cache.sequences; s += 64) {
+        end = load(s, end);
+        if (end > u) break;
+      }
+    }
+    // the last one that starts at u or before it, past those without a token
+    return block + 63 - __builtin_clzll(__ballot(before <= u && tokens > 0));
+  }
+  __device__ __forceinline__ int64_t start(int worker) const { return units * worker / WORKERS; }
+  __device__ __forceinline__ int worker(int64_t u) const { return static_cast<int>(((u + 1) * WORKERS - 1) / units); }
+};
+
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
+                              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)));
 }
 
 template <int DP_, bool E4M3_>
@@ -244,14 +279,16 @@ struct Decode {
   static constexpr int kRowBytes = E4M3 ? DP : 2 * DP;
   static constexpr int kPitch = kRowBytes < 128 ? 128 : kRowBytes;
   static constexpr int kSlots = kPitch / 16, kLoadRows = 64 / kSlots;
-  static constexpr int TS = kPitch >= 256 ? 32 : 64;     // tokens of a stage
-  static constexpr int W = kPitch >= 512 ? 2 : 4;        // wavefronts
-  static constexpr int kThreads = 64 * W, kChunk = W * TS, kSub = TS / 16;
+  static constexpr int TS = kPitch >= 256 ? 32 : 64, kSub = TS / 16;  // tokens of a stage, and parts of 16
   static constexpr int kTile = TS * kPitch;
   static constexpr int kStage = 2 * kTile + (E4M3 ? 512 : 0);
-  static constexpr int kLds = 2 * W * kStage;
+  static constexpr int kLds = 2 * kStage;
+  // one a SIMD of 256 CUs where the LDS holds them (a fifth one a CU ends after the others:
+  // 64 x 8192 tokens in bf16 470 us for 381)
+  static constexpr int kWorkers = 256 * (160 * 1024 / kLds < 4 ? 160 * 1024 / kLds : 4);
   static constexpr int kLoads = 2 * (TS / kLoadRows) + (E4M3 ? 2 * kSub : 0);  // of a whole stage
-  static_assert(W * kHeads * (DP + 2) * 4 <= kLds, "the wavefronts' results fit where the stages were");
+  static constexpr int kPartial = kHeads * (DP + 2);  // floats: sums, then maximum and total of each head
+  using Dealt = Shares<kWorkers, TS>;
 
   __device__ static __forceinline__ int swizzle(int row) {
     return kPitch == 128 ? ((row & 2) << 1) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
@@ -259,65 +296,52 @@ struct Decode {
 
   static __device__ void run(const DecodeArgs& a, uint8_t* lds) {
     const CacheArgs& c = a.cache;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, quarter = lane >> 4;
-    const int head_parts = (a.group + kHeads - 1) / kHeads, parts = c.kv_heads * head_parts;
-    const int64_t units = units_before(a, c.sequences, kChunk, parts);
-    if (units == 0) return;
+    const int lane = threadIdx.x, col = lane & 15, quarter = lane >> 4;
+    Dealt shares(a);
     const int worker = blockIdx.x;
-    int64_t unit = run_start(units, worker);
-    const int64_t end = run_start(units, worker + 1);
+    int64_t unit = shares.start(worker);
+    const int64_t end = shares.start(worker + 1);
     if (unit >= end) return;
-    // the sequence of the first unit
-    int sequence = 0;
-    int64_t base = 0;  // units before it
-    for (;; sequence += 64) {
-      int64_t own = 0;
-      if (sequence + lane < c.sequences) {
-        bool whole;
-        own = (tokens_of(a, sequence + lane, whole) + kChunk - 1) / kChunk * parts;
-      }
-      int64_t upto = own;
-#pragma unroll
-      for (int w = 1; w < 64; w <<= 1) {
-        const int64_t left = __shfl_up(upto, w);
-        if (lane >= w) upto += left;
-      }
-      const uint64_t past = __ballot(base + upto > unit);
-      if (past != 0) {
-        const int first = __builtin_ctzll(past);
-        sequence += first;
-        base += __shfl(upto, first) - __shfl(own, first);
-        break;
-      }
-      base += __shfl(upto, 63);
-    }
+    int sequence = __builtin_amdgcn_readfirstlane(shares.find(unit));
 
-    uint8_t* const mine = lds + 2 * wave * kStage;
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_bytes)mine));
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_bytes)lds));
     const float sc = a.scale * 1.44269504088896340736f;
     const int row_bytes = E4M3 ? c.dim : 2 * c.dim;
-    const auto clear = [&] {  // pads, where no load writes
-      if (row_bytes == kPitch) return;
-      for (int i = lane; i < 2 * kStage / 16; i += 64) *reinterpret_cast<u32x4*>(mine + 16 * i) = (u32x4){0, 0, 0, 0};
+    if (row_bytes < kPitch) {  // pads, where no load writes
+      for (int i = lane; i < kLds / 16; i += 64) *reinterpret_cast<u32x4*>(lds + 16 * i) = (u32x4){0, 0, 0, 0};
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    };
-    clear();
+    }
 
     while (unit < end) {
-      sequence = __builtin_amdgcn_readfirstlane(sequence);
-      bool whole;
-      const int64_t tokens = tokens_of(a, sequence, whole), chunks = (tokens + kChunk - 1) / kChunk;
-      if (chunks == 0 || unit >= base + chunks * parts) {
-        base += chunks * parts;
+      if (sequence >= shares.block + 64) shares.load(shares.block + 64, unit);
+      const int at = sequence - shares.block;
+      const int64_t tokens = lane_value(shares.tokens, at), chunks = Dealt::chunks(tokens), base = lane_value(shares.before, at);
+      if (unit >= base + chunks * shares.parts) {
         ++sequence;
         continue;
       }
       const int part = static_cast<int>((unit - base) / chunks);
       const int64_t seg = base + part * chunks;  // its first unit
-      const int head = part / head_parts, first_head = (part - head * head_parts) * kHeads;
-      const int64_t from = unit - seg, to = (end - seg < chunks ? end - seg : chunks);
+      const int head = part / shares.head_parts, first_head = (part - head * shares.head_parts) * kHeads;
+      int64_t stage = unit - seg;
+      const int64_t from = stage, to = end - seg < chunks ? end - seg : chunks;
+      bool bad = !__builtin_amdgcn_readlane(shares.whole, at);
 
+      // The pages of the next 64 16-token parts, one a lane.
+      const int32_t* table = c.table + sequence * c.table_stride;
+      int pages = 0;
+      const auto look_up = [&](int64_t next) {
+        const int64_t first = next * TS + lane * 16;
+        pages = 0;
+        if (first < tokens) {
+          pages = table[first >> c.page_log2];
+          if (pages < 0 || pages >= c.pages) {
+            bad = true;
+            pages = 0;
+          }
+        }
+      };
+      look_up(stage);
       // q of 16 heads as the second operand
       bf16x8 q[DP / 32];
       const int g = first_head + col;
@@ -330,30 +354,11 @@ struct Decode {
         if (g < a.group && d < c.dim) v = *reinterpret_cast<const u32x4*>(qp + d);
         q[j] = __builtin_bit_cast(bf16x8, v);
       }
-#pragma unroll
-      for (int j = 0; j < DP / 32; ++j) arrived(q[j]);
-      bool bad = !whole;
-      const int32_t* table = c.table + sequence * c.table_stride;
-      const int64_t stages = (tokens + TS - 1) / TS, last = stages < to * W ? stages : to * W;
-      int64_t stage = from * W + wave;
+      arrived(pages);
 
-      // The pages of this wavefront's next 64 16-token parts, one a lane.
-      int pages = 0;
-      const auto look_up = [&](int64_t next) {
-        const int64_t first = (next + lane / kSub * W) * TS + lane % kSub * 16;
-        pages = 0;
-        if (first < tokens) {
-          pages = table[first >> c.page_log2];
-          if (pages < 0 || pages >= c.pages) {
-            bad = true;
-            pages = 0;
-          }
-        }
-        arrived(pages);
-      };
       const auto issue = [&](int64_t next, int slot, int ahead) {
         const int64_t first = next * TS;
-        const uint32_t at = lds_at + slot * kStage;
+        const uint32_t to_stage = lds_at + slot * kStage;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read here last
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
@@ -365,7 +370,7 @@ struct Decode {
           for (int i = 0; i < 16 / kLoadRows; ++i) {
             const int row = i * kLoadRows + lane / kSlots, piece = (lane % kSlots) ^ swizzle(row);
             const uint32_t off = row * row_bytes + 16 * piece;
-            const uint32_t to_lds = at + (16 * u + i * kLoadRows) * kPitch;
+            const uint32_t to_lds = to_stage + (16 * u + i * kLoadRows) * kPitch;
             if (16 * piece < row_bytes) {
               load_to_lds(c.k + row0 * row_bytes, off, to_lds);
               load_to_lds(c.v + row0 * row_bytes, off, to_lds + kTile);
@@ -373,20 +378,23 @@ struct Decode {
           }
           if constexpr (E4M3) {
             if (lane < 4) {
-              load_to_lds<4>(c.k_scales + row0, 4 * lane, at + 2 * kTile + 16 * u);
-              load_to_lds<4>(c.v_scales + row0, 4 * lane, at + 2 * kTile + 256 + 16 * u);
+              load_to_lds<4>(c.k_scales + row0, 4 * lane, to_stage + 2 * kTile + 16 * u);
+              load_to_lds<4>(c.v_scales + row0, 4 * lane, to_stage + 2 * kTile + 256 + 16 * u);
             }
           }
         }
       };
 
+      issue(stage, 0, 0);
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) arrived(q[j]);
       float m = -INFINITY, l = 0.0f;
       f32x4 out[DP / 16];
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) out[t] = (f32x4){0, 0, 0, 0};
 
       const auto compute = [&](int64_t stage, int slot) {
-        const uint8_t* kt = mine + slot * kStage;
+        const uint8_t* kt = lds + slot * kStage;
         const uint8_t* vt = kt + kTile;
         const int64_t left64 = tokens - stage * TS;
         const int left = left64 < TS ? static_cast<int>(left64) : TS;
@@ -429,7 +437,7 @@ struct Decode {
           }
           const float top = quarter_max(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                               fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
-          if (__any(top * sc > m * sc + 8.0f)) {  // see the packed form: weights reach 2^8
+          if (__any(top * sc > m * sc + 8.0f)) {  // as over packed sequences: weights reach 2^8
             const float next = fmaxf(m, top), alpha = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - next) * sc);
             m = next;
             l *= alpha;
@@ -463,18 +471,15 @@ struct Decode {
 
       constexpr int kAhead = 64 / kSub;  // stages of a look-up
       int slot = 0, ahead = 0;
-      if (stage < last) {
-        look_up(stage);
-        issue(stage, 0, 0);
-      }
-      for (; stage < last; stage += W, slot ^= 1) {
-        if (stage + W < last) {
+      for (; stage < to; ++stage, slot ^= 1) {
+        if (stage + 1 < to) {
           if (++ahead == kAhead) {
             ahead = 0;
-            look_up(stage + W);
+            look_up(stage + 1);
+            arrived(pages);
           }
-          issue(stage + W, slot ^ 1, ahead);
-          if ((stage + W + 1) * TS <= tokens)
+          issue(stage + 1, slot ^ 1, ahead);
+          if ((stage + 2) * TS <= tokens)
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
           else
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -484,53 +489,28 @@ struct Decode {
         compute(stage, slot);
       }
 
-      // the wavefronts' results, where their stages were
       l = quarter_sum(l);
       if (__any(bad)) l = NAN;
-      __syncthreads();
-      float* const sums = reinterpret_cast<float*>(lds);  // [W][16][DP], then [W][16][2]
-      float* const stats = sums + W * kHeads * DP;
+      if (g < a.group) {
+        if (from == 0 && to == chunks) {
+          const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+          uint16_t* o = a.out + (static_cast<int64_t>(sequence) * c.kv_heads * a.group + head * a.group + g) * c.dim;
 #pragma unroll
-      for (int t = 0; t < DP / 16; ++t)
-        *reinterpret_cast<f32x4*>(sums + (wave * kHeads + col) * DP + 16 * t + 4 * quarter) = out[t];
-      if (quarter == 0) {
-        stats[(wave * kHeads + col) * 2] = m;
-        stats[(wave * kHeads + col) * 2 + 1] = l;
-      }
-      __syncthreads();
-      const bool finished = from == 0 && to == chunks;
-      float* const to_sums = a.partial + static_cast<int64_t>(2 * worker + (from == 0 ? 1 : 0)) * kHeads * (DP + 2);
-      for (int i = threadIdx.x; i < kHeads * DP / 4; i += kThreads) {
-        const int hd = i / (DP / 4), d = 4 * (i % (DP / 4));
-        if (first_head + hd >= a.group || d >= c.dim) continue;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < W; ++w) top = fmaxf(top, stats[(w * kHeads + hd) * 2]);
-        float total = 0.0f;
-        f32x4 sum = {0, 0, 0, 0};
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const float mw = stats[(w * kHeads + hd) * 2];
-          const float by = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - top) * sc);
-          const float lw = stats[(w * kHeads + hd) * 2 + 1];
-          total += lw != lw ? lw : by * lw;
-          const f32x4 x = *reinterpret_cast<const f32x4*>(sums + (w * kHeads + hd) * DP + d);
-          if (by != 0.0f) sum += by * x;
-        }
-        if (finished) {
-          const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-          uint16_t* o = a.out + (static_cast<int64_t>(sequence) * c.kv_heads * a.group + head * a.group + first_head + hd) * c.dim + d;
-          *reinterpret_cast<u32x2*>(o) = pack4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
+          for (int t = 0; t < DP / 16; ++t) {
+            const int d = 16 * t + 4 * quarter;
+            if (d < c.dim)
+              *reinterpret_cast<u32x2*>(o + d) = pack4(out[t][0] * inverse, out[t][1] * inverse, out[t][2] * inverse, out[t][3] * inverse);
+          }
         } else {
-          *reinterpret_cast<f32x4*>(to_sums + hd * DP + d) = sum;
-          if (d == 0) {
-            to_sums[kHeads * DP + 2 * hd] = top;
-            to_sums[kHeads * DP + 2 * hd + 1] = total;
+          float* p = a.partial + static_cast<int64_t>(2 * worker + (from == 0 ? 1 : 0)) * kPartial;
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) *reinterpret_cast<f32x4*>(p + col * DP + 16 * t + 4 * quarter) = out[t];
+          if (quarter == 0) {
+            p[kHeads * DP + 2 * col] = m;
+            p[kHeads * DP + 2 * col + 1] = l;
           }
         }
       }
-      __syncthreads();
-      clear();
       unit = seg + to;
     }
   }
@@ -553,8 +533,7 @@ struct Decode {
       typedef int i32x2 __attribute__((vector_size(8)));
       typedef __attribute__((address_space(3))) i32x2* lds_i32x2;
       const int i = a >> 1, row = 16 * (u + (i >> 2)) + 4 * quarter + (i & 3);
-      const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(
-          vt + row * kPitch + 16 * (t ^ swizzle(row)) + 8 * (a & 1)));
+      const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2)(vt + row * kPitch + 16 * (t ^ swizzle(row)) + 8 * (a & 1)));
       const u32x2 lo = codes_to_bf16(static_cast<uint32_t>(w[0]), 1.0f), hi = codes_to_bf16(static_cast<uint32_t>(w[1]), 1.0f);
       return __builtin_bit_cast(bf16x8, (u32x4){lo[0], lo[1], hi[0], hi[1]});
     }
@@ -562,68 +541,109 @@ struct Decode {
 };
 
 template <class D>
-__global__ __launch_bounds__(D::kThreads) void decode_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(64) void decode_kernel(DecodeArgs a) {
   extern __shared__ __align__(1024) uint8_t lds[];
   D::run(a, lds);
 }
 
-// One (sequence, key head, 16 heads) a workgroup: adds its parts where there
-// are several, and writes 0 where the sequence has no token.
-template <class D>
+// One (sequence, head) and LANES x 4 of its columns a workgroup: adds its parts where
+// there are several, and writes 0 where the sequence has no token.
+template <class D, int LANES>
 __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
-  constexpr int DP = D::DP;
+  constexpr int DP = D::DP, kGroups = 256 / LANES;  // parts at a time
   const CacheArgs& c = a.cache;
-  const int head_parts = (a.group + kHeads - 1) / kHeads, parts = c.kv_heads * head_parts;
-  const int sequence = blockIdx.x / parts, part = blockIdx.x - sequence * parts;
-  const int head = part / head_parts, first_head = (part - head * head_parts) * kHeads;
-  bool whole;
-  const int64_t tokens = tokens_of(a, sequence, whole), chunks = (tokens + D::kChunk - 1) / D::kChunk;
+  typename D::Dealt shares(a);
+  const int heads = c.kv_heads * a.group, sequence = blockIdx.x / heads, query_head = blockIdx.x - sequence * heads;
+  const int head = query_head / a.group, g = query_head - head * a.group, hd = g % kHeads;
+  if (c.sequences > 64) {
+    int64_t at = 0;
+    for (int s = 0; s <= sequence; s += 64) at = shares.load(s, at);
+  }
+  const int own = sequence - shares.block;
+  const int64_t chunks = D::Dealt::chunks(lane_value(shares.tokens, own));
   int first = 0, last = -1;
   if (chunks > 0) {
-    const int64_t units = units_before(a, c.sequences, D::kChunk, parts);
-    const int64_t seg = units_before(a, sequence, D::kChunk, parts) + part * chunks;
-    first = run_of(units, seg);
-    last = run_of(units, seg + chunks - 1);
+    const int64_t seg = lane_value(shares.before, own) + (head * shares.head_parts + g / kHeads) * chunks;
+    first = shares.worker(seg);
+    last = shares.worker(seg + chunks - 1);
     if (first == last) return;
   }
   const float sc = a.scale * 1.44269504088896340736f;
-  for (int i = threadIdx.x; i < kHeads * DP / 4; i += 256) {
-    const int hd = i / (DP / 4), d = 4 * (i % (DP / 4));
-    if (first_head + hd >= a.group || d >= c.dim) continue;
-    float top = -INFINITY, total = whole ? 0.0f : NAN;
-    f32x4 sum = {0, 0, 0, 0};
-    for (int w = first; w <= last; ++w) {
-      const float* p = a.partial + static_cast<int64_t>(2 * w + (w == first ? 1 : 0)) * kHeads * (DP + 2);
-      const float mw = p[kHeads * DP + 2 * hd], lw = p[kHeads * DP + 2 * hd + 1];
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p + hd * DP + d);
-      const float next = fmaxf(top, mw);
-      const float old = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - next) * sc);
-      const float by = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mw - next) * sc);
-      total = (total != total ? total : old * total) + (lw != lw ? lw : by * lw);
-      if (old != 0.0f) sum *= old; else sum = (f32x4){0, 0, 0, 0};
-      if (by != 0.0f) sum += by * x;
-      top = next;
+  const int d = 4 * (threadIdx.x % LANES + LANES * blockIdx.y), group = threadIdx.x / LANES;
+  float top = -INFINITY, total = 0.0f;
+  f32x4 sum = {0, 0, 0, 0};
+  // Adds a part to another one, both with sums relative to their own maximum.
+  const auto add = [&](float m, float l, f32x4 x) {
+    const float next = fmaxf(top, m);
+    const float old = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((top - next) * sc);
+    const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - next) * sc);
+    total = (total != total ? total : old * total) + (l != l ? l : by * l);
+    sum = (old == 0.0f ? (f32x4){0, 0, 0, 0} : old * sum) + (by == 0.0f ? (f32x4){0, 0, 0, 0} : by * x);
+    top = next;
+  };
+  constexpr int kAtOnce = 4;
+  for (int w0 = first + group; w0 <= last; w0 += kAtOnce * kGroups) {
+    float m[kAtOnce], l[kAtOnce];
+    f32x4 x[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int w = w0 + i * kGroups;
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+      x[i] = (f32x4){0, 0, 0, 0};
+      // where there are fewer units than workers, some of these have none
+      if (w > last || shares.start(w) >= shares.start(w + 1)) continue;
+      const float* p = a.partial + static_cast<int64_t>(2 * w + (w == first ? 1 : 0)) * D::kPartial;
+      m[i] = p[kHeads * DP + 2 * hd];
+      l[i] = p[kHeads * DP + 2 * hd + 1];
+      if (d < c.dim) x[i] = *reinterpret_cast<const f32x4*>(p + hd * DP + d);
     }
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-    uint16_t* o = a.out + (static_cast<int64_t>(sequence) * c.kv_heads * a.group + head * a.group + first_head + hd) * c.dim + d;
-    *reinterpret_cast<u32x2*>(o) = pack4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) add(m[i], l[i], x[i]);
   }
+  __shared__ f32x4 sums[256];
+  __shared__ float stats[256][2];
+#pragma unroll
+  for (int step = kGroups / 2; step > 0; step >>= 1) {
+    if (group >= step && group < 2 * step) {
+      sums[threadIdx.x] = sum;
+      stats[threadIdx.x][0] = top;
+      stats[threadIdx.x][1] = total;
+    }
+    __syncthreads();
+    if (group < step) {
+      const int other = threadIdx.x + step * LANES;
+      add(stats[other][0], stats[other][1], sums[other]);
+    }
+  }
+  if (group != 0 || d >= c.dim) return;
+  if (!__builtin_amdgcn_readlane(shares.whole, own)) total = NAN;
+  const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+  uint16_t* o = a.out + (static_cast<int64_t>(sequence) * heads + query_head) * c.dim + d;
+  *reinterpret_cast<u32x2*>(o) = pack4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
 }
 
 template <class D>
 hipError_t decode(const DecodeArgs& a, hipStream_t st) {
-  decode_kernel<D><<<kWorkers, D::kThreads, D::kLds, st>>>(a);
+  decode_kernel<D><<<D::kWorkers, 64, D::kLds, st>>>(a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  const int64_t grid = static_cast<int64_t>(a.cache.sequences) * a.cache.kv_heads * ((a.group + kHeads - 1) / kHeads);
-  decode_join_kernel<D><<<static_cast<uint32_t>(grid), 256, 0, st>>>(a);
+  // A few heads may each have hundreds of parts: 16 columns a workgroup then.
+  const uint32_t rows = static_cast<uint32_t>(static_cast<int64_t>(a.cache.sequences) * a.cache.kv_heads * a.group);
+  if (rows <= 256)
+    decode_join_kernel<D, 4><<<dim3(rows, D::DP / 16), 256, 0, st>>>(a);
+  else
+    decode_join_kernel<D, D::DP / 4><<<rows, 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
-int padded(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-
 }  // namespace
 
-size_t decode_space(int dim) { return sizeof(float) * 2 * kWorkers * kHeads * (padded(dim) + 2); }
+size_t decode_space(int dim, bool e4m3) {
+  const auto of = [](auto d) { return sizeof(float) * 2 * decltype(d)::kWorkers * decltype(d)::kPartial; };
+  if (dim <= 64) return e4m3 ? of(Decode<64, true>{}) : of(Decode<64, false>{});
+  if (dim <= 128) return e4m3 ? of(Decode<128, true>{}) : of(Decode<128, false>{});
+  return e4m3 ? of(Decode<256, true>{}) : of(Decode<256, false>{});
+}
 
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t st) {
   if (a.cache.e4m3) {

@@ -183,7 +183,7 @@ def native_paged_attention(q, k_pages, v_pages, page_table, lengths, k_scales, v
     sequences, heads, dim = q.shape
     if sequences:
         lib = N.lib()
-        ws_bytes = lib.glm53_paged_attention_workspace_bytes(sequences, heads, k_pages.shape[1], dim)
+        ws_bytes = lib.glm53_paged_attention_workspace_bytes(dim, k_scales is not None)
         ws = N.workspace(ws_bytes, q.device)
         N.run(q.get_device(), lib.glm53_paged_attention, ctypes.byref(cache), ctypes.byref(q_rows), heads, p_lengths, scale,
               out.data_ptr(), ws.data_ptr(), ws_bytes)

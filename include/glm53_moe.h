@@ -735,7 +735,7 @@ int glm53_kv_read(const glm53_kv_cache* cache, const int32_t* offsets, int64_t r
  * NaN.  The work is split evenly over the card whatever the lengths; parts
  * are joined in their order.  Workspace (256-byte aligned) needs no
  * initialisation. */
-size_t glm53_paged_attention_workspace_bytes(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim);
+size_t glm53_paged_attention_workspace_bytes(int64_t head_dim, int32_t e4m3);
 int glm53_paged_attention(const glm53_kv_cache* cache, const glm53_head_rows* q, int64_t heads, const int32_t* lengths,
                           float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
