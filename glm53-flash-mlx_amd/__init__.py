@@ -58,6 +58,7 @@ from .ownership import (
 )
 from .packed import BankHandle, DecodePlan, PackedFP8ExpertBank, PackedFP8MoE, RoutedDiagnostic
 from .router import Float32Gate
+from .self_attention import AttentionBatch, KVCache, SelfAttention
 
 __all__ = [
     "CheckpointError",
@@ -72,4 +73,5 @@ __all__ = [
     "TensorOwnershipError", "borrowed_ephemeral_tensor", "borrowed_stable_tensor", "materialize_owned",
     "owned_tensor", "require_resident", "resident_concatenate", "rms_norm", "residual_norm", "gated_mlp", "GatedMLP",
     "int4_linear", "quantize_int4", "Int4Linear", "Int4MLP", "FeedForwardBlock", "run_blocks",
+    "packed_attention", "paged_attention", "append_kv", "read_kv", "AttentionBatch", "KVCache", "SelfAttention",
 ]

@@ -48,8 +48,7 @@ int attention_args(const glm53_attention* d, bool backward, AttentionArgs& a) {
   CHECK_ARG(d->offsets != nullptr || d->key_offsets == nullptr, "key_offsets without offsets");
   CHECK_ARG(d->offsets == nullptr || (d->sequences > 0 && d->sequences < kMaxSequences), "sequences must be 1 to 2^24 - 1, got %lld",
             (long long)d->sequences);
-  CHECK_ARG(d->offsets == nullptr || d->key_offsets != nullptr || d->tokens == d->keys,
-            "keys of another number than the queries need key_offsets");
+  CHECK_ARG(d->key_offsets != nullptr || d->tokens == d->keys, "keys of another number than the queries need key_offsets");
   const int64_t sequences = d->offsets != nullptr ? d->sequences : 1;
   CHECK_ARG((d->tokens * d->heads / d->kv_heads / 64 + sequences + 2) * d->kv_heads < kMaxGrid &&
                 (d->keys / 64 + sequences + 2) * d->kv_heads < kMaxGrid,

@@ -255,8 +255,9 @@ struct Forward {
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, s[1][e]);
       top = both_max(top);
-      if (__any(top * c > m * c + kSlack)) {
-        const float next = fmaxf(m, top);
+      const bool grows = top * c > m * c + kSlack;
+      if (__any(grows)) {
+        const float next = grows ? top : m;  // each row by itself: its bits are not its neighbours' matter
         const float alpha = next == -INFINITY ? 1.0f : exp2_fast((m - next) * c);
         m = next;
         l *= alpha;
@@ -530,7 +531,7 @@ struct QueryGradient {
     sum = both_sum(sum);
     if (row >= seg.last) return;
     if (h == 0) {  // where the second kernel's products start
-      a.starts[stat] = -lse / c;
+      a.starts[stat] = lse * (-1.0f / c);
       a.starts[stat + heads * a.tokens] = -(delta + sum);
     }
     if constexpr (DQ) store_operand<DP>(a.d_q + own, d_q, a.scale, dim, h);
@@ -662,7 +663,7 @@ struct KeyGradient {
           const f32x4 d = *reinterpret_cast<const f32x4*>(stats + (DK ? kStats / 4 : 0) + 32 * b + result_row(e, h));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[b][e + i] = DK ? l[i] : l[i] * start_scale;
+            s[b][e + i] = DK ? l[i] : l[i] * start_scale;  // as the first kernel has it
             p[b][e + i] = d[i];
           }
         }

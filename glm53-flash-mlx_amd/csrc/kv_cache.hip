@@ -437,8 +437,9 @@ struct Decode {
           }
           const float top = quarter_max(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                               fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
-          if (__any(top * sc > m * sc + 8.0f)) {  // as over packed sequences: weights reach 2^8
-            const float next = fmaxf(m, top), alpha = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - next) * sc);
+          const bool grows = top * sc > m * sc + 8.0f;  // as over packed sequences: weights reach 2^8
+          if (__any(grows)) {
+            const float next = grows ? top : m, alpha = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - next) * sc);
             m = next;
             l *= alpha;
 #pragma unroll

@@ -668,8 +668,9 @@ typedef struct glm53_head_rows {
 /*   S = scale q k^T over the keys that a query sees, P = softmax(S), out = P v
  * Sequence s has queries offsets[s] .. offsets[s + 1] - 1 of `tokens` and keys
  * key_offsets[s] .. key_offsets[s + 1] - 1 of `keys` (int32 [sequences + 1],
- * ascending; key_offsets NULL: offsets; offsets NULL: one sequence of all, key_offsets
- * NULL too).  causal: query i of n sees keys 0 .. i + (the sequence's keys) -
+ * ascending; key_offsets NULL: offsets, and keys = tokens; offsets NULL: one
+ * sequence of all, key_offsets NULL too).  Offsets out of range are taken as the
+ * nearest one in it; results of sequences whose offsets descend mean nothing.  causal: query i of n sees keys 0 .. i + (the sequence's keys) -
  * n, so that the last query sees them all.  A query that sees no key, and rows of
  * no sequence, are 0.  Query head h reads key head h / (heads / kv_heads).
  * head_dim a multiple of 8 up to 256; tokens * heads and keys * heads below 2^30.
@@ -703,8 +704,8 @@ int glm53_packed_attention_backward(const glm53_attention* attention, void* stre
 
 /* A cache of keys and values: `pages` pages of page_size tokens (a power of two
  * from 16 to 2^16), row (page, head, token) of head_dim values, contiguous and
- * 16-byte aligned.  BF16 as they were given, or (e4m3) E4M3 codes and the byte
- * 127 + e of each row, [pages, kv_heads, page_size]: values code * 2^e, e the
+ * 16-byte aligned.  BF16 as they were given, or (e4m3, head_dim a multiple of
+ * 16) E4M3 codes and the byte 127 + e of each row, [pages, kv_heads, page_size]: values code * 2^e, e the
  * smallest with |x| <= 448 * 2^e for the row's finite x, -117 or more.  An
  * infinity or NaN is stored as NaN.  Every stored value is a BF16 value.
  * Token `position` of sequence s lies in page_table[s, position / page_size]
@@ -735,7 +736,7 @@ int glm53_kv_read(const glm53_kv_cache* cache, const int32_t* offsets, int64_t r
  * NaN.  The work is split evenly over the card whatever the lengths; parts
  * are joined in their order.  Workspace (256-byte aligned) needs no
  * initialisation. */
-size_t glm53_paged_attention_workspace_bytes(int64_t head_dim, int32_t e4m3);
+size_t glm53_paged_attention_workspace_bytes(int64_t head_dim, int32_t e4m3); /* whatever the sequences and heads */
 int glm53_paged_attention(const glm53_kv_cache* cache, const glm53_head_rows* q, int64_t heads, const int32_t* lengths,
                           float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
