@@ -86,6 +86,11 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       for (int s = LANES / 2; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, LANES));
       const int e = row_exponent(top);
       const float by = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      if (e == 120) {  // the next code after 240 is 2^128, no bf16 number
+        const float most = 240.0f / by;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = f[j] > most ? most : f[j] < -most ? -most : f[j];
+      }
       u32x2 codes = {0, 0};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {

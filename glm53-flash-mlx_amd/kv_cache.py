@@ -10,7 +10,8 @@ page_size].  Rows are bfloat16, or E4M3 codes (uint8) with one power of two a ro
 
 E4M3 has an exponent of its own, so a row's power of two only has to bring it
 into range; it costs no precision that a finer scale would keep, and every
-value that a cache holds is a bfloat16 value: reading back is exact.  An
+value that a cache holds is a bfloat16 value (the largest bfloat16 numbers, which
+a code would round to 2^128, are stored as 240 * 2^120): reading back is exact.  An
 infinity or NaN is stored as NaN.  Half the bytes of a bfloat16 cache, and a
 token's attention over a cache takes the time of its bytes.
 

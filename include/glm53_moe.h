@@ -706,8 +706,8 @@ int glm53_packed_attention_backward(const glm53_attention* attention, void* stre
  * from 16 to 2^16), row (page, head, token) of head_dim values, contiguous and
  * 16-byte aligned.  BF16 as they were given, or (e4m3, head_dim a multiple of
  * 16) E4M3 codes and the byte 127 + e of each row, [pages, kv_heads, page_size]: values code * 2^e, e the
- * smallest with |x| <= 448 * 2^e for the row's finite x, -117 or more.  An
- * infinity or NaN is stored as NaN.  Every stored value is a BF16 value.
+ * smallest with |x| <= 448 * 2^e for the row's finite x, -117 or more (at e =
+ * 120 codes end at 240: 256 * 2^120 is no BF16 number).  An infinity or NaN is stored as NaN.  Every stored value is a BF16 value.
  * Token `position` of sequence s lies in page_table[s, position / page_size]
  * (int32 [sequences, table_stride], of which max_pages are a sequence's). */
 typedef struct glm53_kv_cache {

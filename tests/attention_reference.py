@@ -88,6 +88,13 @@ def check(got, want, what=""):
     assert bool((over <= 0).all()), f"{what}: off by {float(off.max())}, {float((off / bound.clamp(min=1e-300)).max())} of the bound"
 
 
+def power(e):
+    """2^e in 64 bits by its exponent's bits: a power function's may be off by one step."""
+    import torch
+
+    return (e.long() + 1023 << 52).view(torch.float64)
+
+
 def stored(x, quantised):
     """What a cache holds of rows x [..., dim]: in 64 bits, finite x."""
     import torch
@@ -95,8 +102,9 @@ def stored(x, quantised):
     x = x.double()
     if not quantised:
         return x
-    part, power = torch.frexp(x.abs().amax(-1, keepdim=True))  # top = part * 2^power, part in [0.5, 1)
-    e = (power - 9 + (part > 0.875)).clamp(min=-117).masked_fill(part == 0, -117)
-    y = torch.ldexp(x, -e.double())
-    spacing = torch.ldexp(torch.ones_like(y), torch.frexp(y.abs().clamp(min=2.0**-6))[1].double() - 4)
-    return torch.ldexp(torch.round(y / spacing) * spacing, e.double())
+    part, exponent = torch.frexp(x.abs().amax(-1, keepdim=True))  # top = part * 2^exponent, part in [0.5, 1)
+    e = (exponent - 9 + (part > 0.875)).clamp(min=-117).masked_fill(part == 0, -117)
+    y = x * power(-e)
+    y = torch.where(e == 120, y.clamp(-240, 240), y)  # the next code would be 2^128
+    spacing = power(torch.frexp(y.abs().clamp(min=2.0**-6))[1] - 4)
+    return torch.round(y / spacing) * spacing * power(e)
