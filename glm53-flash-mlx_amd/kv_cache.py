@@ -178,7 +178,7 @@ def native_read_kv(k_pages, v_pages, page_table, offsets, rows: int, k_scales, v
 def native_paged_attention(q, k_pages, v_pages, page_table, lengths, k_scales, v_scales, scale: float):
     """The native call behind glm53::paged_attention."""
     cache, table = _descriptor(k_pages, v_pages, page_table, k_scales, v_scales)
-    out = q.new_empty(q.shape)
+    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     q, q_rows = head_rows(q)
     lengths, p_lengths = index_pointer(lengths)
     sequences, heads, dim = q.shape

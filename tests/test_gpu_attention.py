@@ -231,6 +231,22 @@ def test_single_gradients_are_the_joint_ones(dev):
             assert g is None or torch.equal(g, want[name]), (wanted, name)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_gradients_of_short_sequences(dev, dim):
+    """Rows of few keys have large results, whose rounding shifts a whole row's dS:
+    d_q must be off by its own rounding alone.  That is at most half a step, 2^-8 of a
+    step's lowest value, equally likely anywhere, so 2^-7 / sqrt(12) of the root mean
+    square at most; and 5% for everything in FP32 and dS's two parts (2^-17)."""
+    import torch
+
+    lengths = torch.randint(8, 101, (30,), generator=torch.Generator().manual_seed(3)).tolist()
+    offsets = offsets_of(lengths)
+    q, k, v, d_out = inputs(dev, offsets[-1], offsets[-1], 8, 2, dim)
+    got = gradients(q, k, v, d_out, index(offsets, dev))["d_q"].double()
+    want = attention64(q, k, v, offsets, offsets, True, None, d_out)["d_q"][0]
+    assert float((got - want).norm() / want.norm()) <= 1.05 * 2.0**-7 / 12**0.5
+
+
 def test_gradients_against_differences(dev):
     """The slope of a weighted sum of results along random directions: bf16
     results differ by steps, so the difference is taken of the 64-bit formula,
