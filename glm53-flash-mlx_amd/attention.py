@@ -22,6 +22,8 @@ from . import ops as _ops
 
 MAX_HEAD_DIM = 256
 MAX_STRIDE = 1 << 22  # elements from one token, or one head, to the next
+MAX_HEAD_SPAN = 1 << 30  # of a token's heads together
+MIN_SCALE = 2.0**-64
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor | None = None,
@@ -35,7 +37,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     key_offsets: the same for keys, where they are not the queries' own (a
     chunk of a prompt over all of its keys).  causal: the last query of a sequence
     sees all of its keys, each one before it one key less.  Queries that see no key,
-    and rows of no sequence, are 0.  scale: 1 / sqrt(dim) where None, positive.
+    and rows of no sequence, are 0.  scale: 1 / sqrt(dim) where None, 2^-64 or more.
 
     heads a multiple of kv_heads, dim a multiple of 8 up to 256.  q, k and v
     may be views of one tensor (a joint projection's) without a copy.
@@ -84,8 +86,8 @@ def check_offsets(name: str, t: torch.Tensor | None) -> None:
 
 def check_scale(scale: float | None, dim: int) -> float:
     scale = dim**-0.5 if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not MIN_SCALE <= scale < math.inf:
+        raise ValueError(f"scale must be finite and 2^-64 or more, got {scale}")
     return scale
 
 
@@ -98,7 +100,7 @@ def head_rows(t: torch.Tensor) -> tuple[torch.Tensor, N.HeadRows]:
         row = 0
     if heads == 1:
         head = 0
-    if one != 1 or (row | head) & 7 or max(row, head) > MAX_STRIDE or t.data_ptr() & 15:
+    if one != 1 or (row | head) & 7 or max(row, head) > MAX_STRIDE or heads * head > MAX_HEAD_SPAN or t.data_ptr() & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         row, head = heads * dim, dim
     return t, N.HeadRows(t.data_ptr(), row, head)

@@ -14,13 +14,18 @@ namespace {
 constexpr int64_t kMaxRows = int64_t{1} << 30;
 constexpr int64_t kMaxSequences = int64_t{1} << 24;
 constexpr int64_t kMaxGrid = int64_t{1} << 23;  // workgroups of up to 512 threads: a grid has fewer than 2^32
+constexpr int64_t kMaxCopied = 4 * kMaxGrid;    // rows, four a workgroup, that one call writes to or reads from a cache
+// The rows' logarithms over this are where the gradients' products start: still finite.
+constexpr float kLeastScale = 0x1p-64f;
 
-int head_rows(const glm53_head_rows& r, const char* name, bool wanted, Rows16& out) {
+int head_rows(const glm53_head_rows& r, int64_t heads, const char* name, bool wanted, Rows16& out) {
   CHECK_ARG(!wanted || r.data != nullptr, "null pointer argument: %s", name);
   CHECK_ARG(aligned(r.data, 16), "%s must be 16-byte aligned", name);
   for (const int64_t stride : {r.token_stride, r.head_stride})
     CHECK_ARG(stride >= 0 && stride <= kMaxRowStride && stride % 8 == 0, "%s: stride %lld is no multiple of 8 up to %lld",
               name, (long long)stride, (long long)kMaxRowStride);
+  CHECK_ARG(heads * r.head_stride <= kMaxHeadSpan, "%s: %lld heads at a stride of %lld lie more than %lld elements apart", name,
+            (long long)heads, (long long)r.head_stride, (long long)kMaxHeadSpan);
   out = Rows16{static_cast<const uint16_t*>(r.data), r.token_stride, r.head_stride};
   return GLM53_OK;
 }
@@ -35,7 +40,7 @@ int head_shape(int64_t heads, int64_t kv_heads, int64_t dim) {
 }
 
 int check_scale(float scale) {
-  CHECK_ARG(scale > 0.0f && std::isfinite(scale), "scale must be positive and finite");
+  CHECK_ARG(scale >= kLeastScale && std::isfinite(scale), "scale must be finite and 2^-64 or more");
   return GLM53_OK;
 }
 
@@ -54,9 +59,9 @@ int attention_args(const glm53_attention* d, bool backward, AttentionArgs& a) {
                 (d->keys / 64 + sequences + 2) * d->kv_heads < kMaxGrid,
             "too many tiles for a grid");
   a = AttentionArgs{};
-  if (int rc = head_rows(d->q, "q", d->tokens > 0, a.q)) return rc;
-  if (int rc = head_rows(d->k, "k", d->keys > 0, a.k)) return rc;
-  if (int rc = head_rows(d->v, "v", d->keys > 0, a.v)) return rc;
+  if (int rc = head_rows(d->q, d->heads, "q", d->tokens > 0, a.q)) return rc;
+  if (int rc = head_rows(d->k, d->kv_heads, "k", d->keys > 0, a.k)) return rc;
+  if (int rc = head_rows(d->v, d->kv_heads, "v", d->keys > 0, a.v)) return rc;
   a.offsets = d->offsets;
   a.key_offsets = d->key_offsets;
   a.tokens = d->tokens;
@@ -72,7 +77,7 @@ int attention_args(const glm53_attention* d, bool backward, AttentionArgs& a) {
   CHECK_ARG(d->tokens == 0 || d->out != nullptr, "null pointer argument: out");
   CHECK_ARG(aligned(d->out, 16), "out must be 16-byte aligned");
   if (!backward) return GLM53_OK;
-  if (int rc = head_rows(d->d_out, "d_out", d->tokens > 0, a.d_out)) return rc;
+  if (int rc = head_rows(d->d_out, d->heads, "d_out", d->tokens > 0, a.d_out)) return rc;
   CHECK_ARG(d->tokens == 0 || d->lse != nullptr, "null pointer argument: lse");
   a.d_q = static_cast<uint16_t*>(d->d_q);
   a.d_k = static_cast<uint16_t*>(d->d_k);
@@ -149,11 +154,11 @@ int glm53_kv_append(const glm53_kv_cache* cache, const glm53_head_rows* k, const
   AppendArgs a{};
   if (int rc = cache_args(cache, a.cache)) return rc;
   CHECK_ARG(k != nullptr && v != nullptr, "null pointer argument: rows");
-  CHECK_ARG(tokens >= 0 && tokens < kMaxRows, "invalid number of tokens %lld", (long long)tokens);
+  CHECK_ARG(tokens >= 0 && tokens < kMaxCopied, "invalid number of tokens %lld", (long long)tokens);
   CHECK_ARG(offsets != nullptr || tokens == cache->sequences, "one token a sequence is %lld tokens, got %lld",
             (long long)cache->sequences, (long long)tokens);
-  if (int rc = head_rows(*k, "k", tokens > 0, a.rows_k)) return rc;
-  if (int rc = head_rows(*v, "v", tokens > 0, a.rows_v)) return rc;
+  if (int rc = head_rows(*k, cache->kv_heads, "k", tokens > 0, a.rows_k)) return rc;
+  if (int rc = head_rows(*v, cache->kv_heads, "v", tokens > 0, a.rows_v)) return rc;
   if (tokens == 0 || cache->sequences == 0) return GLM53_OK;
   CHECK_ARG(lengths != nullptr, "null pointer argument: lengths");
   a.tokens = tokens;
@@ -166,7 +171,7 @@ int glm53_kv_append(const glm53_kv_cache* cache, const glm53_head_rows* k, const
 int glm53_kv_read(const glm53_kv_cache* cache, const int32_t* offsets, int64_t rows, void* k, void* v, void* stream) {
   ReadArgs a{};
   if (int rc = cache_args(cache, a.cache)) return rc;
-  CHECK_ARG(rows >= 0 && rows < kMaxRows, "invalid number of rows %lld", (long long)rows);
+  CHECK_ARG(rows >= 0 && rows < kMaxCopied, "invalid number of rows %lld", (long long)rows);
   CHECK_ARG(aligned(k, 16) && aligned(v, 16), "k and v must be 16-byte aligned");
   if (rows == 0 || (k == nullptr && v == nullptr)) return GLM53_OK;
   CHECK_ARG(offsets != nullptr, "null pointer argument: offsets");
@@ -190,7 +195,7 @@ int glm53_paged_attention(const glm53_kv_cache* cache, const glm53_head_rows* q,
   if (int rc = head_shape(heads, cache->kv_heads, cache->head_dim)) return rc;
   if (int rc = check_scale(scale)) return rc;
   CHECK_ARG(q != nullptr, "null pointer argument: q");
-  if (int rc = head_rows(*q, "q", cache->sequences > 0, a.q)) return rc;
+  if (int rc = head_rows(*q, heads, "q", cache->sequences > 0, a.q)) return rc;
   if (cache->sequences == 0) return GLM53_OK;
   CHECK_ARG(lengths && out, "null pointer argument");
   CHECK_ARG(aligned(out, 16), "out must be 16-byte aligned");

@@ -11,6 +11,7 @@ constexpr int64_t kMaxHeadDim = 256;
 // Elements from one token, or one head, to the next: a tile's rows lie within
 // 32-bit byte offsets of its first one.
 constexpr int64_t kMaxRowStride = int64_t{1} << 22;
+constexpr int64_t kMaxHeadSpan = int64_t{1} << 30;  // a token's heads, together
 
 // Rows of one head each: element d of head h of token t at p + t * token + h * head + d.
 struct Rows16 {

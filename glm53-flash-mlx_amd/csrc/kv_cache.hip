@@ -198,8 +198,6 @@ namespace {
 
 constexpr int kHeads = 16;  // columns of the MFMA
 
-typedef __attribute__((address_space(3))) uint8_t* lds_bytes;
-
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -309,7 +307,7 @@ struct Decode {
     if (unit >= end) return;
     int sequence = __builtin_amdgcn_readfirstlane(shares.find(unit));
 
-    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_bytes)lds));
+    const uint32_t lds_at = lds_address(lds);
     const float sc = a.scale * 1.44269504088896340736f;
     const int row_bytes = E4M3 ? c.dim : 2 * c.dim;
     if (row_bytes < kPitch) {  // pads, where no load writes

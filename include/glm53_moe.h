@@ -660,7 +660,7 @@ int glm53_int4_linear(const glm53_int4_weight* weight, const void* x, int64_t ro
  * ---------------------------------------------------------------------- */
 /* Rows of one head each in BF16: element d of head h of token t at data + t *
  * token_stride + h * head_stride + d.  16-byte aligned, strides multiples of 8
- * elements up to 2^22. */
+ * elements up to 2^22, heads * head_stride up to 2^30. */
 typedef struct glm53_head_rows {
   const void* data;
   int64_t token_stride, head_stride;
@@ -670,9 +670,9 @@ typedef struct glm53_head_rows {
  * key_offsets[s] .. key_offsets[s + 1] - 1 of `keys` (int32 [sequences + 1],
  * ascending; key_offsets NULL: offsets, and keys = tokens; offsets NULL: one
  * sequence of all, key_offsets NULL too).  Offsets out of range are taken as the
- * nearest one in it; results of sequences whose offsets descend mean nothing.  causal: query i of n sees keys 0 .. i + (the sequence's keys) -
- * n, so that the last query sees them all.  A query that sees no key, and rows of
- * no sequence, are 0.  Query head h reads key head h / (heads / kv_heads).
+ * nearest one in it; results of sequences whose offsets descend mean nothing.
+ * causal: query i of n sees keys 0 .. i + (the sequence's keys) - n, so that the
+ * last query sees them all.  A query that sees no key, and rows of no sequence, are 0.  Query head h reads key head h / (heads / kv_heads).
  * head_dim a multiple of 8 up to 256; tokens * heads and keys * heads below 2^30.
  * Scores, softmax and sums are FP32; P is rounded to BF16 as an operand, out once. */
 typedef struct glm53_attention {
@@ -692,7 +692,7 @@ typedef struct glm53_attention {
   void* workspace; /* 256-byte aligned, needs no initialisation */
   size_t workspace_bytes;
   int32_t causal;
-  float scale; /* above 0 */
+  float scale; /* 2^-64 or more */
 } glm53_attention;
 int glm53_packed_attention(const glm53_attention* attention, void* stream);
 /* delta = sum(d_out out), dP = d_out v^T, dS = P (dP - delta); d_q = scale dS
@@ -705,9 +705,10 @@ int glm53_packed_attention_backward(const glm53_attention* attention, void* stre
 /* A cache of keys and values: `pages` pages of page_size tokens (a power of two
  * from 16 to 2^16), row (page, head, token) of head_dim values, contiguous and
  * 16-byte aligned.  BF16 as they were given, or (e4m3, head_dim a multiple of
- * 16) E4M3 codes and the byte 127 + e of each row, [pages, kv_heads, page_size]: values code * 2^e, e the
- * smallest with |x| <= 448 * 2^e for the row's finite x, -117 or more (at e =
- * 120 codes end at 240: 256 * 2^120 is no BF16 number).  An infinity or NaN is stored as NaN.  Every stored value is a BF16 value.
+ * 16) E4M3 codes and the byte 127 + e of each row, [pages, kv_heads,
+ * page_size]: values code * 2^e, e the smallest with |x| <= 448 * 2^e for the row's
+ * finite x, -117 or more (at e = 120 codes end at 240: 256 * 2^120 is no BF16
+ * number).  An infinity or NaN is stored as NaN.  Every stored value is a BF16 value.
  * Token `position` of sequence s lies in page_table[s, position / page_size]
  * (int32 [sequences, table_stride], of which max_pages are a sequence's). */
 typedef struct glm53_kv_cache {
@@ -723,7 +724,8 @@ typedef struct glm53_kv_cache {
 /* Writes `tokens` new rows of each head: sequence s's, offsets[s] ..
  * offsets[s + 1] - 1 (NULL: one each), at its positions lengths[s] on.  Rows whose
  * position has no page, or one outside the cache, are not written.  Two
- * sequences that share the page they write to overwrite each other. */
+ * sequences that share the page they write to overwrite each other.  Fewer than
+ * 2^25 rows a call, here and below. */
 int glm53_kv_append(const glm53_kv_cache* cache, const glm53_head_rows* k, const glm53_head_rows* v, int64_t tokens,
                     const int32_t* offsets, const int32_t* lengths, void* stream);
 /* Reads sequence s's positions 0 .. offsets[s + 1] - offsets[s] - 1 into rows

@@ -159,6 +159,23 @@ def test_append_read_and_paged_refusals(N, libso):
     assert libso.glm53_kv_read(ctypes.byref(cache), None, 0, FAKE, FAKE, None) == N.OK
 
 
+def test_limits_of_offsets_and_grids(N, libso):
+    """What 32-bit offsets, a grid and the gradients' start values hold."""
+    far = N.HeadRows(FAKE, 512, 1 << 22)
+    for call in (libso.glm53_packed_attention, libso.glm53_packed_attention_backward):
+        assert call(_attention(N, heads=512, kv_heads=512, q=far), None) == N.INVALID_ARGUMENT
+        assert "apart" in libso.glm53_last_error().decode()
+        assert call(_attention(N, scale=2.0**-65), None) == N.INVALID_ARGUMENT
+        assert "scale" in libso.glm53_last_error().decode()
+    assert _paged(N, libso, _cache(N), heads=512, q=far) == N.INVALID_ARGUMENT
+    assert "apart" in libso.glm53_last_error().decode()
+    cache = _cache(N)
+    assert _append(N, libso, cache, tokens=1 << 25, offsets=FAKE) == N.INVALID_ARGUMENT
+    assert "tokens" in libso.glm53_last_error().decode()
+    assert libso.glm53_kv_read(ctypes.byref(cache), FAKE, 1 << 25, FAKE, FAKE, None) == N.INVALID_ARGUMENT
+    assert "rows" in libso.glm53_last_error().decode()
+
+
 def test_struct_layouts(N, tmp_path):
     structs = {"glm53_head_rows": N.HeadRows, "glm53_attention": N.Attention, "glm53_kv_cache": N.KVCache}
     lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{ROOT / "include" / "glm53_moe.h"}"', "int main(void) {"]
