@@ -151,11 +151,21 @@ int64_t tile_numbers(int64_t rows, bool packed, int sequences, int size) {
 
 // ------------------------------------------------------------- forward ---
 //
-// W wavefronts of RB x 32 rows; a tile of 64 keys is multiplied while the next
-// one is loaded.  Scores are computed as S^T (keys the result's rows), so a
-// lane holds 32 of its row's 64 scores, a row's maximum and sum are within a
-// lane and its counterpart 32 lanes away, and the weights go into the second
-// product (out^T = v^T P^T) from the registers they are in.
+// W wavefronts of 32 rows; a tile of 64 keys is multiplied while the next one is
+// loaded.  Scores are computed as S^T (keys the result's rows), so a lane holds
+// 32 of its row's 64 scores, a row's maximum and sum are within a lane and its
+// counterpart 32 lanes away, and the weights go into the second product (out^T
+// = v^T P^T) from the registers they are in.  One pass over the keys: sums
+// relative to a running maximum, in FP32; the weights are rounded to bf16 as the
+// matrix instruction takes them, the result once.
+//
+// Bound by a SIMD's two wavefronts, which take turns at its matrix unit and its
+// vector unit: a tile of 128 columns is 2,048 clocks of products for both, and the
+// 32 exponentials, maxima, sums and conversions of each lane are about as many.
+// 4,096 + 4,096 tokens, 16 / 4 heads of 128, all seen: 254 us, 1,081 TFLOP/s, the
+// matrix unit busy half of the time (228 us without the softmax's instructions);
+// 64 rows a wavefront, which halve the LDS reads, leave one wavefront a SIMD and
+// were slower.  16,384 causal tokens, 8 / 1 heads: 522 us, 1,053 TFLOP/s.
 
 template <int DP_, bool EXACT, int W_>
 struct Forward {
@@ -210,7 +220,7 @@ struct Forward {
     f32x16 out[T];
     float m, l;  // m in units of scores; l: this lane's part
     uint32_t dirty = 0;
-    // How: kPlain, kMasked, or kCareful (see finite_part)
+    // `how`: kPlain, kMasked, or kCareful (see finite_part)
     const auto compute = [&](int step, auto stage, auto how) {
       constexpr int kHow = decltype(how)::value;
       const int kt = stage * 2 * Tile::kBytes, vt = kt + Tile::kBytes;
@@ -257,7 +267,7 @@ struct Forward {
       top = both_max(top);
       const bool grows = top * c > m * c + kSlack;
       if (__any(grows)) {
-        const float next = grows ? top : m;  // each row by itself: its bits are not its neighbours' matter
+        const float next = grows ? top : m;  // a row's bits do not depend on its neighbours in the wavefront
         const float alpha = next == -INFINITY ? 1.0f : exp2_fast((m - next) * c);
         m = next;
         l *= alpha;
@@ -351,7 +361,8 @@ __global__ __launch_bounds__(F::kThreads, F::DP == 256 ? 1 : 2) void attention_k
 //
 // Two kernels, each with one side of the scores for its own and a loop over the other:
 // no sum is shared, so every gradient is added in a fixed order, for seven
-// products instead of five.
+// products instead of five (8,192 tokens in three sequences, 32 / 8 heads of 128:
+// 357 us and 420 us of all gradients' 777, 800 TFLOP/s of the products made).
 //
 // delta from the rounded `out` is off by as much as `out` is, and puts that into
 // every dS of its row.  The rows' sums of dS, which are 0, say by how much:
@@ -359,7 +370,8 @@ __global__ __launch_bounds__(F::kThreads, F::DP == 256 ? 1 : 2) void attention_k
 // bf16 parts, so that both gradients are off by one operand's rounding at most
 // (relative error 0.0024 instead of 0.0026 to 0.0029).
 
-// d_q: a lane's row as in the forward pass, a tile of 64 keys at a time.
+// d_q: a lane's row as in the forward pass, a tile of 64 keys at a time.  Bound as
+// that is, by four runs of products for its two.
 template <int DP_, bool EXACT, int W_, bool DQ>
 struct QueryGradient {
   static constexpr int DP = DP_, W = W_;
@@ -555,12 +567,14 @@ struct QueryGradient {
 
 // d_k and d_v: a lane's key and a tile of rows at a time.  Scores are computed
 // with rows the result's rows, so that P and dS are the second operands of
-// d_v^T += d_out^T P and d_k^T += q^T dS as they are.  Of the four wavefronts two
-// and two share 32 keys, each with half of a tile's rows, and add up at the end: a
-// workgroup has 64 keys and half as many turns, so that the first keys of a
-// causal sequence, which all rows see, take no longer than the card takes for the
-// rest (8,192 tokens in three sequences, 8 key heads: DKDV us; 128 keys a
-// workgroup: 777).
+// d_v^T += d_out^T P and d_k^T += q^T dS as they are.  A wavefront has 32 keys
+// and all of a tile's rows (RW = 1), or two wavefronts share 32 keys, each with half
+// of a tile's rows, and add up at the end (RW = 2): a workgroup has 64 keys then and
+// half as many turns, so that the first keys of a causal sequence, which all rows
+// see, do not outlast the rest (wide_key_tiles has both sides).  Bound by
+// its one wavefront a SIMD, which has the gradients' sums in 128 registers of a lane
+// and no other one to multiply beside its weights, and by LDS: loading the
+// tiles costs 18% of it.
 template <int DP_, bool EXACT, int NB_, int RW_, bool DK, bool DV>
 struct KeyGradient {
   static constexpr int DP = DP_, NB = NB_, RW = RW_;  // NB blocks of 32 rows a wavefront and turn, RW wavefronts' rows a tile

@@ -215,10 +215,10 @@ struct HeadTile {
 };
 
 // Tiles that a mask cuts: a weight that is 0 because its place is masked must
-// take nothing from the values there, not even 0 x NaN.  So the values of such a
-// tile are multiplied with their infinities and NaNs replaced by 0 (`dirty`
-// where there was one), and what the mask lets through of those is added
-// afterwards by add_nonfinite.
+// take nothing from the values there, not even 0 x NaN.  So the careful pass
+// multiplies the values of such a tile with their infinities and NaNs replaced
+// by 0 (`dirty` where there was one), and what the mask lets through of those is
+// added afterwards by add_nonfinite.
 __device__ __forceinline__ bf16x8 finite_part(bf16x8 v, uint32_t& dirty) {
   u32x4 w = __builtin_bit_cast(u32x4, v);
 #pragma unroll

@@ -23,7 +23,12 @@ and FakeTensor / meta propagation gets the output shapes without a device.
   and ``glm53::gated_mlp_backward`` -- ``gated_mlp``, differentiable where
   `keep` has it return G, U and h;
 * ``glm53::int4_linear(x, weight, scales, offsets?, bias?)`` -- ``int4_linear``,
-  and ``glm53::joined_swiglu(joined, limit)``, the activation of ``Int4MLP``.
+  and ``glm53::joined_swiglu(joined, limit)``, the activation of ``Int4MLP``;
+* ``glm53::packed_attention(q, k, v, offsets?, key_offsets?, causal, scale,
+  keep)`` and ``glm53::packed_attention_backward`` -- ``packed_attention``,
+  differentiable where `keep` has it return the rows' logarithms;
+* ``glm53::append_kv``, ``glm53::read_kv`` and ``glm53::paged_attention`` -- the
+  key-value cache; the first changes the pages that it is given.
 
 The MoE ops take the module by an integer key (``register_owner``): the
 module keeps its weights, its per-(device, stream) native plans and its
