@@ -211,11 +211,11 @@ struct Forward {
     const int lim = prefix(r);
     bf16x8 q[DP / 16];
     load_operand<DP>(q, a.q.p + token * a.q.token + query_head * a.q.head, dim, h);
+    const typename Tile::Places at(lds_at, lane);  // while these are on their way
 #pragma unroll
     for (int j = 0; j < DP / 16; ++j) arrived(q[j]);
     const int all_see = __builtin_amdgcn_readfirstlane(lim), some_see = __builtin_amdgcn_readlane(lim, 31);
 
-    const typename Tile::Places at(lds_at, lane);
     const float c = a.scale * kLog2e;
     f32x16 out[T];
     float m, l;  // m in units of scores; l: this lane's part
