@@ -227,8 +227,15 @@ __device__ __forceinline__ int64_t tokens_of(const DecodeArgs& a, int s, bool& w
   return n < 0 ? 0 : n > most ? most : n;
 }
 
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
+                              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)));
+}
+
 // How the work is dealt: units are chunks of all heads' parts of every sequence.
-// Wavefronts ask; 64 sequences' numbers lie in a wavefront's lanes at a time.
+// Wavefronts ask; 64 sequences' numbers lie in a wavefront's lanes at a time.  More than
+// 64 are 64 runs of them first, a lane's each, of which one is looked at (1,000
+// sequences of 60 tokens, 32 / 8 heads: 64 us; all of them by 64: 74).
 template <int WORKERS, int CHUNK>
 struct Shares {
   const DecodeArgs& a;
@@ -237,11 +244,39 @@ struct Shares {
   int block;                          // sequences block .. block + 63 are in the lanes
   int64_t tokens, before;             // of the lane's sequence, and the units before it
   bool whole;
+  int run;                            // sequences of a run
+  int64_t run_before, run_units;      // of the lane's run
 
   __device__ __forceinline__ explicit Shares(const DecodeArgs& a)
       : a(a), lane(threadIdx.x & 63), head_parts((a.group + kHeads - 1) / kHeads), parts(a.cache.kv_heads * head_parts) {
-    units = 0;
-    for (int s = 0; s < a.cache.sequences; s += 64) units = load(s, units);
+    const int sequences = a.cache.sequences;
+    if (sequences <= 64) {
+      units = load(0, 0);
+      return;
+    }
+    run = (sequences + 63) / 64;
+    run_units = 0;
+    for (int i = 0; i < run; i += 8) {
+#pragma unroll
+      for (int j = i; j < i + 8; ++j) {
+        const int s = lane * run + j;
+        bool unused;
+        if (j < run && s < sequences) run_units += chunks(tokens_of(a, s, unused));
+      }
+    }
+    run_units *= parts;
+    const int64_t upto = sum_upto(run_units);
+    run_before = upto - run_units;
+    units = __shfl(upto, 63);
+  }
+  // The sum of this lane's value and of those of the lanes before it.
+  __device__ __forceinline__ int64_t sum_upto(int64_t v) const {
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      const int64_t left = __shfl_up(v, w);
+      if (lane >= w) v += left;
+    }
+    return v;
   }
   __device__ __forceinline__ static int64_t chunks(int64_t tokens) { return (tokens + CHUNK - 1) / CHUNK; }
   // Takes the 64 sequences from s on, `at` units behind the start; the units behind their end.
@@ -250,22 +285,16 @@ struct Shares {
     tokens = 0;
     whole = true;
     if (s + lane < a.cache.sequences) tokens = tokens_of(a, s + lane, whole);
-    const int64_t own = chunks(tokens) * parts;
-    int64_t upto = own;
-#pragma unroll
-    for (int w = 1; w < 64; w <<= 1) {
-      const int64_t left = __shfl_up(upto, w);
-      if (lane >= w) upto += left;
-    }
+    const int64_t own = chunks(tokens) * parts, upto = sum_upto(own);
     before = at + upto - own;
     return at + __shfl(upto, 63);
   }
   // The sequence of unit u.
   __device__ __forceinline__ int find(int64_t u) {
-    int64_t end = units;
     if (a.cache.sequences > 64) {
-      end = 0;
-      for (int s = 0; s < a.cache.sequences; s += 64) {
+      const int in = 63 - __builtin_clzll(__ballot(run_before <= u && run_units > 0));
+      int64_t end = lane_value(run_before, in);
+      for (int s = in * run; s < a.cache.sequences; s += 64) {
         end = load(s, end);
         if (end > u) break;
       }
@@ -277,10 +306,12 @@ struct Shares {
   __device__ __forceinline__ int worker(int64_t u) const { return static_cast<int>(((u + 1) * WORKERS - 1) / units); }
 };
 
-__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
-  return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
-                              static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)));
-}
+// Which wavefronts have parts of one (sequence, head): first .. last, the first one its start.
+struct Split {
+  int sequence, part, first, last;
+  int64_t units;  // of all, from which each wavefront's follow
+  int64_t unused;
+};
 
 template <int DP_, bool E4M3_>
 struct Decode {
@@ -298,6 +329,15 @@ struct Decode {
   static constexpr int kWorkers = 256 * (160 * 1024 / kLds < 4 ? 160 * 1024 / kLds : 4);
   static constexpr int kLoads = 2 * (TS / kLoadRows) + (E4M3 ? 2 * kSub : 0);  // of a whole stage
   static constexpr int kPartial = kHeads * (DP + 2);  // floats: sums, then maximum and total of each head
+  static constexpr size_t kPartials = sizeof(float) * 2 * kWorkers * kPartial, kSpace = kPartials + sizeof(Split) * kWorkers;
+  // What a join finds in its Split: with few (sequence, head) parts each has one, with more of them
+  // each worker has that of the one which it begins and others end.
+  static __device__ __forceinline__ bool by_segment(const DecodeArgs& a, int parts) {
+    return static_cast<int64_t>(a.cache.sequences) * parts <= kWorkers;
+  }
+  static __device__ __forceinline__ Split* splits(const DecodeArgs& a) {
+    return reinterpret_cast<Split*>(reinterpret_cast<uint8_t*>(a.partial) + kPartials);
+  }
   using Dealt = Shares<kWorkers, TS>;
 
   __device__ static __forceinline__ int swizzle(int row) {
@@ -311,6 +351,9 @@ struct Decode {
     const int worker = blockIdx.x;
     int64_t unit = shares.start(worker);
     const int64_t end = shares.start(worker + 1);
+    const bool by_segment = Decode::by_segment(a, shares.parts);
+    Split* splits = Decode::splits(a);
+    if (!by_segment && lane == 0) splits[worker].last = -1;  // overwritten below where there is one
     if (unit >= end) return;
     int sequence = __builtin_amdgcn_readfirstlane(shares.find(unit));
 
@@ -500,6 +543,9 @@ struct Decode {
         compute(stage, slot);
       }
 
+      if (from == 0 && lane == 0 && (by_segment || to != chunks))
+        splits[by_segment ? sequence * shares.parts + part : worker] =
+            Split{sequence, part, worker, to == chunks ? worker : shares.worker(seg + chunks - 1), shares.units, 0};
       l = quarter_sum(l);
       if (__any(bad)) l = NAN;
       if (g < a.group) {
@@ -557,30 +603,47 @@ __global__ __launch_bounds__(64) void decode_kernel(DecodeArgs a) {
   D::run(a, lds);
 }
 
-// One (sequence, head) and LANES x 4 of its columns a workgroup: adds its parts where
-// there are several, and writes 0 where the sequence has no token.
+// One head of a Split and LANES x 4 of its columns a workgroup: adds its parts where there
+// are several.  Sequences without a token are written here too.  Takes 4 to 9 us, a
+// launch and three loads that wait for each other; finding each head's parts from
+// the lengths took 5 to 7 up to 64 sequences, 34 for 256 and 460 for 1,000.
 template <class D, int LANES>
 __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
   constexpr int DP = D::DP, kGroups = 256 / LANES;  // parts at a time
   const CacheArgs& c = a.cache;
-  typename D::Dealt shares(a);
-  const int heads = c.kv_heads * a.group, sequence = blockIdx.x / heads, query_head = blockIdx.x - sequence * heads;
-  const int head = query_head / a.group, g = query_head - head * a.group, hd = g % kHeads;
-  if (c.sequences > 64) {
-    int64_t at = 0;
-    for (int s = 0; s <= sequence; s += 64) at = shares.load(s, at);
+  const int heads = c.kv_heads * a.group, head_parts = (a.group + kHeads - 1) / kHeads, parts = c.kv_heads * head_parts;
+  const bool by_segment = D::by_segment(a, parts);
+  const Split split = D::splits(a)[blockIdx.x];
+  const int hd = blockIdx.y;
+  if (blockIdx.z == 0) {
+    const int stride = by_segment ? c.sequences : D::kWorkers;
+    for (int s = by_segment ? blockIdx.x / parts : blockIdx.x; s < c.sequences; s += stride) {
+      bool whole;
+      if (tokens_of(a, s, whole) != 0) continue;
+      const uint32_t none = whole ? 0u : 0x7FC07FC0u;
+      u32x2* o = reinterpret_cast<u32x2*>(a.out + static_cast<int64_t>(s) * heads * c.dim);
+      const int row = c.dim / 4, all = heads * row;
+      // a part's head, or every gridDim.y-th head
+      if (by_segment) {
+        const int part = blockIdx.x % parts, g = part % head_parts * kHeads + hd;
+        if (g < a.group)
+          for (int i = threadIdx.x; i < row; i += 256) o[(part / head_parts * a.group + g) * row + i] = (u32x2){none, none};
+        return;
+      }
+      for (int i = hd * 256 + threadIdx.x; i < all; i += gridDim.y * 256) o[i] = (u32x2){none, none};
+    }
   }
-  const int own = sequence - shares.block;
-  const int64_t chunks = D::Dealt::chunks(lane_value(shares.tokens, own));
-  int first = 0, last = -1;
-  if (chunks > 0) {
-    const int64_t seg = lane_value(shares.before, own) + (head * shares.head_parts + g / kHeads) * chunks;
-    first = shares.worker(seg);
-    last = shares.worker(seg + chunks - 1);
-    if (first == last) return;
+  if (by_segment) {
+    bool unused;
+    if (tokens_of(a, blockIdx.x / parts, unused) == 0) return;  // has no Split
   }
+  if (split.last <= split.first) return;
+  const int first = split.first, last = split.last, g = split.part % head_parts * kHeads + hd;
+  if (split.last < 0 || g >= a.group) return;
+  const int sequence = split.sequence, query_head = split.part / head_parts * a.group + g;
+  const auto start = [&](int worker) { return split.units * worker / D::kWorkers; };
   const float sc = a.scale * 1.44269504088896340736f;
-  const int d = 4 * (threadIdx.x % LANES + LANES * blockIdx.y), group = threadIdx.x / LANES;
+  const int d = 4 * (threadIdx.x % LANES + LANES * blockIdx.z), group = threadIdx.x / LANES;
   float top = -INFINITY, total = 0.0f;
   f32x4 sum = {0, 0, 0, 0};
   // Adds a part to another one, both with sums relative to their own maximum.
@@ -603,7 +666,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
       l[i] = 0.0f;
       x[i] = (f32x4){0, 0, 0, 0};
       // where there are fewer units than workers, some of these have none
-      if (w > last || shares.start(w) >= shares.start(w + 1)) continue;
+      if (w > last || start(w) >= start(w + 1)) continue;
       const float* p = a.partial + static_cast<int64_t>(2 * w + (w == first ? 1 : 0)) * D::kPartial;
       m[i] = p[kHeads * DP + 2 * hd];
       l[i] = p[kHeads * DP + 2 * hd + 1];
@@ -628,7 +691,6 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
     }
   }
   if (group != 0 || d >= c.dim) return;
-  if (!__builtin_amdgcn_readlane(shares.whole, own)) total = NAN;
   const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
   uint16_t* o = a.out + (static_cast<int64_t>(sequence) * heads + query_head) * c.dim + d;
   *reinterpret_cast<u32x2*>(o) = pack4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
@@ -638,19 +700,21 @@ template <class D>
 hipError_t decode(const DecodeArgs& a, hipStream_t st) {
   decode_kernel<D><<<D::kWorkers, 64, D::kLds, st>>>(a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  const int most = a.group < kHeads ? a.group : kHeads, parts = a.cache.kv_heads * ((a.group + kHeads - 1) / kHeads);
+  const int64_t segments = static_cast<int64_t>(a.cache.sequences) * parts, heads = a.cache.kv_heads * a.group;
+  const uint32_t splits = static_cast<uint32_t>(segments < D::kWorkers ? segments : D::kWorkers);
   // A few heads may each have hundreds of parts: 16 columns a workgroup then.
-  const uint32_t rows = static_cast<uint32_t>(static_cast<int64_t>(a.cache.sequences) * a.cache.kv_heads * a.group);
-  if (rows <= 256)
-    decode_join_kernel<D, 4><<<dim3(rows, D::DP / 16), 256, 0, st>>>(a);
+  if (a.cache.sequences * heads <= 256)
+    decode_join_kernel<D, 4><<<dim3(splits, most, D::DP / 16), 256, 0, st>>>(a);
   else
-    decode_join_kernel<D, D::DP / 4><<<rows, 256, 0, st>>>(a);
+    decode_join_kernel<D, D::DP / 4><<<dim3(splits, most), 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
 size_t decode_space(int dim, bool e4m3) {
-  const auto of = [](auto d) { return sizeof(float) * 2 * decltype(d)::kWorkers * decltype(d)::kPartial; };
+  const auto of = [](auto d) { return decltype(d)::kSpace; };
   if (dim <= 64) return e4m3 ? of(Decode<64, true>{}) : of(Decode<64, false>{});
   if (dim <= 128) return e4m3 ? of(Decode<128, true>{}) : of(Decode<128, false>{});
   return e4m3 ? of(Decode<256, true>{}) : of(Decode<256, false>{});

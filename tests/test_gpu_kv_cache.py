@@ -300,6 +300,35 @@ def test_many_sequences(dev, sequences):
     decode(dev, [(13 * i) % 90 for i in range(sequences)], 4, 2, 64, 16, True)
 
 
+@pytest.mark.parametrize("sequences, heads, kv_heads, longest, long", [
+    (130, 24, 1, 40, 0),  # two parts of a key head
+    (300, 8, 8, 70, 0),  # more (sequence, head) parts than workers
+    (1023, 1, 1, 5, 0), (1024, 1, 1, 5, 0), (1025, 1, 1, 5, 0),
+    (1030, 2, 1, 20, 4000),  # one of them over many workers
+    (4200, 1, 1, 3, 0),  # runs of more than 64 sequences
+])
+@pytest.mark.parametrize("quantised", [False, True])
+def test_batches(dev, sequences, heads, kv_heads, longest, long, quantised):
+    import torch
+
+    lengths = torch.randint(0, longest + 1, (sequences,), generator=torch.Generator().manual_seed(sequences)).tolist()
+    lengths[:3], lengths[-70:] = [0] * 3, [0] * 70  # starts and ends with sequences without a token
+    if long:
+        lengths[sequences // 2] = long
+    decode(dev, lengths, heads, kv_heads, 64, 16, quantised)
+
+
+@pytest.mark.parametrize("sequences", [3, 200, 1100])
+def test_tables_without_a_page(dev, sequences):
+    """0 where there is no token, NaN where there is one and no page."""
+    import torch
+
+    cache = make_cache(dev, 2, 16, 2, 80, False)
+    lengths = torch.arange(sequences, dtype=torch.int32) % 3
+    got = cache.attend(normal(dev, sequences, 6, 80), torch.zeros(sequences, 0, dtype=torch.int32, device=dev), lengths.to(dev)).cpu()
+    assert bool((got[lengths == 0] == 0).all()) and bool(got[lengths > 0].isnan().all())
+
+
 @pytest.mark.parametrize("scale", [1e-3, 1.0])
 def test_scales(dev, scale):
     decode(dev, [100, 40], 4, 2, 64, 16, True, scale)
