@@ -106,6 +106,11 @@ def head_rows(t: torch.Tensor) -> tuple[torch.Tensor, N.HeadRows]:
     return t, N.HeadRows(t.data_ptr(), row, head)
 
 
+def result_like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape; for a contiguous one by the call that is 0.6 us shorter."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def index_pointer(t: torch.Tensor | None) -> tuple[torch.Tensor | None, int | None]:
     if t is None:
         return None, None
@@ -129,7 +134,7 @@ def native_packed_attention(q, k, v, offsets, key_offsets, causal: bool, scale: 
     """The native call behind glm53::packed_attention: the result, and the
     rows' logarithms where kept."""
     tokens, heads, _ = q.shape
-    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)  # the first is 0.6 us shorter
+    out = result_like(q)
     lse = q.new_empty((k.shape[1], tokens * (heads // k.shape[1])), dtype=torch.float32) if keep else None
     if tokens:
         d, alive = _descriptor(q, k, v, offsets, key_offsets, out, lse, causal, scale)
@@ -141,7 +146,7 @@ def native_packed_attention_backward(q, k, v, offsets, key_offsets, out, lse, d_
                                      wanted: list[bool]):
     """The native call behind glm53::packed_attention_backward: the gradients
     of q, k and v that are `wanted`, None in place of the others."""
-    grads = [t.new_empty(t.shape) if w else None for t, w in zip((q, k, v), wanted)]
+    grads = [result_like(t) if w else None for t, w in zip((q, k, v), wanted)]
     if q.shape[0] == 0 or k.shape[0] == 0:
         return [None if g is None else g.zero_() for g in grads]
     d, alive = _descriptor(q, k, v, offsets, key_offsets, out, lse, causal, scale)

@@ -319,12 +319,16 @@ __device__ __forceinline__ Segment find_segment(const int32_t* offsets, int sequ
     s = __builtin_ctzll(__ballot(own > low && __popcll(have & ((uint64_t{1} << lane) - 1)) == rank));
     g.tile = order == kLastFirst ? low : __builtin_amdgcn_readlane(own, s) - 1 - low;
   } else {
-    int count = 0;
-    for (int i = 0; i < segments; i += 64) {
-      mine = boundary(i + lane);
-      count += __popcll(__ballot(i + lane < segments && mine / size + i + lane <= t));
+    // the last segment that starts at t or before it, of s .. s + span - 1
+    s = 0;
+    for (int span = segments, step;; span = step) {
+      step = (span + 63) / 64;
+      const int i = s + lane * step;
+      mine = boundary(i);
+      const uint64_t upto = __ballot(lane * step < span && i < segments && mine / size + i <= t);
+      s += step * (__popcll(upto) - 1);
+      if (step == 1) break;
     }
-    s = __builtin_amdgcn_readfirstlane(count) - 1;  // boundary 0 counts for every t
   }
   if (segments < 64) {
     g.first = __builtin_amdgcn_readlane(mine, s);

@@ -13,11 +13,15 @@ namespace {
 // for one row.
 __device__ __forceinline__ int sequence_of(const int32_t* offsets, int sequences, int row) {
   const int lane = threadIdx.x & 63;
-  int count = 0;
-  for (int i = 0; i <= sequences; i += 64)
-    count += __popcll(__ballot(i + lane <= sequences && offsets[i + lane] <= row));
-  count = __builtin_amdgcn_readfirstlane(count);
-  return count >= 1 && count <= sequences ? count - 1 : -1;
+  int s = -1;  // the last one that starts at the row or before it is one of s .. s + span - 1
+  for (int span = sequences + 2, step;; span = step) {
+    step = (span + 63) / 64;
+    const int i = s + lane * step;
+    const uint64_t upto = __ballot(lane * step < span && i <= sequences && (i < 0 || offsets[i] <= row));
+    s += step * (__popcll(upto) - 1);
+    if (step == 1) break;
+  }
+  return s < sequences ? s : -1;
 }
 
 // Number of the cache row of a sequence's position, without its head: page *

@@ -28,7 +28,7 @@ import torch
 
 from . import _native as N
 from . import ops as _ops
-from .attention import check_dim, check_heads, check_offsets, check_scale, head_rows, index_pointer
+from .attention import check_dim, check_heads, check_offsets, check_scale, head_rows, index_pointer, result_like
 
 
 def append_kv(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -178,7 +178,7 @@ def native_read_kv(k_pages, v_pages, page_table, offsets, rows: int, k_scales, v
 def native_paged_attention(q, k_pages, v_pages, page_table, lengths, k_scales, v_scales, scale: float):
     """The native call behind glm53::paged_attention."""
     cache, table = _descriptor(k_pages, v_pages, page_table, k_scales, v_scales)
-    out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+    out = result_like(q)
     q, q_rows = head_rows(q)
     lengths, p_lengths = index_pointer(lengths)
     sequences, heads, dim = q.shape

@@ -398,6 +398,15 @@ def test_many_sequences(dev, sequences):
     run(dev, lengths, lengths, 2, 1, 64, True)
 
 
+@pytest.mark.parametrize("sequences", [4094, 4095, 4200])
+def test_searched_in_several_steps(dev, sequences):
+    """More sequences than 64 * 64 segments, some of them empty."""
+    import torch
+
+    lengths = torch.randint(0, 4, (sequences,), generator=torch.Generator().manual_seed(1)).tolist()
+    run(dev, lengths, lengths, 2, 1, 64, True)
+
+
 @pytest.mark.parametrize("lengths", [[2300, 2100], [4300, 0, 100]])
 def test_long_sequences_first(dev, lengths):
     """Lengths whose tiles are taken longest first."""

@@ -87,6 +87,17 @@ def test_written_and_read_back(dev, quantised, dim, page_size):
         assert torch.equal(g.double(), stored(x, quantised))
 
 
+@pytest.mark.parametrize("sequences", [62, 63, 64, 4094, 4095, 5000])
+def test_rows_of_many_sequences(dev, sequences):
+    import torch
+
+    lengths = torch.randint(0, 4, (sequences,), generator=torch.Generator().manual_seed(2)).tolist()
+    cache, table, k, v, offsets = filled(dev, lengths, 16, 1, 16, False)
+    got = cache.read(table, index(offsets, dev), offsets[-1] + 5)
+    for rows, want in zip(got, (k, v)):
+        assert torch.equal(rows[:-5], want) and not bool(rows[-5:].any())
+
+
 @pytest.mark.parametrize("dim", [8, 24, 72, 136])
 def test_bf16_rows_of_other_widths(dev, dim):
     import torch
