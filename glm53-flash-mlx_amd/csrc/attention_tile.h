@@ -85,6 +85,12 @@ __device__ __forceinline__ const void* uniform_address(const void* p) {
   return reinterpret_cast<const void*>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
+// Direct global -> LDS load of 4 bytes a lane, each from an address of its own, to lds + 4 lane.
+__device__ __forceinline__ void load_dword_to_lds(const void* p, uint32_t lds) {
+  lds = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+
 // Direct global -> LDS load of 16 or 4 bytes a lane, base + off, to lds + 16 (4) lane.
 template <int BYTES = 16>
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t off, uint32_t lds) {

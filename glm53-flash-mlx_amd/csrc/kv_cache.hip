@@ -326,12 +326,12 @@ struct Decode {
   static constexpr int kSlots = kPitch / 16, kLoadRows = 64 / kSlots;
   static constexpr int TS = kPitch >= 256 ? 32 : 64, kSub = TS / 16;  // tokens of a stage, and parts of 16
   static constexpr int kTile = TS * kPitch;
-  static constexpr int kStage = 2 * kTile + (E4M3 ? 512 : 0);
+  static constexpr int kStage = 2 * kTile + (E4M3 ? 128 : 0);
   static constexpr int kLds = 2 * kStage;
   // one a SIMD of 256 CUs where the LDS holds them (a fifth one a CU ends after the others:
   // 64 x 8192 tokens in bf16 470 us for 381)
   static constexpr int kWorkers = 256 * (160 * 1024 / kLds < 4 ? 160 * 1024 / kLds : 4);
-  static constexpr int kLoads = 2 * (TS / kLoadRows) + (E4M3 ? 2 * kSub : 0);  // of a whole stage
+  static constexpr int kLoads = 2 * (TS / kLoadRows) + E4M3;  // of a whole stage
   static constexpr int kPartial = kHeads * (DP + 2);  // floats: sums, then maximum and total of each head
   static constexpr size_t kPartials = sizeof(float) * 2 * kWorkers * kPartial, kSpace = kPartials + sizeof(Split) * kWorkers;
   // What a join finds in its Split: with few (sequence, head) parts each has one, with more of them
@@ -433,12 +433,13 @@ struct Decode {
               load_to_lds(c.v + row0 * row_bytes, off, to_lds + kTile);
             }
           }
-          if constexpr (E4M3) {
-            if (lane < 4) {
-              load_to_lds<4>(c.k_scales + row0, 4 * lane, to_stage + 2 * kTile + 16 * u);
-              load_to_lds<4>(c.v_scales + row0, 4 * lane, to_stage + 2 * kTile + 256 + 16 * u);
-            }
-          }
+        }
+        if constexpr (E4M3) {  // a stage's scales by one instruction: 4 tokens a lane, keys' and then values'
+          const int u = (lane & 15) >> 2, page = __shfl(pages, ahead * kSub + u);
+          const int64_t row = ((static_cast<int64_t>(page) * c.kv_heads + head) << c.page_log2) +
+                              ((first + 16 * u) & ((1 << c.page_log2) - 1)) + 4 * (lane & 3);
+          if (lane < 32 && u < kSub && first + 16 * u < tokens)
+            load_dword_to_lds((lane < 16 ? c.k_scales : c.v_scales) + row, to_stage + 2 * kTile);
         }
       };
 
@@ -476,7 +477,7 @@ struct Decode {
                 s[b] = mfma16(__builtin_bit_cast(bf16x8, (u32x4){x2[0], x2[1], x3[0], x3[1]}), q[2 * j + 1], s[b]);
               }
               const uint32_t ks = *reinterpret_cast<const uint32_t*>(vt + kTile + 16 * (u + b) + 4 * quarter);
-              const uint32_t ws = *reinterpret_cast<const uint32_t*>(vt + kTile + 256 + 16 * (u + b) + 4 * quarter);
+              const uint32_t ws = *reinterpret_cast<const uint32_t*>(vt + kTile + 64 + 16 * (u + b) + 4 * quarter);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 s[b][r] *= scale_value((ks >> (8 * r)) & 255);
