@@ -269,6 +269,7 @@ _SIGNATURES = {
     "glm53_int4_linear": (ctypes.c_int, [P, P, I64, P, P, SZ, P]),
     "glm53_packed_attention": (ctypes.c_int, [P, P]),
     "glm53_packed_attention_backward_workspace_bytes": (SZ, [I64, I64]),
+    "glm53_packed_attention_backward_split_bytes": (SZ, [I64] * 6),
     "glm53_packed_attention_backward": (ctypes.c_int, [P, P]),
     "glm53_kv_append": (ctypes.c_int, [P, P, P, I64, P, P, P]),
     "glm53_kv_read": (ctypes.c_int, [P, P, I64, P, P, P]),

@@ -154,6 +154,9 @@ def native_packed_attention_backward(q, k, v, offsets, key_offsets, out, lse, d_
     d.d_q, d.d_k, d.d_v = (None if g is None else g.data_ptr() for g in grads)
     lib = N.lib()
     d.workspace_bytes = lib.glm53_packed_attention_backward_workspace_bytes(q.shape[0], q.shape[1])
+    if wanted[1] or wanted[2]:
+        d.workspace_bytes += lib.glm53_packed_attention_backward_split_bytes(d.tokens, d.keys, d.sequences, d.heads, d.kv_heads,
+                                                                             d.head_dim)
     ws = N.workspace(d.workspace_bytes, q.device)
     d.workspace = ws.data_ptr()
     N.run(q.get_device(), lib.glm53_packed_attention_backward, ctypes.byref(d))

@@ -44,6 +44,10 @@ int check_scale(float scale) {
   return GLM53_OK;
 }
 
+size_t split_bytes(const AttentionArgs& a, int splits) {
+  return splits > 1 ? 2 * sizeof(float) * static_cast<size_t>(splits) * a.keys * a.kv_heads * a.dim : 0;
+}
+
 int attention_args(const glm53_attention* d, bool backward, AttentionArgs& a) {
   CHECK_ARG(d != nullptr, "attention descriptor is null");
   CHECK_ARG(d->tokens >= 0 && d->keys >= 0, "invalid shape tokens=%lld keys=%lld", (long long)d->tokens, (long long)d->keys);
@@ -87,6 +91,9 @@ int attention_args(const glm53_attention* d, bool backward, AttentionArgs& a) {
   CHECK_ARG(need == 0 || (d->workspace && d->workspace_bytes >= need && aligned(d->workspace, 256)),
             "attention's gradients need a 256-byte aligned workspace of %zu bytes", need);
   a.starts = static_cast<float*>(d->workspace);
+  a.splits = attention_row_splits(a);
+  if (d->workspace_bytes < need + split_bytes(a, a.splits)) a.splits = 1;
+  a.sums = reinterpret_cast<float*>(static_cast<uint8_t*>(d->workspace) + need);
   return GLM53_OK;
 }
 
@@ -140,6 +147,21 @@ int glm53_packed_attention(const glm53_attention* attention, void* stream) {
 size_t glm53_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t heads) {
   if (tokens <= 0 || heads <= 0 || tokens >= kMaxRows / heads) return 0;
   return round_up(2 * sizeof(float) * static_cast<size_t>(tokens * heads));
+}
+
+size_t glm53_packed_attention_backward_split_bytes(int64_t tokens, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads,
+                                                   int64_t head_dim) {
+  if (tokens <= 0 || keys <= 0 || heads <= 0 || tokens >= kMaxRows / heads || keys >= kMaxRows / heads || kv_heads <= 0 ||
+      heads % kv_heads != 0 || head_dim <= 0 || head_dim > kMaxHeadDim || sequences >= kMaxSequences)
+    return 0;
+  AttentionArgs a{};
+  a.tokens = tokens;
+  a.keys = keys;
+  a.sequences = static_cast<int>(sequences > 0 ? sequences : 1);
+  a.kv_heads = static_cast<int>(kv_heads);
+  a.group = static_cast<int>(heads / kv_heads);
+  a.dim = static_cast<int>(head_dim);
+  return split_bytes(a, attention_row_splits(a));
 }
 
 int glm53_packed_attention_backward(const glm53_attention* attention, void* stream) {

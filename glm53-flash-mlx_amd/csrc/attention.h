@@ -37,7 +37,14 @@ struct AttentionArgs {
   Rows16 d_out;
   uint16_t *d_q, *d_k, *d_v;   // contiguous; null: not wanted
   float* starts;               // [2, kv_heads, tokens * group]: -lse / (scale log2 e), -delta
+  int splits;                  // of the rows that a workgroup of d_k and d_v takes
+  float* sums;                 // [splits, keys, kv_heads, dim] of d_k, then the same of d_v; where splits > 1
 };
+
+// Into how many parts the rows of one tile of keys are best cut, at most: each has
+// kLeastTurns turns of a workgroup.
+constexpr int kLeastTurns = 16;
+int attention_row_splits(const AttentionArgs& a);
 
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t st);
 hipError_t launch_attention_backward(const AttentionArgs& a, hipStream_t st);

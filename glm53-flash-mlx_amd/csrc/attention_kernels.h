@@ -117,6 +117,20 @@ __device__ __forceinline__ void store_operand(uint16_t* p, const f32x16 (&x)[DP 
     }
 }
 
+template <int DP>
+__device__ __forceinline__ void store_sums(float* p, const f32x16 (&x)[DP / 32], int dim, int h) {
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int d = 32 * t + result_row(e, h);
+      if (d < dim) *reinterpret_cast<f32x4*>(p + d) = (f32x4){x[t][e], x[t][e + 1], x[t][e + 2], x[t][e + 3]};
+    }
+}
+__device__ __forceinline__ float* sums_of(const AttentionArgs& a, int gradient, int split) {
+  return a.sums + (static_cast<int64_t>(gradient) * a.splits + split) * a.keys * a.kv_heads * a.dim;
+}
+
 template <int T>
 __device__ __forceinline__ bool nonfinite(const f32x16 (&x)[T]) {
   float sum = 0.0f;
@@ -509,6 +523,7 @@ struct QueryGradient {
           const int left = lim - step * kKeys - 32 * kb - 4 * h;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
+#pragma clang fp contract(off)  // the same sum whether or not dS is needed for itself
             s[e] = exp2_fast(fmaf(s[e], c, -lse)) * p[e];
             if (kHow != kPlain && result_row(e, 0) >= left) s[e] = 0.0f;
             sum += s[e];
@@ -571,7 +586,9 @@ struct QueryGradient {
 // and all of a tile's rows (RW = 1), or two wavefronts share 32 keys, each with half
 // of a tile's rows, and add up at the end (RW = 2): a workgroup has 64 keys then and
 // half as many turns, so that the first keys of a causal sequence, which all rows
-// see, do not outlast the rest (wide_key_tiles has both sides).  Bound by
+// see, do not outlast the rest (wide_key_tiles has both sides).  With few keys and heads
+// the turns of a tile are split over workgroups, whose FP32 sums key_gradient_join_kernel
+// adds in their order (attention_row_splits).  Bound by
 // its one wavefront a SIMD, which has the gradients' sums in 128 registers of a lane
 // and no other one to multiply beside its weights, and by LDS: loading the
 // tiles costs 18% of it.
@@ -589,7 +606,7 @@ struct KeyGradient {
     const int dim = EXACT ? DP : a.dim;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int half = wave / KW;  // whose rows of a tile
-    const int head = blockIdx.x % a.kv_heads, number = blockIdx.x / a.kv_heads;
+    const int head = blockIdx.x % a.kv_heads, split = blockIdx.x / a.kv_heads % a.splits, number = blockIdx.x / a.kv_heads / a.splits;
     const Segment seg = find_segment(a.key_offsets != nullptr ? a.key_offsets : a.offsets, a.sequences, a.keys, 1, kKeys, number,
                                      tiles, a.causal ? kFirstFirst : kInOrder);
     const int key0 = seg.first + seg.tile * kKeys;
@@ -617,8 +634,17 @@ struct KeyGradient {
     };
     const int h = lane >> 5, key = key0 + 32 * (wave % KW) + (lane & 31), k = key < seg.last ? key : seg.last - 1;
     const int from = sees(k), from_all = __builtin_amdgcn_readlane(from, 31), from_some = __builtin_amdgcn_readfirstlane(from);
-    const int start = __builtin_amdgcn_readfirstlane(sees(key0));
-    const int steps = start < last_row ? (last_row - start + RT - 1) / RT : 0;
+    int start = __builtin_amdgcn_readfirstlane(sees(key0));
+    int steps = start < last_row ? (last_row - start + RT - 1) / RT : 0;
+    if (a.splits > 1) {  // this workgroup's share of the turns, in as many parts as have kLeastTurns
+      const int64_t all = steps;
+      const int parts = steps >= 2 * kLeastTurns ? (steps / kLeastTurns < a.splits ? steps / kLeastTurns : a.splits) : 1;
+      const int first = static_cast<int>(split < parts ? all * split / parts : all);
+      const int end = static_cast<int>(split < parts ? all * (split + 1) / parts : all);
+      if (end < all) last_row = start + end * RT;
+      start += first * RT;
+      steps = end - first;
+    }
 
     if (dim < DP) {
 #pragma unroll
@@ -832,6 +858,11 @@ struct KeyGradient {
     const int64_t o = (static_cast<int64_t>(key) * a.kv_heads + head) * dim;
     if constexpr (RW == 1) {
       if (key >= seg.last) return;
+      if (a.splits > 1) {
+        if (DK) store_sums<DP>(sums_of(a, 0, split) + o, d_k, dim, h);
+        if (DV) store_sums<DP>(sums_of(a, 1, split) + o, d_v, dim, h);
+        return;
+      }
       if (DK) store_operand<DP>(a.d_k + o, d_k, a.scale, dim, h);
       if (DV) store_operand<DP>(a.d_v + o, d_v, 1.0f, dim, h);
       return;
@@ -850,7 +881,7 @@ struct KeyGradient {
     if (DV) give(d_v, DK ? T / 2 : 0);
     __syncthreads();
     if (key >= seg.last) return;
-    const auto finish = [&](const f32x16 (&x)[T], int slot, float scale, uint16_t* to) {
+    const auto finish = [&](const f32x16 (&x)[T], int slot, float scale, uint16_t* to, float* partial) {
 #pragma unroll
       for (int t = 0; t < T; ++t)
         if ((t < T / 2) == (half == 0))
@@ -858,13 +889,16 @@ struct KeyGradient {
           for (int e = 0; e < 4; ++e) {
             const f32x4 y = sums(wave ^ KW, slot + t % (T / 2))[e];
             const int d = 32 * t + result_row(4 * e, h);
-            if (d < dim)
+            if (d >= dim) continue;
+            if (a.splits > 1)
+              *reinterpret_cast<f32x4*>(partial + o + d) = (f32x4){x[t][4 * e], x[t][4 * e + 1], x[t][4 * e + 2], x[t][4 * e + 3]} + y;
+            else
               *reinterpret_cast<u32x2*>(to + o + d) = pack4((x[t][4 * e] + y[0]) * scale, (x[t][4 * e + 1] + y[1]) * scale,
                                                             (x[t][4 * e + 2] + y[2]) * scale, (x[t][4 * e + 3] + y[3]) * scale);
           }
     };
-    if (DK) finish(d_k, 0, a.scale, a.d_k);
-    if (DV) finish(d_v, DK ? T / 2 : 0, 1.0f, a.d_v);
+    if (DK) finish(d_k, 0, a.scale, a.d_k, sums_of(a, 0, split));
+    if (DV) finish(d_v, DK ? T / 2 : 0, 1.0f, a.d_v, sums_of(a, 1, split));
   }
 };
 
@@ -890,7 +924,28 @@ template <class F>
 hipError_t launch_key_gradient(const AttentionArgs& a, hipStream_t st) {
   if (a.keys == 0) return hipSuccess;
   const int64_t tiles = tile_numbers(a.keys, a.offsets != nullptr, a.sequences, F::kKeys);
-  key_gradient_kernel<F><<<static_cast<uint32_t>(tiles * a.kv_heads), F::kThreads, F::kLds, st>>>(a, Divisor(a.group), static_cast<int>(tiles));
+  key_gradient_kernel<F><<<static_cast<uint32_t>(tiles * a.kv_heads * a.splits), F::kThreads, F::kLds, st>>>(a, Divisor(a.group), static_cast<int>(tiles));
+  return hipGetLastError();
+}
+
+// Adds the parts of d_k (blockIdx.y 0) or d_v in their order: four values a thread.  Bound
+// by the bytes of the parts.
+__global__ __launch_bounds__(256) void key_gradient_join_kernel(AttentionArgs a) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4, all = a.keys * a.kv_heads * a.dim;
+  uint16_t* to = blockIdx.y == 0 ? a.d_k : a.d_v;
+  if (i >= all || to == nullptr) return;
+  const float* p = sums_of(a, blockIdx.y, 0) + i;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll 4
+  for (int s = 1; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4*>(p + s * all);
+  const float by = blockIdx.y == 0 ? a.scale : 1.0f;
+  *reinterpret_cast<u32x2*>(to + i) = pack4(sum[0] * by, sum[1] * by, sum[2] * by, sum[3] * by);
+}
+
+hipError_t join_key_gradients(const AttentionArgs& a, hipStream_t st) {
+  if (a.splits == 1 || a.keys == 0) return hipSuccess;
+  const int64_t quads = a.keys * a.kv_heads * a.dim / 4;
+  key_gradient_join_kernel<<<dim3(static_cast<uint32_t>((quads + 255) / 256), 2), 256, 0, st>>>(a);
   return hipGetLastError();
 }
 
@@ -910,13 +965,15 @@ hipError_t backward(const AttentionArgs& a, hipStream_t st) {
   if (e != hipSuccess) return e;
   // both gradients of 256 columns at once would not leave a lane registers for the scores
   if (DP < 256 && a.d_k != nullptr && a.d_v != nullptr) {
-    if (wide_key_tiles(a)) return launch_key_gradient<KeyGradient<DP, EXACT, NB, 1, DP < 256, true>>(a, st);
-    return launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, DP < 256, true>>(a, st);
+    e = wide_key_tiles(a) ? launch_key_gradient<KeyGradient<DP, EXACT, NB, 1, DP < 256, true>>(a, st)
+                          : launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, DP < 256, true>>(a, st);
+    return e != hipSuccess ? e : join_key_gradients(a, st);
   }
   if (a.d_k != nullptr)
     if (e = launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, true, false>>(a, st); e != hipSuccess) return e;
-  if (a.d_v != nullptr) return launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, false, true>>(a, st);
-  return hipSuccess;
+  if (a.d_v != nullptr)
+    if (e = launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, false, true>>(a, st); e != hipSuccess) return e;
+  return a.d_k != nullptr || a.d_v != nullptr ? join_key_gradients(a, st) : hipSuccess;
 }
 
 template <class F>

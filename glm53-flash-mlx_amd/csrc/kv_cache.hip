@@ -118,7 +118,7 @@ __device__ __forceinline__ u32x2 codes_to_bf16(uint32_t codes, float scale) {
 __device__ __forceinline__ float scale_value(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // A wavefront reads one token.  Bound by the bytes: 34,096 tokens of 8 heads of 128
-// from E4M3 33.8 us, 6.2 TB/s (partly of the last-level cache).
+// from E4M3 33.5 us, 6.2 TB/s (partly of the last-level cache).
 template <bool E4M3, int LANES>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const CacheArgs& c = a.cache;
@@ -204,8 +204,8 @@ namespace {
 // heads of 128).
 //
 // That case reads 5.3 TB/s, 64 sequences of up to 8,192 tokens 5.7 in bf16 and 4.8 in
-// E4M3 (165 us); a copy on the card reaches 5.0.  The smallest call takes 6.2 us here,
-// loads that wait for each other (lengths, table, keys), and 5.2 in the join.
+// E4M3 (160 us); a copy on the card reaches 5.0.  The smallest call takes 6.2 us here,
+// loads that wait for each other (lengths, table, keys), and 4.7 in the join.
 
 constexpr int kHeads = 16;  // columns of the MFMA
 

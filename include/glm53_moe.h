@@ -700,6 +700,11 @@ int glm53_packed_attention(const glm53_attention* attention, void* stream);
  * in FP32 in a fixed order.  P and dS are rounded to BF16 as operands.  Rows
  * of no sequence get 0.  Results may not overlap inputs. */
 size_t glm53_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t heads);
+/* What a workspace may have beyond that: with these bytes (0: none are wanted) the
+ * rows of few key heads' gradients are split over the card, and their FP32 parts
+ * added in their order.  Without, the call takes longer. */
+size_t glm53_packed_attention_backward_split_bytes(int64_t tokens, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads,
+                                                   int64_t head_dim);
 int glm53_packed_attention_backward(const glm53_attention* attention, void* stream);
 
 /* A cache of keys and values: `pages` pages of page_size tokens (a power of two

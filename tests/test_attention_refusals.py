@@ -90,6 +90,19 @@ def test_attention_without_rows_and_workspace_sizes(N, libso):
     assert 0 < paged(64, 0) <= paged(128, 1) <= paged(256, 1) < 1 << 26
 
 
+def test_split_bytes(libso):
+    """Parts of few key heads' gradients: FP32 [splits, keys, kv_heads, dim] of d_k and d_v."""
+    size = libso.glm53_packed_attention_backward_split_bytes
+    for refused in ((0, 8, 1, 8, 1, 64), (8, 0, 1, 8, 1, 64), (1 << 28, 8, 1, 8, 1, 64), (4096, 4096, 1, 8, 3, 64),
+                    (4096, 4096, 1, 8, 0, 64), (4096, 4096, 1, 8, 1, 512), (4096, 4096, 1 << 24, 8, 1, 64)):
+        assert size(*refused) == 0
+    assert size(8192, 8192, 1, 8, 1, 128) == 8 * 8192 * 128 * 8  # 128 tiles
+    assert size(8192, 8192, 0, 8, 1, 128) == size(8192, 8192, 1, 8, 1, 128)  # no offsets
+    assert size(8192, 8192, 30, 8, 1, 128) == 0  # short sequences
+    assert size(4096, 4096, 1, 16, 8, 128) == 0  # tiles enough
+    assert size(100, 100, 1, 8, 1, 128) == 0
+
+
 def _cache(N, **changes):
     c = N.KVCache(k_pages=FAKE, v_pages=FAKE, k_scales=None, v_scales=None, page_table=FAKE, pages=4, page_size=16, kv_heads=2,
                   head_dim=64, sequences=3, max_pages=2, table_stride=2, e4m3=0)

@@ -98,6 +98,45 @@ def test_longer(dev, dim, causal):
     run(dev, [1100, 900], [1100, 900], 4, 2, dim, causal)
 
 
+@pytest.mark.parametrize("queries, keys, heads, kv_heads, dim, causal", [
+    ([3000], [3000], 8, 1, 128, True), ([2900, 0, 350], [2900, 0, 350], 8, 1, 64, True), ([2900], [2900], 8, 1, 96, False),
+    ([1500], [1500], 8, 2, 256, True), ([1500], [1500], 8, 2, 200, False), ([5000], [70], 6, 2, 128, False),
+    ([5000], [70], 6, 2, 128, True), ([600, 2500], [2600, 500], 5, 1, 128, True),
+])
+def test_gradients_of_few_keys(dev, queries, keys, heads, kv_heads, dim, causal):
+    """The rows of a tile of keys are split, and the parts added; every subset of
+    gradients alone has the joint call's bits, and without the workspace for the
+    parts the call gives the same results but for their rounding."""
+    import torch
+
+    N = submodule("_native")
+    size = N.lib().glm53_packed_attention_backward_split_bytes
+    assert size(sum(queries), sum(keys), len(queries), heads, kv_heads, dim) > 0
+    q, k, v, d_out, args, got = run(dev, queries, keys, heads, kv_heads, dim, causal)
+    A = submodule("attention")
+    out, lse = A.native_packed_attention(q, k, v, *args, causal, dim**-0.5, True)
+
+    def gradients_of(wanted):
+        return A.native_packed_attention_backward(q, k, v, *args, out, lse, d_out, causal, dim**-0.5, wanted)
+
+    for wanted in ([False, True, False], [False, False, True], [False, True, True]):
+        for g, name in zip(gradients_of(wanted), ("d_q", "d_k", "d_v")):
+            assert g is None or torch.equal(g, got[name]), (wanted, name)
+
+
+def test_parts_and_infinities(dev):
+    """An infinity in a row of one part reaches the keys that the row sees, and no other."""
+    import torch
+
+    q, k, v, d_out = inputs(dev, 3000, 3000, 4, 1, 64)
+    want = gradients(q, k, v, d_out)
+    d_out[1500, 1, 3] = float("inf")
+    got = gradients(q, k, v, d_out)
+    assert bool(got["d_v"][:1501, 0, 3].isinf().all())
+    for name in ("d_k", "d_v"):
+        assert torch.equal(got[name][1501:], want[name][1501:])
+
+
 @pytest.mark.parametrize("dim, causal, heads, tokens", [(128, False, 8, 4200), (64, False, 8, 4200), (96, False, 8, 4200),
                                                         (128, True, 32, 2100), (64, True, 32, 2100)])
 def test_wide_key_tiles(dev, dim, causal, heads, tokens):
