@@ -702,7 +702,7 @@ int glm53_packed_attention(const glm53_attention* attention, void* stream);
 size_t glm53_packed_attention_backward_workspace_bytes(int64_t tokens, int64_t heads);
 /* What a workspace may have beyond that: with these bytes (0: none are wanted) the
  * rows of few key heads' gradients are split over the card, and their FP32 parts
- * added in their order.  Without, the call takes longer. */
+ * added in their order (up to 134 MB, of heads of 256).  Without, the call takes longer. */
 size_t glm53_packed_attention_backward_split_bytes(int64_t tokens, int64_t keys, int64_t sequences, int64_t heads, int64_t kv_heads,
                                                    int64_t head_dim);
 int glm53_packed_attention_backward(const glm53_attention* attention, void* stream);

@@ -105,8 +105,7 @@ def test_longer(dev, dim, causal):
 ])
 def test_gradients_of_few_keys(dev, queries, keys, heads, kv_heads, dim, causal):
     """The rows of a tile of keys are split, and the parts added; every subset of
-    gradients alone has the joint call's bits, and without the workspace for the
-    parts the call gives the same results but for their rounding."""
+    gradients alone has the joint call's bits."""
     import torch
 
     N = submodule("_native")
@@ -122,6 +121,30 @@ def test_gradients_of_few_keys(dev, queries, keys, heads, kv_heads, dim, causal)
     for wanted in ([False, True, False], [False, False, True], [False, True, True]):
         for g, name in zip(gradients_of(wanted), ("d_q", "d_k", "d_v")):
             assert g is None or torch.equal(g, got[name]), (wanted, name)
+
+
+def test_without_the_workspace_of_parts(dev):
+    """The native call with the least workspace does not split, and is right too."""
+    import ctypes
+
+    import torch
+
+    A, N = submodule("attention"), submodule("_native")
+    q, k, v, d_out = inputs(dev, 2000, 2000, 8, 1, 128)
+    out, lse = A.native_packed_attention(q, k, v, None, None, True, 128**-0.5, True)
+    d, alive = A._descriptor(q, k, v, None, None, out, lse, True, 128**-0.5)
+    d_out, d.d_out = A.head_rows(d_out)
+    got = {"d_q": torch.empty_like(q), "d_k": torch.empty_like(k), "d_v": torch.empty_like(v)}
+    d.d_q, d.d_k, d.d_v = (t.data_ptr() for t in got.values())
+    least = N.lib().glm53_packed_attention_backward_workspace_bytes(2000, 8)
+    assert N.lib().glm53_packed_attention_backward_split_bytes(2000, 2000, 0, 8, 1, 128) > 0
+    guarded = torch.full((least + 4096,), 77, dtype=torch.uint8, device=dev)
+    d.workspace, d.workspace_bytes = guarded.data_ptr(), least
+    N.run(q.get_device(), N.lib().glm53_packed_attention_backward, ctypes.byref(d))
+    want = attention64(q, k, v, [0, 2000], [0, 2000], True, None, d_out)
+    for name in got:
+        check(got[name], want[name], name)
+    assert bool((guarded[least:] == 77).all())
 
 
 def test_parts_and_infinities(dev):
