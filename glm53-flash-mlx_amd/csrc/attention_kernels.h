@@ -20,7 +20,8 @@ namespace {
 // How a tile is multiplied: every place of it seen; some masked; or masked,
 // with infinities and NaNs in masked places kept from the results.  The last is the price
 // of a kernel's second pass, which follows where the first one's results are
-// not all finite: they may be what 0 x NaN made of a masked place.
+// not all finite: they may be what 0 x NaN made of a masked place, or sums that
+// passed FP32's range.
 enum How { kPlain, kMasked, kCareful };
 template <int N>
 using Constant = std::integral_constant<int, N>;
@@ -49,7 +50,10 @@ __device__ __forceinline__ void products(bool begin) {
 constexpr float kLog2e = 1.44269504088896340736f;
 // A row's maximum is kept until a new one is this many powers of two above it:
 // the weights 2^(s - m) then reach 2^8, which changes no relative rounding, and
-// few tiles after the first rescale their sums.
+// few tiles after the first rescale their sums.  Sums of such weights times values
+// may pass FP32's range where their mean does not: the second pass takes a row whose
+// results were not finite with weights 2^-40 of these, whose sum is below 1 over 2^30
+// keys.  Powers of two change no bit, but of values below 2^-86 beside such large ones.
 constexpr float kSlack = 8.0f;
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -232,9 +236,12 @@ struct Forward {
 
     const float c = a.scale * kLog2e;
     f32x16 out[T];
+    // whole tiles two at a time: their places in LDS are constants then
+    const int whole = all_see / kKeys & ~1;
     float m, l;  // m in units of scores; l: this lane's part
+    float by = 1.0f;  // of the row's weights as operands, in the second pass
     uint32_t dirty = 0;
-    // `how`: kPlain, kMasked, or kCareful (see finite_part)
+    // `how`: kPlain, kMasked, or kCareful (see finite_part), which takes whole tiles too
     const auto compute = [&](int step, auto stage, auto how) {
       constexpr int kHow = decltype(how)::value;
       const int kt = stage * 2 * Tile::kBytes, vt = kt + Tile::kBytes;
@@ -252,13 +259,16 @@ struct Forward {
           for (int t = 0; t < T; ++t) x[t] = at.across(vt, n - 2 * kGroups, t);
         }
       };
-      read(0);
-      read(1);
+      // the second pass reads none ahead: its registers, the most of both, would put the first one's into
+      // memory (4,096 causal tokens, 16 / 4 heads of 256: 207 us, with two ahead 230; of 200: 233 and 257)
+      constexpr int kAhead = kHow == kCareful ? 0 : 2;
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) read(n);
       products(true);
 #pragma unroll
       for (int n = 0; n < 2 * kGroups; ++n) {
         fence();
-        read(n + 2);
+        read(n + kAhead);
         f32x16& x = s[n / kGroups];
 #pragma unroll
         for (int j = 0; j < 4; ++j) x = mfma32(f[n % 3][j], q[4 * (n % kGroups) + j], n % kGroups + j == 0 ? zero16() : x);
@@ -299,6 +309,7 @@ struct Forward {
         for (int e = 8 * (i & 1); e < 8 * (i & 1) + 8; ++e) {
           x[e] = exp2_fast(fmaf(x[e], c, -mc));
           sum += x[e];
+          if constexpr (kHow == kCareful) x[e] *= by;
         }
         l += sum;
         next = operand8(x, i & 1);
@@ -309,11 +320,11 @@ struct Forward {
       for (int i = 0; i < 4; ++i) {
         fence();
         const int n = 2 * kGroups + i;
-        read(n + 2);
+        read(n + kAhead);
         const bf16x8 p = next;
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-          if constexpr (kHow == kCareful) f[n % 3][t] = finite_part(f[n % 3][t], dirty);
+          if constexpr (kHow == kCareful) f[n % 3][t] = finite_part(f[n % 3][t], dirty, step < whole ? 0 : kSigns);
           out[t] = mfma32(f[n % 3][t], p, out[t]);
         }
         if (i < 3) weigh(i + 1);
@@ -322,15 +333,13 @@ struct Forward {
       products(false);
     };
 
-    // whole tiles two at a time: their places in LDS are constants then
-    const int whole = all_see / kKeys & ~1;
     const auto pass = [&](auto how) {
       m = -INFINITY;
       l = 0.0f;
 #pragma unroll
       for (int t = 0; t < T; ++t) out[t] = zero16();
       int step = 0;
-      for (; step < whole; step += 2) {
+      for (; decltype(how)::value != kCareful && step < whole; step += 2) {
         loads_done();
         issue(step + 1);
         compute(step, Constant<0>{}, Constant<kPlain>{});
@@ -345,7 +354,9 @@ struct Forward {
       }
     };
     pass(Constant<kMasked>{});
-    if (voted<W>(nonfinite(out), lds, wave)) {
+    const bool wrong = nonfinite(out);
+    if (voted<W>(wrong, lds, wave)) {
+      if (both_sum(wrong ? 1.0f : 0.0f) != 0.0f) by = 0x1p-40f;
       issue(0);
       pass(Constant<kCareful>{});
       if (__any(dirty != 0))
@@ -353,7 +364,7 @@ struct Forward {
                           [&](int key) { return key < lim; });
     }
 
-    const float total = both_sum(l), inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    const float total = both_sum(l), inverse = total == 0.0f ? 0.0f : 1.0f / (total * by);
     if (row >= seg.last) return;
     const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
     store_operand<DP>(a.out + (token * heads + query_head) * dim, out, inverse, dim, h);

@@ -225,11 +225,13 @@ struct HeadTile {
 // multiplies the values of such a tile with their infinities and NaNs replaced
 // by 0 (`dirty` where there was one), and what the mask lets through of those is
 // added afterwards by add_nonfinite.
-__device__ __forceinline__ bf16x8 finite_part(bf16x8 v, uint32_t& dirty) {
+// With `signs` 0 a tile stays as it is.
+constexpr uint32_t kSigns = 0x80008000u;
+__device__ __forceinline__ bf16x8 finite_part(bf16x8 v, uint32_t& dirty, uint32_t signs = kSigns) {
   u32x4 w = __builtin_bit_cast(u32x4, v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t bad = ((w[i] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;  // exponents all ones
+    const uint32_t bad = ((w[i] & 0x7F807F80u) + 0x00800080u) & signs;  // exponents all ones
     dirty |= bad;
     w[i] &= ~(bad | (bad - (bad >> 15)));
   }
