@@ -1,5 +1,7 @@
 // The paged key-value cache: rows written (and quantised), rows read back,
 // and the attention of one token a sequence over its pages.
+#include <type_traits>
+
 #include "attention_tile.h"
 #include "kv_cache.h"
 
@@ -207,7 +209,14 @@ namespace {
 // E4M3 (160 us); a copy on the card reaches 5.0.  The smallest call takes 6.2 us here,
 // loads that wait for each other (lengths, table, keys), and 4.7 in the join.
 
+// Sums of weights, which reach 2^8, times values may pass FP32's range where their mean
+// does not, and a weight times its row's power of two a bf16 operand's.  A head whose part of
+// a run is not finite takes the run again with weights kSmaller of these, whose sum is
+// below 1 over 2^31 tokens (powers of two change no bit, but of values below 2^-86 beside
+// such large ones); the join takes all of its parts so.
+//
 constexpr int kHeads = 16;  // columns of the MFMA
+constexpr float kSmaller = 0x1p-40f;
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -310,6 +319,20 @@ struct Shares {
   __device__ __forceinline__ int worker(int64_t u) const { return static_cast<int>(((u + 1) * WORKERS - 1) / units); }
 };
 
+// Whether not all of a lane's sums are finite.
+__device__ __forceinline__ bool nonfinite(const f32x4& x) {
+  return fmaf(x[0], 0.0f, x[1] * 0.0f) + fmaf(x[2], 0.0f, x[3] * 0.0f) != 0.0f;
+}
+template <int T>
+__device__ __forceinline__ bool nonfinite(const f32x4 (&x)[T]) {
+  f32x4 sum = {0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum[r] = fmaf(x[t][r], 0.0f, sum[r]);
+  return nonfinite(sum);
+}
+
 // Which wavefronts have parts of one (sequence, head): first .. last, the first one its start.
 struct Split {
   int sequence, part, first, last;
@@ -332,7 +355,7 @@ struct Decode {
   // 64 x 8192 tokens in bf16 470 us for 381)
   static constexpr int kWorkers = 256 * (160 * 1024 / kLds < 4 ? 160 * 1024 / kLds : 4);
   static constexpr int kLoads = 2 * (TS / kLoadRows) + E4M3;  // of a whole stage
-  static constexpr int kPartial = kHeads * (DP + 2);  // floats: sums, then maximum and total of each head
+  static constexpr int kPartial = kHeads * (DP + 2);  // floats: sums, then maximum and total of each head (negative: both kSmaller)
   static constexpr size_t kPartials = sizeof(float) * 2 * kWorkers * kPartial, kSpace = kPartials + sizeof(Split) * kWorkers;
   // What a join finds in its Split: with few (sequence, head) parts each has one, with more of them
   // each worker has that of the one which it begins and others end.
@@ -380,8 +403,7 @@ struct Decode {
       const int part = static_cast<int>((unit - base) / chunks);
       const int64_t seg = base + part * chunks;  // its first unit
       const int head = part / shares.head_parts, first_head = (part - head * shares.head_parts) * kHeads;
-      int64_t stage = unit - seg;
-      const int64_t from = stage, to = end - seg < chunks ? end - seg : chunks;
+      const int64_t from = unit - seg, to = end - seg < chunks ? end - seg : chunks;
       bool bad = !__builtin_amdgcn_readlane(shares.whole, at);
 
       // The pages of the next 64 16-token parts, one a lane.
@@ -398,7 +420,7 @@ struct Decode {
           }
         }
       };
-      look_up(stage);
+      look_up(from);
       // q of 16 heads as the second operand
       bf16x8 q[DP / 32];
       const int g = first_head + col;
@@ -443,15 +465,13 @@ struct Decode {
         }
       };
 
-      issue(stage, 0, 0);
+      issue(from, 0, 0);
 #pragma unroll
       for (int j = 0; j < DP / 32; ++j) arrived(q[j]);
-      float m = -INFINITY, l = 0.0f;
+      float m, l, by = 1.0f;  // by: of the head's weights as operands, when the run is taken again
       f32x4 out[DP / 16];
-#pragma unroll
-      for (int t = 0; t < DP / 16; ++t) out[t] = (f32x4){0, 0, 0, 0};
 
-      const auto compute = [&](int64_t stage, int slot) {
+      const auto compute = [&](int64_t stage, int slot, auto again) {
         const uint8_t* kt = lds + slot * kStage;
         const uint8_t* vt = kt + kTile;
         const int64_t left64 = tokens - stage * TS;
@@ -511,8 +531,9 @@ struct Decode {
           for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float w = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc, -mc));
+              float w = __builtin_amdgcn_exp2f(fmaf(s[b][r], sc, -mc));
               l += w;
+              if constexpr (again) w *= by;
               p[4 * b + r] = static_cast<__bf16>(!E4M3 ? w : left < TS && 16 * b + r >= here ? 0.0f : w * vs[b][r]);
             }
 #pragma unroll
@@ -529,23 +550,38 @@ struct Decode {
       };
 
       constexpr int kAhead = 64 / kSub;  // stages of a look-up
-      int slot = 0, ahead = 0;
-      for (; stage < to; ++stage, slot ^= 1) {
-        if (stage + 1 < to) {
-          if (++ahead == kAhead) {
-            ahead = 0;
-            look_up(stage + 1);
-            arrived(pages);
-          }
-          issue(stage + 1, slot ^ 1, ahead);
-          if ((stage + 2) * TS <= tokens)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
-          else
+      const auto pass = [&](auto again) {  // of stages from .. to - 1, of which the first one's loads are on their way
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) out[t] = (f32x4){0, 0, 0, 0};
+        int slot = 0, ahead = 0;
+        for (int64_t stage = from; stage < to; ++stage, slot ^= 1) {
+          if (stage + 1 < to) {
+            if (++ahead == kAhead) {
+              ahead = 0;
+              look_up(stage + 1);
+              arrived(pages);
+            }
+            issue(stage + 1, slot ^ 1, ahead);
+            if ((stage + 2) * TS <= tokens)
+              asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+            else
+              asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        } else {
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          }
+          compute(stage, slot, again);
         }
-        compute(stage, slot);
+      };
+      pass(std::false_type{});
+      const bool wrong = nonfinite(out);
+      if (__any(wrong)) {
+        if (quarter_sum(wrong ? 1.0f : 0.0f) != 0.0f) by = kSmaller;
+        look_up(from);
+        arrived(pages);
+        issue(from, 0, 0);
+        pass(std::true_type{});
       }
 
       if (from == 0 && lane == 0 && (by_segment || to != chunks))
@@ -555,7 +591,7 @@ struct Decode {
       if (__any(bad)) l = NAN;
       if (g < a.group) {
         if (from == 0 && to == chunks) {
-          const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+          const float inverse = l == 0.0f ? 0.0f : 1.0f / (l * by);
           uint16_t* o = a.out + (static_cast<int64_t>(sequence) * c.kv_heads * a.group + head * a.group + g) * c.dim;
 #pragma unroll
           for (int t = 0; t < DP / 16; ++t) {
@@ -569,7 +605,7 @@ struct Decode {
           for (int t = 0; t < DP / 16; ++t) *reinterpret_cast<f32x4*>(p + col * DP + 16 * t + 4 * quarter) = out[t];
           if (quarter == 0) {
             p[kHeads * DP + 2 * col] = m;
-            p[kHeads * DP + 2 * col + 1] = l;
+            p[kHeads * DP + 2 * col + 1] = by == 1.0f ? l : -l * by;  // the sign says by which the sums are
           }
         }
       }
@@ -676,6 +712,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
       m[i] = p[kHeads * DP + 2 * hd];
       l[i] = p[kHeads * DP + 2 * hd + 1];
       if (d < c.dim) x[i] = *reinterpret_cast<const f32x4*>(p + hd * DP + d);
+      if (l[i] < 0.0f) x[i] = (f32x4){NAN, NAN, NAN, NAN};
     }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) add(m[i], l[i], x[i]);
@@ -696,6 +733,17 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
     }
   }
   if (group != 0 || d >= c.dim) return;
+  if (nonfinite(sum)) {  // past FP32's range, a part with smaller weights, or no numbers: one part after the other
+    top = -INFINITY;
+    total = 0.0f;
+    sum = (f32x4){0, 0, 0, 0};
+    for (int w = first; w <= last; ++w) {
+      if (start(w) >= start(w + 1)) continue;
+      const float* p = a.partial + static_cast<int64_t>(2 * w + (w == first ? 1 : 0)) * D::kPartial;
+      const float l = p[kHeads * DP + 2 * hd + 1], by = l < 0.0f ? 1.0f : kSmaller;
+      add(p[kHeads * DP + 2 * hd], fabsf(l) * by, by * *reinterpret_cast<const f32x4*>(p + hd * DP + d));
+    }
+  }
   const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
   uint16_t* o = a.out + (static_cast<int64_t>(sequence) * heads + query_head) * c.dim + d;
   *reinterpret_cast<u32x2*>(o) = pack4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
