@@ -13,7 +13,6 @@ The reference's attention is sparse and recurrent and has no counterpart.
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -23,7 +22,7 @@ from . import ops as _ops
 MAX_HEAD_DIM = 256
 MAX_STRIDE = 1 << 22  # elements from one token, or one head, to the next
 MAX_HEAD_SPAN = 1 << 30  # of a token's heads together
-MIN_SCALE = 2.0**-64
+MIN_SCALE, MAX_SCALE = 2.0**-64, 2.0**127  # the largest: its product with log2 e is an FP32 number
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor | None = None,
@@ -37,7 +36,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     key_offsets: the same for keys, where they are not the queries' own (a
     chunk of a prompt over all of its keys).  causal: the last query of a sequence
     sees all of its keys, each one before it one key less.  Queries that see no key,
-    and rows of no sequence, are 0.  scale: 1 / sqrt(dim) where None, 2^-64 or more.
+    and rows of no sequence, are 0.  scale: 1 / sqrt(dim) where None, 2^-64 to 2^127.
 
     heads a multiple of kv_heads, dim a multiple of 8 up to 256.  q, k and v
     may be views of one tensor (a joint projection's) without a copy.
@@ -86,8 +85,8 @@ def check_offsets(name: str, t: torch.Tensor | None) -> None:
 
 def check_scale(scale: float | None, dim: int) -> float:
     scale = dim**-0.5 if scale is None else float(scale)
-    if not MIN_SCALE <= scale < math.inf:
-        raise ValueError(f"scale must be finite and 2^-64 or more, got {scale}")
+    if not MIN_SCALE <= scale <= MAX_SCALE:
+        raise ValueError(f"scale must be from 2^-64 to 2^127, got {scale}")
     return scale
 
 

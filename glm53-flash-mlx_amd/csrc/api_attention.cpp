@@ -1,7 +1,5 @@
 // C ABI of attention (declared in include/glm53_moe.h): packed sequences with
 // their gradients, the paged key-value cache and one token over it.
-#include <cmath>
-
 #include "api_util.h"
 #include "attention.h"
 #include "kv_cache.h"
@@ -17,6 +15,7 @@ constexpr int64_t kMaxGrid = int64_t{1} << 23;  // workgroups of up to 512 threa
 constexpr int64_t kMaxCopied = 4 * kMaxGrid;    // rows, four a workgroup, that one call writes to or reads from a cache
 // The rows' logarithms over this are where the gradients' products start: still finite.
 constexpr float kLeastScale = 0x1p-64f;
+constexpr float kMostScale = 0x1p127f;  // its product with log2 e: still finite
 
 int head_rows(const glm53_head_rows& r, int64_t heads, const char* name, bool wanted, Rows16& out) {
   CHECK_ARG(!wanted || r.data != nullptr, "null pointer argument: %s", name);
@@ -40,7 +39,7 @@ int head_shape(int64_t heads, int64_t kv_heads, int64_t dim) {
 }
 
 int check_scale(float scale) {
-  CHECK_ARG(scale >= kLeastScale && std::isfinite(scale), "scale must be finite and 2^-64 or more");
+  CHECK_ARG(scale >= kLeastScale && scale <= kMostScale, "scale must be from 2^-64 to 2^127");
   return GLM53_OK;
 }
 

@@ -692,7 +692,7 @@ typedef struct glm53_attention {
   void* workspace; /* 256-byte aligned, needs no initialisation */
   size_t workspace_bytes;
   int32_t causal;
-  float scale; /* 2^-64 or more */
+  float scale; /* 2^-64 to 2^127 */
 } glm53_attention;
 int glm53_packed_attention(const glm53_attention* attention, void* stream);
 /* delta = sum(d_out out), dP = d_out v^T, dS = P (dP - delta); d_q = scale dS
