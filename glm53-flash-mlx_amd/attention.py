@@ -36,7 +36,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     key_offsets: the same for keys, where they are not the queries' own (a
     chunk of a prompt over all of its keys).  causal: the last query of a sequence
     sees all of its keys, each one before it one key less.  Queries that see no key,
-    and rows of no sequence, are 0.  scale: 1 / sqrt(dim) where None, 2^-64 to 2^127.
+    and rows of no sequence, are 0, those whose largest scaled score is beyond FP32 NaN.
+    scale: 1 / sqrt(dim) where None, 2^-64 to 2^127.
 
     heads a multiple of kv_heads, dim a multiple of 8 up to 256.  q, k and v
     may be views of one tensor (a joint projection's) without a copy.

@@ -364,12 +364,14 @@ struct Forward {
                           [&](int key) { return key < lim; });
     }
 
-    const float total = both_sum(l), inverse = total == 0.0f ? 0.0f : 1.0f / (total * by);
+    // no key seen; or scores that are no FP32 numbers once scaled, which leave no weights: NaN
+    const float none = m * c == INFINITY ? NAN : 0.0f;
+    const float total = both_sum(l), inverse = total == 0.0f ? none : 1.0f / (total * by);
     if (row >= seg.last) return;
     const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
     store_operand<DP>(a.out + (token * heads + query_head) * dim, out, inverse, dim, h);
     if (a.lse != nullptr && h == 0)
-      a.lse[static_cast<int64_t>(head) * a.tokens * a.group + row] = total == 0.0f ? 0.0f : m * c + __builtin_amdgcn_logf(total);
+      a.lse[static_cast<int64_t>(head) * a.tokens * a.group + row] = total == 0.0f ? none : m * c + __builtin_amdgcn_logf(total);
   }
 };
 

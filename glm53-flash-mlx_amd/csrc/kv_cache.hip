@@ -333,6 +333,10 @@ __device__ __forceinline__ bool nonfinite(const f32x4 (&x)[T]) {
   return nonfinite(sum);
 }
 
+// What a sum without a weight is divided into, with the largest scaled score: NaN of scores
+// that are no FP32 numbers once scaled, 0 where there are none.
+__device__ __forceinline__ float without_weights(float top) { return top == INFINITY ? NAN : 0.0f; }
+
 // Which wavefronts have parts of one (sequence, head): first .. last, the first one its start.
 struct Split {
   int sequence, part, first, last;
@@ -591,7 +595,7 @@ struct Decode {
       if (__any(bad)) l = NAN;
       if (g < a.group) {
         if (from == 0 && to == chunks) {
-          const float inverse = l == 0.0f ? 0.0f : 1.0f / (l * by);
+          const float inverse = l == 0.0f ? without_weights(m * sc) : 1.0f / (l * by);
           uint16_t* o = a.out + (static_cast<int64_t>(sequence) * c.kv_heads * a.group + head * a.group + g) * c.dim;
 #pragma unroll
           for (int t = 0; t < DP / 16; ++t) {
@@ -744,7 +748,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
       add(p[kHeads * DP + 2 * hd], fabsf(l) * by, by * *reinterpret_cast<const f32x4*>(p + hd * DP + d));
     }
   }
-  const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+  const float inverse = total == 0.0f ? without_weights(top * sc) : 1.0f / total;
   uint16_t* o = a.out + (static_cast<int64_t>(sequence) * heads + query_head) * c.dim + d;
   *reinterpret_cast<u32x2*>(o) = pack4(sum[0] * inverse, sum[1] * inverse, sum[2] * inverse, sum[3] * inverse);
 }

@@ -672,7 +672,9 @@ typedef struct glm53_head_rows {
  * sequence of all, key_offsets NULL too).  Offsets out of range are taken as the
  * nearest one in it; results of sequences whose offsets descend mean nothing.
  * causal: query i of n sees keys 0 .. i + (the sequence's keys) - n, so that the
- * last query sees them all.  A query that sees no key, and rows of no sequence, are 0.  Query head h reads key head h / (heads / kv_heads).
+ * last query sees them all.  A query that sees no key, and rows of no sequence, are 0;
+ * one whose largest scaled score is beyond FP32 is NaN.  Query head h reads key head
+ * h / (heads / kv_heads).
  * head_dim a multiple of 8 up to 256; tokens * heads and keys * heads below 2^30.
  * Scores, softmax and sums are FP32; P is rounded to BF16 as an operand, out once. */
 typedef struct glm53_attention {

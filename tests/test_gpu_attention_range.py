@@ -77,3 +77,17 @@ def test_rows_and_columns_beside_large_ones_keep_their_bits(dev):
     w[150] = float("nan")
     again = M.packed_attention(q, k, w)
     assert torch.equal(again[:150], got[:150]) and bool(again[150:].isnan().all())
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_scores_that_no_number_holds(dev, causal):
+    """Scaled scores past FP32's range give NaN, of results and of what they reach, not 0."""
+    q, k, v, d_out = inputs(dev, 150, 150, 2, 1, 64)
+    want = gradients(q, k, v, d_out, index([0, 60, 150], dev), causal=causal, scale=4.0)
+    q, k = q.clone(), k.clone()
+    q[70, 1], k[60:62, 0] = 2.0**60, 2.0**61  # 2^127 of scores, which are numbers
+    got = gradients(q, k, v, d_out, index([0, 60, 150], dev), causal=causal, scale=4.0)
+    assert bool(got["out"][70, 1].isnan().all()) and bool(got["d_q"][70, 1].isnan().all())
+    assert bool(got["d_k"][60].isnan().all()) and bool(got["d_v"][60].isnan().all())
+    for name in got:  # the other sequence
+        assert (got[name][:60] == want[name][:60]).all(), name

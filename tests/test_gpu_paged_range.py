@@ -85,3 +85,16 @@ def test_other_heads_keep_their_bits(dev, quantised):
     got = cache.attend(q, table, index(lengths, dev))
     assert torch.equal(got[1], want[1]) and torch.equal(got[0, :2], want[0, :2])
     assert bool(((got[0, 2:].double() - 2.0**126).abs() <= 2 * 2.0**-8 * 2.0**126).all())
+
+
+@pytest.mark.parametrize("lengths", [[1], [50], [20_000]])
+def test_scores_that_no_number_holds(dev, lengths):
+    """Scaled scores past FP32's range give NaN, not 0: in one part, and joined."""
+    n = lengths[0]
+    k, v = normal(dev, n, 1, 64, seed=1), normal(dev, n, 1, 64, seed=2)
+    k[n // 2] = 2.0**60
+    cache, table, _ = cached(dev, lengths, k, v, 16, False)
+    q = normal(dev, 1, 2, 64, seed=4)
+    q[0, 1] = 2.0**60
+    got = cache.attend(q, table, index(lengths, dev), scale=4.0)  # of 2^126
+    assert bool(got[0, 1].isnan().all())
