@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 
 from .norms import residual_norm, rms_norm
+from .self_attention import AttentionBatch
 
 
 class FeedForwardBlock(torch.nn.Module):
@@ -54,6 +55,8 @@ def run_blocks(blocks, residual: torch.Tensor, final_weight: torch.Tensor | None
     blocks = list(blocks)
     if not blocks:
         raise ValueError("run_blocks needs a block")
+    if isinstance(batch, AttentionBatch):
+        batch = batch.for_step()
     normed = None
     for block, after in zip(blocks, blocks[1:] + [None]):
         weight = final_weight if after is None else after.norm_weight

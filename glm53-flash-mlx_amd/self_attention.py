@@ -35,6 +35,24 @@ class KVCache:
                                v_scales=self.v_scales, scale=scale)
 
 
+class _After:
+    """The field ``AttentionBatch.after``: what was given, else made of the
+    lengths as they are when it is asked for.  What was made so is not taken as
+    given where it is handed on, as dataclasses.replace does."""
+
+    def __get__(self, batch, owner=None):
+        if batch is None:
+            return None  # the field's default
+        if batch._given is not None or batch.offsets is not None:
+            return batch._given
+        made = batch._tokens()
+        made.of_lengths = True
+        return made
+
+    def __set__(self, batch, value):
+        batch._given = None if getattr(value, "of_lengths", False) else value
+
+
 @dataclasses.dataclass
 class AttentionBatch:
     """Which rows of a step are whose, the same for every layer.
@@ -43,15 +61,15 @@ class AttentionBatch:
     new token a sequence).  With a cache: page_table and lengths as for
     ``append_kv``, and for chunks of prompts that are in the cache already
     key_offsets, the offsets of lengths + new tokens, and keys, their last one, as a number.
-    after: lengths + 1 of single tokens, made here where it is not given (a captured step gives
-    its own, and changes it with lengths)."""
+    after: what single tokens' sequences hold with them, lengths + 1 where it is not
+    given: as lengths are when a step runs, a captured one too."""
 
     offsets: torch.Tensor | None = None
     page_table: torch.Tensor | None = None
     lengths: torch.Tensor | None = None
     key_offsets: torch.Tensor | None = None
     keys: int | None = None
-    after: torch.Tensor | None = None
+    after: torch.Tensor | None = _After()
 
     def __post_init__(self):
         if (self.page_table is None) != (self.lengths is None):
@@ -60,8 +78,15 @@ class AttentionBatch:
             raise ValueError("a batch without a cache has offsets, and no key_offsets")
         if (self.key_offsets is None) != (self.keys is None) or (self.key_offsets is not None and self.offsets is None):
             raise ValueError("key_offsets and keys are given together, with offsets")
-        if self.offsets is None and self.after is None:
-            self.after = self.lengths + 1
+
+    def _tokens(self) -> torch.Tensor:
+        return self.lengths + 1
+
+    def for_step(self) -> "AttentionBatch":
+        """The same with `after` made once, for all layers of a step."""
+        if self.offsets is not None or self._given is not None:
+            return self
+        return dataclasses.replace(self, after=self._tokens())
 
 
 class SelfAttention(torch.nn.Module):

@@ -1,0 +1,50 @@
+"""CPU tests of AttentionBatch: what a step takes from it."""
+
+from __future__ import annotations
+
+import dataclasses
+
+from conftest import pkg
+
+
+def single(**changes):
+    import torch
+
+    table = torch.zeros(3, 2, dtype=torch.int32)
+    return pkg().AttentionBatch(**{**dict(page_table=table, lengths=torch.tensor([4, 0, 9], dtype=torch.int32)), **changes})
+
+
+def test_after_follows_the_lengths():
+    """In place, by assignment, and in a copy with other lengths."""
+    import torch
+
+    batch = single()
+    assert batch.after.tolist() == [5, 1, 10]
+    batch.lengths += 1
+    assert batch.after.tolist() == [6, 2, 11] and batch.for_step().after.tolist() == [6, 2, 11]
+    batch.lengths = torch.tensor([7, 7, 7], dtype=torch.int32)
+    assert batch.after.tolist() == [8, 8, 8]
+    other = dataclasses.replace(batch, lengths=batch.lengths + 5)
+    assert other.after.tolist() == [13, 13, 13]
+    other.lengths += 1
+    assert other.after.tolist() == [14, 14, 14]
+    taken = single(after=batch.after)  # another batch's, made there
+    assert taken.after.tolist() == [5, 1, 10]
+
+
+def test_an_own_after_stays():
+    import torch
+
+    own = torch.tensor([1, 2, 3], dtype=torch.int32)
+    batch = single(after=own)
+    batch.lengths += 1
+    assert batch.after is own and batch.for_step() is batch
+    assert dataclasses.replace(batch, lengths=batch.lengths + 1).after is own
+
+
+def test_packed_rows_have_none():
+    import torch
+
+    offsets = torch.tensor([0, 2, 5], dtype=torch.int32)
+    batch = pkg().AttentionBatch(offsets)
+    assert batch.after is None and batch.for_step() is batch

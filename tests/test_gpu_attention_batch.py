@@ -1,0 +1,102 @@
+"""GPU tests of SelfAttention over a cache as a serving loop uses it: a batch
+kept over steps, idle slots, prompts behind cached tokens."""
+
+from __future__ import annotations
+
+import pytest
+
+from conftest import pkg
+from test_gpu_self_attention import index, model, tables
+
+pytestmark = pytest.mark.gpu
+
+
+def cached_blocks(dev, quantised=False, pages=16):
+    """Two layers of attention and MLPs, and a function that gives them empty caches."""
+    blocks, final = model(dev)
+
+    def fresh():
+        for b in blocks:
+            if hasattr(b.mlp, "cache"):
+                b.mlp.cache = pkg().KVCache(pages, 16, b.mlp.kv_heads, b.mlp.head_dim, quantised=quantised, device=dev)
+
+    return blocks, final, fresh
+
+
+def rows(dev, n, seed=0):
+    import torch
+
+    return torch.randn(n, 256, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).to(dev)
+
+
+@pytest.mark.parametrize("through", ["run_blocks", "module"])
+def test_a_batch_kept_over_steps(dev, through):
+    """Lengths that grow in place: each step's bits are those of a batch made for it."""
+    import torch
+
+    M = pkg()
+    blocks, final, fresh = cached_blocks(dev)
+    table = tables(dev, 2, 8)
+
+    def step(x, batch):
+        if through == "run_blocks":
+            return M.run_blocks(blocks, x, final, batch)[1]
+        return blocks[0].mlp(x, batch)
+
+    with torch.no_grad():
+        got = {}
+        for kept in (True, False):
+            fresh()
+            batch = M.AttentionBatch(page_table=table, lengths=index([0, 5], dev))
+            got[kept] = []
+            for n in range(20):
+                if not kept:
+                    batch = M.AttentionBatch(page_table=table, lengths=index([n, 5 + n], dev))
+                got[kept].append(step(rows(dev, 2, n), batch))
+                batch.lengths += 1
+        for a, b in zip(got[True], got[False]):
+            assert torch.equal(a, b)
+
+
+def test_a_captured_step_follows_the_lengths(dev):
+    """Without an `after` of its own, and with the lengths changed alone."""
+    import torch
+
+    M = pkg()
+    blocks, final, fresh = cached_blocks(dev)
+    table = tables(dev, 2, 8)
+    x, lengths = rows(dev, 2), index([0, 3], dev)
+    batch = M.AttentionBatch(page_table=table, lengths=lengths)
+    with torch.no_grad():
+        want = []
+        fresh()
+        for n in range(10):
+            want.append(M.run_blocks(blocks, rows(dev, 2, n), final, M.AttentionBatch(page_table=table, lengths=index([n, 3 + n], dev)))[1])
+        fresh()
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            M.run_blocks(blocks, x, final, batch)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = M.run_blocks(blocks, x, final, batch)[1]
+        for n in range(10):
+            x.copy_(rows(dev, 2, n))
+            lengths.copy_(index([n, 3 + n], dev))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[n]), n
+
+
+def test_a_compiled_step(dev):
+    import torch
+
+    M = pkg()
+    blocks, final, fresh = cached_blocks(dev)
+    fresh()
+    batch = M.AttentionBatch(page_table=tables(dev, 2, 8), lengths=index([0, 3], dev))
+    with torch.no_grad():
+        step = torch.compile(lambda x: M.run_blocks(blocks, x, final, batch)[1], backend="eager")
+        for n in range(3):
+            assert torch.equal(step(rows(dev, 2, n)), M.run_blocks(blocks, rows(dev, 2, n), final, batch)[1])
+            batch.lengths += 1
