@@ -62,7 +62,8 @@ class AttentionBatch:
     ``append_kv``, and for chunks of prompts that are in the cache already
     key_offsets, the offsets of lengths + new tokens, and keys, their last one, as a number.
     after: what single tokens' sequences hold with them, lengths + 1 where it is not
-    given: as lengths are when a step runs, a captured one too."""
+    given: as lengths are when a step runs, a captured one too.  A slot of single tokens is idle,
+    and its attention 0, where it holds nothing and has no first page (a negative one)."""
 
     offsets: torch.Tensor | None = None
     page_table: torch.Tensor | None = None
@@ -80,7 +81,10 @@ class AttentionBatch:
             raise ValueError("key_offsets and keys are given together, with offsets")
 
     def _tokens(self) -> torch.Tensor:
-        return self.lengths + 1
+        after, table = self.lengths + 1, self.page_table
+        if table.shape[:1] == after.shape and table.shape[1] > 0:  # others are refused where they are used
+            after = torch.where(table[:, 0] < 0, self.lengths, after)
+        return after
 
     def for_step(self) -> "AttentionBatch":
         """The same with `after` made once, for all layers of a step."""

@@ -48,3 +48,13 @@ def test_packed_rows_have_none():
     offsets = torch.tensor([0, 2, 5], dtype=torch.int32)
     batch = pkg().AttentionBatch(offsets)
     assert batch.after is None and batch.for_step() is batch
+
+
+def test_idle_slots_hold_nothing():
+    """A slot without a first page keeps its length: 0 where it is idle, a token without a page where it is not."""
+    import torch
+
+    table = torch.tensor([[3, -1], [-1, -1], [-1, 2]], dtype=torch.int32)
+    batch = single(page_table=table, lengths=torch.tensor([4, 0, 9], dtype=torch.int32))
+    assert batch.after.tolist() == [5, 0, 9] and batch.for_step().after.tolist() == [5, 0, 9]
+    assert single(page_table=table[:, :0]).after.tolist() == [5, 1, 10]

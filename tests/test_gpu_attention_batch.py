@@ -100,3 +100,34 @@ def test_a_compiled_step(dev):
         for n in range(3):
             assert torch.equal(step(rows(dev, 2, n)), M.run_blocks(blocks, rows(dev, 2, n), final, batch)[1])
             batch.lengths += 1
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_idle_slots(dev, quantised):
+    """A slot without tokens and pages: attention gives it 0, the blocks a finite row, the
+    other slots their own bits; one whose sequence has lost its page is NaN."""
+    import torch
+
+    M = pkg()
+    blocks, final, fresh = cached_blocks(dev, quantised, pages=17)
+    table = tables(dev, 2, 8)
+    idle = torch.cat([table[:1], torch.full((1, 8), -1, dtype=torch.int32, device=dev), table[1:]])
+    x = rows(dev, 3)
+    with torch.no_grad():
+        fresh()
+        batch = M.AttentionBatch(page_table=idle, lengths=index([0, 0, 5], dev))
+        for n in range(3):
+            got = M.run_blocks(blocks, x, final, batch)[1]
+            assert bool(got.isfinite().all())
+            batch.lengths += index([1, 0, 1], dev)
+        assert not bool(blocks[0].mlp(x, batch)[1].any())
+        # the same steps with a page for the idle slot: its neighbours' rows
+        fresh()
+        spare = M.AttentionBatch(page_table=idle.masked_fill(idle < 0, 16), lengths=index([0, 0, 5], dev))
+        for n in range(3):
+            want = M.run_blocks(blocks, x, final, spare)[1]
+            spare.lengths += index([1, 0, 1], dev)
+        assert torch.equal(got[[0, 2]], want[[0, 2]])
+        lost = M.AttentionBatch(page_table=idle, lengths=index([3, 7, 8], dev))
+        got = M.run_blocks(blocks, x, final, lost)[1]
+        assert bool(got[1].isnan().all()) and bool(got[[0, 2]].isfinite().all())
