@@ -56,7 +56,7 @@ def run_blocks(blocks, residual: torch.Tensor, final_weight: torch.Tensor | None
     if not blocks:
         raise ValueError("run_blocks needs a block")
     if isinstance(batch, AttentionBatch):
-        batch = batch.for_step()
+        residual, batch = batch.refuse(residual), batch.for_step()
     normed = None
     for block, after in zip(blocks, blocks[1:] + [None]):
         weight = final_weight if after is None else after.norm_weight

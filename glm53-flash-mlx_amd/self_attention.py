@@ -4,6 +4,7 @@ cache in serving.  No positions are encoded."""
 
 from __future__ import annotations
 
+import copy
 import dataclasses
 
 import torch
@@ -59,8 +60,10 @@ class AttentionBatch:
 
     offsets int32 [sequences + 1]: packed rows (None with a page_table: one
     new token a sequence).  With a cache: page_table and lengths as for
-    ``append_kv``, and for chunks of prompts that are in the cache already
-    key_offsets, the offsets of lengths + new tokens, and keys, their last one, as a number.
+    ``append_kv``.  Packed rows then attend to each other alone, so that their sequences
+    hold nothing yet (a step with a length that is not 0 gives NaN), or to all that
+    their sequences hold with them, by key_offsets, the offsets of lengths + new
+    tokens, and keys, their last one, as a number.
     after: what single tokens' sequences hold with them, lengths + 1 where it is not
     given: as lengths are when a step runs, a captured one too.  A slot of single tokens is idle,
     and its attention 0, where it holds nothing and has no first page (a negative one)."""
@@ -73,6 +76,7 @@ class AttentionBatch:
     after: torch.Tensor | None = _After()
 
     def __post_init__(self):
+        self._refused = False
         if (self.page_table is None) != (self.lengths is None):
             raise ValueError("page_table and lengths are given together")
         if self.page_table is None and (self.offsets is None or self.key_offsets is not None):
@@ -81,16 +85,27 @@ class AttentionBatch:
             raise ValueError("key_offsets and keys are given together, with offsets")
 
     def _tokens(self) -> torch.Tensor:
-        after, table = self.lengths + 1, self.page_table
-        if table.shape[:1] == after.shape and table.shape[1] > 0:  # others are refused where they are used
-            after = torch.where(table[:, 0] < 0, self.lengths, after)
-        return after
+        table = self.page_table
+        if table.shape[:1] == self.lengths.shape and table.shape[1] > 0:
+            return self.lengths + (table[:, 0] >= 0)
+        return self.lengths + 1  # tables that do not fit are refused where they are used
+
+    def refuse(self, x: torch.Tensor) -> torch.Tensor:
+        """x; NaN in its place where the batch has packed rows leave out tokens that
+        their sequences hold.  Decided on the device: the lengths are there."""
+        if self._refused or self.offsets is None or self.page_table is None or self.key_offsets is not None:
+            return x
+        return torch.where(self.lengths.any(), float("nan"), x)
 
     def for_step(self) -> "AttentionBatch":
-        """The same with `after` made once, for all layers of a step."""
-        if self.offsets is not None or self._given is not None:
+        """The same for all layers of a step: `after` made once, refused (or not) already."""
+        if self.offsets is None and self._given is not None or self.page_table is None:
             return self
-        return dataclasses.replace(self, after=self._tokens())
+        step = copy.copy(self)
+        if self.offsets is None:
+            step.after = self._tokens()
+        step._refused = True
+        return step
 
 
 class SelfAttention(torch.nn.Module):
@@ -136,6 +151,7 @@ class SelfAttention(torch.nn.Module):
             raise RuntimeError("a batch with a page table needs a cache")
         if not self.causal:
             raise RuntimeError("a cache is of causal attention")
+        k = batch.refuse(k)
         self.cache.append(k, v, batch.page_table, batch.lengths, batch.offsets)
         if batch.offsets is None:
             return self.cache.attend(q, batch.page_table, batch.after, scale=self.scale)

@@ -58,3 +58,22 @@ def test_idle_slots_hold_nothing():
     batch = single(page_table=table, lengths=torch.tensor([4, 0, 9], dtype=torch.int32))
     assert batch.after.tolist() == [5, 0, 9] and batch.for_step().after.tolist() == [5, 0, 9]
     assert single(page_table=table[:, :0]).after.tolist() == [5, 1, 10]
+
+
+def test_packed_rows_of_sequences_that_hold_tokens_are_refused():
+    """Without key_offsets: NaN in place of what a step works on, once a step."""
+    import torch
+
+    def ints(*values):
+        return torch.tensor(values, dtype=torch.int32)
+
+    x, table = torch.arange(20.0).view(10, 2), torch.zeros(4, 2, dtype=torch.int32)
+    batch = pkg().AttentionBatch(ints(1, 3, 3, 6, 8), table, ints(0, 5, 2, 0))
+    assert bool(batch.refuse(x).isnan().all())
+    step = batch.for_step()
+    assert step.refuse(x) is x and step.lengths is batch.lengths and step.after is None
+    batch.lengths.zero_()
+    assert torch.equal(batch.refuse(x), x)
+    for other in (pkg().AttentionBatch(ints(1, 3, 3, 6, 8), table, ints(0, 5, 2, 0), ints(1, 3, 8, 13, 15), 15),
+                  pkg().AttentionBatch(ints(0, 3)), single()):
+        assert other.refuse(x) is x

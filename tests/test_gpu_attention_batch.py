@@ -131,3 +131,39 @@ def test_idle_slots(dev, quantised):
         lost = M.AttentionBatch(page_table=idle, lengths=index([3, 7, 8], dev))
         got = M.run_blocks(blocks, x, final, lost)[1]
         assert bool(got[1].isnan().all()) and bool(got[[0, 2]].isfinite().all())
+
+
+@pytest.mark.parametrize("through", ["run_blocks", "module"])
+def test_prompts_behind_cached_tokens_need_key_offsets(dev, through):
+    """Without them a step whose sequences hold tokens, which its rows would leave out, is NaN,
+    captured and replayed too; over empty sequences it has the bits of a step without a cache."""
+    import torch
+
+    M = pkg()
+    blocks, final, fresh = cached_blocks(dev)
+    x, offsets, lengths = rows(dev, 60), index([0, 20, 35, 58], dev), index([0, 0, 0], dev)
+    batch = M.AttentionBatch(offsets, tables(dev, 3, 5), lengths)
+
+    def step(batch):
+        return M.run_blocks(blocks, x, final, batch)[1] if through == "run_blocks" else blocks[0].mlp(x, batch)
+
+    with torch.no_grad():
+        fresh()
+        want = step(M.AttentionBatch(offsets))
+        assert torch.equal(step(batch), want)
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            step(batch)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = step(batch)
+        for values in ([0, 0, 0], [0, 12, 0], [3, 3, 3], [0, 0, 0]):
+            lengths.copy_(index(values, dev))
+            graph.replay()
+            torch.cuda.synchronize()
+            for got in (out, step(batch)):
+                if any(values):
+                    assert bool(got[:58].isnan().all())
+                else:
+                    assert torch.equal(got, want)
