@@ -108,11 +108,25 @@ class AttentionBatch:
         return step
 
 
+class _ReadBack(torch.autograd.Function):
+    """Keys and values as a cache gives them for those that were written to it:
+    no gradient finds the way back, so that a backward pass raises."""
+
+    @staticmethod
+    def forward(ctx, k_new, v_new, k, v):
+        return k.view_as(k), v.view_as(v)
+
+    @staticmethod
+    def backward(ctx, d_k, d_v):
+        raise RuntimeError("keys and values that went through a cache have no gradient")
+
+
 class SelfAttention(torch.nn.Module):
     """``o_proj(attention(qkv_proj(x)))``.  qkv_proj holds the query heads' rows,
     then the key heads', then the values'; both are any module from bfloat16
     rows to bfloat16 rows (nn.Linear, Int4Linear, BlockFP8Linear).  cache: a
-    KVCache, for batches with a page table."""
+    KVCache, for batches with a page table; what is read from it has no gradient, and a
+    backward pass through it raises."""
 
     takes_batch = True
 
@@ -156,7 +170,9 @@ class SelfAttention(torch.nn.Module):
         if batch.offsets is None:
             return self.cache.attend(q, batch.page_table, batch.after, scale=self.scale)
         if batch.key_offsets is not None:
-            k, v = self.cache.read(batch.page_table, batch.key_offsets, batch.keys)
+            k_new, v_new, (k, v) = k, v, self.cache.read(batch.page_table, batch.key_offsets, batch.keys)
+            if torch.is_grad_enabled() and (k_new.requires_grad or v_new.requires_grad):
+                k, v = _ReadBack.apply(k_new, v_new, k, v)
         return packed_attention(q, k, v, batch.offsets, batch.key_offsets, scale=self.scale)
 
     def to_int4(self, group_size: int = 64, symmetric: bool = False) -> "SelfAttention":

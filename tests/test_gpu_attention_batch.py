@@ -167,3 +167,32 @@ def test_prompts_behind_cached_tokens_need_key_offsets(dev, through):
                     assert bool(got[:58].isnan().all())
                 else:
                     assert torch.equal(got, want)
+
+
+def test_no_gradient_through_a_cache(dev):
+    """Results over what a cache holds raise in a backward pass, instead of gradients that lack
+    what went through it; a prompt's own rows have theirs."""
+    import torch
+
+    M = pkg()
+    a = M.SelfAttention(256, 8, 2, 64, device=dev)
+    a.cache = M.KVCache(16, 16, 2, 64, device=dev)
+    table, x, offsets = tables(dev, 2, 8), rows(dev, 20), index([0, 10, 20], dev)
+    y = a(x, M.AttentionBatch(offsets, table, index([0, 0], dev)))
+    got = torch.autograd.grad(y.float().square().sum(), list(a.parameters()))
+    y = a(x, M.AttentionBatch(offsets))
+    want = torch.autograd.grad(y.float().square().sum(), list(a.parameters()))
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    chunk = M.AttentionBatch(offsets, table, index([10, 10], dev), index([0, 20, 40], dev), 40)
+    y = a(x, chunk)
+    with torch.no_grad():
+        assert torch.equal(y, a(x, chunk))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        y.float().sum().backward()
+    y = a(x[:2], M.AttentionBatch(page_table=table, lengths=index([20, 20], dev)))
+    with pytest.raises(RuntimeError, match="autograd"):
+        y.float().sum().backward()
+    assert all(p.grad is None or p is a.o_proj.weight for p in a.parameters())
+    for p in a.parameters():  # served with frozen weights: nothing asks for one
+        p.requires_grad_(False)
+    assert not a(x, chunk).requires_grad
