@@ -965,7 +965,9 @@ hipError_t join_key_gradients(const AttentionArgs& a, hipStream_t st) {
 // Whether to take 128 keys a workgroup, which load each row half as often as 64: where
 // they are enough for every CU, and twice as many in causal sequences, whose tiles have
 // different amounts of work (8,192 tokens in two sequences, 16 / 4 heads, all seen: 927 us
-// with 128 keys, 1026 with 64; 4,096 causal tokens, 16 / 4 heads of 96: 556 and 401).
+// with 128 keys, 1026 with 64; 4,096 causal tokens, 16 / 4 heads of 96: 556 and 401).  With
+// 32,768 keys of all heads, of up to 64 values and all seen, their rows are split too (all
+// gradients of 4,096 tokens, 32 / 8 heads: 528 us; unsplit 536, split with 64 keys 545).
 bool wide_key_tiles(const AttentionArgs& a) { return a.keys * a.kv_heads / 128 >= (a.causal ? 512 : 256); }
 
 template <int DP, bool EXACT, int NB>
