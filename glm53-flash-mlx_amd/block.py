@@ -55,7 +55,7 @@ def run_blocks(blocks, residual: torch.Tensor, final_weight: torch.Tensor | None
     blocks = list(blocks)
     if not blocks:
         raise ValueError("run_blocks needs a block")
-    if isinstance(batch, AttentionBatch):
+    if isinstance(batch, AttentionBatch) and any(getattr(getattr(b, "mlp", None), "takes_batch", False) for b in blocks):
         residual, batch = batch.refuse(residual), batch.for_step()
     normed = None
     for block, after in zip(blocks, blocks[1:] + [None]):

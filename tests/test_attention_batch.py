@@ -77,3 +77,18 @@ def test_packed_rows_of_sequences_that_hold_tokens_are_refused():
     for other in (pkg().AttentionBatch(ints(1, 3, 3, 6, 8), table, ints(0, 5, 2, 0), ints(1, 3, 8, 13, 15), 15),
                   pkg().AttentionBatch(ints(0, 3)), single()):
         assert other.refuse(x) is x
+
+
+def test_blocks_without_attention_do_not_see_the_batch():
+    """Not even one that attention would refuse."""
+    import torch
+
+    class Same(torch.nn.Module):
+        mlp, eps, norm_weight = None, 1e-5, None
+
+        def forward(self, residual, normed=None, next_weight=None, batch=None):
+            return residual, normed
+
+    table, ints = torch.zeros(1, 2, dtype=torch.int32), torch.tensor([0, 4], dtype=torch.int32)
+    x = torch.ones(4, 8)
+    assert pkg().run_blocks([Same()], x, None, pkg().AttentionBatch(ints, table, ints[1:]))[0] is x
