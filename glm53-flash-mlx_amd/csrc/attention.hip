@@ -5,10 +5,10 @@ namespace glm53 {
 
 hipError_t launch_attention(const AttentionArgs& a, hipStream_t st) {
   if (a.dim > 128) return launch_attention_wide(a, st);
-  if (a.dim == 128) return launch_forward<Forward<128, true, 4>>(a, st);
-  if (a.dim == 64) return launch_forward<Forward<64, true, 4>>(a, st);
-  if (a.dim > 64) return launch_forward<Forward<128, false, 4>>(a, st);
-  return launch_forward<Forward<64, false, 4>>(a, st);
+  if (a.dim == 128) return launch_forward<Forward<128, true>>(a, st);
+  if (a.dim == 64) return launch_forward<Forward<64, true>>(a, st);
+  if (a.dim > 64) return launch_forward<Forward<128, false>>(a, st);
+  return launch_forward<Forward<64, false>>(a, st);
 }
 
 int attention_row_splits(const AttentionArgs& a) {

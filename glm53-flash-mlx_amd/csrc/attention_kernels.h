@@ -39,7 +39,7 @@ __device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
 // Around a run of products: its wavefront goes first on its SIMD, so that the
 // other one there comes to its weights while this one multiplies (16,384 causal
-// tokens, 8 heads of 128: 505 us, without 560).
+// tokens, 8 / 1 heads of 128, when it was built: 505 us, without 560).
 __device__ __forceinline__ void products(bool begin) {
   if (begin)
     __builtin_amdgcn_s_setprio(1);
@@ -185,9 +185,9 @@ int64_t tile_numbers(int64_t rows, bool packed, int sequences, int size) {
 // 64 rows a wavefront, which halve the LDS reads, leave one wavefront a SIMD and
 // were slower.  16,384 causal tokens, 8 / 1 heads: 522 us, 1,053 TFLOP/s.
 
-template <int DP_, bool EXACT, int W_>
+template <int DP_, bool EXACT>
 struct Forward {
-  static constexpr int DP = DP_, W = W_;
+  static constexpr int DP = DP_, W = 4;
   static constexpr int kRows = 32 * W, kThreads = 64 * W, kKeys = 64, T = DP / 32;
   using Tile = HeadTile<DP, kKeys, W>;
   static constexpr int kLds = 4 * Tile::kBytes;  // two stages of keys and values
@@ -365,13 +365,13 @@ struct Forward {
     }
 
     // no key seen; or scores that are no FP32 numbers once scaled, which leave no weights: NaN
-    const float none = m * c == INFINITY ? NAN : 0.0f;
-    const float total = both_sum(l), inverse = total == 0.0f ? none : 1.0f / (total * by);
+    const float total = both_sum(l);
     if (row >= seg.last) return;
+    const float top = m * c, none = top == INFINITY ? NAN : 0.0f, inverse = total == 0.0f ? none : 1.0f / (total * by);
     const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
     store_operand<DP>(a.out + (token * heads + query_head) * dim, out, inverse, dim, h);
     if (a.lse != nullptr && h == 0)
-      a.lse[static_cast<int64_t>(head) * a.tokens * a.group + row] = total == 0.0f ? none : m * c + __builtin_amdgcn_logf(total);
+      a.lse[static_cast<int64_t>(head) * a.tokens * a.group + row] = total == 0.0f ? none : top + __builtin_amdgcn_logf(total);
   }
 };
 
@@ -399,14 +399,14 @@ __global__ __launch_bounds__(F::kThreads, F::DP == 256 ? 1 : 2) void attention_k
 
 // d_q: a lane's row as in the forward pass, a tile of 64 keys at a time.  Bound as
 // that is, by four runs of products for its two.
-template <int DP_, bool EXACT, int W_, bool DQ>
+template <int DP_, bool EXACT, bool DQ>
 struct QueryGradient {
-  static constexpr int DP = DP_, W = W_;
+  static constexpr int DP = DP_, W = 4;
   static constexpr int kRows = 32 * W, kThreads = 64 * W, kKeys = 64, T = DP / 32;
   static constexpr int kAhead = DP >= 128 ? 1 : 2;  // the registers leave no more
   // Rows of up to 256 keys, whose `out` is no mean of many and whose delta is off by more,
   // take their sums of dS in a pass of their own first (d_q of 30 sequences of 8 to 100
-  // tokens off by 0.0022 instead of 0.0029).
+  // tokens off by 0.0023 instead of 0.0029).
   static constexpr int kFewSteps = 4;
   using Tile = HeadTile<DP, kKeys, W>;
   static constexpr int kLds = 4 * Tile::kBytes;
@@ -677,7 +677,9 @@ struct KeyGradient {
       const int token0 = group.quotient(row0);
       const uint16_t* qp = a.q.p + token0 * a.q.token + head * a.group * a.q.head;
       const uint16_t* op = a.d_out.p + token0 * a.d_out.token + head * a.group * a.d_out.head;
-      const auto offset = [&](const Rows16& x) {  // start, and so row0, is a token's first row
+      // row0 may lie inside token0 where a group does not divide RT, so that every row's token and
+      // head are found; load_even needs whole tokens a tile, which `even` says
+      const auto offset = [&](const Rows16& x) {
         return [&](int n) {
           const int token = group.quotient(row0 + n), g = row0 + n - token * a.group;
           return static_cast<uint32_t>(token - token0) * static_cast<uint32_t>(2 * x.token) + static_cast<uint32_t>(g) * static_cast<uint32_t>(2 * x.head);
@@ -974,15 +976,17 @@ template <int DP, bool EXACT, int NB>
 hipError_t backward(const AttentionArgs& a, hipStream_t st) {
   hipError_t e = hipSuccess;
   if (a.d_q != nullptr)
-    e = launch_query_gradient<QueryGradient<DP, EXACT, 4, true>>(a, st);
+    e = launch_query_gradient<QueryGradient<DP, EXACT, true>>(a, st);
   else if (a.d_k != nullptr)
-    e = launch_query_gradient<QueryGradient<DP, EXACT, 4, false>>(a, st);  // for delta
+    e = launch_query_gradient<QueryGradient<DP, EXACT, false>>(a, st);  // for delta
   if (e != hipSuccess) return e;
   // both gradients of 256 columns at once would not leave a lane registers for the scores
-  if (DP < 256 && a.d_k != nullptr && a.d_v != nullptr) {
-    e = wide_key_tiles(a) ? launch_key_gradient<KeyGradient<DP, EXACT, NB, 1, DP < 256, true>>(a, st)
-                          : launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, DP < 256, true>>(a, st);
-    return e != hipSuccess ? e : join_key_gradients(a, st);
+  if constexpr (DP < 256) {
+    if (a.d_k != nullptr && a.d_v != nullptr) {
+      e = wide_key_tiles(a) ? launch_key_gradient<KeyGradient<DP, EXACT, NB, 1, true, true>>(a, st)
+                            : launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, true, true>>(a, st);
+      return e != hipSuccess ? e : join_key_gradients(a, st);
+    }
   }
   if (a.d_k != nullptr)
     if (e = launch_key_gradient<KeyGradient<DP, EXACT, NB, 2, true, false>>(a, st); e != hipSuccess) return e;

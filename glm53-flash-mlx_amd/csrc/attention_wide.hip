@@ -5,8 +5,8 @@
 namespace glm53 {
 
 hipError_t launch_attention_wide(const AttentionArgs& a, hipStream_t st) {
-  if (a.dim == 256) return launch_forward<Forward<256, true, 4>>(a, st);
-  return launch_forward<Forward<256, false, 4>>(a, st);
+  if (a.dim == 256) return launch_forward<Forward<256, true>>(a, st);
+  return launch_forward<Forward<256, false>>(a, st);
 }
 
 hipError_t launch_attention_backward_wide(const AttentionArgs& a, hipStream_t st) {
