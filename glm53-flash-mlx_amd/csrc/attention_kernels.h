@@ -180,10 +180,10 @@ int64_t tile_numbers(int64_t rows, bool packed, int sequences, int size) {
 // Bound by a SIMD's two wavefronts, which take turns at its matrix unit and its
 // vector unit: a tile of 128 columns is 2,048 clocks of products for both, and the
 // 32 exponentials, maxima, sums and conversions of each lane are about as many.
-// 4,096 + 4,096 tokens, 16 / 4 heads of 128, all seen: 254 us, 1,081 TFLOP/s, the
-// matrix unit busy half of the time (228 us without the softmax's instructions);
-// 64 rows a wavefront, which halve the LDS reads, leave one wavefront a SIMD and
-// were slower.  16,384 causal tokens, 8 / 1 heads: 522 us, 1,053 TFLOP/s.
+// 4,096 + 4,096 tokens, 16 / 4 heads of 128, all seen: 242 us, 1,138 TFLOP/s, the
+// matrix unit busy half of the time (228 us without the softmax's instructions, when all took
+// 254); 64 rows a wavefront, which halve the LDS reads, leave one wavefront a SIMD and
+// were slower.  16,384 causal tokens, 8 / 1 heads: 477 us, 1,153 TFLOP/s.
 
 template <int DP_, bool EXACT>
 struct Forward {

@@ -206,16 +206,15 @@ namespace {
 // heads of 128).
 //
 // That case reads 5.3 TB/s, 64 sequences of up to 8,192 tokens 5.7 in bf16 and 4.8 in
-// E4M3 (160 us); a copy on the card reaches 5.0.  The smallest call takes 6.2 us here,
-// loads that wait for each other (lengths, table, keys), and 4.7 in the join.
+// E4M3 (160 us); a copy on the card reaches 5.0.  The smallest call takes 6.7 us here,
+// loads that wait for each other (lengths, table, keys), and 4.9 in the join.
 
 // Sums of weights, which reach 2^8, times values may pass FP32's range where their mean
 // does not, and a weight times its row's power of two a bf16 operand's.  A head whose part of
 // a run is not finite takes the run again with weights kSmaller of these, whose sum is
 // below 1 over 2^31 tokens (powers of two change no bit, but of values below 2^-86 beside
 // such large ones); the join takes all of its parts so.
-//
-constexpr int kHeads = 16;  // columns of the MFMA
+constexpr int kHeads = 16;  // columns of the MFMA: more heads of a key head read its cache once for 16 each
 constexpr float kSmaller = 0x1p-40f;
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
