@@ -86,7 +86,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     over that sequence's first lengths[s] tokens in the cache.
 
     lengths int32 [sequences].  A sequence without a token gives 0, one with a
-    token that has no page in the cache NaN.  scale: 1 / sqrt(dim) where None.
+    token that has no page in the cache NaN, and so does a head whose largest scaled
+    score is beyond FP32.  scale: 1 / sqrt(dim) where None, 2^-64 to 2^127.
     The softmax and all sums are FP32, its weights are rounded to bf16 as
     operands, the result once."""
     N.same_device(q, k_pages, v_pages, page_table, lengths, k_scales, v_scales)

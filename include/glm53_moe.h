@@ -742,7 +742,8 @@ int glm53_kv_read(const glm53_kv_cache* cache, const int32_t* offsets, int64_t r
 /* One query a sequence, q [sequences, heads], over its positions 0 ..
  * lengths[s] - 1; out BF16 [sequences, heads, head_dim] contiguous.  A sequence
  * without a token gives 0, one with a position that has no page in the cache
- * NaN.  The work is split evenly over the card whatever the lengths; parts
+ * NaN, a head whose largest scaled score is beyond FP32 NaN; scale 2^-64 to
+ * 2^127.  The work is split evenly over the card whatever the lengths; parts
  * are joined in their order.  Workspace (256-byte aligned) needs no
  * initialisation. */
 size_t glm53_paged_attention_workspace_bytes(int64_t head_dim, int32_t e4m3); /* whatever the sequences and heads */
